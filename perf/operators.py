@@ -302,7 +302,7 @@ def _plain_append_one(s, x, pool, scales, seq, at, page, slot):
     tail = tail[kept].long()
     filled = (old % p)[kept]
     before = scales[tail]
-    now = torch.where(most >= 0, most / 127.0, scales)
+    now = torch.where(most >= 0, most * (1.0 / 127.0), scales)
     now[tail] = torch.maximum(now[tail], before)
     scales.copy_(now)
     ratio = torch.where(now[tail] > 0, before / now[tail], torch.zeros_like(before))
