@@ -16,6 +16,8 @@ SYMBOLS = [
     "shlo_max_axis", "shlo_contiguous", "shlo_eval", "shlo_kernel_new", "shlo_kernel_free",
     "shlo_kernel_apply", "shlo_compile", "shlo_fn_free", "shlo_apply", "shlo_libm_erff_range",
     "shlo_count_nonzero", "shlo_current_stream", "shlo_launch_count", "shlo_device_ptr", "shlo_mul_mat_noalloc",
+    "shlo_rope_phases", "shlo_rope_noalloc", "shlo_kv_append_noalloc", "shlo_kv_gather_noalloc",
+    "shlo_kv_attend_workspace", "shlo_kv_attend_noalloc",
 ]
 
 
@@ -29,6 +31,24 @@ TRACE_FN = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.POINTER(c_arr)
                             ctypes.POINTER(c_arr), ctypes.POINTER(ctypes.c_int), ctypes.c_int,
                             ctypes.c_void_p, ctypes.c_size_t)
 FREE_FN = ctypes.CFUNCTYPE(None, ctypes.c_void_p)
+
+
+
+class KvPool(ctypes.Structure):
+    """shlo_kv_pool."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("pages", ctypes.c_int64), ("page_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64),
+                ("scale_page_stride", ctypes.c_int64), ("scale_head_stride", ctypes.c_int64),
+                ("heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("page_tokens", ctypes.c_int32)]
+
+
+class KvBatch(ctypes.Structure):
+    """shlo_kv_batch."""
+    _fields_ = [("starts", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("tables", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("seqs", ctypes.c_int32), ("table_pages", ctypes.c_int32),
+                ("tokens", ctypes.c_int32)]
+
 
 _lib = None
 
@@ -94,6 +114,16 @@ def load() -> ctypes.CDLL:
     L.shlo_mul_mat_noalloc.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
                                        ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                        ctypes.c_void_p]
+    p, i32, i64, u8 = ctypes.c_void_p, ctypes.c_int32, ctypes.c_int64, ctypes.c_uint8
+    f32, f64 = ctypes.c_float, ctypes.c_double
+    pool, batch = ctypes.POINTER(KvPool), ctypes.POINTER(KvBatch)
+    L.shlo_rope_phases.argtypes = [i32, f64, i32, f64, f64, f64, f64, p, ctypes.POINTER(f32)]
+    L.shlo_rope_noalloc.argtypes = [p, i64, i64, p, p, p, i64, i64, i64, i32, i32, i32, u8, ctypes.c_uint32, f32, p]
+    L.shlo_kv_append_noalloc.argtypes = [pool, batch, p, i64, i64, p, i64, i64, u8, p]
+    L.shlo_kv_gather_noalloc.argtypes = [pool, p, i64, i32, i32, p, p, i64, p, i64, i64, p, i64, i64, u8, p]
+    L.shlo_kv_attend_workspace.argtypes = [ctypes.POINTER(ctypes.c_size_t)]
+    L.shlo_kv_attend_noalloc.argtypes = [pool, batch, p, i64, i64, i32, u8, f32, i32, i32, p, i64, i64, p, p,
+                                         ctypes.c_size_t, p]
     special = {"shlo_last_error", "shlo_empty", "shlo_retain", "shlo_release", "shlo_kernel_free", "shlo_fn_free"}
     for name in SYMBOLS:
         if name not in special:

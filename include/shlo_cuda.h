@@ -189,6 +189,91 @@ int shlo_device_ptr(shlo_arr a, void **ptr, int *device);
 int shlo_mul_mat_noalloc(const float *w, const float *x, float *y, int64_t K, int64_t M, int64_t R, int64_t N,
                          int64_t w_batch_stride, void *stream);
 
+/* ---- decoder operators (no counterpart in the reference, whose modules keep nothing between calls) ----
+   Rotary positions, a paged key/value cache in 8 bits, and the attention that
+   reads it, for hosts that generate token by token. The *_noalloc functions
+   work on caller-owned device memory of the current device, allocate nothing,
+   and queue their work on `stream` (a cudaStream_t; NULL is the default
+   stream). Activations are float16 or float32 (`dtype`), given by a pointer and
+   two strides in values, of a token and of a head; the values of a head are
+   contiguous. Indices are int32 on the device. A host that has no memory of
+   its own uses the "shlo_rope" kernel and the shlo_kv_* functions on arrays. */
+
+/* The phases of `rot` turned dimensions, [rot / 2] int64 on the host: pair i
+   turns by base^(-2i / rot) radians a position, kept as turns a position in
+   units of 2^-64. `scaling` for contexts `by` times longer: 0 none; 1 every
+   frequency divided by `by`; 2 the base raised so that the slowest pair turns
+   `by` times slower; 3 pairs that turn `fast` times or more over `trained`
+   positions kept, those of at most `slow` turns divided, a ramp over the pairs
+   between; 4 the same ends blended by the turns. *factor is what the results
+   are multiplied by (1, or 0.1 ln(by) + 1 for 3). */
+int shlo_rope_phases(int32_t rot, double base, int32_t scaling, double by, double trained, double fast, double slow,
+                     int64_t *phases, float *factor);
+/* Turn the first `rot` of `dim` dimensions of x[tokens][heads][dim] by each
+   token's position into y, the others copied:
+   (a, b) -> factor (a cos - b sin, b cos + a sin). y may be x itself. flags: 1
+   pairs side by side (2i, 2i + 1) instead of half the part apart
+   (i, i + rot / 2); 2 turned back (the gradient of the turn). Positions may be
+   negative; angles are exact to 2^-32 turns at every position. */
+int shlo_rope_noalloc(const void *x, int64_t x_token, int64_t x_head, const int32_t *positions, const int64_t *phases,
+                      void *y, int64_t y_token, int64_t y_head, int64_t tokens, int32_t heads, int32_t dim, int32_t rot,
+                      uint8_t dtype, uint32_t flags, float factor, void *stream);
+
+/* A paged cache: `pages` pages of `page_tokens` tokens (16, 32, 64, 128 or 256)
+   for `heads` key/value heads of `head_dim` values (a multiple of 16, up to
+   256). A value is its int8 times the scale of its page and head. k and v have
+   the same strides, in bytes (multiples of 16), so pages may be laid out by
+   heads or by tokens; the scales' strides are in floats. */
+typedef struct {
+	int8_t *k, *v;
+	float *k_scale, *v_scale;
+	int64_t pages;
+	int64_t page_stride, head_stride, token_stride;
+	int64_t scale_page_stride, scale_head_stride;
+	int32_t heads, head_dim, page_tokens;
+} shlo_kv_pool;
+/* A batch of sequences, all arrays on the device: sequence s has the rows
+   starts[s] .. starts[s + 1] - 1 of the call's activations as its newest tokens
+   (starts[0] = 0, ascending; no rows is allowed), lens[s] tokens in all with
+   them, and page tables[s * table_stride + i] for its tokens
+   i * page_tokens ... An entry outside the cache (-1, say) is a page it does
+   not have. */
+typedef struct {
+	const int32_t *starts, *lens, *tables;
+	int64_t table_stride;
+	int32_t seqs, table_pages, tokens; /* tokens: the rows of the activations */
+} shlo_kv_batch;
+
+/* Round the batch's new keys and values into their pages. Where a page's
+   largest magnitude grows, its older tokens are rounded again; a page whose
+   first token is among the new ones starts afresh. Values that are not finite
+   make the page's scale NaN. No two sequences of a call may write one page
+   (copy a shared last page first). A call repeated changes nothing. */
+int shlo_kv_append_noalloc(const shlo_kv_pool *pool, const shlo_kv_batch *batch, const void *k, int64_t k_token,
+                           int64_t k_head, const void *v, int64_t v_token, int64_t v_head, uint8_t dtype, void *stream);
+/* The values that the cache holds for n tokens (sequence seq[i], position
+   pos[i]) into k and v [n][heads][head_dim] (pointers and strides multiples of
+   16 bytes); a token that the tables do not hold reads as zeros. */
+int shlo_kv_gather_noalloc(const shlo_kv_pool *pool, const int32_t *tables, int64_t table_stride, int32_t seqs,
+                           int32_t table_pages, const int32_t *seq, const int32_t *pos, int64_t n, void *k,
+                           int64_t k_token, int64_t k_head, void *v, int64_t v_token, int64_t v_head, uint8_t dtype,
+                           void *stream);
+/* The bytes of workspace that an attention call needs on the current device. */
+int shlo_kv_attend_workspace(size_t *bytes);
+/* out = soft_max(scale q k^T) v over the cache, per row of the batch and query
+   head; `heads` is a multiple of the cache's, consecutive ones sharing a
+   key/value head. A row at position p (the newest token's is lens - 1) sees the
+   tokens t < lens, with `causal` t <= p, with `window` > 0 t > p - window, in
+   pages that its table has. A row that sees none gives 0, and -inf in lse. lse
+   (float32 [tokens][heads], or NULL) is the logarithm of the sum of the
+   exponentials of the scaled scores. The workspace must be zero before the
+   first call that uses it; calls leave it ready for the next, on one stream at
+   a time. The same call gives the same bits. */
+int shlo_kv_attend_noalloc(const shlo_kv_pool *pool, const shlo_kv_batch *batch, const void *q, int64_t q_token,
+                           int64_t q_head, int32_t heads, uint8_t dtype, float scale, int32_t causal, int32_t window,
+                           void *out, int64_t out_token, int64_t out_head, float *lse, void *workspace,
+                           size_t workspace_bytes, void *stream);
+
 /* ---- test-driver helpers (Mlx.lean:69-73) ---- */
 
 /* smlx_libm_erff_range: this platform's binary32 erff over `count`
