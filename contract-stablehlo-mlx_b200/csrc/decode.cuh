@@ -52,28 +52,30 @@ size_t attend_work_bytes(int sms);
 int launch_kv_attend(const AttendCall &c, int sms, cudaStream_t st);
 
 // The new tokens of sequence s and its length, with the caller's arrays held
-// to the batch: starts to [0, tokens], the length to 0 and above.
+// to the batch: starts to [0, tokens], the length to 0 and above. `starts` and
+// `lens` are the batch's arrays or a block's copies of them.
 struct SeqSpan {
   int start, n, len;
 };
-__device__ __forceinline__ SeqSpan seq_span(const shlo_kv_batch &b, int s) {
+__device__ __forceinline__ SeqSpan seq_span(const int32_t *starts, const int32_t *lens, int tokens, int s) {
   SeqSpan r;
-  r.start = min(max(__ldg(b.starts + s), 0), b.tokens);
-  r.n = max(min(max(__ldg(b.starts + s + 1), 0), b.tokens) - r.start, 0);
-  r.len = max(__ldg(b.lens + s), 0);
+  r.start = min(max(starts[s], 0), tokens);
+  r.n = max(min(max(starts[s + 1], 0), tokens) - r.start, 0);
+  r.len = max(lens[s], 0);
   return r;
 }
-// The sequence that owns slot `slot` where sequence s has the slots from
-// starts[s] * num / 2^shift + extra * s on: the last whose first is not above it.
-__device__ __forceinline__ int slot_base(const shlo_kv_batch &b, int s, int num, int shift, int extra) {
-  const int64_t at = min(max(__ldg(b.starts + s), 0), b.tokens);
+// Slots: sequence s has those from starts[s] * num / 2^shift + extra * s on.
+__device__ __forceinline__ int slot_base(const int32_t *starts, int tokens, int s, int num, int shift, int extra) {
+  const int64_t at = min(max(starts[s], 0), tokens);
   return (int)((at * num) >> shift) + extra * s;
 }
-__device__ __forceinline__ int slot_owner(const shlo_kv_batch &b, int slot, int num, int shift, int extra) {
-  int lo = 0, hi = b.seqs - 1;
+// The owner of a slot: the last sequence, from `lo` on, whose first is not above it.
+__device__ __forceinline__ int slot_owner(const int32_t *starts, int tokens, int seqs, int lo, int slot, int num, int shift,
+                                          int extra) {
+  int hi = seqs - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
-    if (slot_base(b, mid, num, shift, extra) <= slot) lo = mid;
+    if (slot_base(starts, tokens, mid, num, shift, extra) <= slot) lo = mid;
     else hi = mid - 1;
   }
   return lo;

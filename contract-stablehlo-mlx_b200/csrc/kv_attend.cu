@@ -55,19 +55,43 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t *>(&v);
 }
-__device__ __forceinline__ uint4 ld_stream16(const int8_t *p) {
+// Copy N bytes from global to this lane's place in shared memory, past L1; zeros where `ok` is false.
+template <int N>
+__device__ __forceinline__ void copy_async(uint32_t dst, const int8_t *src) {
+  if constexpr (N == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(N) : "memory");
+}
+template <int N>
+__device__ __forceinline__ void copy_async(uint32_t dst, const int8_t *src, bool ok) {
+  const int n = ok ? N : 0;
+  if constexpr (N == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(N), "r"(n) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t p) {
   uint4 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(p) : "memory");
   return r;
 }
-__device__ __forceinline__ uint2 ld_stream8(const int8_t *p) {
+__device__ __forceinline__ uint2 lds8(uint32_t p) {
   uint2 r;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "l"(p));
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(p) : "memory");
   return r;
 }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // DP: the head width rounded up to 64, 128 or 256; NT: row tiles of 8; TERMS: 1
-// (float16 queries) or 2 (float32).
+// (float16 queries) or 2 (float32). A step is 16 MT keys of a warp: its keys'
+// and its values' bytes are a piece each, in one ring of R pieces (keys 0, values
+// 0, keys 1, ...): the piece R on is asked for as soon as one is used up. A lane
+// copies the bytes it will read itself to a place of its own (so the ring needs
+// no barrier and no reads conflict): the ring, not the warps' number, covers the
+// memory's latency.
 template <typename T, int DP, int NT>
 struct Shape {
   static constexpr int TERMS = sizeof(T) == 2 ? 1 : 2;
@@ -76,92 +100,195 @@ struct Shape {
   static constexpr int GRAN = kWarps * MT * 16;
   static constexpr int KS = DP / 16;            // 16-wide steps of the first product
   static constexpr int OSTRIDE = DP + 4;
+  static constexpr int PER_SM = DP == 64 ? (NT == 1 ? 4 : 3) : DP == 128 ? (NT == 1 ? 3 : 2) : 2;
+  static constexpr int PIECE = MT * 16 * DP;    // bytes
+  static constexpr int R = DP == 64 ? 5 : 3;
   // shared memory, in 4-byte words
   static constexpr int Q_WORDS = KS * 32 * 2 * NT * TERMS;
+  static constexpr int RING_WORDS = kWarps * R * PIECE / 4;
   static constexpr int O_WORDS = kWarps * ROWS * OSTRIDE;
-  static constexpr int JOIN_WORDS = (kAttendMaxBlocks / kJoin + 2) * ROWS;
-  static constexpr int BODY = O_WORDS > JOIN_WORDS ? O_WORDS : JOIN_WORDS;
-  static constexpr int WORDS = Q_WORDS + BODY + 3 * kWarps * ROWS + 2 * (kThreads + 4) + 4;
+  static constexpr int JOIN_WORDS = 2 * (kJoin + 1) * ROWS;
+  static constexpr int BODY = O_WORDS > JOIN_WORDS ? O_WORDS : JOIN_WORDS;  // the warps' results, then a join's factors
+  static constexpr int BATCH = 258;  // the batch's arrays, up to 128 sequences
+  static constexpr int WORDS = 2 * Q_WORDS + RING_WORDS + BODY + 2 * kWarps * ROWS + 2 * ROWS + 2 * (kThreads + 4) + 16 + 4 + BATCH;
 };
 
-template <typename T, int DP, int NT, int PER_SM>
-__global__ void __launch_bounds__(kThreads, PER_SM) k_kv_attend_rows(const AttendArgs a, int min_gran) {
+// A block goes from segment to segment: a warp that is done with one asks for
+// the next one's first pieces and queries before the block's results meet, so
+// the memory is busy meanwhile. Per segment two barriers: the queries are
+// staged, the results are written.
+template <typename T, int DP, int NT>
+__global__ void __launch_bounds__(kThreads, Shape<T, DP, NT>::PER_SM) k_kv_attend_rows(const AttendArgs a, int min_gran) {
   using S = Shape<T, DP, NT>;
   constexpr int ROWS = S::ROWS, MT = S::MT, GRAN = S::GRAN, KS = S::KS, TERMS = S::TERMS, OS = S::OSTRIDE;
   constexpr int KC = DP / 64;        // 16-byte pieces a lane reads of a key row
   constexpr int VW = DP / 32;        // 4-byte words a lane reads of a value row
+  constexpr int R = S::R;
+  constexpr int QV = (DP + 127) / 128;  // groups of four dimensions a lane stages of a query row
+  constexpr int TL = 32 / MT;           // steps of a chunk of pages
   extern __shared__ __align__(16) uint32_t smem[];
-  uint32_t *const qs = smem;                                   // [TERMS][NT][KS][32][2]
-  float *const body = reinterpret_cast<float *>(smem + S::Q_WORDS);
-  float *const wm = body + S::BODY, *const wl = wm + kWarps * ROWS, *const rs = wl + kWarps * ROWS;
-  long long *const sched = reinterpret_cast<long long *>(rs + kWarps * ROWS);
-  unsigned *const flag = reinterpret_cast<unsigned *>(sched + kThreads + 4);
+  uint32_t *const qs0 = smem;                                  // [2][TERMS][NT][KS / 2][32][2][2]
+  uint32_t *const rings = smem + 2 * S::Q_WORDS;
+  float *const body = reinterpret_cast<float *>(rings + S::RING_WORDS);
+  float *const wm = body + S::BODY, *const wl = wm + kWarps * ROWS, *const rs0 = wl + kWarps * ROWS;  // rs0 [2][ROWS]
+  long long *const sched = reinterpret_cast<long long *>(rs0 + 2 * ROWS);
+  Place *const place = reinterpret_cast<Place *>(sched + kThreads + 4);
+  unsigned *const flag = reinterpret_cast<unsigned *>(place) + 16;
+  int *const batch = reinterpret_cast<int *>(flag + 4);
+  static_assert(sizeof(Place) <= 64, "its room in shared memory");
 
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, g = lane / 4, c = lane % 4;
   const int D = a.pool.head_dim, PT = 1 << a.page_shift;
-  Cursor cur;
-  if (!schedule<ROWS, GRAN, kThreads>(a, min_gran, sched, cur)) return;
+  Line line;
+  BatchArrays ba;
+  if (!schedule<ROWS, GRAN, kThreads>(a, min_gran, sched, batch, S::BATCH, ba, line)) return;
 
-  while (cur.at < cur.end && cur.head < a.pool.heads) {
-    RowTile t;
-    const int units = tile_of_slot<ROWS, GRAN>(a, cur.slot, t);
-    if (units == 0) {  // a slot without a tile
-      cur.slot++;
-      if (cur.slot == a.slots) {
-        cur.slot = 0;
-        cur.head++;
-      }
-      continue;
-    }
-    const int take = (int)min((long long)(units - cur.off), cur.end - cur.at);
-    const long long u0 = cur.at - cur.off, u1 = u0 + units;
-    const int head = cur.head;
-
-    // The rows' queries as the first product's right side: step (j, s) of lane
-    // (g, c) has row g's dimensions d, d + 2 and d + 1, d + 3, d = 64 j + 16 c + 4 s.
-    if constexpr (TERMS == 2) {
-      for (int row = warp; row < ROWS; row += kWarps) {
-        float m = 0.0f;
-        if (row < t.rows) {
-          const int r = t.row0 + row;
-          const T *q = static_cast<const T *>(a.q) + (int64_t)(t.start + r / a.group) * a.q_token +
-                       (int64_t)(head * a.group + r % a.group) * a.q_head;
-          for (int d = lane; d < D; d += 32) m = fmaxf(m, fabsf((float)q[d]));
-        }
+  // Rings: a lane's 16 bytes of copy i of a piece are at [i][lane].
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(rings) + warp * (R * S::PIECE) + lane * 16;
+  const uint32_t vring = ring - lane * 16 + lane * (VW == 2 ? 8 : 16);
+  const int64_t tok = a.pool.token_stride, tok8 = 8 * tok;
+  const int64_t klane = g * tok + 16 * c, vlane = 2 * c * tok + (VW == 2 ? 8 : 16) * g;
+  const bool wide = D == DP;
+  auto copy_k = [&](int slot, int head, int key, int pages, int at) {  // (the caller commits)
+    const uint32_t dst = ring + slot * S::PIECE;
 #pragma unroll
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    for (int mt = 0; mt < MT; mt++) {
+      const int pg = __shfl_sync(~0u, pages, at + mt);
+      const int8_t *src = a.pool.k + ((int64_t)head * a.pool.head_stride + (int64_t)max(pg, 0) * a.pool.page_stride +
+                                      ((key + mt * 16) & (PT - 1)) * tok + klane);
+      const int8_t *src8 = src + tok8;
+      if (wide && pg >= 0) {
+#pragma unroll
+        for (int j = 0; j < KC; j++) {
+          copy_async<16>(dst + (mt * 2 * KC + j) * 512, src + 64 * j);
+          copy_async<16>(dst + ((mt * 2 + 1) * KC + j) * 512, src8 + 64 * j);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < KC; j++) {
+          const bool ok = pg >= 0 && 64 * j + 16 * c < D;
+          copy_async<16>(dst + (mt * 2 * KC + j) * 512, src + 64 * j, ok);
+          copy_async<16>(dst + ((mt * 2 + 1) * KC + j) * 512, src8 + 64 * j, ok);
+        }
+      }
+    }
+  };
+  auto copy_v = [&](int slot, int head, int key, int pages, int at) {
+    constexpr int N = VW == 2 ? 8 : 16, VC = VW == 2 ? 1 : VW / 4;
+    const uint32_t dst = vring + slot * S::PIECE;
+#pragma unroll
+    for (int mt = 0; mt < MT; mt++) {
+      const int pg = __shfl_sync(~0u, pages, at + mt);
+      const int8_t *p[4];
+      p[0] = a.pool.v + ((int64_t)head * a.pool.head_stride + (int64_t)max(pg, 0) * a.pool.page_stride +
+                         ((key + mt * 16) & (PT - 1)) * tok + vlane);
+      p[1] = p[0] + tok;
+      p[2] = p[0] + tok8;
+      p[3] = p[2] + tok;
+      if (wide && pg >= 0) {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+          for (int j = 0; j < VC; j++) copy_async<N>(dst + ((mt * 4 + k) * VC + j) * (32 * N), p[k] + 128 * j);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+          for (int j = 0; j < VC; j++)
+            copy_async<N>(dst + ((mt * 4 + k) * VC + j) * (32 * N), p[k] + 128 * j, pg >= 0 && 128 * j + N * g < D);
+      }
+    }
+  };
+  // Keys of step i of this warp: key0 + i * GRAN + [0, 16 MT).
+  auto first_key = [&](const Segment &sg) { return (sg.t.lo / GRAN + sg.off) * GRAN + warp * (MT * 16); };
+  // Pages of the coming steps are held across the lanes, 32 tiles of 16 keys (TL
+  // steps) at a time; -1: no row of the tile sees a key of it, or there is none.
+  auto step_pages = [&](const Segment &sg, int step) -> int {
+    step += lane / MT;
+    const int key = first_key(sg) + step * GRAN + (lane % MT) * 16;
+    if (step >= sg.take || key >= sg.t.hi || key + 16 <= sg.t.lo) return -1;
+    const int p = __ldg(a.batch.tables + (int64_t)sg.t.seq * a.batch.table_stride + (key >> a.page_shift));
+    return p >= 0 && p < a.pool.pages ? p : -1;
+  };
+  // A segment's first pieces and its queries. The queries are the first
+  // product's right side: step (j, s) of lane (g, c) has row g's dimensions d,
+  // d + 2 and d + 1, d + 3, d = 64 j + 16 c + 4 s.
+  auto begin = [&](const Segment &sg, int buf) -> int {
+    constexpr int RW = ROWS / kWarps;
+    const int pages = step_pages(sg, 0), key = first_key(sg);
+    T raw[RW][QV][4];  // asked for before the pages are waited for
+#pragma unroll
+    for (int i = 0; i < RW; i++) {
+      const int row = warp + i * kWarps, r = sg.t.row0 + row;
+      const T *q = static_cast<const T *>(a.q) + (int64_t)(sg.t.start + r / a.group) * a.q_token +
+                   (int64_t)(sg.head * a.group + r % a.group) * a.q_head;
+#pragma unroll
+      for (int k = 0; k < QV; k++) {
+        const int d = 4 * (lane + 32 * k);
+#pragma unroll
+        for (int j = 0; j < 4; j++) raw[i][k][j] = row < sg.t.rows && d < D ? q[d + j] : (T)0.0f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < R; i++) {
+      if (i / 2 < sg.take) {
+        if (i % 2 == 0) copy_k(i, sg.head, key + i / 2 * GRAN, pages, i / 2 * MT);
+        else copy_v(i, sg.head, key + i / 2 * GRAN, pages, i / 2 * MT);
+      }
+      copy_commit();
+    }
+    uint32_t *const qs = qs0 + buf * S::Q_WORDS;
+#pragma unroll
+    for (int i = 0; i < RW; i++) {
+      const int row = warp + i * kWarps;
+      float f[QV][4], m = 0.0f;
+#pragma unroll
+      for (int k = 0; k < QV; k++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          f[k][j] = (float)raw[i][k][j];
+          m = fmaxf(m, fabsf(f[k][j]));
+        }
+      if constexpr (TERMS == 2) {
+#pragma unroll
+        for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, x));
         // a power of two that brings the row's largest value to [2^13, 2^14)
         int e = 0;
-        if (m > 0.0f && m <= 3.402823466e38f) e = 13 - ilogbf(m);
-        if (lane == 0) rs[row] = (float)max(-126, min(126, e));
-      }
-      __syncthreads();
-    }
-    for (int i = threadIdx.x; i < KS * 32 * NT; i += kThreads) {
-      const int l = i % 32, ks = (i / 32) % KS, nt = i / (32 * KS);
-      const int row = nt * 8 + l / 4, d = 64 * (ks / 4) + 16 * (l % 4) + 4 * (ks % 4);
-      float f[4] = {0.f, 0.f, 0.f, 0.f};
-      if (row < t.rows && d < D) {
-        const int r = t.row0 + row;
-        const T *q = static_cast<const T *>(a.q) + (int64_t)(t.start + r / a.group) * a.q_token +
-                     (int64_t)(head * a.group + r % a.group) * a.q_head + d;
-        float sc = 1.0f;
-        if constexpr (TERMS == 2) sc = exp2f(rs[row]);
+        if (m > 0.0f && m <= 3.402823466e38f) e = max(-126, min(126, 13 - ilogbf(m)));
+        const float up = __int_as_float((127 + e) << 23);
+        if (lane == 0) rs0[buf * ROWS + row] = __int_as_float((127 - e) << 23);
 #pragma unroll
-        for (int j = 0; j < 4; j++) f[j] = (float)q[j] * sc;
-      }
-      uint32_t *dst = qs + (nt * KS + ks) * 64 + l * 2;
-      dst[0] = pack_half(f[0], f[2]);
-      dst[1] = pack_half(f[1], f[3]);
-      if constexpr (TERMS == 2) {
-        float lo[4];
+        for (int k = 0; k < QV; k++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) lo[j] = f[j] - __half2float(__float2half_rn(f[j]));
-        dst[NT * KS * 64] = pack_half(lo[0], lo[2]);
-        dst[NT * KS * 64 + 1] = pack_half(lo[1], lo[3]);
+          for (int j = 0; j < 4; j++) f[k][j] *= up;
+      }
+#pragma unroll
+      for (int k = 0; k < QV; k++) {
+        const int d = 4 * (lane + 32 * k);
+        if (d >= DP) break;
+        const int ks = (d / 64) * 4 + (d % 16) / 4, l = (row % 8) * 4 + (d % 64) / 16;
+        uint32_t *dst = qs + ((row / 8) * KS + ks / 2 * 2) * 64 + l * 4 + ks % 2 * 2;
+        *reinterpret_cast<uint2 *>(dst) = make_uint2(pack_half(f[k][0], f[k][2]), pack_half(f[k][1], f[k][3]));
+        if constexpr (TERMS == 2) {
+          float lo[4];
+#pragma unroll
+          for (int j = 0; j < 4; j++) lo[j] = f[k][j] - __half2float(__float2half_rn(f[k][j]));
+          *reinterpret_cast<uint2 *>(dst + NT * KS * 64) = make_uint2(pack_half(lo[0], lo[2]), pack_half(lo[1], lo[3]));
+        }
       }
     }
+    return pages;
+  };
+
+  seek<ROWS, GRAN, kThreads>(a, ba, line, place);
+  __syncthreads();
+  Place p = *place;
+  Segment sg;
+  if (!next_segment<ROWS, GRAN>(a, ba, p, sg)) return;
+  int buf = 0, pages = begin(sg, 0);
+  for (;;) {
     __syncthreads();
+    const uint32_t *const qs = qs0 + buf * S::Q_WORDS;
 
     // Each lane's two rows (columns 2c, 2c + 1 of the transposed products) of each tile of 8.
     int lo[NT][2], hi[NT][2];
@@ -171,11 +298,11 @@ __global__ void __launch_bounds__(kThreads, PER_SM) k_kv_attend_rows(const Atten
 #pragma unroll
       for (int e = 0; e < 2; e++) {
         const int row = nt * 8 + 2 * c + e;
-        const int pos = t.first + (t.row0 + row) / a.group;
+        const int pos = sg.t.first + (sg.t.row0 + row) / a.group;
         lo[nt][e] = row_lo(a, pos);
-        hi[nt][e] = row < t.rows ? row_hi(a, t.keys, pos) : 0;
+        hi[nt][e] = row < sg.t.rows ? row_hi(a, sg.t.keys, pos) : 0;
         col[nt][e] = a.scale_log2;
-        if constexpr (TERMS == 2) col[nt][e] *= exp2f(-rs[row]);
+        if constexpr (TERMS == 2) col[nt][e] *= rs0[buf * ROWS + row];
       }
 
     float o[NT][VW * 2][4], m[NT][2], l[NT][2], vmax = 0.0f;
@@ -188,77 +315,44 @@ __global__ void __launch_bounds__(kThreads, PER_SM) k_kv_attend_rows(const Atten
       m[nt][0] = m[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.0f;
     }
+    float ksl = 0.0f, ratio_l = 0.0f;  // of the lane's tile: keys' scale, 2^14 values' scale / largest so far
+    uint32_t holes = 0;
+    int pages_next = -1, slot = 0;  // slot: of the piece that comes next
+    const int key0 = first_key(sg);
 
-    const int32_t *table = a.batch.tables + (int64_t)t.seq * a.batch.table_stride;
-    const int8_t *kbase = a.pool.k + (int64_t)head * a.pool.head_stride, *vbase = a.pool.v + (int64_t)head * a.pool.head_stride;
-    const float *ksc = a.pool.k_scale + (int64_t)head * a.pool.scale_head_stride;
-    const float *vsc = a.pool.v_scale + (int64_t)head * a.pool.scale_head_stride;
-    // Keys of step i of this warp: key0 + i * GRAN + [0, 16 MT).
-    const int key0 = (t.lo / GRAN + cur.off) * GRAN + warp * (MT * 16);
-    auto page_of = [&](int key) -> int {  // -1: no such key
-      if (key >= t.keys) return -1;
-      const int p = __ldg(table + (key >> a.page_shift));
-      return p >= 0 && p < a.pool.pages ? p : -1;
-    };
-    uint4 kr[MT][2][KC];
-    uint32_t vr[MT][4][VW];
-    float ks_[MT], vs_[MT];
-    int page[MT], page_next[MT];
-    auto load_k = [&](int key, const int (&pg)[MT]) {
-#pragma unroll
-      for (int mt = 0; mt < MT; mt++) {
-        const int8_t *row = kbase + (int64_t)pg[mt] * a.pool.page_stride +
-                            (int64_t)((key + mt * 16 + g) & (PT - 1)) * a.pool.token_stride + 16 * c;
-        ks_[mt] = pg[mt] >= 0 ? __ldg(ksc + (int64_t)pg[mt] * a.pool.scale_page_stride) : 0.0f;
-#pragma unroll
-        for (int h2 = 0; h2 < 2; h2++)
-#pragma unroll
-          for (int j = 0; j < KC; j++) {
-            kr[mt][h2][j] = make_uint4(0x0u, 0x0u, 0x0u, 0x0u);
-            if (pg[mt] >= 0 && 64 * j + 16 * c < D) kr[mt][h2][j] = ld_stream16(row + h2 * 8 * a.pool.token_stride + 64 * j);
-          }
-      }
-    };
-    auto load_v = [&](int key, const int (&pg)[MT]) {
-#pragma unroll
-      for (int mt = 0; mt < MT; mt++) {
-        const int8_t *row = vbase + (int64_t)pg[mt] * a.pool.page_stride +
-                            (int64_t)((key + mt * 16 + 2 * c) & (PT - 1)) * a.pool.token_stride;
-        const float sv = pg[mt] >= 0 ? __ldg(vsc + (int64_t)pg[mt] * a.pool.scale_page_stride) : 0.0f;
-        vs_[mt] = fabsf(sv) <= 3.402823466e38f ? sv : __int_as_float(0x7fc00000);
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const int8_t *p = row + (int64_t)((k & 1) + (k >> 1) * 8) * a.pool.token_stride;
-          if constexpr (VW == 2) {
-            uint2 r = make_uint2(0u, 0u);
-            if (pg[mt] >= 0 && 8 * g < D) r = ld_stream8(p + 8 * g);
-            vr[mt][k][0] = r.x;
-            vr[mt][k][1] = r.y;
-          } else {
-#pragma unroll
-            for (int j = 0; j < VW / 4; j++) {
-              uint4 r = make_uint4(0u, 0u, 0u, 0u);
-              if (pg[mt] >= 0 && 128 * j + 16 * g < D) r = ld_stream16(p + 128 * j + 16 * g);
-              vr[mt][k][4 * j] = r.x;
-              vr[mt][k][4 * j + 1] = r.y;
-              vr[mt][k][4 * j + 2] = r.z;
-              vr[mt][k][4 * j + 3] = r.w;
-            }
-          }
-        }
-      }
-    };
-#pragma unroll
-    for (int mt = 0; mt < MT; mt++) {
-      page[mt] = page_of(key0 + mt * 16);
-      page_next[mt] = take > 1 ? page_of(key0 + GRAN + mt * 16) : -1;
-    }
-    load_k(key0, page);
-    load_v(key0, page);
-
-    for (int i = 0; i < take; i++) {
+    for (int i = 0; i < sg.take; i++) {
       const int key = key0 + i * GRAN;
-      // S^T: [16 keys][8 rows] a tile
+      const int at = (i % TL) * MT;
+      if (at == 0) {
+        if (i) pages = pages_next;
+        pages_next = i + TL < sg.take ? step_pages(sg, i + TL) : -1;
+        holes = __ballot_sync(~0u, pages < 0);
+        float vs = 0.0f;
+        ksl = 0.0f;
+        if (pages >= 0) {
+          ksl = __ldg(a.pool.k_scale + ((int64_t)sg.head * a.pool.scale_head_stride + (int64_t)pages * a.pool.scale_page_stride));
+          vs = __ldg(a.pool.v_scale + ((int64_t)sg.head * a.pool.scale_head_stride + (int64_t)pages * a.pool.scale_page_stride));
+        }
+        const bool finite = fabsf(vs) <= 3.402823466e38f;
+        float top = finite ? fmaxf(vmax, fabsf(vs)) : vmax;
+#pragma unroll
+        for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+        if (top != vmax) {
+          const float f = __fdiv_rn(vmax, top);
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int w = 0; w < VW * 2; w++)
+#pragma unroll
+              for (int j = 0; j < 4; j++) o[nt][w][j] *= f;
+          vmax = top;
+        }
+        // a scale that is not finite makes the weights of the keys that are seen NaN
+        ratio_l = !finite ? __int_as_float(0x7fc00000) : vmax > 0.0f ? __fdiv_rn(vs, vmax) * 16384.0f : 0.0f;
+      }
+      const bool hole = (holes >> at & ((1u << MT) - 1)) != 0;
+      // S^T: [16 keys][8 rows] a tile. R - 1 pieces were committed after these keys.
+      copy_wait<R - 1>();
       float s[MT][NT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; mt++)
@@ -266,35 +360,57 @@ __global__ void __launch_bounds__(kThreads, PER_SM) k_kv_attend_rows(const Atten
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
           for (int j = 0; j < 4; j++) s[mt][nt][j] = 0.0f;
+      uint4 kr[MT][2], b[TERMS][NT];
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) {
-        uint2 b[TERMS][NT];
+        if (ks % 4 == 0) {
 #pragma unroll
-        for (int tm = 0; tm < TERMS; tm++)
+          for (int mt = 0; mt < MT; mt++)
 #pragma unroll
-          for (int nt = 0; nt < NT; nt++)
-            b[tm][nt] = *reinterpret_cast<const uint2 *>(qs + ((tm * NT + nt) * KS + ks) * 64 + lane * 2);
+            for (int h2 = 0; h2 < 2; h2++) kr[mt][h2] = lds16(ring + slot * S::PIECE + ((mt * 2 + h2) * KC + ks / 4) * 512);
+        }
+        if (ks % 2 == 0) {
+#pragma unroll
+          for (int tm = 0; tm < TERMS; tm++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+              b[tm][nt] = *reinterpret_cast<const uint4 *>(qs + ((tm * NT + nt) * KS + ks) * 64 + lane * 4);
+        }
 #pragma unroll
         for (int mt = 0; mt < MT; mt++) {
-          const uint32_t w0 = (&kr[mt][0][ks / 4].x)[ks % 4] ^ 0x80808080u, w1 = (&kr[mt][1][ks / 4].x)[ks % 4] ^ 0x80808080u;
+          const uint32_t w0 = (&kr[mt][0].x)[ks % 4] ^ 0x80808080u, w1 = (&kr[mt][1].x)[ks % 4] ^ 0x80808080u;
           const uint32_t af[4] = {half_pair<0x4240>(w0), half_pair<0x4240>(w1), half_pair<0x4341>(w0), half_pair<0x4341>(w1)};
 #pragma unroll
           for (int tm = 0; tm < TERMS; tm++)
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) mma16816(s[mt][nt], af, b[tm][nt].x, b[tm][nt].y);
+            for (int nt = 0; nt < NT; nt++)
+              mma16816(s[mt][nt], af, ks % 2 ? b[tm][nt].z : b[tm][nt].x, ks % 2 ? b[tm][nt].w : b[tm][nt].y);
         }
       }
+      // The piece R on takes the place of these (none past the segment: its end
+      // leaves nothing on the way that could land on the next one's pieces).
+      auto refill = [&](int steps, bool keys) {
+        if (i + steps < sg.take) {
+          const int from = at + steps * MT < 32 ? pages : pages_next, tile = (at + steps * MT) & 31;
+          if (keys) copy_k(slot, sg.head, key + steps * GRAN, from, tile);
+          else copy_v(slot, sg.head, key + steps * GRAN, from, tile);
+        }
+        copy_commit();
+        slot = slot + 1 == R ? 0 : slot + 1;
+      };
+      refill(R / 2, R % 2 == 0);
+
       // scores in units of log2, the unseen at -inf
-      const bool edge = key < t.lo_all || key + MT * 16 > t.hi_all;
+      float ks_[MT];
+#pragma unroll
+      for (int mt = 0; mt < MT; mt++) ks_[mt] = __shfl_sync(~0u, ksl, at + mt);
+      const bool edge = key < sg.t.lo_all || key + MT * 16 > sg.t.hi_all;
 #pragma unroll
       for (int mt = 0; mt < MT; mt++)
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
           for (int j = 0; j < 4; j++) s[mt][nt][j] *= ks_[mt] * col[nt][j & 1];
-      bool hole = false;
-#pragma unroll
-      for (int mt = 0; mt < MT; mt++) hole |= page[mt] < 0;
       uint32_t seen = ~0u;  // bit (mt * NT + nt) * 4 + j
       if (edge || hole) {
         seen = 0;
@@ -305,19 +421,11 @@ __global__ void __launch_bounds__(kThreads, PER_SM) k_kv_attend_rows(const Atten
 #pragma unroll
             for (int j = 0; j < 4; j++) {
               const int kk = key + mt * 16 + g + (j >> 1) * 8;
-              const bool y = page[mt] >= 0 && kk >= lo[nt][j & 1] && kk < hi[nt][j & 1];
+              const bool y = !(holes >> (at + mt) & 1) && kk >= lo[nt][j & 1] && kk < hi[nt][j & 1];
               if (!y) s[mt][nt][j] = -INFINITY;
               seen |= (y ? 1u : 0u) << ((mt * NT + nt) * 4 + j);
             }
       }
-      // the next step's keys, now that these are used up
-#pragma unroll
-      for (int mt = 0; mt < MT; mt++) {
-        page[mt] = page_next[mt];
-        page_next[mt] = i + 2 < take ? page_of(key + 2 * GRAN + mt * 16) : -1;
-      }
-      if (i + 1 < take) load_k(key + GRAN, page);
-
       bool moved = false;
       float mn[NT][2];
 #pragma unroll
@@ -333,11 +441,7 @@ __global__ void __launch_bounds__(kThreads, PER_SM) k_kv_attend_rows(const Atten
           mn[nt][e] = x;
           moved |= x != m[nt][e];
         }
-      float vtop = vmax;
-#pragma unroll
-      for (int mt = 0; mt < MT; mt++) vtop = fmaxf(vtop, fabsf(vs_[mt]));
-      if (__any_sync(~0u, moved) || vtop != vmax) {
-        const float vr_ = vtop != vmax ? __fdiv_rn(vmax, vtop) : 1.0f;
+      if (__any_sync(~0u, moved)) {
 #pragma unroll
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -345,50 +449,69 @@ __global__ void __launch_bounds__(kThreads, PER_SM) k_kv_attend_rows(const Atten
             const float f = m[nt][e] == -INFINITY ? 0.0f : ex2(m[nt][e] - mn[nt][e]);
             l[nt][e] *= f;
             m[nt][e] = mn[nt][e];
-            const float fo = f * vr_;
 #pragma unroll
             for (int w = 0; w < VW * 2; w++) {
-              o[nt][w][e] *= fo;
-              o[nt][w][2 + e] *= fo;
+              o[nt][w][e] *= f;
+              o[nt][w][2 + e] *= f;
             }
           }
-        vmax = vtop;
       }
+      float top[NT][2];  // (a row that has seen nothing yet subtracts 0)
+#pragma unroll
+      for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) top[nt][e] = m[nt][e] == -INFINITY ? 0.0f : m[nt][e];
+      copy_wait<R - 1>();
 #pragma unroll
       for (int mt = 0; mt < MT; mt++) {
-        // 2^14 sv / largest sv; a scale that is not finite makes the weights of the keys that are seen NaN
-        const float ratio = vmax > 0.0f ? __fdiv_rn(vs_[mt], vmax) * 16384.0f : vs_[mt];
+        const float ratio = __shfl_sync(~0u, ratio_l, at + mt);
         uint32_t pb[TERMS][NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-          float p[4];
+          float w[4];
 #pragma unroll
           for (int j = 0; j < 4; j++) {
-            const float top = m[nt][j & 1] == -INFINITY ? 0.0f : m[nt][j & 1];
-            const float e = ex2(s[mt][nt][j] - top);
+            const float e = ex2(s[mt][nt][j] - top[nt][j & 1]);
             l[nt][j & 1] += e;
-            p[j] = e * ratio;
+            w[j] = e * ratio;
           }
           if (edge || hole) {
 #pragma unroll
             for (int j = 0; j < 4; j++)
-              if (!(seen >> ((mt * NT + nt) * 4 + j) & 1)) p[j] = 0.0f;
+              if (!(seen >> ((mt * NT + nt) * 4 + j) & 1)) w[j] = 0.0f;
           }
-          const uint32_t p01 = pack_half(p[0], p[1]), p23 = pack_half(p[2], p[3]);
+          const uint32_t p01 = pack_half(w[0], w[1]), p23 = pack_half(w[2], w[3]);
           pb[0][nt][0] = transpose8x8(p01);
           pb[0][nt][1] = transpose8x8(p23);
           if constexpr (TERMS == 2) {
             const float2 h01 = __half22float2(*reinterpret_cast<const __half2 *>(&p01));
             const float2 h23 = __half22float2(*reinterpret_cast<const __half2 *>(&p23));
-            pb[1][nt][0] = transpose8x8(pack_half(p[0] - h01.x, p[1] - h01.y));
-            pb[1][nt][1] = transpose8x8(pack_half(p[2] - h23.x, p[3] - h23.y));
+            pb[1][nt][0] = transpose8x8(pack_half(w[0] - h01.x, w[1] - h01.y));
+            pb[1][nt][1] = transpose8x8(pack_half(w[2] - h23.x, w[3] - h23.y));
           }
         }
         // O^T += V^T P^T: word w of a lane holds dimensions 4w .. 4w + 3 of four keys
+        uint32_t vr[4][4];
 #pragma unroll
         for (int w = 0; w < VW; w++) {
-          const uint32_t x0 = vr[mt][0][w] ^ 0x80808080u, x1 = vr[mt][1][w] ^ 0x80808080u;
-          const uint32_t x2 = vr[mt][2][w] ^ 0x80808080u, x3 = vr[mt][3][w] ^ 0x80808080u;
+          if (w % 4 == 0) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              if constexpr (VW == 2) {
+                const uint2 r = lds8(vring + slot * S::PIECE + (mt * 4 + k) * 256);
+                vr[k][0] = r.x;
+                vr[k][1] = r.y;
+              } else {
+                const uint4 r = lds16(vring + slot * S::PIECE + ((mt * 4 + k) * (VW / 4) + w / 4) * 512);
+                vr[k][0] = r.x;
+                vr[k][1] = r.y;
+                vr[k][2] = r.z;
+                vr[k][3] = r.w;
+              }
+            }
+          }
+          const uint32_t x0 = vr[0][w % 4] ^ 0x80808080u, x1 = vr[1][w % 4] ^ 0x80808080u;
+          const uint32_t x2 = vr[2][w % 4] ^ 0x80808080u, x3 = vr[3][w % 4] ^ 0x80808080u;
           const uint32_t a01 = __byte_perm(x0, x1, 0x5140), b01 = __byte_perm(x0, x1, 0x7362);
           const uint32_t a23 = __byte_perm(x2, x3, 0x5140), b23 = __byte_perm(x2, x3, 0x7362);
           const uint32_t f0[4] = {half_pair<0x4140>(a01), half_pair<0x4342>(a01), half_pair<0x4140>(a23), half_pair<0x4342>(a23)};
@@ -402,10 +525,14 @@ __global__ void __launch_bounds__(kThreads, PER_SM) k_kv_attend_rows(const Atten
             }
         }
       }
-      if (i + 1 < take) load_v(key + GRAN, page);
+      refill((R + 1) / 2, R % 2 == 1);
     }
 
-    // The warps' results meet in shared memory.
+    // The next segment is on its way before this one's results meet in shared memory.
+    Segment ns;
+    const bool more = next_segment<ROWS, GRAN>(a, ba, p, ns);
+    if (more) pages = begin(ns, buf ^ 1);
+
     const float unscale = vmax * 0x1p-14f;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
@@ -430,11 +557,11 @@ __global__ void __launch_bounds__(kThreads, PER_SM) k_kv_attend_rows(const Atten
         }
       }
     __syncthreads();
-    const bool whole = take == units;
-    float *part = whole ? nullptr : partial_at<ROWS, DP>(a, blockIdx.x, cur.off == 0);
+    const bool whole = sg.take == sg.units;
+    float *part = whole ? nullptr : partial_at<ROWS, DP>(a, blockIdx.x, sg.off == 0);
     for (int i = threadIdx.x; i < ROWS * DP / 4; i += kThreads) {
       const int row = i / (DP / 4), d = (i % (DP / 4)) * 4;
-      if (row >= t.rows) break;
+      if (row >= sg.t.rows) break;
       float top = -INFINITY, sum = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps; w++) top = fmaxf(top, wm[w * ROWS + row]);
@@ -450,14 +577,8 @@ __global__ void __launch_bounds__(kThreads, PER_SM) k_kv_attend_rows(const Atten
         r.w = __fmaf_rn(f, v.w, r.w);
       }
       if (whole) {
-        if (d < D) {
-          const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-          write_out<T>(a, t, head, row, d, sum == 0.0f ? 0.0f : r.x * inv);
-          write_out<T>(a, t, head, row, d + 1, sum == 0.0f ? 0.0f : r.y * inv);
-          write_out<T>(a, t, head, row, d + 2, sum == 0.0f ? 0.0f : r.z * inv);
-          write_out<T>(a, t, head, row, d + 3, sum == 0.0f ? 0.0f : r.w * inv);
-        }
-        if (d == 0) write_lse(a, t, head, row, top, sum);
+        if (d < D) write_out<T>(a, sg.t, sg.head, row, d, r, sum);
+        if (d == 0) write_lse(a, sg.t, sg.head, row, top, sum);
       } else {
         *reinterpret_cast<float4 *>(part + row * DP + d) = r;
         if (d == 0) {
@@ -466,30 +587,26 @@ __global__ void __launch_bounds__(kThreads, PER_SM) k_kv_attend_rows(const Atten
         }
       }
     }
-    if (!whole) arrive<T, ROWS, DP, kThreads>(a, t, cur, u0, u1, body, flag);
-    __syncthreads();
-    cur.at += take;
-    cur.off = 0;
-    cur.slot++;
-    if (cur.slot == a.slots) {
-      cur.slot = 0;
-      cur.head++;
-    }
+    if (!whole) arrive<T, ROWS, DP, kThreads>(a, sg, line, body, flag);
+    if (!more) break;
+    sg = ns;
+    buf ^= 1;
   }
 }
 
-template <typename T, int DP, int NT, int PER_SM>
+template <typename T, int DP, int NT>
 int launch_rows(AttendArgs a, int sms, cudaStream_t st) {
   using S = Shape<T, DP, NT>;
   constexpr size_t smem = S::WORDS * 4;
-  auto *kern = k_kv_attend_rows<T, DP, NT, PER_SM>;
+  static_assert((smem + 1024) * S::PER_SM <= 228 * 1024, "blocks of an SM");
+  auto *kern = k_kv_attend_rows<T, DP, NT>;
   if (smem > 48 * 1024) SHLO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   a.slots = (int)(((int64_t)a.batch.tokens * a.group) / S::ROWS + a.batch.seqs);
   // No more blocks than granules there can be.
   const int64_t room = ((int64_t)a.batch.table_pages << a.page_shift) / S::GRAN + 1;
   int64_t most = (int64_t)a.slots * a.pool.heads;
   most = most > (1 << 20) ? most : most * room;
-  const int64_t full = (int64_t)sms * PER_SM;
+  const int64_t full = (int64_t)sms * S::PER_SM;
   int64_t grid = most < full ? most : full;
   if (grid > kAttendMaxBlocks) grid = kAttendMaxBlocks;
   if (grid < 1) grid = 1;
@@ -500,14 +617,13 @@ int launch_rows(AttendArgs a, int sms, cudaStream_t st) {
 template <typename T>
 int dispatch_rows(const AttendArgs &a, int nt, int sms, cudaStream_t st) {
   const int D = a.pool.head_dim;
-  if (nt == 1) {
-    if (D <= 64) return launch_rows<T, 64, 1, 4>(a, sms, st);
-    if (D <= 128) return launch_rows<T, 128, 1, 3>(a, sms, st);
-    return launch_rows<T, 256, 1, 2>(a, sms, st);
+  if (nt == 1 || D > 128) {
+    if (D <= 64) return launch_rows<T, 64, 1>(a, sms, st);
+    if (D <= 128) return launch_rows<T, 128, 1>(a, sms, st);
+    return launch_rows<T, 256, 1>(a, sms, st);
   }
-  if (D <= 64) return launch_rows<T, 64, 2, 3>(a, sms, st);
-  if (D <= 128) return launch_rows<T, 128, 2, 2>(a, sms, st);
-  return launch_rows<T, 256, 2, 2>(a, sms, st);
+  if (D <= 64) return launch_rows<T, 64, 2>(a, sms, st);
+  return launch_rows<T, 128, 2>(a, sms, st);
 }
 
 constexpr size_t kCounterBytes = 2 * kAttendMaxBlocks * sizeof(unsigned);
@@ -523,7 +639,11 @@ size_t attend_work_bytes(int sms) {
     const size_t b = (size_t)blocks * 2 * rows * (dp + 2) * 4;
     if (b > most) most = b;
   };
-  of(8, 64, 4); of(8, 128, 3); of(8, 256, 2); of(16, 64, 3); of(16, 128, 2); of(16, 256, 2);
+  of(8, 64, Shape<__half, 64, 1>::PER_SM);
+  of(8, 128, Shape<__half, 128, 1>::PER_SM);
+  of(8, 256, Shape<__half, 256, 1>::PER_SM);
+  of(16, 64, Shape<__half, 64, 2>::PER_SM);
+  of(16, 128, Shape<__half, 128, 2>::PER_SM);
   return kCounterBytes + most;
 }
 
@@ -552,6 +672,8 @@ int launch_kv_attend(const AttendCall &c, int sms, cudaStream_t st) {
   a.group = group;
   a.slots = 0;
   a.causal = c.causal; a.window = c.window;
+  const int64_t per = 4;
+  a.out_wide = (uintptr_t)c.out % (4 * size) == 0 && c.out_token % per == 0 && c.out_head % per == 0;
   a.scale_log2 = c.scale * 1.44269504088896341f;
   a.page_shift = 31 - __builtin_clz((unsigned)c.pool.page_tokens);
   a.above = 0;

@@ -7,17 +7,19 @@
 // kRows. A tile sees the keys [lo, hi) of its rows; a granule is kGran keys from
 // a multiple of kGran. A unit is one tile of one key/value head: all its
 // granules. The units of all heads lie on one line of W granules, which the N
-// blocks cut into equal parts, so ragged lengths and few long sequences load
-// every block alike. A block computes the line itself from `starts` and `lens`
-// (the host knows neither), by a scan over slots: sequence s has the slots from
-// floor(starts[s] * group / kRows) + s on, always enough for its tiles.
+// blocks cut into equal chunks, whatever units they fall in, so ragged lengths
+// and few long sequences load every block alike. A block computes the line
+// itself from `starts` and `lens` (the host knows neither), by a scan over slots:
+// sequence s has the slots from floor(starts[s] * group / kRows) + s on, always
+// enough for its tiles. (Measured and left: four chunks a block of falling size,
+// taken from a counter. 64 x 8192 keys took 246 us instead of 230: every cut
+// costs a block about 8 us, more than the unevenness it evens out.)
 //
-// Joining. A unit cut between blocks leaves one partial result a block: the sum
+// Joining. A unit cut between chunks leaves one partial result a chunk: the sum
 // of exp2(score - m) v without the division, m and the sum l, in 32 bits. At
-// most two a block: of the unit it starts in the middle of, and of the one it
+// most two a chunk: of the unit it starts in the middle of, and of the one it
 // leaves unfinished. The block that arrives last joins them, always in the
-// order of the keys, so the result does not depend on who is last; more than
-// kJoin partials are joined in groups of kJoin first.
+// order of the keys; more than kJoin partials are joined in groups of kJoin first.
 #pragma once
 
 #include "decode.cuh"
@@ -34,17 +36,18 @@ struct AttendArgs {
   int group;         // query heads a key/value head
   int slots;         // slots of the work list
   int causal, window;
+  int out_wide;      // out allows stores of four values
   float scale_log2;  // scale * log2(e)
   int page_shift;
   // Which sequences this launch takes: those with rows (new tokens * group) in
   // (above, upto].
   int64_t above, upto;
   unsigned *counters;  // [2][kAttendMaxBlocks], zero between calls
-  float *partials;     // [blocks][2][rows * (dim + 2)]
+  float *partials;     // [chunks][2][rows * (dim + 2)]
 };
 
 constexpr int kAttendMaxBlocks = 1024;
-constexpr int kJoin = 16;
+constexpr int kJoin = 64;
 
 // A tile of rows and what it sees.
 struct RowTile {
@@ -63,16 +66,26 @@ __device__ __forceinline__ int row_lo(const AttendArgs &a, int pos) {
 }
 
 // The tile of a slot; returns its granules (0: the slot has no tile here).
+// t.seq, when `after` is set, is the owner of an earlier slot: the search goes
+// on from it, one sequence at a time.
 template <int ROWS, int GRAN>
-__device__ __forceinline__ int tile_of_slot(const AttendArgs &a, int slot, RowTile &t) {
+__device__ __forceinline__ int tile_of_slot(const AttendArgs &a, const int32_t *starts, const int32_t *lens, int slot,
+                                            RowTile &t, bool after) {
   constexpr int SH = ROWS == 8 ? 3 : ROWS == 16 ? 4 : ROWS == 64 ? 6 : 7;
   static_assert(1 << SH == ROWS, "rows of a tile");
-  const int s = slot_owner(a.batch, slot, a.group, SH, 1);
-  const SeqSpan sp = seq_span(a.batch, s);
-  const int64_t rows = (int64_t)sp.n * a.group;
-  const int64_t row0 = (int64_t)(slot - slot_base(a.batch, s, a.group, SH, 1)) * ROWS;
-  if (row0 < 0 || row0 >= rows || rows <= a.above || rows > a.upto) return 0;
+  const int tokens = a.batch.tokens, seqs = a.batch.seqs;
+  int s;
+  if (after) {
+    s = t.seq;
+    while (s + 1 < seqs && slot_base(starts, tokens, s + 1, a.group, SH, 1) <= slot) s++;
+  } else {
+    s = slot_owner(starts, tokens, seqs, 0, slot, a.group, SH, 1);
+  }
   t.seq = s;
+  const SeqSpan sp = seq_span(starts, lens, tokens, s);
+  const int64_t rows = (int64_t)sp.n * a.group;
+  const int64_t row0 = (int64_t)(slot - slot_base(starts, tokens, s, a.group, SH, 1)) * ROWS;
+  if (row0 < 0 || row0 >= rows || rows <= a.above || rows > a.upto) return 0;
   t.row0 = (int)row0;
   t.rows = (int)min((int64_t)ROWS, rows - row0);
   t.start = sp.start;
@@ -91,24 +104,106 @@ __device__ __forceinline__ int tile_of_slot(const AttendArgs &a, int slot, RowTi
   return (t.hi + GRAN - 1) / GRAN - t.lo / GRAN;
 }
 
-// A block's part of the line, and where it stands on it.
-struct Cursor {
-  long long per_head;    // granules a head
-  long long total;       // W
-  int blocks;            // blocks with work
-  long long at, end;     // this block's part
-  int head, slot, off;   // the unit `at` is in, and the granule in it
+// The line.
+struct Line {
+  long long per_head;      // granules a head
+  long long total;         // W
+  int blocks;              // blocks with work
+  long long before, mine;  // this thread's slots' granules on a head's line
+};
+// A place on it: what is left of a chunk, and the unit and granule that begins at.
+struct Place {
+  long long at, end;
+  int head, slot, off, seq;
 };
 
-// All threads call it; NT threads, `sh` shared memory of NT + 4 long longs. A
-// block without work returns false.
+// The chunk that a granule of the line belongs to.
+__device__ __forceinline__ int chunk_of(const Line &c, long long x) {
+  return (int)(((x + 1) * c.blocks - 1) / c.total);
+}
+
+// The batch's arrays as the block reads them: its own copies where they fit.
+struct BatchArrays {
+  const int32_t *starts, *lens;
+};
+
+// Find the beginning of the block's chunk: the thread that holds its slot writes
+// it to `to` (shared memory), which all may read after a barrier.
 template <int ROWS, int GRAN, int NT>
-__device__ bool schedule(const AttendArgs &a, int min_gran, long long *sh, Cursor &c) {
+__device__ void seek(const AttendArgs &a, const BatchArrays &ba, const Line &c, Place *to) {
+  const long long at = c.total * blockIdx.x / c.blocks;
+  const int head = (int)(at / c.per_head);
+  long long r = at - head * c.per_head - c.before;
+  if (r < 0 || r >= c.mine) return;
+  const int per = (a.slots + NT - 1) / NT, s0 = min((int)threadIdx.x * per, a.slots);
+  RowTile u;
+  int s = s0;
+  for (; s < a.slots; s++) {
+    const int g = tile_of_slot<ROWS, GRAN>(a, ba.starts, ba.lens, s, u, s > s0);
+    if (r < g) break;
+    r -= g;
+  }
+  to->at = at;
+  to->end = c.total * (blockIdx.x + 1) / c.blocks;
+  to->head = head;
+  to->slot = s;
+  to->off = (int)r;
+  to->seq = u.seq;
+}
+
+// One unit's part of a chunk: granules off .. off + take of `units`; the unit
+// begins at u0 on the line.
+struct Segment {
+  RowTile t;
+  int head, off, take, units;
+  long long u0;
+};
+// The next one from `p` on (false: the chunk is at its end).
+template <int ROWS, int GRAN>
+__device__ __forceinline__ bool next_segment(const AttendArgs &a, const BatchArrays &ba, Place &p, Segment &g) {
+  while (p.at < p.end && p.head < a.pool.heads) {
+    g.t.seq = p.seq;
+    const int units = tile_of_slot<ROWS, GRAN>(a, ba.starts, ba.lens, p.slot, g.t, true);
+    const int off = p.off;
+    p.seq = g.t.seq;
+    g.head = p.head;
+    p.off = 0;
+    p.slot++;
+    if (p.slot == a.slots) {
+      p.slot = p.seq = 0;
+      p.head++;
+    }
+    if (units == 0) continue;  // a slot without a tile
+    g.off = off;
+    g.units = units;
+    g.take = (int)min((long long)(units - off), p.end - p.at);
+    g.u0 = p.at - off;
+    p.at += g.take;
+    return true;
+  }
+  return false;
+}
+
+// Lay out the line. All threads call it; NT threads, `sh` shared memory of NT +
+// 4 long longs, `copy` of `room` ints for the batch's arrays (each thread
+// searches them: from global memory every step of a search would wait for L2).
+// False: the block has no work.
+template <int ROWS, int GRAN, int NT>
+__device__ bool schedule(const AttendArgs &a, int min_gran, long long *sh, int *copy, int room, BatchArrays &ba, Line &c) {
+  ba.starts = a.batch.starts;
+  ba.lens = a.batch.lens;
+  const int seqs = a.batch.seqs;
+  if (2 * seqs + 1 <= room) {
+    for (int i = threadIdx.x; i < 2 * seqs + 1; i += NT) copy[i] = i <= seqs ? __ldg(ba.starts + i) : __ldg(ba.lens + i - seqs - 1);
+    __syncthreads();
+    ba.starts = copy;
+    ba.lens = copy + seqs + 1;
+  }
   const int chunk = (a.slots + NT - 1) / NT;
   const int s0 = min((int)threadIdx.x * chunk, a.slots), s1 = min(s0 + chunk, a.slots);
   long long mine = 0;
   RowTile t;
-  for (int s = s0; s < s1; s++) mine += tile_of_slot<ROWS, GRAN>(a, s, t);
+  for (int s = s0; s < s1; s++) mine += tile_of_slot<ROWS, GRAN>(a, ba.starts, ba.lens, s, t, s > s0);
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   long long sum = mine;
 #pragma unroll
@@ -125,54 +220,45 @@ __device__ bool schedule(const AttendArgs &a, int min_gran, long long *sh, Curso
     if (w < warp) before += v;
     all += v;
   }
-  before += sum - mine;
+  c.before = before + sum - mine;
+  c.mine = mine;
   c.per_head = all;
   c.total = all * a.pool.heads;
   if (c.total == 0) return false;
   const long long fit = c.total / min_gran;
   c.blocks = (int)(fit < 1 ? 1 : fit < (long long)gridDim.x ? fit : (long long)gridDim.x);
-  if ((int)blockIdx.x >= c.blocks) return false;
-  c.at = c.total * blockIdx.x / c.blocks;
-  c.end = c.total * (blockIdx.x + 1) / c.blocks;
-  c.head = (int)(c.at / all);
-  const long long rem = c.at - c.head * all;
   __syncthreads();
-  if (rem >= before && rem < before + mine) {
-    long long r = rem - before;
-    int s = s0;
-    for (; s < s1; s++) {
-      const int g = tile_of_slot<ROWS, GRAN>(a, s, t);
-      if (r < g) break;
-      r -= g;
-    }
-    sh[0] = s;
-    sh[1] = r;
-  }
-  __syncthreads();
-  c.slot = (int)sh[0];
-  c.off = (int)sh[1];
-  __syncthreads();
-  return true;
+  return (int)blockIdx.x < c.blocks;
 }
 
-// The block that a granule of the line belongs to.
-__device__ __forceinline__ int block_of(const Cursor &c, long long x) {
-  return (int)(((x + 1) * c.blocks - 1) / c.total);
-}
-
-// Where block `i` keeps its partial: 0 of a unit begun by an earlier block, 1
-// of one that it begins.
+// Where chunk `i` keeps its partial: 0 of a unit begun in an earlier chunk, 1 of
+// one that begins in it.
 template <int ROWS, int DP>
 __device__ __forceinline__ float *partial_at(const AttendArgs &a, int i, int which) {
   return a.partials + ((int64_t)i * 2 + which) * (ROWS * (DP + 2));
 }
 
+// Four values of a row, divided by the sum l (a row that saw nothing: 0). The
+// caller's strides may be odd: one 2- or 4-byte store each where they are.
 template <typename T>
-__device__ __forceinline__ void write_out(const AttendArgs &a, const RowTile &t, int head, int row, int d, float v) {
+__device__ __forceinline__ void write_out(const AttendArgs &a, const RowTile &t, int head, int row, int d, float4 v, float l) {
   const int r = t.row0 + row, tok = t.start + r / a.group, h = head * a.group + r % a.group;
   T *o = static_cast<T *>(a.out) + (int64_t)tok * a.out_token + (int64_t)h * a.out_head + d;
-  if constexpr (sizeof(T) == 2) *o = __float2half_rn(v);
-  else *o = v;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  if (l == 0.0f) v = make_float4(0.f, 0.f, 0.f, 0.f);
+  v.x *= inv; v.y *= inv; v.z *= inv; v.w *= inv;
+  if constexpr (sizeof(T) == 2) {
+    const __half2 p = __floats2half2_rn(v.x, v.y), q = __floats2half2_rn(v.z, v.w);
+    if (a.out_wide) {
+      *reinterpret_cast<uint2 *>(o) = make_uint2(*reinterpret_cast<const uint32_t *>(&p), *reinterpret_cast<const uint32_t *>(&q));
+    } else {
+      o[0] = p.x; o[1] = p.y; o[2] = q.x; o[3] = q.y;
+    }
+  } else if (a.out_wide) {
+    *reinterpret_cast<float4 *>(o) = v;
+  } else {
+    o[0] = v.x; o[1] = v.y; o[2] = v.z; o[3] = v.w;
+  }
 }
 __device__ __forceinline__ void write_lse(const AttendArgs &a, const RowTile &t, int head, int row, float m, float l) {
   if (!a.lse) return;
@@ -186,94 +272,111 @@ __device__ __forceinline__ float join_factor(float m, float top) {
   return m == -INFINITY ? 0.0f : exp2f(m - top);
 }
 
-// Join the partials of blocks i0 .. i0 + n - 1 (the first one's slot is
-// `which0`, the others' 0; `step` blocks apart) into `dst` (a partial), or into
-// the output when dst is null. NT threads; fac: shared memory of (n + 2) * ROWS floats.
+// Join the partials of chunks i0 .. i0 + n - 1 (the first one's slot is
+// `which0`, the others' 0; `step` chunks apart) into `dst` (a partial), or into
+// the output when dst is null. NT threads; fac: shared memory of 2 (n + 1) ROWS
+// floats. Everything is read with all threads' loads in flight at once: one
+// after another, each would wait for L2.
 template <typename T, int ROWS, int DP, int NT>
 __device__ void join(const AttendArgs &a, const RowTile &t, int head, int i0, int n, int step, int which0, float *dst,
                      float *fac) {
   auto src = [&](int k) -> const float * { return partial_at<ROWS, DP>(a, i0 + k * step, k == 0 ? which0 : 0); };
-  for (int i = threadIdx.x; i < n * ROWS; i += NT) {
-    const int k = i / ROWS, row = i % ROWS;
-    fac[i] = __ldcg(src(k) + ROWS * DP + row);
+  float *const ms = fac, *const ls = fac + n * ROWS, *const top = ls + n * ROWS, *const sum = top + ROWS;
+  for (int i = threadIdx.x; i < 2 * n * ROWS; i += NT) {
+    const int k = (i / ROWS) % n;
+    fac[i] = __ldcg(src(k) + ROWS * DP + (i >= n * ROWS ? ROWS : 0) + i % ROWS);
   }
   __syncthreads();
-  float *const top = fac + n * ROWS, *const sum = top + ROWS;
   for (int row = threadIdx.x; row < ROWS; row += NT) {
     float m = -INFINITY;
-    for (int k = 0; k < n; k++) m = fmaxf(m, fac[k * ROWS + row]);
-    float l = 0.0f;
-    for (int k = 0; k < n; k++) {
-      const float f = join_factor(fac[k * ROWS + row], m);
-      fac[k * ROWS + row] = f;
-      l = __fmaf_rn(f, __ldcg(src(k) + ROWS * DP + ROWS + row), l);
-    }
+    for (int k = 0; k < n; k++) m = fmaxf(m, ms[k * ROWS + row]);
     top[row] = m;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n * ROWS; i += NT) ms[i] = join_factor(ms[i], top[i % ROWS]);
+  __syncthreads();
+  for (int row = threadIdx.x; row < ROWS; row += NT) {
+    float l = 0.0f;
+    for (int k = 0; k < n; k++) l = __fmaf_rn(ms[k * ROWS + row], ls[k * ROWS + row], l);
     sum[row] = l;
     if (dst) {
-      dst[ROWS * DP + row] = m;
+      dst[ROWS * DP + row] = top[row];
       dst[ROWS * DP + ROWS + row] = l;
     } else if (row < t.rows) {
-      write_lse(a, t, head, row, m, l);
+      write_lse(a, t, head, row, top[row], l);
     }
   }
   __syncthreads();
-  // In place where dst is the first partial: each thread reads a value of it before it writes it.
-  for (int i = threadIdx.x; i < t.rows * DP / 4; i += NT) {
-    const int row = i / (DP / 4), d = (i % (DP / 4)) * 4;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int k = 0; k < n; k++) {
-      const float4 v = __ldcg(reinterpret_cast<const float4 *>(src(k) + row * DP + d));
-      const float f = fac[k * ROWS + row];
-      o.x = __fmaf_rn(f, v.x, o.x);
-      o.y = __fmaf_rn(f, v.y, o.y);
-      o.z = __fmaf_rn(f, v.z, o.z);
-      o.w = __fmaf_rn(f, v.w, o.w);
+  // In place where dst is the first partial: a thread reads a value of it before it
+  // writes it. Two vectors a thread, eight partials of each at a time.
+  const int items = t.rows * DP / 4;
+  for (int i0_ = threadIdx.x; i0_ < items; i0_ += 2 * NT) {
+    float4 o[2];
+    o[0] = o[1] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int i1_ = min(i0_ + NT, items - 1);
+    for (int k0 = 0; k0 < n; k0 += 8) {
+      float4 v[2][8];
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        v[0][j] = v[1][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (k0 + j < n) {
+          v[0][j] = __ldcg(reinterpret_cast<const float4 *>(src(k0 + j)) + i0_);
+          v[1][j] = __ldcg(reinterpret_cast<const float4 *>(src(k0 + j)) + i1_);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; j++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const float f = k0 + j < n ? ms[(k0 + j) * ROWS + (e ? i1_ : i0_) / (DP / 4)] : 0.0f;
+          o[e].x = __fmaf_rn(f, v[e][j].x, o[e].x);
+          o[e].y = __fmaf_rn(f, v[e][j].y, o[e].y);
+          o[e].z = __fmaf_rn(f, v[e][j].z, o[e].z);
+          o[e].w = __fmaf_rn(f, v[e][j].w, o[e].w);
+        }
     }
-    if (dst) {
-      *reinterpret_cast<float4 *>(dst + row * DP + d) = o;
-    } else if (d < a.pool.head_dim) {
-      const float l = sum[row];
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      write_out<T>(a, t, head, row, d, l == 0.0f ? 0.0f : o.x * inv);
-      write_out<T>(a, t, head, row, d + 1, l == 0.0f ? 0.0f : o.y * inv);
-      write_out<T>(a, t, head, row, d + 2, l == 0.0f ? 0.0f : o.z * inv);
-      write_out<T>(a, t, head, row, d + 3, l == 0.0f ? 0.0f : o.w * inv);
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      const int i = e ? i0_ + NT : i0_, row = i / (DP / 4), d = (i % (DP / 4)) * 4;
+      if (i >= items) break;
+      if (dst) *reinterpret_cast<float4 *>(dst + row * DP + d) = o[e];
+      else if (d < a.pool.head_dim) write_out<T>(a, t, head, row, d, o[e], sum[row]);
     }
   }
   __syncthreads();
 }
 
-// Called by all threads of a block after it wrote its partial of a unit of the
-// line's granules [u0, u1): joins what is complete. `flag`: shared memory.
+// Called by all threads of a block after it wrote its partial of a segment:
+// joins what is complete. `flag`: shared memory.
 template <typename T, int ROWS, int DP, int NT>
-__device__ void arrive(const AttendArgs &a, const RowTile &t, const Cursor &c, long long u0, long long u1, float *fac,
-                       unsigned *flag) {
-  const int i0 = block_of(c, u0), i1 = block_of(c, u1 - 1), n = i1 - i0 + 1;
+__device__ void arrive(const AttendArgs &a, const Segment &g, const Line &c, float *fac, unsigned *flag) {
+  const int i0 = chunk_of(c, g.u0), i1 = chunk_of(c, g.u0 + g.units - 1), n = i1 - i0 + 1;
   auto last = [&](unsigned *ctr, int of) {
-    __threadfence();
+    // One thread's fences order the whole block's writes (they come before it at
+    // the barrier) and reads: a fence of every thread would wait for the copies
+    // that all of them have on the way.
     __syncthreads();
-    if (threadIdx.x == 0) *flag = atomicInc(ctr, (unsigned)of - 1) == (unsigned)of - 1;  // wraps to 0
+    if (threadIdx.x == 0) {
+      __threadfence();
+      *flag = atomicInc(ctr, (unsigned)of - 1) == (unsigned)of - 1;  // wraps to 0
+      __threadfence();
+    }
     __syncthreads();
-    const bool yes = *flag != 0;
-    __syncthreads();
-    if (yes) __threadfence();
-    return yes;
+    return *flag != 0;
   };
   if (n <= kJoin) {
-    if (last(a.counters + i0, n)) join<T, ROWS, DP, NT>(a, t, c.head, i0, n, 1, 1, nullptr, fac);
+    if (last(a.counters + i0, n)) join<T, ROWS, DP, NT>(a, g.t, g.head, i0, n, 1, 1, nullptr, fac);
     return;
   }
   const int k = ((int)blockIdx.x - i0) / kJoin, g0 = i0 + k * kJoin, gn = min(kJoin, i1 - g0 + 1);
   const int groups = (n + kJoin - 1) / kJoin;
-  // (a group of one needs no count; its block's counter may be another unit's)
+  // (a group of one needs no count; its chunk's counter may be another unit's)
   if (gn > 1) {
     if (!last(a.counters + g0, gn)) return;
-    join<T, ROWS, DP, NT>(a, t, c.head, g0, gn, 1, k == 0, partial_at<ROWS, DP>(a, g0, k == 0), fac);
+    join<T, ROWS, DP, NT>(a, g.t, g.head, g0, gn, 1, k == 0, partial_at<ROWS, DP>(a, g0, k == 0), fac);
   }
   if (last(a.counters + kAttendMaxBlocks + i0, groups))
-    join<T, ROWS, DP, NT>(a, t, c.head, i0, groups, kJoin, 1, nullptr, fac);
+    join<T, ROWS, DP, NT>(a, g.t, g.head, i0, groups, kJoin, 1, nullptr, fac);
 }
 
 }  // namespace shlo

@@ -111,9 +111,9 @@ template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const AppendArgs a) {
   const shlo_kv_pool &pool = a.pool;
   const int PT = pool.page_tokens, sh = 31 - __clz(PT), slot = blockIdx.x, h = blockIdx.y, z = blockIdx.z;
-  const int b = slot_owner(a.batch, slot, 1, sh, 2);
-  const SeqSpan sp = seq_span(a.batch, b);
-  const int slot0 = slot_base(a.batch, b, 1, sh, 2);
+  const int b = slot_owner(a.batch.starts, a.batch.tokens, a.batch.seqs, 0, slot, 1, sh, 2);
+  const SeqSpan sp = seq_span(a.batch.starts, a.batch.lens, a.batch.tokens, b);
+  const int slot0 = slot_base(a.batch.starts, a.batch.tokens, b, 1, sh, 2);
   const int first = sp.len - sp.n;  // the first new token's position
   const int from = max(first, 0);
   const int page_of = (from >> sh) + (slot - slot0);

@@ -2,8 +2,8 @@
 the attention that reads it, for hosts that generate token by token.
 
 The *_noalloc functions take device tensors of the caller's own -- objects with
-data_ptr(), shape, stride(), dtype and element_size(), as a torch.Tensor has them;
-nothing here imports torch -- and queue their work on `stream` (a cudaStream_t as
+data_ptr(), shape, stride(), dtype, numel(), element_size() and is_contiguous(), as a
+torch.Tensor has them; nothing here imports torch -- and queue their work on `stream` (a cudaStream_t as
 an integer; 0 is the default stream). They allocate nothing. Every one is one call
 of include/shlo_cuda.h, whose comments say what it computes; errors raise ShloError.
 """
@@ -18,8 +18,17 @@ from ._lib import KvBatch, KvPool, ShloError, check, load
 
 SCALINGS = {"none": 0, "linear": 1, "base": 2, "ramp": 3, "blend": 4}
 
-_FLOATS = {"torch.float16": M.dtF16, "torch.float32": M.dtF32}
-_I32, _I64, _I8, _F32 = "torch.int32", "torch.int64", "torch.int8", "torch.float32"
+_NAMES = {"torch.float16": M.dtF16, "torch.float32": M.dtF32, "torch.int32": M.dtI32, "torch.int64": M.dtI64,
+          "torch.int8": M.dtI8}
+_codes: dict = {}  # a dtype object seen before -> its code (None: not carried)
+
+
+def _code(x):
+    d = x.dtype
+    try:
+        return _codes[d]
+    except KeyError:
+        return _codes.setdefault(d, _NAMES.get(str(d)))
 
 
 def rope_phases(rot: int, base: float = 10000.0, scaling: str = "none", by: float = 1.0, trained: float = 0.0,
@@ -34,48 +43,49 @@ def rope_phases(rot: int, base: float = 10000.0, scaling: str = "none", by: floa
     return out, f.value
 
 
-def _float(x, what):
-    t = _FLOATS.get(str(x.dtype))
-    if t is None:
-        raise ShloError("%s: %s not carried (float16 or float32)" % (what, x.dtype))
-    return t
-
-
-def _want(x, dtype, ndim, what):
-    if str(x.dtype) != dtype or len(x.shape) != ndim:
-        raise ShloError("%s: %s of rank %d, %s of rank %d expected" % (what, x.dtype, len(x.shape), dtype, ndim))
-
-
-def _packed(x, what):
-    """The last axis's values are contiguous."""
-    if x.shape[-1] > 1 and x.stride()[-1] != 1:
-        raise ShloError("%s: the last axis is strided" % what)
-
-
 def _rows(x, what):
-    """[tokens, heads, dim]: its token and head strides."""
-    if len(x.shape) != 3:
-        raise ShloError("%s: rank %d, [tokens, heads, dim] expected" % (what, len(x.shape)))
-    _packed(x, what)
-    s = x.stride()
-    return s[0], s[1]
+    """A float [tokens, heads, dim] whose last axis is contiguous: (shape, strides, type code)."""
+    c, n, s = _code(x), x.shape, x.stride()
+    if c != M.dtF16 and c != M.dtF32:
+        raise ShloError("%s: %s not carried (float16 or float32)" % (what, x.dtype))
+    if len(n) != 3:
+        raise ShloError("%s: rank %d, [tokens, heads, dim] expected" % (what, len(n)))
+    if s[2] != 1 and n[2] > 1:
+        raise ShloError("%s: the last axis is strided" % what)
+    return n, s, c
+
+
+def _list(x, code, what):
+    """A contiguous vector of a type: its length."""
+    n = x.shape
+    if _code(x) != code or len(n) != 1:
+        raise ShloError("%s: %s of rank %d, a vector of int%d expected" % (what, x.dtype, len(n), 32 if code == M.dtI32 else 64))
+    if n[0] > 1 and x.stride()[0] != 1:
+        raise ShloError("%s: the last axis is strided" % what)
+    return n[0]
+
+
+def _tables(x, what):
+    """int32 [sequences, pages], rows at any distance: (shape, row stride)."""
+    n, s = x.shape, x.stride()
+    if _code(x) != M.dtI32 or len(n) != 2:
+        raise ShloError("%s: %s of rank %d, int32 of rank 2 expected" % (what, x.dtype, len(n)))
+    if n[1] > 1 and s[1] != 1:
+        raise ShloError("%s: the last axis is strided" % what)
+    return n, s[0]
 
 
 def rope_noalloc(x, positions, phases, out, *, interleaved=False, inverse=False, factor=1.0, stream=0):
     """x [tokens, heads, dim] turned by positions (int32 [tokens]) into out; phases: rope_phases' on the device."""
-    dt = _float(x, "rope")
-    xs, ys = _rows(x, "rope: x"), _rows(out, "rope: out")
-    t, h, d = x.shape
-    if tuple(out.shape) != (t, h, d) or str(out.dtype) != str(x.dtype):
+    n, xs, dt = _rows(x, "rope: x")
+    m, ys, dy = _rows(out, "rope: out")
+    if m != n or dy != dt:
         raise ShloError("rope: out is not x's shape and type")
-    _want(positions, _I32, 1, "rope: positions")
-    _want(phases, _I64, 1, "rope: phases")
-    _packed(positions, "rope: positions")
-    _packed(phases, "rope: phases")
-    if positions.shape[0] != t:
+    t, h, d = n
+    if _list(positions, M.dtI32, "rope: positions") != t:
         raise ShloError("rope: %d positions for %d tokens" % (positions.shape[0], t))
     check(load().shlo_rope_noalloc(x.data_ptr(), xs[0], xs[1], positions.data_ptr(), phases.data_ptr(), out.data_ptr(),
-                                   ys[0], ys[1], t, h, d, 2 * phases.shape[0], dt,
+                                   ys[0], ys[1], t, h, d, 2 * _list(phases, M.dtI64, "rope: phases"), dt,
                                    (1 if interleaved else 0) | (2 if inverse else 0), factor, stream))
 
 
@@ -86,62 +96,47 @@ class Pool:
     __slots__ = ("c", "keep")
 
     def __init__(self, k, v, k_scale, v_scale):
-        for x, what in ((k, "cache: k"), (v, "cache: v")):
-            _want(x, _I8, 4, what)
-            _packed(x, what)
-        for x, what in ((k_scale, "cache: k_scale"), (v_scale, "cache: v_scale")):
-            _want(x, _F32, 2, what)
-        p, h, t, d = k.shape
-        s, z = k.stride(), k_scale.stride()
-        if tuple(v.shape) != (p, h, t, d) or tuple(v.stride()) != tuple(s):
-            raise ShloError("cache: k and v differ in shape or strides")
-        if tuple(k_scale.shape) != (p, h) or tuple(v_scale.shape) != (p, h) or tuple(v_scale.stride()) != tuple(z):
-            raise ShloError("cache: the scales are not [pages, heads] with the same strides")
+        n, m, s, z = k.shape, k_scale.shape, k.stride(), k_scale.stride()
+        if _code(k) != M.dtI8 or _code(v) != M.dtI8 or len(n) != 4:
+            raise ShloError("cache: k and v are int8 [pages, heads, page_tokens, head_dim]")
+        if v.shape != n or v.stride() != s or s[3] != 1:
+            raise ShloError("cache: k and v differ in shape or strides, or their last axis is strided")
+        if _code(k_scale) != M.dtF32 or _code(v_scale) != M.dtF32 or m != n[:2] or v_scale.shape != m or v_scale.stride() != z:
+            raise ShloError("cache: the scales are not float32 [pages, heads] with the same strides")
         self.keep = (k, v, k_scale, v_scale)
-        self.c = KvPool(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), p, s[0], s[1], s[2], z[0],
-                        z[1], h, d, t)
+        self.c = KvPool(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n[0], s[0], s[1], s[2],
+                        z[0], z[1], n[1], n[3], n[2])
 
 
 def _batch(starts, lens, tables, tokens):
-    _want(starts, _I32, 1, "batch: starts")
-    _want(lens, _I32, 1, "batch: lens")
-    _want(tables, _I32, 2, "batch: tables")
-    _packed(starts, "batch: starts")
-    _packed(lens, "batch: lens")
-    _packed(tables, "batch: tables")
-    n, w = tables.shape
-    if starts.shape[0] != n + 1 or lens.shape[0] != n:
-        raise ShloError("batch: %d starts and %d lengths for tables of %d sequences" % (starts.shape[0], lens.shape[0], n))
-    return KvBatch(starts.data_ptr(), lens.data_ptr(), tables.data_ptr(), tables.stride()[0], n, w, tokens)
+    (n, w), stride = _tables(tables, "batch: tables")
+    a, b = _list(starts, M.dtI32, "batch: starts"), _list(lens, M.dtI32, "batch: lens")
+    if a != n + 1 or b != n:
+        raise ShloError("batch: %d starts and %d lengths for tables of %d sequences" % (a, b, n))
+    return KvBatch(starts.data_ptr(), lens.data_ptr(), tables.data_ptr(), stride, n, w, tokens)
 
 
 def append_noalloc(pool: Pool, k, v, starts, lens, tables, *, stream=0):
     """k and v [tokens, heads, dim] rounded into the pages of their sequences."""
-    dt = _float(k, "kv_append")
-    ks, vs = _rows(k, "kv_append: k"), _rows(v, "kv_append: v")
-    t, h, d = k.shape
-    if tuple(v.shape) != (t, h, d) or str(v.dtype) != str(k.dtype) or h != pool.c.heads or d != pool.c.head_dim:
-        raise ShloError("kv_append: k and v are not [tokens, %d, %d] of one type" % (pool.c.heads, pool.c.head_dim))
-    check(load().shlo_kv_append_noalloc(pool.c, _batch(starts, lens, tables, t), k.data_ptr(), ks[0], ks[1],
-                                        v.data_ptr(), vs[0], vs[1], dt, stream))
+    n, ks, dt = _rows(k, "kv_append: k")
+    m, vs, dv = _rows(v, "kv_append: v")
+    c = pool.c
+    if m != n or dv != dt or n[1] != c.heads or n[2] != c.head_dim:
+        raise ShloError("kv_append: k and v are not [tokens, %d, %d] of one type" % (c.heads, c.head_dim))
+    check(load().shlo_kv_append_noalloc(c, _batch(starts, lens, tables, n[0]), k.data_ptr(), ks[0], ks[1], v.data_ptr(),
+                                        vs[0], vs[1], dt, stream))
 
 
 def gather_noalloc(pool: Pool, tables, seq, pos, k, v, *, stream=0):
     """The cache's values of tokens (seq[i], pos[i]) into k and v [n, heads, dim]."""
-    dt = _float(k, "kv_gather")
-    ks, vs = _rows(k, "kv_gather: k"), _rows(v, "kv_gather: v")
-    _want(tables, _I32, 2, "kv_gather: tables")
-    _want(seq, _I32, 1, "kv_gather: seq")
-    _want(pos, _I32, 1, "kv_gather: pos")
-    for x, what in ((tables, "tables"), (seq, "seq"), (pos, "pos")):
-        _packed(x, "kv_gather: " + what)
-    n = seq.shape[0]
-    shape = (n, pool.c.heads, pool.c.head_dim)
-    if pos.shape[0] != n or tuple(k.shape) != shape or tuple(v.shape) != shape or str(v.dtype) != str(k.dtype):
-        raise ShloError("kv_gather: pos, k and v are not of %d tokens, %d heads of %d" % shape)
-    check(load().shlo_kv_gather_noalloc(pool.c, tables.data_ptr(), tables.stride()[0], tables.shape[0],
-                                        tables.shape[1], seq.data_ptr(), pos.data_ptr(), n, k.data_ptr(), ks[0], ks[1],
-                                        v.data_ptr(), vs[0], vs[1], dt, stream))
+    n, ks, dt = _rows(k, "kv_gather: k")
+    m, vs, dv = _rows(v, "kv_gather: v")
+    (seqs, width), stride = _tables(tables, "kv_gather: tables")
+    c, t = pool.c, _list(seq, M.dtI32, "kv_gather: seq")
+    if _list(pos, M.dtI32, "kv_gather: pos") != t or n != (t, c.heads, c.head_dim) or m != n or dv != dt:
+        raise ShloError("kv_gather: pos, k and v are not of %d tokens, %d heads of %d" % (t, c.heads, c.head_dim))
+    check(load().shlo_kv_gather_noalloc(c, tables.data_ptr(), stride, seqs, width, seq.data_ptr(), pos.data_ptr(), t,
+                                        k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], dt, stream))
 
 
 def attend_workspace() -> int:
@@ -154,19 +149,19 @@ def attend_workspace() -> int:
 def attend_noalloc(pool: Pool, q, starts, lens, tables, out, *, workspace, scale, lse=None, causal=True, window=0,
                    stream=0):
     """q [tokens, query heads, dim] against the cache into out (and lse, float32 [tokens, query heads])."""
-    dt = _float(q, "kv_attend")
-    qs, os_ = _rows(q, "kv_attend: q"), _rows(out, "kv_attend: out")
-    t, h, d = q.shape
-    if d != pool.c.head_dim:
-        raise ShloError("kv_attend: queries of width %d, the cache's heads are %d wide" % (d, pool.c.head_dim))
-    if tuple(out.shape) != (t, h, d) or str(out.dtype) != str(q.dtype):
+    n, qs, dt = _rows(q, "kv_attend: q")
+    m, os_, do = _rows(out, "kv_attend: out")
+    t, h, d = n
+    c = pool.c
+    if d != c.head_dim:
+        raise ShloError("kv_attend: queries of width %d, the cache's heads are %d wide" % (d, c.head_dim))
+    if m != n or do != dt:
         raise ShloError("kv_attend: out is not q's shape and type")
-    lp = 0
+    lp = None
     if lse is not None:
-        _want(lse, _F32, 2, "kv_attend: lse")
-        if tuple(lse.shape) != (t, h) or (t and h and tuple(lse.stride()) != (h, 1)):
-            raise ShloError("kv_attend: lse is not a contiguous [%d, %d]" % (t, h))
+        if _code(lse) != M.dtF32 or lse.shape != (t, h) or (t and h and not lse.is_contiguous()):
+            raise ShloError("kv_attend: lse is not a contiguous float32 [%d, %d]" % (t, h))
         lp = lse.data_ptr()
-    check(load().shlo_kv_attend_noalloc(pool.c, _batch(starts, lens, tables, t), q.data_ptr(), qs[0], qs[1], h, dt,
-                                        scale, 1 if causal else 0, window, out.data_ptr(), os_[0], os_[1], lp,
+    check(load().shlo_kv_attend_noalloc(c, _batch(starts, lens, tables, t), q.data_ptr(), qs[0], qs[1], h, dt, scale,
+                                        1 if causal else 0, window, out.data_ptr(), os_[0], os_[1], lp,
                                         workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream))
