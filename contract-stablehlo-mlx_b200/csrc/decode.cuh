@@ -47,6 +47,7 @@ struct AttendCall {
   int32_t window;
   void *work;
   size_t work_bytes;
+  int *err;  // the device's word for launches that gave up a wait
 };
 size_t attend_work_bytes(int sms);
 int launch_kv_attend(const AttendCall &c, int sms, cudaStream_t st);

@@ -107,7 +107,7 @@ struct Shape {
   static constexpr int Q_WORDS = KS * 32 * 2 * NT * TERMS;
   static constexpr int RING_WORDS = kWarps * R * PIECE / 4;
   static constexpr int O_WORDS = kWarps * ROWS * OSTRIDE;
-  static constexpr int JOIN_WORDS = 2 * (kJoin + 1) * ROWS;
+  static constexpr int JOIN_WORDS = 2 * (kJoin<ROWS> + 1) * ROWS;
   static constexpr int BODY = O_WORDS > JOIN_WORDS ? O_WORDS : JOIN_WORDS;  // the warps' results, then a join's factors
   static constexpr int BATCH = 258;  // the batch's arrays, up to 128 sequences
   static constexpr int WORDS = 2 * Q_WORDS + RING_WORDS + BODY + 2 * kWarps * ROWS + 2 * ROWS + 2 * (kThreads + 4) + 16 + 4 + BATCH;
@@ -644,7 +644,8 @@ size_t attend_work_bytes(int sms) {
   of(8, 256, Shape<__half, 256, 1>::PER_SM);
   of(16, 64, Shape<__half, 64, 2>::PER_SM);
   of(16, 128, Shape<__half, 128, 2>::PER_SM);
-  return kCounterBytes + most;
+  const size_t tiles = attend_tiles_partial_bytes(sms);
+  return kCounterBytes + (tiles > most ? tiles : most);
 }
 
 int launch_kv_attend(const AttendCall &c, int sms, cudaStream_t st) {
@@ -680,8 +681,20 @@ int launch_kv_attend(const AttendCall &c, int sms, cudaStream_t st) {
   a.upto = (int64_t)1 << 40;
   a.counters = static_cast<unsigned *>(c.work);
   a.partials = reinterpret_cast<float *>(static_cast<char *>(c.work) + kCounterBytes);
-  // Tiles of 8 rows where the sequences have 8 or fewer on average, else 16.
-  const int nt = (int64_t)c.batch.tokens * group <= (int64_t)8 * c.batch.seqs ? 1 : 2;
+  a.q_wide = (uintptr_t)c.q % 16 == 0 && c.q_token % 8 == 0 && c.q_head % 8 == 0;
+  a.err = c.err;
+  // Tiles of 8 rows where the sequences have 8 or fewer on average, else 16. Above
+  // 16, float16 sequences of more than 16 rows go to the tiles of 128 (in which a
+  // 16-row tile would cost as much as a full one), in a launch of their own.
+  const int64_t rows = (int64_t)c.batch.tokens * group;
+  const int nt = rows <= (int64_t)8 * c.batch.seqs ? 1 : 2;
+  if (c.dtype == kF16 && rows > (int64_t)16 * c.batch.seqs) {
+    AttendArgs big = a;
+    big.above = 16;
+    SHLO_TRY(launch_attend_tiles(big, sms, st));
+    if (c.batch.seqs == 1) return 0;
+    a.upto = 16;
+  }
   return c.dtype == kF16 ? dispatch_rows<__half>(a, nt, sms, st) : dispatch_rows<float>(a, nt, sms, st);
 }
 
@@ -707,7 +720,7 @@ int shlo_kv_attend_noalloc(const shlo_kv_pool *pool, const shlo_kv_batch *batch,
   Device *dev;
   SHLO_TRY(current_device(&dev));
   AttendCall c{*pool, *batch, q, q_token, q_head, out, out_token, out_head, lse, heads, dtype, scale, causal != 0, window,
-               workspace, workspace_bytes};
+               workspace, workspace_bytes, dev->pipe_err_dev};
   return launch_kv_attend(c, dev->sm_count, (cudaStream_t)stream);
 }
 

@@ -37,6 +37,7 @@ struct AttendArgs {
   int slots;         // slots of the work list
   int causal, window;
   int out_wide;      // out allows stores of four values
+  int q_wide;        // q allows 16-byte loads
   float scale_log2;  // scale * log2(e)
   int page_shift;
   // Which sequences this launch takes: those with rows (new tokens * group) in
@@ -44,10 +45,16 @@ struct AttendArgs {
   int64_t above, upto;
   unsigned *counters;  // [2][kAttendMaxBlocks], zero between calls
   float *partials;     // [chunks][2][rows * (dim + 2)]
+  int *err;            // set by a launch that gave up a wait
 };
 
 constexpr int kAttendMaxBlocks = 1024;
-constexpr int kJoin = 64;
+// Partials joined at once: what a join's factors take in shared memory bounds it.
+template <int ROWS> constexpr int kJoin = ROWS == 128 ? 32 : 64;
+
+// kv_attend_tiles.cu: tiles of 128 rows, float16.
+int launch_attend_tiles(const AttendArgs &a, int sms, cudaStream_t st);
+size_t attend_tiles_partial_bytes(int sms);
 
 // A tile of rows and what it sees.
 struct RowTile {
@@ -350,6 +357,7 @@ __device__ void join(const AttendArgs &a, const RowTile &t, int head, int i0, in
 // joins what is complete. `flag`: shared memory.
 template <typename T, int ROWS, int DP, int NT>
 __device__ void arrive(const AttendArgs &a, const Segment &g, const Line &c, float *fac, unsigned *flag) {
+  constexpr int J = kJoin<ROWS>;
   const int i0 = chunk_of(c, g.u0), i1 = chunk_of(c, g.u0 + g.units - 1), n = i1 - i0 + 1;
   auto last = [&](unsigned *ctr, int of) {
     // One thread's fences order the whole block's writes (they come before it at
@@ -364,19 +372,19 @@ __device__ void arrive(const AttendArgs &a, const Segment &g, const Line &c, flo
     __syncthreads();
     return *flag != 0;
   };
-  if (n <= kJoin) {
+  if (n <= J) {
     if (last(a.counters + i0, n)) join<T, ROWS, DP, NT>(a, g.t, g.head, i0, n, 1, 1, nullptr, fac);
     return;
   }
-  const int k = ((int)blockIdx.x - i0) / kJoin, g0 = i0 + k * kJoin, gn = min(kJoin, i1 - g0 + 1);
-  const int groups = (n + kJoin - 1) / kJoin;
+  const int k = ((int)blockIdx.x - i0) / J, g0 = i0 + k * J, gn = min(J, i1 - g0 + 1);
+  const int groups = (n + J - 1) / J;
   // (a group of one needs no count; its chunk's counter may be another unit's)
   if (gn > 1) {
     if (!last(a.counters + g0, gn)) return;
     join<T, ROWS, DP, NT>(a, g.t, g.head, g0, gn, 1, k == 0, partial_at<ROWS, DP>(a, g0, k == 0), fac);
   }
   if (last(a.counters + kAttendMaxBlocks + i0, groups))
-    join<T, ROWS, DP, NT>(a, g.t, g.head, i0, groups, kJoin, 1, nullptr, fac);
+    join<T, ROWS, DP, NT>(a, g.t, g.head, i0, groups, J, 1, nullptr, fac);
 }
 
 }  // namespace shlo

@@ -289,6 +289,30 @@ def test_attend(kind, page, hk, group, D, lens, news, layout):
 
 
 @pytest.mark.parametrize("kind", ["f16", "f32"])
+@pytest.mark.parametrize("page,hk,group,D,lens,news,layout", [
+    (16, 1, 1, 16, [17], [17], "heads"),
+    (64, 1, 8, 128, [3000], [20], "heads"),
+    (16, 2, 3, 128, [400, 129, 1000, 5], [300, 129, 1, 5], "tokens"),
+    (128, 1, 5, 256, [500, 64], [200, 64], "heads"),
+    (256, 2, 2, 240, [700], [90], "tokens"),
+    (32, 1, 16, 64, [260, 1], [260, 1], "heads"),
+    (64, 3, 1, 80, [128, 127, 0, 129], [128, 127, 130, 129], "tokens"),
+    (16, 1, 4, 48, [2500, 33], [40, 33], "heads")])
+def test_attend_prompts(kind, page, hk, group, D, lens, news, layout):
+    """Many rows a sequence: tiles of 128 rows that end inside a token's heads, units cut between blocks, rows of
+    sequences that have none to see."""
+    c = Case(kind, page, hk, group, D, lens, news, layout, seed=7)
+    work = torch.zeros(Dc.attend_workspace(), dtype=torch.uint8, device="cuda")
+    pool = pool_of(c.cache, layout)
+    for causal, window in ((True, 0), (False, 0), (True, 100)):
+        got = c.run(causal, window, work=work, pool=pool)
+        c.check(got, causal, window)
+        again = c.run(causal, window, work=work, pool=pool)
+        assert again[0].tobytes() == got[0].tobytes() and again[1].tobytes() == got[1].tobytes()
+    assert int(work[:8192].to(torch.int32).sum()) == 0
+
+
+@pytest.mark.parametrize("kind", ["f16", "f32"])
 @pytest.mark.parametrize("hk,group,D,lens", [(1, 8, 128, [40001]), (2, 4, 64, [30000, 3]), (1, 1, 256, [9000]),
                                              (1, 16, 128, [20000, 11000])])
 def test_attend_long_contexts_split_and_joined(kind, hk, group, D, lens):
