@@ -339,8 +339,8 @@ __global__ void __launch_bounds__(kThreadsT, Tiles<DP>::PER_SM) k_kv_attend_tile
       // (the values are N-major).
       const uint32_t id_s = 1u << 4 | (uint32_t)(KT >> 3) << 17 | (uint32_t)(kRowsT >> 4) << 24;
       const uint32_t id_o = 1u << 4 | 1u << 16 | (uint32_t)(D >> 3) << 17 | (uint32_t)(kRowsT >> 4) << 24;
-      auto scores = [&](int j) {
-        if (!bar_wait(k_full, (done + j) & 1, gone)) return;
+      // (every warp has waited for the keys: see below)
+      auto scores = [&]() {
         tm_after();
         for (int k = 0; k < D / 16; k++) {
           const uint32_t off = (k % 4) * 32;
@@ -357,13 +357,18 @@ __global__ void __launch_bounds__(kThreadsT, Tiles<DP>::PER_SM) k_kv_attend_tile
           mma_ts(o_at, s_at + k * 8, operand(smem_at(vs) + k * 2048, KT * 128), id_o, j > 0 || k > 0);
         tm_commit(pv_done);
         // S takes P's place: the next scores wait for the product that reads P
-        if (j + 1 < n && bar_wait(pv_done, ph, gone)) scores(j + 1);
+        if (j + 1 < n && bar_wait(pv_done, ph, gone)) scores();
       };
-      if (tid == 0) scores(0);
+      // A warp waits for a tile's keys (their scales lie beside them) before it lets
+      // the product that reads them start: later, the barrier might be two phases
+      // on and look as if it had yet to come.
+      ok = warp_wait(k_full, done & 1, gone);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (tid == 0 && ok) scores();
       __syncwarp();
-      for (int j = 0; j < n; j++) {
+      for (int j = 0; j < n && ok; j++) {
         const uint32_t ph = (done + j) & 1;
-        if (!warp_wait(k_full, ph, gone) || !warp_wait(qk_done, ph, gone)) {
+        if (!warp_wait(qk_done, ph, gone)) {
           ok = false;
           break;
         }
@@ -388,8 +393,8 @@ __global__ void __launch_bounds__(kThreadsT, Tiles<DP>::PER_SM) k_kv_attend_tile
           }
         };
         float top = -INFINITY;
-#pragma unroll
-        for (int ch = 0; ch < KT / 32; ch++) {
+#pragma unroll 1
+        for (int ch = 0; ch < KT / 32; ch++) {  // (unrolled, the loops overflow the instruction cache)
           float v[32];
           tm_ld32(s_at + lanes + ch * 32, v);
           masked(v, ch);
@@ -404,20 +409,18 @@ __global__ void __launch_bounds__(kThreadsT, Tiles<DP>::PER_SM) k_kv_attend_tile
           l *= f;
           m = mn;
           if (j) {  // (the first product writes O)
+#pragma unroll 1
+            for (int ch = 0; ch * 32 < D; ch++) {
+              float v[32];
+              tm_ld32(o_at + lanes + ch * 32, v);
 #pragma unroll
-            for (int ch = 0; ch < DP / 32; ch++) {
-              if (ch * 32 < D) {
-                float v[32];
-                tm_ld32(o_at + lanes + ch * 32, v);
-#pragma unroll
-                for (int x = 0; x < 32; x++) v[x] *= f;
-                tm_st32(o_at + lanes + ch * 32, v);
-              }
+              for (int x = 0; x < 32; x++) v[x] *= f;
+              tm_st32(o_at + lanes + ch * 32, v);
             }
           }
         }
         const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
+#pragma unroll 1
         for (int ch = 0; ch < KT / 32; ch++) {
           float v[32];
           tm_ld32(s_at + lanes + ch * 32, v);
@@ -445,6 +448,7 @@ __global__ void __launch_bounds__(kThreadsT, Tiles<DP>::PER_SM) k_kv_attend_tile
         }
         tm_wait_st();
         tm_before();
+        if (j + 1 < n && !warp_wait(k_full, ph ^ 1, gone)) ok = false;
         __syncwarp();
         if (lane == 0) bar_arrive(p_full);
         if (tid == 0) outputs(j);
@@ -456,7 +460,7 @@ __global__ void __launch_bounds__(kThreadsT, Tiles<DP>::PER_SM) k_kv_attend_tile
       float *part = whole ? nullptr : partial_at<kRowsT, DP>(a, blockIdx.x, sg.off == 0);
       const float unscale = vtop * 0x1p-7f;
       if (ok) {
-#pragma unroll
+#pragma unroll 1
         for (int ch = 0; ch < DP / 32; ch++) {
           if (ch * 32 < D) {
             float v[32];
