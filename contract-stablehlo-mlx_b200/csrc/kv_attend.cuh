@@ -50,9 +50,10 @@ struct AttendArgs {
 
 constexpr int kAttendMaxBlocks = 1024;
 // Partials joined at once: what a join's factors take in shared memory bounds it.
-template <int ROWS> constexpr int kJoin = ROWS == 128 ? 32 : 64;
+template <int ROWS> constexpr int kJoin = ROWS >= 128 ? 32 : 64;
+template <int ROWS> constexpr int kRowShift = ROWS == 8 ? 3 : ROWS == 16 ? 4 : ROWS == 128 ? 7 : 8;
 
-// kv_attend_tiles.cu: tiles of 128 rows, float16.
+// kv_attend_tiles.cu: tiles of 256 rows (128 of heads wider than 128), float16.
 int launch_attend_tiles(const AttendArgs &a, int sms, cudaStream_t st);
 size_t attend_tiles_partial_bytes(int sms);
 
@@ -78,8 +79,7 @@ __device__ __forceinline__ int row_lo(const AttendArgs &a, int pos) {
 template <int ROWS, int GRAN>
 __device__ __forceinline__ int tile_of_slot(const AttendArgs &a, const int32_t *starts, const int32_t *lens, int slot,
                                             RowTile &t, bool after) {
-  constexpr int SH = ROWS == 8 ? 3 : ROWS == 16 ? 4 : ROWS == 64 ? 6 : 7;
-  static_assert(1 << SH == ROWS, "rows of a tile");
+  constexpr int SH = kRowShift<ROWS>;
   const int tokens = a.batch.tokens, seqs = a.batch.seqs;
   int s;
   if (after) {
@@ -180,7 +180,16 @@ __device__ __forceinline__ bool next_segment(const AttendArgs &a, const BatchArr
       p.slot = p.seq = 0;
       p.head++;
     }
-    if (units == 0) continue;  // a slot without a tile
+    if (units == 0) {  // a slot without a tile: neither has the rest of its sequence's
+      constexpr int SH = kRowShift<ROWS>;
+      if (p.slot > 0)
+        p.slot = p.seq + 1 < a.batch.seqs ? max(p.slot, slot_base(ba.starts, a.batch.tokens, p.seq + 1, a.group, SH, 1)) : a.slots;
+      if (p.slot >= a.slots) {
+        p.slot = p.seq = 0;
+        p.head++;
+      }
+      continue;
+    }
     g.off = off;
     g.units = units;
     g.take = (int)min((long long)(units - off), p.end - p.at);
