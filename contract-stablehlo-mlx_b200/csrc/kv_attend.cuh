@@ -22,6 +22,8 @@
 // order of the keys; more than kJoin partials are joined in groups of kJoin first.
 #pragma once
 
+#include <type_traits>
+
 #include "decode.cuh"
 
 namespace shlo {
@@ -324,41 +326,46 @@ __device__ void join(const AttendArgs &a, const RowTile &t, int head, int i0, in
   }
   __syncthreads();
   // In place where dst is the first partial: a thread reads a value of it before it
-  // writes it. Two vectors a thread, eight partials of each at a time.
+  // writes it. Sixteen loads a thread on their way: eight vectors of two partials,
+  // or two of eight.
   const int items = t.rows * DP / 4;
-  for (int i0_ = threadIdx.x; i0_ < items; i0_ += 2 * NT) {
-    float4 o[2];
-    o[0] = o[1] = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int i1_ = min(i0_ + NT, items - 1);
-    for (int k0 = 0; k0 < n; k0 += 8) {
-      float4 v[2][8];
+  auto vectors = [&](auto per, auto batch) {
+    constexpr int V = decltype(per)::value, B = decltype(batch)::value;
+    for (int first = threadIdx.x; first < items; first += V * NT) {
+      float4 o[V];
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        v[0][j] = v[1][j] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (k0 + j < n) {
-          v[0][j] = __ldcg(reinterpret_cast<const float4 *>(src(k0 + j)) + i0_);
-          v[1][j] = __ldcg(reinterpret_cast<const float4 *>(src(k0 + j)) + i1_);
-        }
+      for (int e = 0; e < V; e++) o[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k0 = 0; k0 < n; k0 += B) {
+        float4 v[V][B];
+#pragma unroll
+        for (int j = 0; j < B; j++)
+#pragma unroll
+          for (int e = 0; e < V; e++) {
+            v[e][j] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (k0 + j < n && first + e * NT < items) v[e][j] = __ldcg(reinterpret_cast<const float4 *>(src(k0 + j)) + first + e * NT);
+          }
+#pragma unroll
+        for (int j = 0; j < B; j++)
+#pragma unroll
+          for (int e = 0; e < V; e++) {
+            const float f = k0 + j < n && first + e * NT < items ? ms[(k0 + j) * ROWS + (first + e * NT) / (DP / 4)] : 0.0f;
+            o[e].x = __fmaf_rn(f, v[e][j].x, o[e].x);
+            o[e].y = __fmaf_rn(f, v[e][j].y, o[e].y);
+            o[e].z = __fmaf_rn(f, v[e][j].z, o[e].z);
+            o[e].w = __fmaf_rn(f, v[e][j].w, o[e].w);
+          }
       }
 #pragma unroll
-      for (int j = 0; j < 8; j++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const float f = k0 + j < n ? ms[(k0 + j) * ROWS + (e ? i1_ : i0_) / (DP / 4)] : 0.0f;
-          o[e].x = __fmaf_rn(f, v[e][j].x, o[e].x);
-          o[e].y = __fmaf_rn(f, v[e][j].y, o[e].y);
-          o[e].z = __fmaf_rn(f, v[e][j].z, o[e].z);
-          o[e].w = __fmaf_rn(f, v[e][j].w, o[e].w);
-        }
+      for (int e = 0; e < V; e++) {
+        const int i = first + e * NT, row = i / (DP / 4), d = (i % (DP / 4)) * 4;
+        if (i >= items) break;
+        if (dst) *reinterpret_cast<float4 *>(dst + row * DP + d) = o[e];
+        else if (d < a.pool.head_dim) write_out<T>(a, t, head, row, d, o[e], sum[row]);
+      }
     }
-#pragma unroll
-    for (int e = 0; e < 2; e++) {
-      const int i = e ? i0_ + NT : i0_, row = i / (DP / 4), d = (i % (DP / 4)) * 4;
-      if (i >= items) break;
-      if (dst) *reinterpret_cast<float4 *>(dst + row * DP + d) = o[e];
-      else if (d < a.pool.head_dim) write_out<T>(a, t, head, row, d, o[e], sum[row]);
-    }
-  }
+  };
+  if (ROWS >= 128 && n <= 2) vectors(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
+  else vectors(std::integral_constant<int, 2>{}, std::integral_constant<int, 8>{});
   __syncthreads();
 }
 

@@ -4,7 +4,7 @@
 // The formulas are kv_attend.cu's. A block holds RT tiles of 128 rows' queries in
 // shared memory and goes over KT keys at a time: S = Q K^T into tensor
 // memory, the weights P = e^(s - m) (sv / largest sv) 2^7 as float16 over S,
-// O += P V with P from tensor memory. Three kinds of warps hand tiles to each
+// O += P V with P from tensor memory. Four kinds of warps hand tiles to each
 // other by mbarriers, with two places of scores, so that the products of one
 // tile of keys run beside the exponentials of another:
 //   four a row tile   a row a thread: scores from tensor memory, masks, m and l in
@@ -12,6 +12,7 @@
 //   four              the keys' and values' bytes, which bulk copies bring to shared
 //                     memory RS tiles ahead, to float16 integers (exact) in the
 //                     128-byte swizzled layout; once for all row tiles
+//   one               asks for the bytes, their pages and scales
 //   one               one thread issues the products
 // Keys lie in shared memory with their dimensions contiguous, for both products:
 // K-major for the first, N-major for the second, so nothing is transposed.
@@ -165,22 +166,23 @@ struct Tiles {
   static constexpr int KT = DP == 256 ? 32 : 64;   // keys a tile
   static constexpr int RT = DP == 256 ? 1 : 2;     // row tiles
   static constexpr int ROWS = RT * kRowsT;
-  static constexpr int THREADS = (4 * RT + 5) * 32;
+  static constexpr int THREADS = (4 * RT + 6) * 32;
   static constexpr int O_COL = RT * 2 * KT;        // S of tile r, place b at (2 r + b) KT; P lies over S, two weights a column
   static constexpr int TM_COLS = 512;
   static constexpr int Q_BYTES = kRowsT * DP * 2, K_BYTES = KT * DP * 2;
   static constexpr int NS = 3, RS = 3;             // stages of keys and values: as float16 (the scores run two tiles ahead of the outputs), as bytes
   static constexpr int GROUPS = KT / 16;
-  static constexpr int META = 2 * GROUPS + 4;      // a stage's scales of keys and of values, its holes, whether the scores need care
+  static constexpr int META = 2 * GROUPS + 4;      // a tile's scales of keys and of values, its holes, whether the scores need care
+  static constexpr int NM = 8;                     // such sets: those asked for (RS), converted (NS) and under the softmax
   static constexpr int BATCH = 1024;
-  static constexpr int MISC = 256 + (THREADS + 4) * 8 + 64 + BATCH * 4 + NS * META * 4 + 64;
+  static constexpr int MISC = 256 + (THREADS + 4) * 8 + 64 + BATCH * 4 + NM * META * 4 + 64;
   static constexpr int BYTES = 1024 + RT * Q_BYTES + 2 * NS * K_BYTES + RS * K_BYTES + MISC;
 };
 
 template <int DP>
 __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const AttendArgs a, int min_gran) {
   using S = Tiles<DP>;
-  constexpr int KT = S::KT, GROUPS = S::GROUPS, META = S::META, RT = S::RT, NS = S::NS, RS = S::RS, ROWS = S::ROWS, THREADS = S::THREADS;
+  constexpr int KT = S::KT, GROUPS = S::GROUPS, META = S::META, NM = S::NM, RT = S::RT, NS = S::NS, RS = S::RS, ROWS = S::ROWS, THREADS = S::THREADS;
   extern __shared__ uint8_t raw_smem[];
   uint8_t *const base = raw_smem + ((1024 - (smem_at(raw_smem) & 1023)) & 1023);
   uint8_t *const qs = base, *const ks = qs + RT * S::Q_BYTES, *const vs = ks + NS * S::K_BYTES;
@@ -193,7 +195,7 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
   Place *const place = reinterpret_cast<Place *>(sched + THREADS + 4);
   int *const batch = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(place) + 64);
   float *const meta = reinterpret_cast<float *>(batch + S::BATCH);
-  unsigned *const flag = reinterpret_cast<unsigned *>(meta + NS * META);
+  unsigned *const flag = reinterpret_cast<unsigned *>(meta + NM * META);
   volatile int *const gone = reinterpret_cast<volatile int *>(flag + 1);
   uint32_t *const tm_slot = reinterpret_cast<uint32_t *>(flag + 2);
   float *const vtop_s = reinterpret_cast<float *>(flag + 3);
@@ -251,34 +253,123 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
       return pg >= 0 && pg < a.pool.pages ? pg : -1;
     };
     const int rts = (sg.t.rows + kRowsT - 1) / kRowsT;  // row tiles with rows
+    const int n = sg.take;
+    // The asking warp's: pages and scales are held across its lanes, 32 groups of 16
+    // keys (TL tiles: a stretch) at a time, and asked for a stretch ahead: on a
+    // tile's own path they would be two more waits for L2.
+    constexpr int TL = 32 / GROUPS;
+    const int64_t tok = a.pool.token_stride;
+    int pg = -1, pg_next = -1;
+    int64_t off = 0, off_next = 0;  // of the group's first key
+    float kscale = 0.0f, vscale = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
+    auto pages = [&](int j) {
+      const int key = key0 + j * KT + lane * 16;
+      pg_next = j + lane / GROUPS < n ? page_at(key) : -1;
+      off_next = (int64_t)sg.head * a.pool.head_stride + (int64_t)max(pg_next, 0) * a.pool.page_stride + (int64_t)(key & (PT - 1)) * tok;
+    };
+    auto ask_scales = [&]() {
+      ks_next = vs_next = 0.0f;
+      if (pg_next >= 0) {
+        ks_next = __ldg(a.pool.k_scale + ((int64_t)sg.head * a.pool.scale_head_stride + (int64_t)pg_next * a.pool.scale_page_stride));
+        vs_next = __ldg(a.pool.v_scale + ((int64_t)sg.head * a.pool.scale_head_stride + (int64_t)pg_next * a.pool.scale_page_stride));
+      }
+    };
+    auto turn = [&]() {  // to the next stretch
+      pg = pg_next;
+      off = off_next;
+      kscale = ks_next;
+      vscale = vs_next;
+    };
+    // The bytes of tile j into its stage. What is not there is left as it lies: any
+    // byte is a finite value, and no row sees it.
+    auto copy_tile = [&](int j) {
+      const uint32_t rs = (done + j) % RS, to = smem_at(raw) + rs * S::K_BYTES;
+      uint64_t *const bar = raw_full + rs;
+      const int at = j % TL * GROUPS;
+      const bool joined = tok == D;  // a group's 16 rows are one run of bytes: a lane copies one group's keys or values
+      const int group = joined ? lane / 2 : lane % GROUPS;
+      const int q = __shfl_sync(~0u, pg, (at + group) & 31);
+      const int64_t o = __shfl_sync(~0u, off, (at + group) & 31);
+      if (joined) {
+        if (lane < 2 * GROUPS && q >= 0)
+          copy_bulk(to + ((lane & 1) * KT + group * 16) * D, (lane & 1 ? a.pool.v : a.pool.k) + o, 16 * D, bar);
+      } else {
+#pragma unroll 1
+        for (int i = lane; i < 2 * KT; i += 32) {  // one row a copy; GROUPS divides 32, so a lane keeps its group
+          const int kv = i / KT, row = i % KT / GROUPS;
+          if (q >= 0) copy_bulk(to + (kv * KT + group * 16 + row) * D, (kv ? a.pool.v : a.pool.k) + o + row * tok, D, bar);
+        }
+      }
+    };
+    // Its scales, for the softmax; and the count of its bytes, with which they are
+    // handed on (a tile is complete when both the count and the bytes are there).
+    auto count_tile = [&](int j, float vtop) {
+      const int at = j % TL * GROUPS;
+      float *mt = meta + (done + j) % NM * META;
+      const float c = kscale * a.scale_log2;
+      // a scale that is not finite makes the weights of the keys that are seen NaN
+      const float ratio = !(fabsf(vscale) <= 3.402823466e38f) ? __int_as_float(0x7fc00000) : vtop > 0.0f ? __fdiv_rn(vscale, vtop) * 128.0f : 0.0f;
+      const uint32_t group_bits = (1u << GROUPS) - 1;
+      const uint32_t holes = __ballot_sync(~0u, pg < 0) >> at & group_bits, odd = __ballot_sync(~0u, !(c >= 0.0f)) >> at & group_bits;
+      if (lane >= at && lane < at + GROUPS) {
+        mt[lane - at] = c;
+        mt[GROUPS + lane - at] = ratio;
+      }
+      if (lane == 0) {
+        mt[2 * GROUPS] = __int_as_float((int)holes);
+        mt[2 * GROUPS + 1] = __int_as_float((int)odd);
+      }
+      __syncwarp();
+      const uint32_t bytes = 2u * (GROUPS - __popc(holes)) * 16u * (uint32_t)D;
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_at(raw_full + (done + j) % RS)), "r"(bytes) : "memory");
+    };
+    constexpr int ASKER = 4 * RT + 5;
+    static_assert(RS <= TL / 2, "the first tiles are of one stretch, and the next one's scales are yet to ask for");
+    if (warp == ASKER) {
+      pages(0);
+      ask_scales();
+      turn();
+      for (int j = 0; j < RS && j < n; j++) copy_tile(j);
+    }
     // The queries, and the largest finite scale of the segment's values.
     if (tid == 0) *vtop_s = 0.0f;
     __syncthreads();
     {
-      constexpr int PIECES = DP / 8;
-      for (int i = tid; i < rts * kRowsT * PIECES; i += THREADS) {
-        const int row = i / PIECES, c = i % PIECES, d = c * 8, r = sg.t.row0 + row;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (row < sg.t.rows && d < D) {
-          const __half *q = static_cast<const __half *>(a.q) + (int64_t)(sg.t.start + r / a.group) * a.q_token +
-                            (int64_t)(sg.head * a.group + r % a.group) * a.q_head + d;
-          if (a.q_wide) {
-            v = *reinterpret_cast<const uint4 *>(q);
-          } else {
-            __half h[8];
+      constexpr int PIECES = DP / 8, BATCH = 4;
+      const int items = rts * kRowsT * PIECES;
+      for (int i0 = tid; i0 < items; i0 += BATCH * THREADS) {  // several loads on their way
+        uint4 v[BATCH];
 #pragma unroll
-            for (int j = 0; j < 8; j++) h[j] = q[j];
-            memcpy(&v, h, 16);
+        for (int k = 0; k < BATCH; k++) {
+          const int i = i0 + k * THREADS, row = i / PIECES, d = i % PIECES * 8, r = sg.t.row0 + row;
+          v[k] = make_uint4(0u, 0u, 0u, 0u);
+          if (row < sg.t.rows && d < D) {
+            const __half *q = static_cast<const __half *>(a.q) + (int64_t)(sg.t.start + r / a.group) * a.q_token +
+                              (int64_t)(sg.head * a.group + r % a.group) * a.q_head + d;
+            if (a.q_wide) {
+              v[k] = *reinterpret_cast<const uint4 *>(q);
+            } else {
+              __half h[8];
+#pragma unroll
+              for (int j = 0; j < 8; j++) h[j] = q[j];
+              memcpy(&v[k], h, 16);
+            }
           }
         }
-        *reinterpret_cast<uint4 *>(qs + (row / kRowsT) * S::Q_BYTES + (c / 8) * (kRowsT * 128) + (row % kRowsT) * 128 +
-                                   (((c % 8) ^ (row & 7)) * 16)) = v;
+#pragma unroll
+        for (int k = 0; k < BATCH; k++) {
+          const int i = i0 + k * THREADS, row = i / PIECES, c = i % PIECES;
+          if (i < items)
+            *reinterpret_cast<uint4 *>(qs + (row / kRowsT) * S::Q_BYTES + (c / 8) * (kRowsT * 128) + (row % kRowsT) * 128 +
+                                       (((c % 8) ^ (row & 7)) * 16)) = v[k];
+        }
       }
       float top = 0.0f;
       for (int i = tid; i < sg.take * GROUPS; i += THREADS) {
-        const int pg = page_at(key0 + i * 16);
-        if (pg >= 0) {
-          const float s = fabsf(__ldg(a.pool.v_scale + ((int64_t)sg.head * a.pool.scale_head_stride + (int64_t)pg * a.pool.scale_page_stride)));
+        const int q = page_at(key0 + i * 16);
+        if (q >= 0) {
+          const float s = fabsf(__ldg(a.pool.v_scale + ((int64_t)sg.head * a.pool.scale_head_stride + (int64_t)q * a.pool.scale_page_stride)));
           if (s <= 3.402823466e38f) top = fmaxf(top, s);
         }
       }
@@ -289,8 +380,23 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     __syncthreads();
     const float vtop = *vtop_s;
-    const int n = sg.take;
 
+    if (warp == ASKER) {
+      // ---- bytes, pages and scales ----
+      for (int j = 0; j < RS && j < n; j++) count_tile(j, vtop);
+      pages(TL);
+      for (int j = RS; j < n; j++) {
+        const uint32_t t = done + j;
+        if (j % TL == TL / 2) ask_scales();
+        if (j % TL == 0) {
+          turn();
+          pages(j + TL);
+        }
+        if (!warp_wait(raw_free + t % RS, (t / RS & 1) ^ 1, gone)) break;
+        copy_tile(j);
+        count_tile(j, vtop);
+      }
+    } else
     if (warp == 4 * RT + 4) {
       // ---- products ----
       {
@@ -366,72 +472,15 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
           }
         }
       }
-    } else if (warp >= 4 * RT) {
+    } else if (warp >= 4 * RT && warp < 4 * RT + 4) {
       // ---- bytes to float16 ----
       constexpr int CH = DP / 16, KPP = 128 / CH, NI = KT / KPP;  // pieces a key, keys a pass, passes
       const int pt = tid - 128 * RT, key_in = pt / CH, ch = pt % CH;
       const bool live = ch * 16 < D;
-      const int64_t tok = a.pool.token_stride;
       // where this thread's two pieces of 8 go in a stage
       const int db = ch / 4, c0 = (ch % 4) * 2, first = db & 1;  // (the pieces in an order that keeps eight lanes on eight bank groups)
       const int to1 = db * (KT * 128) + key_in * 128 + (((c0 + first) ^ (key_in & 7)) * 16);
       const int to2 = db * (KT * 128) + key_in * 128 + (((c0 + 1 - first) ^ (key_in & 7)) * 16);
-      // The first of these warps asks for the bytes. Pages and scales are held
-      // across its lanes, 32 groups of 16 keys (TL tiles: a stretch) at a time, and
-      // asked for a stretch ahead: on a tile's own path they would be two more
-      // waits for L2.
-      const bool asks = warp == 4 * RT;
-      const bool joined = tok == D;  // a group's 16 rows are one run of bytes
-      constexpr int TL = 32 / GROUPS;
-      int pg = -1, pg_next = -1, stretch = 0;  // stretch: pg's first tile
-      int64_t off = 0, off_next = 0;  // of the group's first key
-      float ksl = 0.0f, ratio = 0.0f, ks_next = 0.0f, vs_next = 0.0f;
-      auto pages = [&](int j) {
-        const int key = key0 + j * KT + lane * 16;
-        pg_next = j + lane / GROUPS < n ? page_at(key) : -1;
-        off_next = (int64_t)sg.head * a.pool.head_stride + (int64_t)max(pg_next, 0) * a.pool.page_stride + (int64_t)(key & (PT - 1)) * tok;
-      };
-      auto ask_scales = [&]() {
-        ks_next = vs_next = 0.0f;
-        if (pg_next >= 0) {
-          ks_next = __ldg(a.pool.k_scale + ((int64_t)sg.head * a.pool.scale_head_stride + (int64_t)pg_next * a.pool.scale_page_stride));
-          vs_next = __ldg(a.pool.v_scale + ((int64_t)sg.head * a.pool.scale_head_stride + (int64_t)pg_next * a.pool.scale_page_stride));
-        }
-      };
-      auto turn = [&]() {  // to the next stretch
-        pg = pg_next;
-        off = off_next;
-        ksl = ks_next * a.scale_log2;
-        // a scale that is not finite makes the weights of the keys that are seen NaN
-        ratio = !(fabsf(vs_next) <= 3.402823466e38f) ? __int_as_float(0x7fc00000) : vtop > 0.0f ? __fdiv_rn(vs_next, vtop) * 128.0f : 0.0f;
-      };
-      // The bytes of tile j into its stage. What is not there is left as it lies: any
-      // byte is a finite value, and no row sees it.
-      auto ask = [&](int j) {
-        const int at = j % TL * GROUPS;
-        const uint32_t rs = (done + j) % RS;
-        uint64_t *const bar = raw_full + rs;
-        const uint32_t to = smem_at(raw) + rs * S::K_BYTES;
-        const int group = joined ? lane / 2 : lane % GROUPS;  // joined: a lane copies one group's keys or values
-        // (from the stretch after the present one where that has come)
-        const bool now = j / TL * TL <= stretch;
-        const int q = __shfl_sync(~0u, now ? pg : pg_next, (at + group) & 31);
-        const int64_t o = __shfl_sync(~0u, now ? off : off_next, (at + group) & 31);
-        const uint32_t there = 2 * __popc(__ballot_sync(~0u, (now ? pg : pg_next) >= 0) >> at & ((1u << GROUPS) - 1));
-        if (lane == 0)
-          asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_at(bar)), "r"(there * 16u * (uint32_t)D) : "memory");
-        __syncwarp();
-        if (joined) {
-          if (lane < 2 * GROUPS && q >= 0)
-            copy_bulk(to + ((lane & 1) * KT + group * 16) * D, (lane & 1 ? a.pool.v : a.pool.k) + o, 16 * D, bar);
-        } else {
-#pragma unroll 1
-          for (int i = lane; i < 2 * KT; i += 32) {  // one row a copy; GROUPS divides 32, so a lane keeps its group
-            const int kv = i / KT, row = i % KT / GROUPS;
-            if (q >= 0) copy_bulk(to + (kv * KT + group * 16 + row) * D, (kv ? a.pool.v : a.pool.k) + o + row * tok, D, bar);
-          }
-        }
-      };
       auto put = [&](uint8_t *to, const uint8_t *from) {
 #pragma unroll
         for (int i = 0; i < NI; i++) {
@@ -448,13 +497,6 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
           *reinterpret_cast<uint4 *>(to + to2 + i * (KPP * 128)) = first ? lo4 : hi4;
         }
       };
-      if (asks) {
-        pages(0);
-        ask_scales();
-        turn();
-        pages(TL);
-        for (int j = 0; j < RS && j < n; j++) ask(j);
-      }
       for (int j = 0; j < n; j++) {
         const uint32_t t = done + j, st = t % NS, rs = t % RS;
         if (!warp_wait(raw_full + rs, t / RS & 1, gone)) break;
@@ -464,33 +506,10 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
           put(ks + st * S::K_BYTES, from);
           put(vs + st * S::K_BYTES, from + KT * D);
         }
-        if (asks) {
-          const int at = j % TL * GROUPS;
-          if (at == 0 && j) {
-            turn();
-            stretch = j;
-            pages(j + TL);
-          }
-          if (j % TL == TL / 2) ask_scales();
-          float *mt = meta + st * META;
-          const uint32_t holes = __ballot_sync(~0u, pg < 0), odd = __ballot_sync(~0u, !(ksl >= 0.0f));
-          if (lane >= at && lane < at + GROUPS) {
-            mt[lane - at] = ksl;
-            mt[GROUPS + lane - at] = ratio;
-          }
-          if (lane == 0) {
-            mt[2 * GROUPS] = __int_as_float((int)(holes >> at & ((1u << GROUPS) - 1)));
-            mt[2 * GROUPS + 1] = __int_as_float((int)(odd >> at & ((1u << GROUPS) - 1)));
-          }
-        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) bar_arrive(kv_full + st);
         if (lane == 0) bar_arrive(raw_free + rs);  // this warp has read the bytes
-        if (asks && j + RS < n) {
-          if (!warp_wait(raw_free + rs, t / RS & 1, gone)) break;
-          ask(j + RS);
-        }
       }
     } else {
       // ---- weights ----
@@ -510,7 +529,7 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
           break;
         }
         tm_after();
-        const float *mt = meta + st * META;
+        const float *mt = meta + (done + j) % NM * META;
         const uint32_t holes = (uint32_t)__float_as_int(mt[2 * GROUPS]);
         const int key = key0 + j * KT;
         // With care: keys that some rows do not see, scales that are negative or no numbers.
