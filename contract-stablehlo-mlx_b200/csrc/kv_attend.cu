@@ -673,8 +673,8 @@ int launch_kv_attend(const AttendCall &c, int sms, cudaStream_t st) {
   a.group = group;
   a.slots = 0;
   a.causal = c.causal; a.window = c.window;
-  const int64_t per = 4;
-  a.out_wide = (uintptr_t)c.out % (4 * size) == 0 && c.out_token % per == 0 && c.out_head % per == 0;
+  auto out_by = [&](int v) { return (uintptr_t)c.out % (v * size) == 0 && c.out_token % v == 0 && c.out_head % v == 0; };
+  a.out_wide = out_by(8) ? 2 : out_by(4) ? 1 : 0;
   a.scale_log2 = c.scale * 1.44269504088896341f;
   a.page_shift = 31 - __builtin_clz((unsigned)c.pool.page_tokens);
   a.above = 0;

@@ -38,7 +38,7 @@ struct AttendArgs {
   int group;         // query heads a key/value head
   int slots;         // slots of the work list
   int causal, window;
-  int out_wide;      // out allows stores of four values
+  int out_wide;      // out allows stores of four values (1), of eight (2)
   int q_wide;        // q allows 16-byte loads
   float scale_log2;  // scale * log2(e)
   int page_shift;

@@ -637,19 +637,40 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
       tm_after();
       const bool whole = sg.take == sg.units;
       float *part = whole ? nullptr : partial_at<ROWS, DP>(a, blockIdx.x, sg.off == 0);
-      const float unscale = vtop * 0x1p-7f;
       if (ok) {
+        const int r = sg.t.row0 + min(row, sg.t.rows - 1);
+        __half *const to = static_cast<__half *>(a.out) + (int64_t)(sg.t.start + r / a.group) * a.out_token +
+                           (int64_t)(sg.head * a.group + r % a.group) * a.out_head;
+        float scale = vtop * 0x1p-7f;
+        if (whole) scale = l == 0.0f ? 0.0f : scale / l;
+        const bool empty = whole && l == 0.0f;  // a row that saw nothing: 0, whatever lies in O
 #pragma unroll 1
         for (int ch = 0; ch * 16 < D; ch++) {
           float v[16];
           tm_ld16(o_at + ch * 16, v);
           if (row < sg.t.rows) {
 #pragma unroll
-            for (int x = 0; x < 4; x++) {
-              const float4 r = make_float4(v[4 * x] * unscale, v[4 * x + 1] * unscale, v[4 * x + 2] * unscale, v[4 * x + 3] * unscale);
-              const int d = ch * 16 + 4 * x;
-              if (whole) write_out<__half>(a, sg.t, sg.head, row, d, r, l);
-              else *reinterpret_cast<float4 *>(part + row * DP + d) = r;
+            for (int x = 0; x < 16; x++) v[x] = empty ? 0.0f : v[x] * scale;
+            if (!whole) {
+#pragma unroll
+              for (int x = 0; x < 4; x++)
+                *reinterpret_cast<float4 *>(part + row * DP + ch * 16 + 4 * x) = make_float4(v[4 * x], v[4 * x + 1], v[4 * x + 2], v[4 * x + 3]);
+            } else {
+              __half2 h[8];
+#pragma unroll
+              for (int x = 0; x < 8; x++) h[x] = __floats2half2_rn(v[2 * x], v[2 * x + 1]);
+              if (a.out_wide == 2) {
+                uint4 w[2];
+                memcpy(w, h, 32);
+                *reinterpret_cast<uint4 *>(to + ch * 16) = w[0];
+                *reinterpret_cast<uint4 *>(to + ch * 16 + 8) = w[1];
+              } else {
+#pragma unroll
+                for (int x = 0; x < 8; x++) {
+                  to[ch * 16 + 2 * x] = h[x].x;
+                  to[ch * 16 + 2 * x + 1] = h[x].y;
+                }
+              }
             }
           }
         }
