@@ -22,7 +22,7 @@ struct KernelInfo {
   int n_inputs;     // binding order of StablehloMlx/Kernels/Shaders.lean
   int param_index;  // which input holds the parameter words
   int n_params;     // words read
-  uint8_t out_dtype;
+  uint8_t out_dtype;    // (kNumDTypes: the first input's)
 };
 
 const KernelInfo kKernels[] = {
@@ -43,6 +43,8 @@ const KernelInfo kKernels[] = {
     {"shlo_mul_mat_bias", KK_MUL_MAT_EP, 5, 4, 7, kF32},  // w, x, bias, residual, p = [mul_mat's six, flags]
     {"shlo_norm_affine", KK_NORM_AFFINE, 4, 3, 4, kF32},  // x, gamma, beta, p = [norm's four]
     {"shlo_attention", KK_ATTENTION, 4, 3, 5, kF32},      // q, k, v, p = [B, S, H, width, scale bits]
+    // Rotary positions (float16 or float32, the result of x's type):
+    {"shlo_rope", KK_ROPE, 4, 3, 6, kNumDTypes},          // x, positions, phases, p = [T, H, D, rot, flags, factor bits]
 };
 
 }  // namespace
@@ -270,8 +272,9 @@ int shlo_kernel_apply(shlo_kernel k, const shlo_arr *inputs, int n_inputs, const
   if (n_outputs != 1) return fail("kernel %s: one output expected", ki.name);
   for (int i = 0; i < n_inputs; i++)
     if (!inputs[i]) return fail("kernel %s: input %d is null", ki.name, i);
-  if (out_dtypes[0] != ki.out_dtype)
-    return fail("kernel %s: output dtype %s, %s expected", ki.name, dtype_name(out_dtypes[0]), dtype_name(ki.out_dtype));
+  const uint8_t out_dtype = ki.out_dtype == kNumDTypes ? inputs[0]->dtype : ki.out_dtype;
+  if (out_dtypes[0] != out_dtype)
+    return fail("kernel %s: output dtype %s, %s expected", ki.name, dtype_name(out_dtypes[0]), dtype_name(out_dtype));
   uint32_t p[8] = {0};
   SHLO_TRY(read_words(inputs[ki.param_index], p, ki.n_params));
   // The op log of a compiled function's recording (fusion.cu): in the capture
@@ -322,6 +325,7 @@ int shlo_kernel_apply(shlo_kernel k, const shlo_arr *inputs, int n_inputs, const
       case KK_MUL_MAT_EP: rc = k_mul_mat_ep(dev, in[0], in[1], p, in[2], in[3], (int)p[6], &o); break;
       case KK_NORM_AFFINE: rc = k_norm_affine(dev, in[0], p, in[1], in[2], &o); break;
       case KK_ATTENTION: rc = k_attention(dev, in[0], in[1], in[2], p, &o); break;
+      case KK_ROPE: rc = k_rope(dev, in[0], in[1], in[2], p, &o); break;
     }
   }
   for (Arr *a : in)

@@ -188,7 +188,7 @@ int device_wait(Device *dev, const char *what);
 // The kernels of shlo_kernel_apply, by name (api.cu's table).
 enum KernelKind {
   KK_MUL_MAT, KK_SOFT_MAX, KK_NORM, KK_SILU, KK_GELU_ERF, KK_ERFF_MAP, KK_DIVIDE, KK_SQRT, KK_F64_EW,
-  KK_F64_OF_F32, KK_F32_OF_F64, KK_MUL_MAT_EP, KK_NORM_AFFINE, KK_ATTENTION
+  KK_F64_OF_F32, KK_F32_OF_F64, KK_MUL_MAT_EP, KK_NORM_AFFINE, KK_ATTENTION, KK_ROPE
 };
 // mul_mat's fused epilogue (k_mul_mat_ep): + bias[m] (its own operand order),
 // then + res[r][m], then gelu_erf (the pinned build's).
@@ -273,6 +273,9 @@ int k_sqrt(Device *dev, Arr *a, const uint32_t *p, Arr **out);
 int k_f64_ew(Device *dev, Arr *a, Arr *b, const uint32_t *p, Arr **out);
 int k_f64_of_f32(Device *dev, Arr *a, const uint32_t *p, Arr **out);
 int k_f32_of_f64(Device *dev, Arr *a, const uint32_t *p, Arr **out);
+
+// ---- decoder operators (decode_arrays.cu) ----
+int k_rope(Device *dev, Arr *x, Arr *positions, Arr *phases, const uint32_t *p, Arr **out);
 
 // ---- built-ins (elementwise.cu) ----
 int op_unary(uint32_t op, Arr *a, Arr **out);

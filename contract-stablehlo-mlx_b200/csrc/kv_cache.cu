@@ -58,48 +58,49 @@ struct AppendArgs {
   int64_t xt[2], xh[2];
 };
 
-// 16 values of x as float (whole: every offset allows 16-byte loads).
+// 16 values of x as they come (WIDE: every offset allows 16-byte loads), kept so
+// between the passes: half the registers of floats for float16.
+template <typename T>
+struct Raw16 {
+  uint4 w[sizeof(T)];
+};
 template <typename T, bool WIDE>
-__device__ __forceinline__ void load16(const T *p, float (&f)[16]) {
+__device__ __forceinline__ void load16(const T *p, Raw16<T> &r) {
   if constexpr (WIDE) {
-    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int i = 0; i < 2; i++) {
-        const uint4 r = *reinterpret_cast<const uint4 *>(p + 8 * i);
-        const __half2 *h = reinterpret_cast<const __half2 *>(&r);
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const float2 g = __half22float2(h[j]);
-          f[8 * i + 2 * j] = g.x;
-          f[8 * i + 2 * j + 1] = g.y;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float4 r = *reinterpret_cast<const float4 *>(p + 4 * i);
-        f[4 * i] = r.x; f[4 * i + 1] = r.y; f[4 * i + 2] = r.z; f[4 * i + 3] = r.w;
-      }
-    }
+    for (int i = 0; i < (int)sizeof(T); i++) r.w[i] = *(reinterpret_cast<const uint4 *>(p) + i);
   } else {
+    T v[16];
 #pragma unroll
-    for (int i = 0; i < 16; i++) f[i] = (float)p[i];
+    for (int i = 0; i < 16; i++) v[i] = p[i];
+    memcpy(&r, v, sizeof r);
   }
+}
+template <typename T>
+__device__ __forceinline__ void floats16(const Raw16<T> &r, float (&f)[16]) {
+  T v[16];
+  memcpy(v, &r, sizeof r);
+#pragma unroll
+  for (int i = 0; i < 16; i++) f[i] = (float)v[i];
+}
+
+// round(x / s), the quotient rounded to binary32 first. x times the reciprocal is
+// within 2^-21 of the quotient relative (2^-14 at 127); away from a tie it
+// rounds to the same integer, near one the division decides.
+__device__ __forceinline__ float quantised(float x, float s, float inv) {
+  const float r = x * inv;
+  float q = rintf(r);
+  if (!(fabsf(fabsf(r - q) - 0.5f) > 0x1p-12f)) q = rintf(__fdiv_rn(x, s));
+  return fminf(fmaxf(q, -127.0f), 127.0f);
 }
 
 __device__ __forceinline__ uint4 pack16(const float (&f)[16], float s) {
-  uint32_t w[4];
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+  // s = 0: every value of the page is 0. s NaN: the page reads as NaN.
+  if (s > 0.0f) {
+    const float inv = __fdiv_rn(1.0f, s);  // (infinite for the smallest s: then the division decides)
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    uint32_t r = 0;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      // s = 0: every value of the page is 0. s NaN: the page reads as NaN.
-      float q = s > 0.0f ? rintf(__fdiv_rn(f[4 * i + j], s)) : 0.0f;
-      q = fminf(fmaxf(q, -127.0f), 127.0f);
-      r |= ((uint32_t)(int)q & 0xffu) << (8 * j);
-    }
-    w[i] = r;
+    for (int i = 0; i < 16; i++) w[i / 4] |= ((uint32_t)(int)quantised(f[i], s, inv) & 0xffu) << (8 * (i % 4));
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
@@ -128,10 +129,12 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const AppendArgs a
   float *scale = (z ? pool.v_scale : pool.k_scale) + (int64_t)page * pool.scale_page_stride + (int64_t)h * pool.scale_head_stride;
   const int old_n = p0 - page_of * PT;  // older tokens that stay in the page
 
-  float keep[kKeep][16];
+  Raw16<T> keep[kKeep];
   float most = 0.0f;
   bool bad = false;
-  auto scan = [&](const float (&f)[16]) {
+  auto scan = [&](const Raw16<T> &r) {
+    float f[16];
+    floats16(r, f);
 #pragma unroll
     for (int j = 0; j < 16; j++) {
       const float m = fabsf(f[j]);
@@ -142,15 +145,15 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const AppendArgs a
 #pragma unroll
   for (int k = 0; k < kKeep; k++) {
     const int i = threadIdx.x + k * kAppendThreads;
-    if (i < items) {
-      load16<T, WIDE>(x + (int64_t)(i / pieces) * a.xt[z] + (i % pieces) * 16, keep[k]);
-      scan(keep[k]);
-    }
+    if (i < items) load16<T, WIDE>(x + (int64_t)(i / pieces) * a.xt[z] + (i % pieces) * 16, keep[k]);
   }
+#pragma unroll
+  for (int k = 0; k < kKeep; k++)
+    if ((int)threadIdx.x + k * kAppendThreads < items) scan(keep[k]);
   for (int i = threadIdx.x + kKeep * kAppendThreads; i < items; i += kAppendThreads) {
-    float f[16];
-    load16<T, WIDE>(x + (int64_t)(i / pieces) * a.xt[z] + (i % pieces) * 16, f);
-    scan(f);
+    Raw16<T> r;
+    load16<T, WIDE>(x + (int64_t)(i / pieces) * a.xt[z] + (i % pieces) * 16, r);
+    scan(r);
   }
   __shared__ float red[kAppendThreads / 32];
   const float old_s = old_n ? *scale : 0.0f;
@@ -184,7 +187,9 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const AppendArgs a
       *p = r;
     }
   }
-  auto put = [&](int i, const float (&f)[16]) {
+  auto put = [&](int i, const Raw16<T> &r) {
+    float f[16];
+    floats16(r, f);
     *reinterpret_cast<uint4 *>(dst + (int64_t)(old_n + i / pieces) * pool.token_stride + (i % pieces) * 16) = pack16(f, s);
   };
 #pragma unroll
@@ -193,9 +198,9 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(const AppendArgs a
     if (i < items) put(i, keep[k]);
   }
   for (int i = threadIdx.x + kKeep * kAppendThreads; i < items; i += kAppendThreads) {
-    float f[16];
-    load16<T, WIDE>(x + (int64_t)(i / pieces) * a.xt[z] + (i % pieces) * 16, f);
-    put(i, f);
+    Raw16<T> r;
+    load16<T, WIDE>(x + (int64_t)(i / pieces) * a.xt[z] + (i % pieces) * 16, r);
+    put(i, r);
   }
 }
 
@@ -209,41 +214,51 @@ struct GatherArgs {
   int64_t yt[2], yh[2];
 };
 
-// V values a thread and step (16 bytes of output); items run over [row][head][piece].
+// A warp reads one token, keys and values, V values a lane and step (16 bytes of
+// output), four steps' loads on their way: the waits for the token's place and
+// page come once a token, not once a value.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) k_kv_gather(const GatherArgs a) {
   const shlo_kv_pool &pool = a.pool;
-  const int pieces = pool.head_dim / V, z = blockIdx.y;
-  const int row_items = pieces * pool.heads;
-  const int8_t *src = z ? pool.v : pool.k;
-  const float *scales = z ? pool.v_scale : pool.k_scale;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < a.n * row_items; i += (int64_t)gridDim.x * 256) {
-    const int64_t row = i / row_items;
-    const int r = (int)(i - row * row_items), h = r / pieces, d = (r - h * pieces) * V;
+  const int pieces = pool.head_dim / V, items = 2 * pieces * pool.heads, lane = threadIdx.x % 32;
+  for (int64_t row = (int64_t)blockIdx.x * 8 + threadIdx.x / 32; row < a.n; row += (int64_t)gridDim.x * 8) {
     const int s = __ldg(a.seq + row), at = __ldg(a.pos + row);
-    T y[V];
+    int page = -1;  // (a token that the tables do not hold reads as zeros)
+    if (s >= 0 && s < a.seqs && at >= 0 && at / pool.page_tokens < a.table_pages)
+      page = __ldg(a.tables + (int64_t)s * a.table_stride + at / pool.page_tokens);
+    const bool there = page >= 0 && page < pool.pages;
+    const int64_t base = (int64_t)page * pool.page_stride + (int64_t)(at % pool.page_tokens) * pool.token_stride;
+    for (int i0 = lane; i0 < items; i0 += 4 * 32) {
+      uint2 q[4];
+      float sc[4];
 #pragma unroll
-    for (int j = 0; j < V; j++) y[j] = (T)0.0f;
-    // A token that the tables do not hold reads as zeros.
-    if (s >= 0 && s < a.seqs && at >= 0 && at / pool.page_tokens < a.table_pages) {
-      const int page = __ldg(a.tables + (int64_t)s * a.table_stride + at / pool.page_tokens);
-      if (page >= 0 && page < pool.pages) {
-        const float sc = __ldg(scales + (int64_t)page * pool.scale_page_stride + (int64_t)h * pool.scale_head_stride);
-        const int8_t *p = src + (int64_t)page * pool.page_stride + (int64_t)h * pool.head_stride +
-                          (int64_t)(at % pool.page_tokens) * pool.token_stride + d;
-        int8_t q[V];
-        if constexpr (V == 8) *reinterpret_cast<uint2 *>(q) = *reinterpret_cast<const uint2 *>(p);
-        else *reinterpret_cast<uint32_t *>(q) = *reinterpret_cast<const uint32_t *>(p);
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-          const float f = (float)q[j] * sc;
-          if constexpr (sizeof(T) == 2) y[j] = __float2half_rn(f);
-          else y[j] = f;
+      for (int k = 0; k < 4; k++) {
+        const int i = i0 + k * 32, z = i >= items / 2, j = i - z * (items / 2), h = j / pieces, d = (j - h * pieces) * V;
+        q[k] = make_uint2(0u, 0u);
+        sc[k] = 0.0f;
+        if (there && i < items) {
+          const int8_t *p = (z ? pool.v : pool.k) + base + (int64_t)h * pool.head_stride + d;
+          if constexpr (V == 8) q[k] = __ldg(reinterpret_cast<const uint2 *>(p));
+          else q[k].x = __ldg(reinterpret_cast<const uint32_t *>(p));
+          sc[k] = __ldg((z ? pool.v_scale : pool.k_scale) + (int64_t)page * pool.scale_page_stride + (int64_t)h * pool.scale_head_stride);
         }
       }
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int i = i0 + k * 32, z = i >= items / 2, j = i - z * (items / 2), h = j / pieces, d = (j - h * pieces) * V;
+        if (i >= items) break;
+        T y[V];
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+          const float f = (float)(int8_t)((e < 4 ? q[k].x : q[k].y) >> (8 * (e % 4))) * sc[k];
+          if constexpr (sizeof(T) == 2) y[e] = __float2half_rn(f);
+          else y[e] = f;
+        }
+        uint4 w;
+        memcpy(&w, y, 16);
+        *reinterpret_cast<uint4 *>(static_cast<T *>(a.y[z]) + row * a.yt[z] + (int64_t)h * a.yh[z] + d) = w;
+      }
     }
-    T *dst = static_cast<T *>(a.y[z]) + row * a.yt[z] + (int64_t)h * a.yh[z] + d;
-    *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(y);
   }
 }
 
@@ -302,9 +317,8 @@ int launch_kv_gather(const shlo_kv_pool &p, const int32_t *tables, int64_t table
   a.n = n;
   a.y[0] = k; a.yt[0] = k_token; a.yh[0] = k_head;
   a.y[1] = v; a.yt[1] = v_token; a.yh[1] = v_head;
-  const int64_t items = n * (p.head_dim / per16) * p.heads;
-  const int64_t want = (items + 255) / 256, cap = (int64_t)sms * 16;
-  const dim3 grid((unsigned)(want < cap ? want : cap), 2);
+  const int64_t want = (n + 7) / 8, cap = (int64_t)sms * 8;
+  const unsigned grid = (unsigned)(want < cap ? want : cap);
   if (dtype == kF16) k_kv_gather<__half, 8><<<grid, 256, 0, st>>>(a);
   else k_kv_gather<float, 4><<<grid, 256, 0, st>>>(a);
   return launch_check("kv_gather");

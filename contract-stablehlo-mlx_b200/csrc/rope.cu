@@ -86,41 +86,58 @@ __global__ void __launch_bounds__(kRopeThreads) k_rope(const RopeArgs a) {
   // (token, head, unit) of this thread's items, kRopeThreads apart
   const int dh = kRopeThreads / units, du = kRopeThreads - dh * units;
   int h = threadIdx.x / units, u = threadIdx.x - h * units, t = 0;
-  for (;;) {
-    while (h >= nh) {
-      h -= nh;
-      t++;
-    }
-    if (t >= nt) break;
-    const T *x = static_cast<const T *>(a.x) + (t0 + t) * a.xt + (h0 + h) * a.xh;
-    T *y = static_cast<T *>(a.y) + (t0 + t) * a.yt + (h0 + h) * a.yh;
-    if (u < ru) {
-      const int o1 = INTER ? 2 * VEC * u : VEC * u, o2 = INTER ? o1 + VEC : o1 + half;
-      T v[2][VEC];
-      load_vec<T, VEC>(x + o1, v[0]);
-      load_vec<T, VEC>(x + o2, v[1]);
+  // Several items' loads go out before the first is stored: a block's life is a
+  // few waits for memory, not one an item.
+  constexpr int AT_ONCE = 3;
+  while (t < nt) {
+    T v[AT_ONCE][2][VEC];
+    T *y[AT_ONCE];
+    int tab[AT_ONCE];  // where the unit's cosines begin; -1: copied; -2: nothing
+    int o2[AT_ONCE];
 #pragma unroll
-      for (int j = 0; j < VEC; j++) {
-        const int at = t * half + (j / PART) * (ru * PART) + u * PART + j % PART;
-        const float c = cs[at], s = sn[at];
-        T &lo = INTER ? v[(2 * j) / VEC][(2 * j) % VEC] : v[0][j];
-        T &hi = INTER ? v[(2 * j + 1) / VEC][(2 * j + 1) % VEC] : v[1][j];
-        const float p = to_f32(lo), q = to_f32(hi);
-        of_f32(lo, __fmaf_rn(p, c, -(q * s)));
-        of_f32(hi, __fmaf_rn(q, c, p * s));
+    for (int k = 0; k < AT_ONCE; k++) {
+      while (h >= nh) {
+        h -= nh;
+        t++;
       }
-      store_vec<T, VEC>(y + o1, v[0]);
-      store_vec<T, VEC>(y + o2, v[1]);
-    } else {
-      T v[VEC];
-      load_vec<T, VEC>(x + a.rot + (u - ru) * VEC, v);
-      store_vec<T, VEC>(y + a.rot + (u - ru) * VEC, v);
+      tab[k] = -2;
+      if (t < nt) {
+        const T *x = static_cast<const T *>(a.x) + (t0 + t) * a.xt + (h0 + h) * a.xh;
+        y[k] = static_cast<T *>(a.y) + (t0 + t) * a.yt + (h0 + h) * a.yh;
+        const int o = u < ru ? (INTER ? 2 * VEC : VEC) * u : a.rot + (u - ru) * VEC;
+        load_vec<T, VEC>(x + o, v[k][0]);
+        y[k] += o;
+        tab[k] = -1;
+        if (u < ru) {
+          tab[k] = t * half + u * PART;
+          o2[k] = INTER ? VEC : half;
+          load_vec<T, VEC>(x + o + o2[k], v[k][1]);
+        }
+      }
+      u += du;
+      h += dh;
+      if (u >= units) {
+        u -= units;
+        h++;
+      }
     }
-    u += du;
-    h += dh;
-    if (u >= units) {
-      u -= units;
-      h++;
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; k++) {
+      if (tab[k] == -2) break;
+      if (tab[k] >= 0) {
+#pragma unroll
+        for (int j = 0; j < VEC; j++) {
+          const int at = tab[k] + (j / PART) * (ru * PART) + j % PART;
+          const float c = cs[at], s = sn[at];
+          T &lo = INTER ? v[k][(2 * j) / VEC][(2 * j) % VEC] : v[k][0][j];
+          T &hi = INTER ? v[k][(2 * j + 1) / VEC][(2 * j + 1) % VEC] : v[k][1][j];
+          const float p = to_f32(lo), q = to_f32(hi);
+          of_f32(lo, __fmaf_rn(p, c, -(q * s)));
+          of_f32(hi, __fmaf_rn(q, c, p * s));
+        }
+        store_vec<T, VEC>(y[k] + o2[k], v[k][1]);
+      }
+      store_vec<T, VEC>(y[k], v[k][0]);
     }
   }
 }
@@ -222,8 +239,8 @@ int shlo_rope_phases(int32_t rot, double base, int32_t scaling, double by, doubl
       // Pairs that turn at least `fast` times over the trained positions keep
       // their frequency, those under `slow` turns are slowed `by` times; a
       // ramp in the pair's index between the two (bounds rounded outward).
-      auto at = [&](double turns) { return rot * logl(trained / (turns * two_pi)) / (2.0L * logl(base)); };
-      long double lo = floorl(at(fast)), hi = ceill(at(slow));
+      const long double per = rot / (2.0L * logl((long double)base));
+      long double lo = floorl(per * logl(trained / (fast * two_pi))), hi = ceill(per * logl(trained / (slow * two_pi)));
       if (lo < 0) lo = 0;
       if (hi > rot - 1) hi = rot - 1;
       long double width = hi - lo;

@@ -18,6 +18,7 @@ SYMBOLS = [
     "shlo_count_nonzero", "shlo_current_stream", "shlo_launch_count", "shlo_device_ptr", "shlo_mul_mat_noalloc",
     "shlo_rope_phases", "shlo_rope_noalloc", "shlo_kv_append_noalloc", "shlo_kv_gather_noalloc",
     "shlo_kv_attend_workspace", "shlo_kv_attend_noalloc",
+    "shlo_kv_new", "shlo_kv_free", "shlo_kv_storage", "shlo_kv_append", "shlo_kv_gather", "shlo_kv_attend",
 ]
 
 
@@ -124,7 +125,16 @@ def load() -> ctypes.CDLL:
     L.shlo_kv_attend_workspace.argtypes = [ctypes.POINTER(ctypes.c_size_t)]
     L.shlo_kv_attend_noalloc.argtypes = [pool, batch, p, i64, i64, i32, u8, f32, i32, i32, p, i64, i64, p, p,
                                          ctypes.c_size_t, p]
-    special = {"shlo_last_error", "shlo_empty", "shlo_retain", "shlo_release", "shlo_kernel_free", "shlo_fn_free"}
+    L.shlo_kv_new.argtypes = [i64, i32, i32, i32, ctypes.POINTER(p)]
+    L.shlo_kv_free.argtypes = [p]
+    L.shlo_kv_free.restype = None
+    L.shlo_kv_storage.argtypes = [p, pool]
+    L.shlo_kv_append.argtypes = [p, c_arr, c_arr, c_arr, c_arr, c_arr]
+    L.shlo_kv_gather.argtypes = [p, c_arr, c_arr, c_arr, u8, ctypes.POINTER(c_arr), ctypes.POINTER(c_arr)]
+    L.shlo_kv_attend.argtypes = [p, c_arr, c_arr, c_arr, c_arr, f32, i32, i32, ctypes.POINTER(c_arr),
+                                 ctypes.POINTER(c_arr)]
+    special = {"shlo_last_error", "shlo_empty", "shlo_retain", "shlo_release", "shlo_kernel_free", "shlo_fn_free",
+               "shlo_kv_free"}
     for name in SYMBOLS:
         if name not in special:
             getattr(L, name).restype = ctypes.c_int

@@ -14,6 +14,7 @@ import ctypes
 import numpy as np
 
 from . import mlx as M
+from . import run as Run
 from ._lib import KvBatch, KvPool, ShloError, check, load
 
 SCALINGS = {"none": 0, "linear": 1, "base": 2, "ramp": 3, "blend": 4}
@@ -165,3 +166,58 @@ def attend_noalloc(pool: Pool, q, starts, lens, tables, out, *, workspace, scale
     check(load().shlo_kv_attend_noalloc(c, _batch(starts, lens, tables, t), q.data_ptr(), qs[0], qs[1], h, dt, scale,
                                         1 if causal else 0, window, out.data_ptr(), os_[0], os_[1], lp,
                                         workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream))
+
+
+# ---- on arrays (mlx.Arr), in the library's own memory ----
+
+def rope(x: M.Arr, positions: M.Arr, phases: M.Arr, *, interleaved=False, inverse=False, factor=1.0) -> M.Arr:
+    """x [tokens, heads, dim] turned by positions (int32 [tokens]); phases: rope_phases' as an int64 array. May be
+    called inside a compiled function."""
+    t, h, d = M.shape(x)
+    words = [t, h, d, 2 * M.shape(phases)[0], (1 if interleaved else 0) | (2 if inverse else 0),
+             int(np.array([factor], np.float32).view(np.uint32)[0])]
+    return M.kernel_apply(Run.kernel("rope"), [x, positions, phases, Run.params(words)], [[t, h, d]],
+                          bytes([M.dtype(x)]), [max(t, 1), 1, 1], [64, 1, 1])[0]
+
+
+class Cache:
+    """A paged key/value cache in 8 bits in the library's memory (shlo_kv_new). Which pages a sequence has is the
+    caller's to say, in the tables; not for compiled functions."""
+
+    __slots__ = ("h", "heads", "head_dim", "page_tokens", "pages")
+
+    def __init__(self, pages: int, heads: int, head_dim: int, page_tokens: int = 64):
+        h = ctypes.c_void_p()
+        check(load().shlo_kv_new(pages, heads, head_dim, page_tokens, ctypes.byref(h)))
+        self.h = h.value
+        self.pages, self.heads, self.head_dim, self.page_tokens = pages, heads, head_dim, page_tokens
+
+    def __del__(self):
+        h = getattr(self, "h", None)
+        if h:
+            try:
+                load().shlo_kv_free(h)
+            except Exception:
+                pass
+            self.h = None
+
+    def storage(self) -> KvPool:
+        p = KvPool()
+        check(load().shlo_kv_storage(self.h, p))
+        return p
+
+    def append(self, k: M.Arr, v: M.Arr, starts: M.Arr, lens: M.Arr, tables: M.Arr) -> None:
+        check(load().shlo_kv_append(self.h, k.h, v.h, starts.h, lens.h, tables.h))
+
+    def gather(self, tables: M.Arr, seq: M.Arr, pos: M.Arr, dtype: int = M.dtF32):
+        k, v = ctypes.c_void_p(), ctypes.c_void_p()
+        check(load().shlo_kv_gather(self.h, tables.h, seq.h, pos.h, dtype, ctypes.byref(k), ctypes.byref(v)))
+        return M.Arr(k.value), M.Arr(v.value)
+
+    def attend(self, q: M.Arr, starts: M.Arr, lens: M.Arr, tables: M.Arr, *, scale: float, causal=True, window=0,
+               lse=False):
+        """The attention's result, or (result, lse)."""
+        o, l = ctypes.c_void_p(), ctypes.c_void_p()
+        check(load().shlo_kv_attend(self.h, q.h, starts.h, lens.h, tables.h, scale, 1 if causal else 0, window,
+                                    ctypes.byref(o), ctypes.byref(l) if lse else None))
+        return (M.Arr(o.value), M.Arr(l.value)) if lse else M.Arr(o.value)

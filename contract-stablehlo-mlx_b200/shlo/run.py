@@ -36,6 +36,7 @@ FUSED = {
     "mul_mat_bias": (["w", "x", "bias", "res", "p"], ["y"]),
     "norm_affine": (["x", "gamma", "beta", "p"], ["y"]),
     "attention": (["q", "k", "v", "p"], ["y"]),
+    "rope": (["x", "positions", "phases", "p"], ["y"]),
 }
 EP_BIAS, EP_BIAS_LHS, EP_RES, EP_RES_LHS, EP_GELU = 1, 2, 4, 8, 16
 

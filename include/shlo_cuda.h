@@ -274,6 +274,32 @@ int shlo_kv_attend_noalloc(const shlo_kv_pool *pool, const shlo_kv_batch *batch,
                            void *out, int64_t out_token, int64_t out_head, float *lse, void *workspace,
                            size_t workspace_bytes, void *stream);
 
+/* ---- the decoder operators on arrays ----
+   Rotary positions are the kernel "shlo_rope" (shlo_kernel_new, shlo_kernel_apply):
+   inputs x [T, H, D], positions int32 [T], phases int64 [rot / 2] and the
+   parameter words [T, H, D, rot, flags, factor bits], as shlo_rope_noalloc's; the
+   result is of x's type. A cache is a handle, since it changes in place; its work
+   is on the device's stream (shlo_current_stream), and it is refused inside a
+   compiled function, whose replays work on private copies. Activations are
+   [tokens, heads, dim] arrays of float16 or float32 (strided views are read in
+   place where a head's values are contiguous), starts, lens and tables int32
+   arrays [seqs + 1], [seqs] and [seqs, table_pages]. */
+typedef struct shlo_kv_s *shlo_kv;
+/* A cache of the library's own storage on the current device, all zeros. */
+int shlo_kv_new(int64_t pages, int32_t heads, int32_t head_dim, int32_t page_tokens, shlo_kv *out);
+/* Drops it; the storage returns to the library's pool in stream order. */
+void shlo_kv_free(shlo_kv kv);
+/* Where its values and scales lie, for copying pages or for the *_noalloc
+   functions; valid until it is freed. */
+int shlo_kv_storage(shlo_kv kv, shlo_kv_pool *pool);
+int shlo_kv_append(shlo_kv kv, shlo_arr k, shlo_arr v, shlo_arr starts, shlo_arr lens, shlo_arr tables);
+/* New arrays [n, heads, head_dim] of `dtype`. */
+int shlo_kv_gather(shlo_kv kv, shlo_arr tables, shlo_arr seq, shlo_arr pos, uint8_t dtype, shlo_arr *k, shlo_arr *v);
+/* A new array of q's shape and type, and of the logarithms [tokens, query heads]
+   where `lse` is not NULL; rows that no sequence has are 0. */
+int shlo_kv_attend(shlo_kv kv, shlo_arr q, shlo_arr starts, shlo_arr lens, shlo_arr tables, float scale, int32_t causal,
+                   int32_t window, shlo_arr *out, shlo_arr *lse);
+
 /* ---- test-driver helpers (Mlx.lean:69-73) ---- */
 
 /* smlx_libm_erff_range: this platform's binary32 erff over `count`
