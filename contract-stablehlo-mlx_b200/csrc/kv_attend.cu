@@ -360,6 +360,9 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DP, NT>::PER_SM) k_kv_atten
         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
           for (int j = 0; j < 4; j++) s[mt][nt][j] = 0.0f;
+      // float32's second terms are summed apart: the matrix instructions cut off what
+      // falls below a sum's last bit.
+      float s2[MT][NT][4] = {};
       uint4 kr[MT][2], b[TERMS][NT];
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) {
@@ -384,8 +387,16 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DP, NT>::PER_SM) k_kv_atten
           for (int tm = 0; tm < TERMS; tm++)
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
-              mma16816(s[mt][nt], af, ks % 2 ? b[tm][nt].z : b[tm][nt].x, ks % 2 ? b[tm][nt].w : b[tm][nt].y);
+              mma16816(tm == 0 ? s[mt][nt] : s2[mt][nt], af, ks % 2 ? b[tm][nt].z : b[tm][nt].x, ks % 2 ? b[tm][nt].w : b[tm][nt].y);
         }
+      }
+      if constexpr (TERMS == 2) {
+#pragma unroll
+        for (int mt = 0; mt < MT; mt++)
+#pragma unroll
+          for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) s[mt][nt][j] += s2[mt][nt][j];
       }
       // The piece R on takes the place of these (none past the segment: its end
       // leaves nothing on the way that could land on the next one's pieces).
@@ -516,13 +527,30 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DP, NT>::PER_SM) k_kv_atten
           const uint32_t a23 = __byte_perm(x2, x3, 0x5140), b23 = __byte_perm(x2, x3, 0x7362);
           const uint32_t f0[4] = {half_pair<0x4140>(a01), half_pair<0x4342>(a01), half_pair<0x4140>(a23), half_pair<0x4342>(a23)};
           const uint32_t f1[4] = {half_pair<0x4140>(b01), half_pair<0x4342>(b01), half_pair<0x4140>(b23), half_pair<0x4342>(b23)};
-#pragma unroll
-          for (int tm = 0; tm < TERMS; tm++)
+          if constexpr (TERMS == 1) {
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
-              mma16816(o[nt][2 * w], f0, pb[tm][nt][0], pb[tm][nt][1]);
-              mma16816(o[nt][2 * w + 1], f1, pb[tm][nt][0], pb[tm][nt][1]);
+              mma16816(o[nt][2 * w], f0, pb[0][nt][0], pb[0][nt][1]);
+              mma16816(o[nt][2 * w + 1], f1, pb[0][nt][0], pb[0][nt][1]);
             }
+          } else {
+            // Over thousands of keys the instructions' cut-off bits would add up (they
+            // all point one way): sixteen keys' sums are added to O by rounding adds.
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+              float t0[4] = {}, t1[4] = {};
+#pragma unroll
+              for (int tm = TERMS - 1; tm >= 0; tm--) {
+                mma16816(t0, f0, pb[tm][nt][0], pb[tm][nt][1]);
+                mma16816(t1, f1, pb[tm][nt][0], pb[tm][nt][1]);
+              }
+#pragma unroll
+              for (int j = 0; j < 4; j++) {
+                o[nt][2 * w][j] += t0[j];
+                o[nt][2 * w + 1][j] += t1[j];
+              }
+            }
+          }
         }
       }
       refill((R + 1) / 2, R % 2 == 1);

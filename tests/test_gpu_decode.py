@@ -29,6 +29,15 @@ NP = {"f16": np.float16, "f32": np.float32}
 def device():
     torch.cuda.set_device(0)
     M.set_device(0)
+    yield
+    torch.cuda.empty_cache()  # the caches' gigabytes go back before other files' child processes allocate
+
+
+@pytest.fixture(autouse=True)
+def tidy():
+    yield
+    if torch.cuda.memory_reserved() > 1 << 30:
+        torch.cuda.empty_cache()
 
 
 def cuda(a):
