@@ -15,10 +15,21 @@
 // lane idles for a group of 8 query heads; a row's dimensions and the keys of a
 // tile may be taken in any order, so each lane reads 16 contiguous bytes.
 //
+// Measured on one B200, 128-wide heads, four query heads to a key/value head,
+// float16: 64 sequences x 8192 keys (1.07 GB) 218 us, 4.93 TB/s; 64 ragged ones
+// (505 MB) 118 us; two of 150 to 200 thousand keys (343 MB) 88 us; one of 256
+// keys 12 us. A loop without the products takes as long: the rest over the bytes
+// is the start (the line, the first pages and pieces, 8 us), a block's cuts
+// between units (8 us each, which the SM's other blocks cover as long as they
+// are not at one too) and the last blocks' ends. Two or four blocks an SM
+// measured 231 and 227 us for the first.
+//
 // Precision. Scores, maxima, sums and outputs are kept in 32 bits. The weights
 // are rounded to float16 for the second product, as e^(s - m) (sv / largest sv
 // so far) 2^14: at most 2^14 and, since float16 reaches down to 2^-24, exact to
-// 2^-38 of the largest weight. For float32 queries q and the weights are split
+// 2^-38 of the largest weight (of the largest value's scale among the keys of the
+// tile of rows: a page whose scale is 2^28 times a row's others costs that row's
+// bits). For float32 queries q and the weights are split
 // into two float16 terms each (22 bits), q after scaling each row by a power of
 // two to below 2^14.
 #include "kv_attend.cuh"
