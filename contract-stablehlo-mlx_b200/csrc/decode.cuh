@@ -50,7 +50,7 @@ struct AttendCall {
   int *err;  // the device's word for launches that gave up a wait
 };
 size_t attend_work_bytes(int sms);
-int launch_kv_attend(const AttendCall &c, int sms, cudaStream_t st);
+int launch_kv_attend(const AttendCall &c, int sms, int device, cudaStream_t st);
 
 // The new tokens of sequence s and its length, with the caller's arrays held
 // to the batch: starts to [0, tokens], the length to 0 and above. `starts` and

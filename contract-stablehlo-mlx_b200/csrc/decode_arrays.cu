@@ -258,7 +258,7 @@ int shlo_kv_attend(shlo_kv kv, shlo_arr q, shlo_arr starts, shlo_arr lens, shlo_
   c.work = work->ptr;
   c.work_bytes = work->bytes;
   c.err = kv->dev->pipe_err_dev;
-  SHLO_TRY(launch_kv_attend(c, kv->dev->sm_count, kv->dev->stream));
+  SHLO_TRY(launch_kv_attend(c, kv->dev->sm_count, kv->dev->id, kv->dev->stream));
   shlo_retain(o);
   *out = o;
   if (l) {

@@ -634,12 +634,13 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DP, NT>::PER_SM) k_kv_atten
 }
 
 template <typename T, int DP, int NT>
-int launch_rows(AttendArgs a, int sms, cudaStream_t st) {
+int launch_rows(AttendArgs a, int sms, int device, cudaStream_t st) {
   using S = Shape<T, DP, NT>;
   constexpr size_t smem = S::WORDS * 4;
   static_assert((smem + 1024) * S::PER_SM <= 228 * 1024, "blocks of an SM");
   auto *kern = k_kv_attend_rows<T, DP, NT>;
-  if (smem > 48 * 1024) SHLO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  static std::atomic<uint64_t> allowed{0};
+  SHLO_TRY(allow_smem((const void *)kern, smem, allowed, device));
   a.slots = (int)(((int64_t)a.batch.tokens * a.group) / S::ROWS + a.batch.seqs);
   // No more blocks than granules there can be.
   const int64_t room = ((int64_t)a.batch.table_pages << a.page_shift) / S::GRAN + 1;
@@ -654,15 +655,15 @@ int launch_rows(AttendArgs a, int sms, cudaStream_t st) {
 }
 
 template <typename T>
-int dispatch_rows(const AttendArgs &a, int nt, int sms, cudaStream_t st) {
+int dispatch_rows(const AttendArgs &a, int nt, int sms, int device, cudaStream_t st) {
   const int D = a.pool.head_dim;
   if (nt == 1 || D > 128) {
-    if (D <= 64) return launch_rows<T, 64, 1>(a, sms, st);
-    if (D <= 128) return launch_rows<T, 128, 1>(a, sms, st);
-    return launch_rows<T, 256, 1>(a, sms, st);
+    if (D <= 64) return launch_rows<T, 64, 1>(a, sms, device, st);
+    if (D <= 128) return launch_rows<T, 128, 1>(a, sms, device, st);
+    return launch_rows<T, 256, 1>(a, sms, device, st);
   }
-  if (D <= 64) return launch_rows<T, 64, 2>(a, sms, st);
-  return launch_rows<T, 128, 2>(a, sms, st);
+  if (D <= 64) return launch_rows<T, 64, 2>(a, sms, device, st);
+  return launch_rows<T, 128, 2>(a, sms, device, st);
 }
 
 constexpr size_t kCounterBytes = 2 * kAttendMaxBlocks * sizeof(unsigned);
@@ -687,7 +688,7 @@ size_t attend_work_bytes(int sms) {
   return kCounterBytes + (tiles > most ? tiles : most);
 }
 
-int launch_kv_attend(const AttendCall &c, int sms, cudaStream_t st) {
+int launch_kv_attend(const AttendCall &c, int sms, int device, cudaStream_t st) {
   SHLO_TRY(check_pool(&c.pool, "kv_attend"));
   SHLO_TRY(check_batch(&c.batch, "kv_attend"));
   if (c.dtype != kF16 && c.dtype != kF32) return fail("kv_attend: %s not carried (float16 or float32)", dtype_name(c.dtype));
@@ -729,12 +730,12 @@ int launch_kv_attend(const AttendCall &c, int sms, cudaStream_t st) {
   const int nt = rows <= (int64_t)8 * c.batch.seqs ? 1 : 2;
   if (c.dtype == kF16 && rows > (int64_t)16 * c.batch.seqs) {
     AttendArgs big = a;
-    big.above = 16;
-    SHLO_TRY(launch_attend_tiles(big, sms, st));
+    if (c.batch.seqs > 1) big.above = 16;  // (one sequence: one launch, whatever rows of q are its own)
+    SHLO_TRY(launch_attend_tiles(big, sms, device, st));
     if (c.batch.seqs == 1) return 0;
     a.upto = 16;
   }
-  return c.dtype == kF16 ? dispatch_rows<__half>(a, nt, sms, st) : dispatch_rows<float>(a, nt, sms, st);
+  return c.dtype == kF16 ? dispatch_rows<__half>(a, nt, sms, device, st) : dispatch_rows<float>(a, nt, sms, device, st);
 }
 
 }  // namespace shlo
@@ -760,7 +761,7 @@ int shlo_kv_attend_noalloc(const shlo_kv_pool *pool, const shlo_kv_batch *batch,
   SHLO_TRY(current_device(&dev));
   AttendCall c{*pool, *batch, q, q_token, q_head, out, out_token, out_head, lse, heads, dtype, scale, causal != 0, window,
                workspace, workspace_bytes, dev->pipe_err_dev};
-  return launch_kv_attend(c, dev->sm_count, (cudaStream_t)stream);
+  return launch_kv_attend(c, dev->sm_count, dev->id, (cudaStream_t)stream);
 }
 
 }  // extern "C"

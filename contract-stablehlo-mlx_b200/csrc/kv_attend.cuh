@@ -55,8 +55,18 @@ constexpr int kAttendMaxBlocks = 1024;
 template <int ROWS> constexpr int kJoin = ROWS >= 128 ? 32 : 64;
 template <int ROWS> constexpr int kRowShift = ROWS == 8 ? 3 : ROWS == 16 ? 4 : ROWS == 128 ? 7 : 8;
 
+// A kernel's dynamic shared memory, allowed once a device: `done` is the launch's
+// own bits (the call itself would be a tenth of a small launch).
+inline int allow_smem(const void *kern, size_t bytes, std::atomic<uint64_t> &done, int device) {
+  const uint64_t bit = (uint64_t)1 << device;
+  if (done.load(std::memory_order_relaxed) & bit) return 0;
+  SHLO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  done.fetch_or(bit);
+  return 0;
+}
+
 // kv_attend_tiles.cu: tiles of 256 rows (128 of heads wider than 128), float16.
-int launch_attend_tiles(const AttendArgs &a, int sms, cudaStream_t st);
+int launch_attend_tiles(const AttendArgs &a, int sms, int device, cudaStream_t st);
 size_t attend_tiles_partial_bytes(int sms);
 
 // A tile of rows and what it sees.

@@ -712,10 +712,11 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
 constexpr int kMinGranules = 4;
 
 template <int DP>
-int launch(AttendArgs a, int sms, cudaStream_t st) {
+int launch(AttendArgs a, int sms, int device, cudaStream_t st) {
   using S = Tiles<DP>;
   auto *kern = k_kv_attend_tiles<DP>;
-  SHLO_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
+  static std::atomic<uint64_t> allowed{0};
+  SHLO_TRY(allow_smem((const void *)kern, S::BYTES, allowed, device));
   a.slots = (int)(((int64_t)a.batch.tokens * a.group) / S::ROWS + a.batch.seqs);
   const int64_t room = ((int64_t)a.batch.table_pages << a.page_shift) / S::KT + 1;
   int64_t most = (int64_t)a.slots * a.pool.heads;
@@ -736,11 +737,11 @@ size_t attend_tiles_partial_bytes(int sms) {
   return blocks * 2 * rows * 4;
 }
 
-int launch_attend_tiles(const AttendArgs &a, int sms, cudaStream_t st) {
+int launch_attend_tiles(const AttendArgs &a, int sms, int device, cudaStream_t st) {
   const int D = a.pool.head_dim;
-  if (D <= 64) return launch<64>(a, sms, st);
-  if (D <= 128) return launch<128>(a, sms, st);
-  return launch<256>(a, sms, st);
+  if (D <= 64) return launch<64>(a, sms, device, st);
+  if (D <= 128) return launch<128>(a, sms, device, st);
+  return launch<256>(a, sms, device, st);
 }
 
 }  // namespace shlo

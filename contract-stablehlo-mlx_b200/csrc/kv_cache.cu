@@ -46,6 +46,7 @@ int check_batch(const shlo_kv_batch *b, const char *what) {
     return fail("%s: %d sequences, %d tokens, tables of %d pages", what, b->seqs, b->tokens, b->table_pages);
   if (b->seqs > (1 << 20) || b->tokens > (1 << 28)) return fail("%s: %d sequences (at most 2^20), %d tokens (at most 2^28)", what, b->seqs, b->tokens);
   if (b->seqs && (!b->starts || !b->lens || (b->table_pages && !b->tables))) return fail("%s: null pointer in the batch", what);
+  if (((uintptr_t)b->starts | (uintptr_t)b->lens | (uintptr_t)b->tables) % 4) return fail("%s: misaligned starts, lens or tables", what);
   if (b->table_pages > (1 << 22)) return fail("%s: tables of %d pages (at most 2^22)", what, b->table_pages);
   return 0;
 }
@@ -324,6 +325,7 @@ int launch_kv_gather(const shlo_kv_pool &p, const int32_t *tables, int64_t table
   if (n < 0 || seqs < 0 || table_pages < 0) return fail("kv_gather: %lld tokens of %d sequences", (long long)n, seqs);
   if (n == 0) return 0;
   if (!seq || !pos || !k || !v || (seqs && table_pages && !tables)) return fail("kv_gather: null pointer");
+  if (((uintptr_t)seq | (uintptr_t)pos | (uintptr_t)tables) % 4) return fail("kv_gather: misaligned tables, seq or pos");
   const int64_t per16 = (int64_t)(16 / dtype_size(dtype));
   if (((uintptr_t)k | (uintptr_t)v) % 16 || k_token % per16 || k_head % per16 || v_token % per16 || v_head % per16)
     return fail("kv_gather: the outputs' pointers and strides are multiples of 16 bytes");

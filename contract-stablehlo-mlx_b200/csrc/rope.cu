@@ -164,6 +164,7 @@ int launch_rope(const RopeCall &c, int sms, cudaStream_t st) {
   if (c.tokens > 0x7fffffff) return fail("rope: %lld tokens, at most 2^31 - 1", (long long)c.tokens);
   const size_t size = dtype_size(c.dtype);
   if (((uintptr_t)c.x | (uintptr_t)c.y) % size) return fail("rope: x or y is not aligned to its type");
+  if ((uintptr_t)c.positions % 4 || (uintptr_t)c.phases % 8) return fail("rope: misaligned positions or phases");
   const bool same = c.x == c.y;
   if (same && (c.x_token != c.y_token || c.x_head != c.y_head))
     return fail("rope: x and y share storage with different strides");

@@ -407,8 +407,8 @@ static int wait_stream(Device *dev, cudaStream_t stream, const char *what) {
       volatile int *perr = dev->pipe_err_host;
       if (perr && *perr) {
         *perr = 0;
-        return fail("%s: a mul_mat launch on device %d gave up waiting for its stage copies (the results are "
-                    "not valid)", what, dev->id);
+        return fail("%s: a launch on device %d gave up waiting for its own copies or products (the results "
+                    "are not valid)", what, dev->id);
       }
       return 0;
     }

@@ -2,8 +2,8 @@
 the attention that reads it, for hosts that generate token by token.
 
 The *_noalloc functions take device tensors of the caller's own -- objects with
-data_ptr(), shape, stride(), dtype, numel(), element_size() and is_contiguous(), as a
-torch.Tensor has them; nothing here imports torch -- and queue their work on `stream` (a cudaStream_t as
+data_ptr(), shape, stride(), dtype, is_cuda, numel(), element_size() and is_contiguous(), as
+a torch.Tensor has them; nothing here imports torch -- and queue their work on `stream` (a cudaStream_t as
 an integer; 0 is the default stream). They allocate nothing. Every one is one call
 of include/shlo_cuda.h, whose comments say what it computes; errors raise ShloError.
 """
@@ -21,10 +21,13 @@ SCALINGS = {"none": 0, "linear": 1, "base": 2, "ramp": 3, "blend": 4}
 
 _NAMES = {"torch.float16": M.dtF16, "torch.float32": M.dtF32, "torch.int32": M.dtI32, "torch.int64": M.dtI64,
           "torch.int8": M.dtI8}
+_F16, _F32, _I8, _I32, _I64 = M.dtF16, M.dtF32, M.dtI8, M.dtI32, M.dtI64
 _codes: dict = {}  # a dtype object seen before -> its code (None: not carried)
 
 
 def _code(x):
+    if not x.is_cuda:
+        raise ShloError("a tensor in host memory: the decoder operators take device memory")
     d = x.dtype
     try:
         return _codes[d]
@@ -47,7 +50,7 @@ def rope_phases(rot: int, base: float = 10000.0, scaling: str = "none", by: floa
 def _rows(x, what):
     """A float [tokens, heads, dim] whose last axis is contiguous: (shape, strides, type code)."""
     c, n, s = _code(x), x.shape, x.stride()
-    if c != M.dtF16 and c != M.dtF32:
+    if c != _F16 and c != _F32:
         raise ShloError("%s: %s not carried (float16 or float32)" % (what, x.dtype))
     if len(n) != 3:
         raise ShloError("%s: rank %d, [tokens, heads, dim] expected" % (what, len(n)))
@@ -69,7 +72,7 @@ def _list(x, code, what):
 def _tables(x, what):
     """int32 [sequences, pages], rows at any distance: (shape, row stride)."""
     n, s = x.shape, x.stride()
-    if _code(x) != M.dtI32 or len(n) != 2:
+    if _code(x) != _I32 or len(n) != 2:
         raise ShloError("%s: %s of rank %d, int32 of rank 2 expected" % (what, x.dtype, len(n)))
     if n[1] > 1 and s[1] != 1:
         raise ShloError("%s: the last axis is strided" % what)
@@ -83,10 +86,10 @@ def rope_noalloc(x, positions, phases, out, *, interleaved=False, inverse=False,
     if m != n or dy != dt:
         raise ShloError("rope: out is not x's shape and type")
     t, h, d = n
-    if _list(positions, M.dtI32, "rope: positions") != t:
+    if _list(positions, _I32, "rope: positions") != t:
         raise ShloError("rope: %d positions for %d tokens" % (positions.shape[0], t))
     check(load().shlo_rope_noalloc(x.data_ptr(), xs[0], xs[1], positions.data_ptr(), phases.data_ptr(), out.data_ptr(),
-                                   ys[0], ys[1], t, h, d, 2 * _list(phases, M.dtI64, "rope: phases"), dt,
+                                   ys[0], ys[1], t, h, d, 2 * _list(phases, _I64, "rope: phases"), dt,
                                    (1 if interleaved else 0) | (2 if inverse else 0), factor, stream))
 
 
@@ -98,11 +101,11 @@ class Pool:
 
     def __init__(self, k, v, k_scale, v_scale):
         n, m, s, z = k.shape, k_scale.shape, k.stride(), k_scale.stride()
-        if _code(k) != M.dtI8 or _code(v) != M.dtI8 or len(n) != 4:
+        if _code(k) != _I8 or _code(v) != _I8 or len(n) != 4:
             raise ShloError("cache: k and v are int8 [pages, heads, page_tokens, head_dim]")
         if v.shape != n or v.stride() != s or s[3] != 1:
             raise ShloError("cache: k and v differ in shape or strides, or their last axis is strided")
-        if _code(k_scale) != M.dtF32 or _code(v_scale) != M.dtF32 or m != n[:2] or v_scale.shape != m or v_scale.stride() != z:
+        if _code(k_scale) != _F32 or _code(v_scale) != _F32 or m != n[:2] or v_scale.shape != m or v_scale.stride() != z:
             raise ShloError("cache: the scales are not float32 [pages, heads] with the same strides")
         self.keep = (k, v, k_scale, v_scale)
         self.c = KvPool(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n[0], s[0], s[1], s[2],
@@ -111,7 +114,7 @@ class Pool:
 
 def _batch(starts, lens, tables, tokens):
     (n, w), stride = _tables(tables, "batch: tables")
-    a, b = _list(starts, M.dtI32, "batch: starts"), _list(lens, M.dtI32, "batch: lens")
+    a, b = _list(starts, _I32, "batch: starts"), _list(lens, _I32, "batch: lens")
     if a != n + 1 or b != n:
         raise ShloError("batch: %d starts and %d lengths for tables of %d sequences" % (a, b, n))
     return KvBatch(starts.data_ptr(), lens.data_ptr(), tables.data_ptr(), stride, n, w, tokens)
@@ -133,8 +136,8 @@ def gather_noalloc(pool: Pool, tables, seq, pos, k, v, *, stream=0):
     n, ks, dt = _rows(k, "kv_gather: k")
     m, vs, dv = _rows(v, "kv_gather: v")
     (seqs, width), stride = _tables(tables, "kv_gather: tables")
-    c, t = pool.c, _list(seq, M.dtI32, "kv_gather: seq")
-    if _list(pos, M.dtI32, "kv_gather: pos") != t or n != (t, c.heads, c.head_dim) or m != n or dv != dt:
+    c, t = pool.c, _list(seq, _I32, "kv_gather: seq")
+    if _list(pos, _I32, "kv_gather: pos") != t or n != (t, c.heads, c.head_dim) or m != n or dv != dt:
         raise ShloError("kv_gather: pos, k and v are not of %d tokens, %d heads of %d" % (t, c.heads, c.head_dim))
     check(load().shlo_kv_gather_noalloc(c, tables.data_ptr(), stride, seqs, width, seq.data_ptr(), pos.data_ptr(), t,
                                         k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], dt, stream))
@@ -159,8 +162,10 @@ def attend_noalloc(pool: Pool, q, starts, lens, tables, out, *, workspace, scale
     if m != n or do != dt:
         raise ShloError("kv_attend: out is not q's shape and type")
     lp = None
+    if not workspace.is_cuda:
+        raise ShloError("kv_attend: the workspace is in host memory")
     if lse is not None:
-        if _code(lse) != M.dtF32 or lse.shape != (t, h) or (t and h and not lse.is_contiguous()):
+        if _code(lse) != _F32 or lse.shape != (t, h) or (t and h and not lse.is_contiguous()):
             raise ShloError("kv_attend: lse is not a contiguous float32 [%d, %d]" % (t, h))
         lp = lse.data_ptr()
     check(load().shlo_kv_attend_noalloc(c, _batch(starts, lens, tables, t), q.data_ptr(), qs[0], qs[1], h, dt, scale,

@@ -442,6 +442,20 @@ def test_attend_rows_outside_the_batch_are_left():
                       cuda(np.zeros((0, 1), np.int32)), out[:0], scale=1.0, workspace=work, stream=stream())
 
 
+@pytest.mark.parametrize("kind", ["f16", "f32"])
+@pytest.mark.parametrize("lens,news", [([40], [2]), ([40], [70]), ([300, 20], [2, 1])])
+def test_attend_buffers_longer_than_the_batch(kind, lens, news):
+    """Activations of a fixed, longer buffer: the batch's rows are right, whichever kernel the buffer's length
+    suggests, and the others stay."""
+    c = Case(kind, 16, 1, 4, 64, [max(a, b) for a, b in zip(lens, news)], news)
+    q = cuda(np.concatenate([c.q, np.repeat(c.q[:1], 200, 0)]))
+    out = torch.full(q.shape, 9.0, dtype=q.dtype, device="cuda")
+    got = c.run(q=q, out=out)
+    T = len(c.q)
+    c.check((got[0][:T], got[1][:T]))
+    assert np.all(got[0][T:] == 9.0) and np.all(got[1][T:] == 9.0)
+
+
 def test_cache_past_32_bit_offsets():
     """Pages past 2^32 bytes of the cache, written, read back and attended to."""
     page, H, D = 256, 2, 256
@@ -495,6 +509,19 @@ def test_another_stream_than_the_default():
     c.check((out.cpu().numpy(), lse))
 
 
+class Shifted:
+    """A tensor's description with an address a byte further on, as a C caller could pass it."""
+
+    def __init__(self, t):
+        self.t = t
+
+    def data_ptr(self):
+        return self.t.data_ptr() + 1
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+
 def test_refusals():
     """Arguments that no kernel takes come back as errors, and nothing is written."""
     c = Case("f16", 16, 2, 2, 64, [20], [1])
@@ -507,6 +534,10 @@ def test_refusals():
             f(*a, **k)
     at = lambda **k: dict(dict(scale=1.0, workspace=work), **k)  # noqa: E731
     refuses("workspace", Dc.attend_noalloc, pool, q, st, ln, tb, out, **at(workspace=work[:-16]))
+    refuses("host memory", Dc.attend_noalloc, pool, q, st.cpu(), ln, tb, out, **at())
+    refuses("host memory", Dc.attend_noalloc, pool, q, st, ln, tb, out, **at(workspace=work.cpu()))
+    refuses("host memory", Dc.rope_noalloc, q.cpu(), ln, ln.long(), out)
+    refuses("misaligned", Dc.attend_noalloc, pool, q, st, Shifted(ln), tb, out, **at())
     refuses("not carried", Dc.attend_noalloc, pool, q.bfloat16(), st, ln, tb, out, **at())
     refuses("window", Dc.attend_noalloc, pool, q, st, ln, tb, out, **at(window=-1))
     refuses("shape and type", Dc.attend_noalloc, pool, q, st, ln, tb, out.float(), **at())
