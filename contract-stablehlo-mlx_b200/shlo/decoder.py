@@ -80,8 +80,12 @@ class Decoder:
         s.tokens, s.pages = 0, []
 
     def step(self, news) -> np.ndarray:
-        """New tokens [n, d] of each (sequence, tokens) in turn -> their outputs [all, d]."""
+        """New tokens [n, d] of each (sequence, tokens) in turn -> their outputs [all, d]. A sequence is named once
+        a step: its tokens of one step are one run of positions."""
         cfg = self.cfg
+        news = list(news)
+        if len({id(s) for s, _ in news}) != len(news):
+            raise ShloError("decoder: a sequence named twice in one step")
         need = [-(-(s.tokens + len(x)) // cfg.page_tokens) - len(s.pages) for s, x in news]
         if sum(need) > len(self.free):
             raise ShloError("decoder: %d pages needed, %d free" % (sum(need), len(self.free)))
