@@ -81,31 +81,33 @@ class Decoder:
 
     def step(self, news) -> np.ndarray:
         """New tokens [n, d] of each (sequence, tokens) in turn -> their outputs [all, d]. A sequence is named once
-        a step: its tokens of one step are one run of positions."""
+        a step: its tokens of one step are one run of positions. A step that fails leaves every sequence's length
+        and pages as they were (rounded again, at most, in the page that its last tokens share with the new ones)."""
         cfg = self.cfg
-        news = list(news)
+        news = [(s, np.asarray(x, np.float32)) for s, x in news]
         if len({id(s) for s, _ in news}) != len(news):
             raise ShloError("decoder: a sequence named twice in one step")
-        need = [-(-(s.tokens + len(x)) // cfg.page_tokens) - len(s.pages) for s, x in news]
+        t = sum(len(x) for _, x in news)
+        lens = [s.tokens + len(x) for s, x in news]
+        need = [-(-n // cfg.page_tokens) - len(s.pages) for (s, _), n in zip(news, lens)]
         if sum(need) > len(self.free):
             raise ShloError("decoder: %d pages needed, %d free" % (sum(need), len(self.free)))
-        positions, lens = [], []
-        for (s, x), n in zip(news, need):
-            s.pages += [self.free.pop() for _ in range(n)]
-            positions.append(np.arange(s.tokens, s.tokens + len(x), dtype=np.int32))
-            s.tokens += len(x)
-            lens.append(s.tokens)
-        width = max(len(s.pages) for s, _ in news)
-        tables = np.array([s.pages + [-1] * (width - len(s.pages)) for s, _ in news], np.int32)
+        # The pages that the step adds stay on the free list until its outputs are there.
+        take = iter(self.free[::-1])
+        pages = [s.pages + [next(take) for _ in range(n)] for (s, _), n in zip(news, need)]
+        width = max(len(p) for p in pages)
+        tables = np.array([p + [-1] * (width - len(p)) for p in pages], np.int32)
         starts = np.concatenate([[0], np.cumsum([len(x) for _, x in news])]).astype(np.int32)
         batch = [M.of_numpy(a) for a in (starts, np.array(lens, np.int32), tables)]
-        at = M.of_numpy(np.concatenate(positions))
-        x = np.concatenate([x for _, x in news]).astype(np.float32)
-        t = len(x)
-        h = M.of_numpy(x)
+        at = M.of_numpy(np.concatenate([np.arange(s.tokens, n, dtype=np.int32) for (s, _), n in zip(news, lens)]))
+        h = M.of_numpy(np.concatenate([x for _, x in news]))
         for li in range(cfg.layers):
             h = self._layer(h, li, t, at, batch)
-        return M.to_numpy(M.reshape(h, [t, cfg.d]))
+        out = M.to_numpy(M.reshape(h, [t, cfg.d]))
+        for (s, _), n, p in zip(news, lens, pages):
+            s.tokens, s.pages = n, p
+        del self.free[len(self.free) - sum(need):]
+        return out
 
     def _dense(self, x, name, bias, m, k, t, res=None, flags=Run.EP_BIAS):
         return Run.mul_mat_bias(self.w[name], x, k, m, t, t, 0, self.w[bias], res, flags)

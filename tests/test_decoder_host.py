@@ -34,6 +34,24 @@ def test_a_sequence_named_twice_is_refused(decoder):
     assert (a.tokens, a.pages, decoder.free, len(decoder.seen)) == (3, pages, free, n)
 
 
+def test_a_step_that_fails_leaves_lengths_and_pages(decoder):
+    a, _ = decoder.start(tokens(3))
+    b, layer = Dd.Sequence(), decoder._layer
+    before = (a.tokens, list(a.pages), list(decoder.free))
+
+    def broken(h, li, t, at, batch):
+        if li == 1:
+            raise ShloError("layer")
+        return h
+    decoder._layer = broken
+    with pytest.raises(ShloError, match="layer"):
+        decoder.step([(a, tokens(6)), (b, tokens(5))])
+    assert (a.tokens, a.pages, decoder.free) == before and (b.tokens, b.pages) == (0, [])
+    decoder._layer = layer
+    decoder.step([(a, tokens(6)), (b, tokens(5))])
+    assert (a.tokens, b.tokens) == (9, 5) and sorted(a.pages + b.pages + decoder.free) == list(range(10))
+
+
 def test_a_step_lays_its_batch_out(decoder):
     a, y = decoder.start(tokens(5))
     assert np.array_equal(y, tokens(5) + 2)
