@@ -88,6 +88,8 @@ class Decoder:
         if len({id(s) for s, _ in news}) != len(news):
             raise ShloError("decoder: a sequence named twice in one step")
         t = sum(len(x) for _, x in news)
+        if t == 0:
+            return np.zeros((0, cfg.d), np.float32)
         lens = [s.tokens + len(x) for s, x in news]
         need = [-(-n // cfg.page_tokens) - len(s.pages) for (s, _), n in zip(news, lens)]
         if sum(need) > len(self.free):

@@ -52,6 +52,14 @@ def test_a_step_that_fails_leaves_lengths_and_pages(decoder):
     assert (a.tokens, b.tokens) == (9, 5) and sorted(a.pages + b.pages + decoder.free) == list(range(10))
 
 
+def test_steps_without_tokens(decoder):
+    a, _ = decoder.start(tokens(4))
+    before = (a.tokens, list(a.pages), list(decoder.free), len(decoder.seen))
+    assert decoder.step([]).shape == (0, 8)
+    assert decoder.step([(a, tokens(0)), (Dd.Sequence(), tokens(0))]).shape == (0, 8)
+    assert (a.tokens, a.pages, decoder.free, len(decoder.seen)) == before
+
+
 def test_a_step_lays_its_batch_out(decoder):
     a, y = decoder.start(tokens(5))
     assert np.array_equal(y, tokens(5) + 2)
