@@ -183,7 +183,7 @@ __device__ __forceinline__ bool next_segment(const AttendArgs &a, const BatchArr
   while (p.at < p.end && p.head < a.pool.heads) {
     g.t.seq = p.seq;
     const int units = tile_of_slot<ROWS, GRAN>(a, ba.starts, ba.lens, p.slot, g.t, true);
-    const int off = p.off;
+    const int off = p.off, slot = p.slot;
     p.seq = g.t.seq;
     g.head = p.head;
     p.off = 0;
@@ -192,10 +192,15 @@ __device__ __forceinline__ bool next_segment(const AttendArgs &a, const BatchArr
       p.slot = p.seq = 0;
       p.head++;
     }
-    if (units == 0) {  // a slot without a tile: neither has the rest of its sequence's
+    if (units == 0) {
+      // A slot without a tile: one before its sequence's first (rows of q that no
+      // sequence has), or one after its last, and then neither has the rest of its.
       constexpr int SH = kRowShift<ROWS>;
-      if (p.slot > 0)
-        p.slot = p.seq + 1 < a.batch.seqs ? max(p.slot, slot_base(ba.starts, a.batch.tokens, p.seq + 1, a.group, SH, 1)) : a.slots;
+      if (p.slot > 0) {
+        const int own = slot_base(ba.starts, a.batch.tokens, p.seq, a.group, SH, 1);
+        if (slot < own) p.slot = own;
+        else p.slot = p.seq + 1 < a.batch.seqs ? max(p.slot, slot_base(ba.starts, a.batch.tokens, p.seq + 1, a.group, SH, 1)) : a.slots;
+      }
       if (p.slot >= a.slots) {
         p.slot = p.seq = 0;
         p.head++;
