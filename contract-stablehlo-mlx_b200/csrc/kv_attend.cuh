@@ -48,7 +48,10 @@ struct AttendArgs {
   unsigned *counters;  // [2][kAttendMaxBlocks], zero between calls
   float *partials;     // [chunks][2][rows * (dim + 2)]
   int *err;            // set by a launch that gave up a wait
+  uint64_t wait_ns;    // after which a wait is given up
 };
+
+constexpr uint64_t kWaitLimitNs = 2000000000ull;
 
 constexpr int kAttendMaxBlocks = 1024;
 // Partials joined at once: what a join's factors take in shared memory bounds it.

@@ -60,25 +60,30 @@ __device__ __forceinline__ bool bar_test(uint64_t *b, uint32_t parity) {  // wit
       : "=r"(ok) : "r"(smem_at(b)), "r"(parity) : "memory");
   return ok != 0;
 }
-// A wait of two seconds at most; it ends early when another warp gave up.
-__device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity, volatile int *gone) {
+// A wait of `limit` nanoseconds at most; it ends early when another warp gave up.
+__device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity, volatile int *gone, uint64_t limit) {
   if (bar_try(b, parity)) return true;
   uint64_t t0, t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
   for (uint32_t i = 1;; i++) {
     if (bar_try(b, parity)) return true;
-    if ((i & 255) == 0) {
+    if ((i & 255) == 0 || limit == 0) {
       asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-      if (*gone || t - t0 > 2000000000ull) {
+      if (*gone || t - t0 >= limit) {
         *gone = 1;
         return false;
       }
     }
   }
 }
-// The same for a whole warp, which goes on or gives up as one.
-__device__ __forceinline__ bool warp_wait(uint64_t *b, uint32_t parity, volatile int *gone) {
-  return __all_sync(~0u, bar_wait(b, parity, gone));
+// What is still on the way when a block gives up is waited for, for two seconds at most.
+__device__ __forceinline__ void bar_drain(uint64_t *b, uint32_t parity) {
+  uint64_t t0, t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
+  do {
+    if (bar_try(b, parity)) return;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  } while (t - t0 < kWaitLimitNs);
 }
 __device__ __forceinline__ float ex2_(float x) {
   float r;
@@ -198,7 +203,7 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
   // Barriers. Of a stage of bytes: there, used up. Of a stage of float16: there, used up. Of
   // a row tile and a place of scores: scores done, weights there, outputs done.
   uint64_t *const kv_full = reinterpret_cast<uint64_t *>(raw + RS * S::K_BYTES), *const kv_free = kv_full + 4, *const raw_full = kv_full + 20, *const raw_free = kv_full + 24;
-  uint64_t *const qk_done = kv_full + 8, *const p_full = kv_full + 12, *const pv_done = kv_full + 16;
+  uint64_t *const qk_done = kv_full + 8, *const p_full = kv_full + 12, *const pv_done = kv_full + 16, *const drained = kv_full + 28;
   long long *const sched = reinterpret_cast<long long *>(kv_full + 32);
   Place *const place = reinterpret_cast<Place *>(sched + THREADS + 4);
   int *const batch = reinterpret_cast<int *>(reinterpret_cast<uint8_t *>(place) + 64);
@@ -207,12 +212,15 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
   volatile int *const gone = reinterpret_cast<volatile int *>(flag + 1);
   uint32_t *const tm_slot = reinterpret_cast<uint32_t *>(flag + 2);
   float *const vtop_s = reinterpret_cast<float *>(flag + 3);
+  int *const asked = reinterpret_cast<int *>(flag + 4);  // tiles of the segment whose bytes were asked for
   float *const fac = reinterpret_cast<float *>(qs);  // a join's factors, when no tile is under way
   static_assert(sizeof(Place) <= 64, "its room in shared memory");
   static_assert(2 * (kJoin<ROWS> + 1) * ROWS * 4 <= RT * S::Q_BYTES + (2 * NS + RS) * S::K_BYTES, "a join's factors");
 
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int D = a.pool.head_dim, PT = 1 << a.page_shift;
+  // A wait of a whole warp, which goes on or gives up as one.
+  auto warp_wait = [&](uint64_t *b, uint32_t parity) { return __all_sync(~0u, bar_wait(b, parity, gone, a.wait_ns)); };
   Line line;
   BatchArrays ba;
   if (!schedule<ROWS, KT, THREADS>(a, min_gran, sched, batch, S::BATCH, ba, line)) return;
@@ -231,6 +239,7 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
       bar_init(p_full + i, 4);
       bar_init(pv_done + i, 1);
     }
+    bar_init(drained, 1);
     *gone = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -339,6 +348,7 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
       ask_scales();
       turn();
       for (int j = 0; j < RS && j < n; j++) copy_tile(j);
+      if (lane == 0) *asked = min(RS, n);
     }
     // The queries, and the largest finite scale of the segment's values.
     if (tid == 0) *vtop_s = 0.0f;
@@ -400,9 +410,10 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
           turn();
           pages(j + TL);
         }
-        if (!warp_wait(raw_free + t % RS, (t / RS & 1) ^ 1, gone)) break;
+        if (!warp_wait(raw_free + t % RS, (t / RS & 1) ^ 1)) break;
         copy_tile(j);
         count_tile(j, vtop);
+        if (lane == 0) *asked = j + 1;
       }
     } else
     if (warp == 4 * RT + 4) {
@@ -469,11 +480,11 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
           }
           if (any) {
             idle = 0;
-          } else if ((++idle & 255) == 0) {  // two seconds of nothing: give up
+          } else if ((++idle & 255) == 0 || a.wait_ns == 0) {  // nothing for too long: give up
             uint64_t now;
             asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
             if (idle == 256) t0 = now;
-            if (__any_sync(~0u, *gone || now - t0 > 2000000000ull)) {
+            if (__any_sync(~0u, *gone || now - t0 >= a.wait_ns)) {
               *gone = 1;
               break;
             }
@@ -507,8 +518,8 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
       };
       for (int j = 0; j < n; j++) {
         const uint32_t t = done + j, st = t % NS, rs = t % RS;
-        if (!warp_wait(raw_full + rs, t / RS & 1, gone)) break;
-        if (j >= NS && !warp_wait(kv_free + st, (t / NS & 1) ^ 1, gone)) break;
+        if (!warp_wait(raw_full + rs, t / RS & 1)) break;
+        if (j >= NS && !warp_wait(kv_free + st, (t / NS & 1) ^ 1)) break;
         if (live) {
           const uint8_t *from = raw + rs * S::K_BYTES + key_in * D + ch * 16;
           put(ks + st * S::K_BYTES, from);
@@ -532,7 +543,7 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
       for (int j = 0; j < n; j++) {
         const uint32_t t = mine + j, b = t & 1, ph = (t >> 1) & 1, st = (done + j) % NS;
         const uint32_t s_at = tm + (2 * rt + b) * KT + lanes;
-        if (!warp_wait(kv_full + st, (done + j) / NS & 1, gone) || !warp_wait(qk_done + 2 * rt + b, ph, gone)) {
+        if (!warp_wait(kv_full + st, (done + j) / NS & 1) || !warp_wait(qk_done + 2 * rt + b, ph)) {
           ok = false;
           break;
         }
@@ -577,7 +588,7 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
           m = mn;
           if (j) {  // (the first product writes O)
             const uint32_t u = t - 1;
-            if (!warp_wait(pv_done + 2 * rt + (u & 1), (u >> 1) & 1, gone)) {
+            if (!warp_wait(pv_done + 2 * rt + (u & 1), (u >> 1) & 1)) {
               ok = false;
               break;
             }
@@ -640,7 +651,7 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
       }
       if (ok) {
         const uint32_t u = mine + n - 1;
-        ok = warp_wait(pv_done + 2 * rt + (u & 1), (u >> 1) & 1, gone);
+        ok = warp_wait(pv_done + 2 * rt + (u & 1), (u >> 1) & 1);
       }
       tm_after();
       const bool whole = sg.take == sg.units;
@@ -699,7 +710,18 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
     for (int r = 0; r < RT; r++) turns[r] += r < rts ? n : 0;
     __syncthreads();
     tm_after();
-    if (*gone) break;
+    if (*gone) {
+      // A warp gave up: the results are not valid, and the host is told. The bytes and
+      // products that are on the way land before the block leaves its memory.
+      if (warp == ASKER)
+        for (int j = max(0, *asked - RS); j < *asked; j++) bar_drain(raw_full + (done - n + j) % RS, (done - n + j) / RS & 1);
+      if (warp == 4 * RT + 4) {
+        if (elect_one()) tm_commit(drained);
+        __syncwarp();
+        bar_drain(drained, 0);
+      }
+      break;
+    }
     if (sg.take != sg.units) arrive<__half, ROWS, DP, THREADS>(a, sg, line, fac, flag);
   }
   __syncthreads();

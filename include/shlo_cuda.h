@@ -308,6 +308,9 @@ int shlo_kv_attend(shlo_kv kv, shlo_arr q, shlo_arr starts, shlo_arr lens, shlo_
    platform erff of this backend is the correctly rounded one (the pinned
    reference build links CORE-MATH's). `out` receives `count` uint32 words. */
 int shlo_libm_erff_range(uint32_t base, uint32_t count, uint32_t *out);
+/* After how many nanoseconds the attention's launches from now on give up a
+   wait (below 0: the two seconds they have otherwise). */
+void shlo_test_attend_wait(int64_t ns);
 /* smlx_count_nonzero: the exact number of nonzero elements, evaluated. */
 int shlo_count_nonzero(shlo_arr a, uint64_t *count);
 

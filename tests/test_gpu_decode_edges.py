@@ -9,6 +9,7 @@ torch = pytest.importorskip("torch")
 
 from shlo import decode as Dc  # noqa: E402
 from shlo import mlx as M  # noqa: E402
+from shlo._lib import ShloError, load  # noqa: E402
 from test_gpu_decode import Case, cuda  # noqa: E402
 
 
@@ -38,3 +39,30 @@ def test_rows_before_the_first_sequence(kind, hk, group, lens, news):
         c.check((got[0][lead:], got[1][lead:]))
         assert np.all(got[0][:lead] == 9.0) and np.all(got[1][:lead] == 9.0)
         assert int(work[:8192].to(torch.int32).sum()) == 0
+
+
+def wait():
+    """The library's own wait for its device, which tells what its launches reported."""
+    torch.cuda.synchronize()
+    M.to_numpy(M.transpose(M.of_numpy(np.zeros((2, 3), np.float32)), [1, 0]))
+
+
+@pytest.mark.parametrize("hk,group,D,lens,news", [(2, 3, 128, [400, 129, 1000, 5], [300, 129, 1, 5]),
+                                                  (1, 8, 64, [3000], [20]), (1, 5, 256, [500, 64], [200, 64])])
+def test_a_launch_that_gives_up_returns_and_is_told(hk, group, D, lens, news):
+    """Waits that run out at once, with bytes and products on the way: the launch returns, the error is told, and
+    the context and later launches are as before."""
+    c = Case("f16", 16, hk, group, D, lens, news, seed=7)
+    first = c.run()
+    lib = load()
+    try:
+        for _ in range(3):
+            lib.shlo_test_attend_wait(0)
+            c.run()
+            lib.shlo_test_attend_wait(-1)
+            with pytest.raises(ShloError, match="gave up"):
+                wait()
+            again = c.run()
+            assert again[0].tobytes() == first[0].tobytes() and again[1].tobytes() == first[1].tobytes()
+    finally:
+        lib.shlo_test_attend_wait(-1)
