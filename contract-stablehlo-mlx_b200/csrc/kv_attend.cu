@@ -668,7 +668,7 @@ int dispatch_rows(const AttendArgs &a, int nt, int sms, int device, cudaStream_t
 
 constexpr size_t kCounterBytes = 2 * kAttendMaxBlocks * sizeof(unsigned);
 
-std::atomic<uint64_t> g_wait_ns{kWaitLimitNs};
+std::atomic<unsigned> g_give_up{0};
 
 }  // namespace
 
@@ -725,7 +725,7 @@ int launch_kv_attend(const AttendCall &c, int sms, int device, cudaStream_t st) 
   a.partials = reinterpret_cast<float *>(static_cast<char *>(c.work) + kCounterBytes);
   a.q_wide = (uintptr_t)c.q % 16 == 0 && c.q_token % 8 == 0 && c.q_head % 8 == 0;
   a.err = c.err;
-  a.wait_ns = g_wait_ns.load(std::memory_order_relaxed);
+  a.give_up = g_give_up.load(std::memory_order_relaxed);
   // Tiles of 8 rows where the sequences have 8 or fewer on average, else 16. Above
   // 16, float16 sequences of more than 16 rows go to the tiles of 128 (in which a
   // 16-row tile would cost as much as a full one), in a launch of their own.
@@ -755,7 +755,7 @@ int shlo_kv_attend_workspace(size_t *bytes) {
   return 0;
 }
 
-void shlo_test_attend_wait(int64_t ns) { g_wait_ns.store(ns < 0 ? kWaitLimitNs : (uint64_t)ns); }
+void shlo_test_attend_give_up(int32_t every) { g_give_up.store(every < 0 ? 0u : (unsigned)every); }
 
 int shlo_kv_attend_noalloc(const shlo_kv_pool *pool, const shlo_kv_batch *batch, const void *q, int64_t q_token,
                            int64_t q_head, int32_t heads, uint8_t dtype, float scale, int32_t causal, int32_t window,

@@ -48,7 +48,7 @@ struct AttendArgs {
   unsigned *counters;  // [2][kAttendMaxBlocks], zero between calls
   float *partials;     // [chunks][2][rows * (dim + 2)]
   int *err;            // set by a launch that gave up a wait
-  uint64_t wait_ns;    // after which a wait is given up
+  unsigned give_up;    // every so many blocks of the tiles give up at once (0: none)
 };
 
 constexpr uint64_t kWaitLimitNs = 2000000000ull;

@@ -60,21 +60,25 @@ __device__ __forceinline__ bool bar_test(uint64_t *b, uint32_t parity) {  // wit
       : "=r"(ok) : "r"(smem_at(b)), "r"(parity) : "memory");
   return ok != 0;
 }
-// A wait of `limit` nanoseconds at most; it ends early when another warp gave up.
-__device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity, volatile int *gone, uint64_t limit) {
+// A wait of two seconds at most; it ends early when another warp gave up.
+__device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity, volatile int *gone) {
   if (bar_try(b, parity)) return true;
   uint64_t t0, t;
   asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
   for (uint32_t i = 1;; i++) {
     if (bar_try(b, parity)) return true;
-    if ((i & 255) == 0 || limit == 0) {
+    if ((i & 255) == 0) {
       asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-      if (*gone || t - t0 >= limit) {
+      if (*gone || t - t0 > kWaitLimitNs) {
         *gone = 1;
         return false;
       }
     }
   }
+}
+// The same for a whole warp, which goes on or gives up as one.
+__device__ __forceinline__ bool warp_wait(uint64_t *b, uint32_t parity, volatile int *gone) {
+  return __all_sync(~0u, bar_wait(b, parity, gone));
 }
 // What is still on the way when a block gives up is waited for, for two seconds at most.
 __device__ __forceinline__ void bar_drain(uint64_t *b, uint32_t parity) {
@@ -219,8 +223,6 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
 
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int D = a.pool.head_dim, PT = 1 << a.page_shift;
-  // A wait of a whole warp, which goes on or gives up as one.
-  auto warp_wait = [&](uint64_t *b, uint32_t parity) { return __all_sync(~0u, bar_wait(b, parity, gone, a.wait_ns)); };
   Line line;
   BatchArrays ba;
   if (!schedule<ROWS, KT, THREADS>(a, min_gran, sched, batch, S::BATCH, ba, line)) return;
@@ -262,6 +264,9 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
   for (int r = 0; r < RT; r++) turns[r] = 0;
 
   while (next_segment<ROWS, KT>(a, ba, p, sg)) {
+    // (After a wait that was given up the units are only counted, all of them: the
+    // counters are zero again for the next launch. What is joined then is not valid.)
+    if (!*gone) {
     const int key0 = (sg.t.lo / KT + sg.off) * KT;
     const int32_t *table = a.batch.tables + (int64_t)sg.t.seq * a.batch.table_stride;
     auto page_at = [&](int key) -> int {  // -1: no row of the tile sees a key of these 16, or there is no page
@@ -410,7 +415,7 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
           turn();
           pages(j + TL);
         }
-        if (!warp_wait(raw_free + t % RS, (t / RS & 1) ^ 1)) break;
+        if (!warp_wait(raw_free + t % RS, (t / RS & 1) ^ 1, gone)) break;
         copy_tile(j);
         count_tile(j, vtop);
         if (lane == 0) *asked = j + 1;
@@ -430,6 +435,7 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
 #pragma unroll
         for (int r = 0; r < RT; r++) next_s[r] = next_o[r] = 0;
         uint64_t t0 = 0;
+        const bool hurried = a.give_up && blockIdx.x % a.give_up == 0;
         for (uint32_t idle = 0; left > 0;) {
           bool any = false;
 #pragma unroll
@@ -480,11 +486,11 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
           }
           if (any) {
             idle = 0;
-          } else if ((++idle & 255) == 0 || a.wait_ns == 0) {  // nothing for too long: give up
+          } else if ((++idle & 255) == 0 || hurried) {  // two seconds of nothing: give up
             uint64_t now;
             asm volatile("mov.u64 %0, %globaltimer;" : "=l"(now));
             if (idle == 256) t0 = now;
-            if (__any_sync(~0u, *gone || now - t0 >= a.wait_ns)) {
+            if (__any_sync(~0u, *gone || hurried || now - t0 > kWaitLimitNs)) {
               *gone = 1;
               break;
             }
@@ -518,8 +524,8 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
       };
       for (int j = 0; j < n; j++) {
         const uint32_t t = done + j, st = t % NS, rs = t % RS;
-        if (!warp_wait(raw_full + rs, t / RS & 1)) break;
-        if (j >= NS && !warp_wait(kv_free + st, (t / NS & 1) ^ 1)) break;
+        if (!warp_wait(raw_full + rs, t / RS & 1, gone)) break;
+        if (j >= NS && !warp_wait(kv_free + st, (t / NS & 1) ^ 1, gone)) break;
         if (live) {
           const uint8_t *from = raw + rs * S::K_BYTES + key_in * D + ch * 16;
           put(ks + st * S::K_BYTES, from);
@@ -543,7 +549,7 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
       for (int j = 0; j < n; j++) {
         const uint32_t t = mine + j, b = t & 1, ph = (t >> 1) & 1, st = (done + j) % NS;
         const uint32_t s_at = tm + (2 * rt + b) * KT + lanes;
-        if (!warp_wait(kv_full + st, (done + j) / NS & 1) || !warp_wait(qk_done + 2 * rt + b, ph)) {
+        if (!warp_wait(kv_full + st, (done + j) / NS & 1, gone) || !warp_wait(qk_done + 2 * rt + b, ph, gone)) {
           ok = false;
           break;
         }
@@ -588,7 +594,7 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
           m = mn;
           if (j) {  // (the first product writes O)
             const uint32_t u = t - 1;
-            if (!warp_wait(pv_done + 2 * rt + (u & 1), (u >> 1) & 1)) {
+            if (!warp_wait(pv_done + 2 * rt + (u & 1), (u >> 1) & 1, gone)) {
               ok = false;
               break;
             }
@@ -651,7 +657,7 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
       }
       if (ok) {
         const uint32_t u = mine + n - 1;
-        ok = warp_wait(pv_done + 2 * rt + (u & 1), (u >> 1) & 1);
+        ok = warp_wait(pv_done + 2 * rt + (u & 1), (u >> 1) & 1, gone);
       }
       tm_after();
       const bool whole = sg.take == sg.units;
@@ -720,7 +726,8 @@ __global__ void __launch_bounds__(Tiles<DP>::THREADS, 1) k_kv_attend_tiles(const
         __syncwarp();
         bar_drain(drained, 0);
       }
-      break;
+      __syncthreads();
+    }
     }
     if (sg.take != sg.units) arrive<__half, ROWS, DP, THREADS>(a, sg, line, fac, flag);
   }

@@ -19,7 +19,7 @@ SYMBOLS = [
     "shlo_rope_phases", "shlo_rope_noalloc", "shlo_kv_append_noalloc", "shlo_kv_gather_noalloc",
     "shlo_kv_attend_workspace", "shlo_kv_attend_noalloc",
     "shlo_kv_new", "shlo_kv_free", "shlo_kv_storage", "shlo_kv_append", "shlo_kv_gather", "shlo_kv_attend",
-    "shlo_test_attend_wait",
+    "shlo_test_attend_give_up",
 ]
 
 
@@ -134,10 +134,10 @@ def load() -> ctypes.CDLL:
     L.shlo_kv_gather.argtypes = [p, c_arr, c_arr, c_arr, u8, ctypes.POINTER(c_arr), ctypes.POINTER(c_arr)]
     L.shlo_kv_attend.argtypes = [p, c_arr, c_arr, c_arr, c_arr, f32, i32, i32, ctypes.POINTER(c_arr),
                                  ctypes.POINTER(c_arr)]
-    L.shlo_test_attend_wait.argtypes = [i64]
-    L.shlo_test_attend_wait.restype = None
+    L.shlo_test_attend_give_up.argtypes = [i32]
+    L.shlo_test_attend_give_up.restype = None
     special = {"shlo_last_error", "shlo_empty", "shlo_retain", "shlo_release", "shlo_kernel_free", "shlo_fn_free",
-               "shlo_kv_free", "shlo_test_attend_wait"}
+               "shlo_kv_free", "shlo_test_attend_give_up"}
     for name in SYMBOLS:
         if name not in special:
             getattr(L, name).restype = ctypes.c_int

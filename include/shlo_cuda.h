@@ -268,8 +268,8 @@ int shlo_kv_attend_workspace(size_t *bytes);
    (float32 [tokens][heads], or NULL) is the logarithm of the sum of the
    exponentials of the scaled scores. The workspace must be zero before the
    first call that uses it; calls leave it ready for the next, on one stream at
-   a time (after a launch that gave up a wait, which the library's next wait
-   reports, zero it again). The same call gives the same bits. */
+   a time, those that gave up a wait (which the library's next wait reports)
+   too. The same call gives the same bits. */
 int shlo_kv_attend_noalloc(const shlo_kv_pool *pool, const shlo_kv_batch *batch, const void *q, int64_t q_token,
                            int64_t q_head, int32_t heads, uint8_t dtype, float scale, int32_t causal, int32_t window,
                            void *out, int64_t out_token, int64_t out_head, float *lse, void *workspace,
@@ -308,9 +308,9 @@ int shlo_kv_attend(shlo_kv kv, shlo_arr q, shlo_arr starts, shlo_arr lens, shlo_
    platform erff of this backend is the correctly rounded one (the pinned
    reference build links CORE-MATH's). `out` receives `count` uint32 words. */
 int shlo_libm_erff_range(uint32_t base, uint32_t count, uint32_t *out);
-/* After how many nanoseconds the attention's launches from now on give up a
-   wait (below 0: the two seconds they have otherwise). */
-void shlo_test_attend_wait(int64_t ns);
+/* Every `every`-th block of the attention's tiles gives up its first wait, as
+   it would after two seconds, in the launches from now on (0: none). */
+void shlo_test_attend_give_up(int32_t every);
 /* smlx_count_nonzero: the exact number of nonzero elements, evaluated. */
 int shlo_count_nonzero(shlo_arr a, uint64_t *count);
 

@@ -49,20 +49,47 @@ def wait():
 
 @pytest.mark.parametrize("hk,group,D,lens,news", [(2, 3, 128, [400, 129, 1000, 5], [300, 129, 1, 5]),
                                                   (1, 8, 64, [3000], [20]), (1, 5, 256, [500, 64], [200, 64])])
-def test_a_launch_that_gives_up_returns_and_is_told(hk, group, D, lens, news):
-    """Waits that run out at once, with bytes and products on the way: the launch returns, the error is told, and
-    the context and later launches are as before."""
+def test_a_launch_that_gives_up_leaves_the_next_one_right(hk, group, D, lens, news):
+    """Waits that are given up: the launch returns, the error is told, and without the workspace being touched the
+    next call gives the bits that it gave before."""
     c = Case("f16", 16, hk, group, D, lens, news, seed=7)
-    first = c.run()
+    work = torch.zeros(Dc.attend_workspace(), dtype=torch.uint8, device="cuda")
+    first = c.run(work=work)
+    c.check(first)
     lib = load()
     try:
-        for _ in range(3):
-            lib.shlo_test_attend_wait(0)
-            c.run()
-            lib.shlo_test_attend_wait(-1)
+        for every in (1, 2, 3):  # of the blocks, so that some units' parts arrive and others' do not
+            lib.shlo_test_attend_give_up(every)
+            c.run(work=work)
+            lib.shlo_test_attend_give_up(0)
             with pytest.raises(ShloError, match="gave up"):
                 wait()
-            again = c.run()
+            assert int(work[:8192].to(torch.int32).sum()) == 0
+            again = c.run(work=work)
             assert again[0].tobytes() == first[0].tobytes() and again[1].tobytes() == first[1].tobytes()
     finally:
-        lib.shlo_test_attend_wait(-1)
+        lib.shlo_test_attend_give_up(0)
+
+
+def test_a_cache_after_a_launch_that_gave_up():
+    """The same through a handle, whose workspace is the library's own: the wait reports it, calls after it are right."""
+    rng = np.random.default_rng(5)
+    cache = Dc.Cache(64, 2, 64, 16)
+    n = 700
+    kv = M.of_numpy(rng.standard_normal((n, 2, 64)).astype(np.float16))
+    q = M.of_numpy(rng.standard_normal((n, 8, 64)).astype(np.float16))
+    batch = [M.of_numpy(a) for a in (np.array([0, n], np.int32), np.array([n], np.int32), np.arange(44, dtype=np.int32)[None])]
+    cache.append(kv, kv, *batch)
+    first = M.to_numpy(cache.attend(q, *batch, scale=0.125))
+    lib = load()
+    try:
+        lib.shlo_test_attend_give_up(2)
+        lost = cache.attend(q, *batch, scale=0.125)
+        lib.shlo_test_attend_give_up(0)
+        after = cache.attend(q, *batch, scale=0.125)  # queued before the error is seen
+        with pytest.raises(ShloError, match="gave up"):
+            M.to_numpy(lost)
+        assert M.to_numpy(after).tobytes() == first.tobytes()
+        assert M.to_numpy(cache.attend(q, *batch, scale=0.125)).tobytes() == first.tobytes()
+    finally:
+        lib.shlo_test_attend_give_up(0)
