@@ -76,6 +76,9 @@ struct Device {
 // The device current on this host thread, initialised on first use.
 int current_device(Device **out);
 int device_by_id(int id, Device **out);
+// The device current in CUDA itself on this host thread, which stays so: of the
+// entry points on caller-owned memory.
+int calling_device(Device **out);
 int current_flavor();
 
 // ---- storage ----

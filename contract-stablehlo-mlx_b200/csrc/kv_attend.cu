@@ -747,10 +747,15 @@ using namespace shlo;
 
 extern "C" {
 
+int shlo_cuda_device(void) {
+  int id;
+  return cudaGetDevice(&id) == cudaSuccess ? id : -1;
+}
+
 int shlo_kv_attend_workspace(size_t *bytes) {
   if (!bytes) return fail("kv_attend workspace: null pointer");
   Device *dev;
-  SHLO_TRY(current_device(&dev));
+  SHLO_TRY(calling_device(&dev));
   *bytes = attend_work_bytes(dev->sm_count);
   return 0;
 }
@@ -763,7 +768,7 @@ int shlo_kv_attend_noalloc(const shlo_kv_pool *pool, const shlo_kv_batch *batch,
                            size_t workspace_bytes, void *stream) {
   if (!pool || !batch) return fail("kv_attend: null descriptor");
   Device *dev;
-  SHLO_TRY(current_device(&dev));
+  SHLO_TRY(calling_device(&dev));
   AttendCall c{*pool, *batch, q, q_token, q_head, out, out_token, out_head, lse, heads, dtype, scale, causal != 0, window,
                workspace, workspace_bytes, dev->pipe_err_dev};
   return launch_kv_attend(c, dev->sm_count, dev->id, (cudaStream_t)stream);

@@ -355,7 +355,7 @@ int shlo_kv_append_noalloc(const shlo_kv_pool *pool, const shlo_kv_batch *batch,
                            int64_t k_head, const void *v, int64_t v_token, int64_t v_head, uint8_t dtype, void *stream) {
   if (!pool || !batch) return fail("kv_append: null descriptor");
   Device *dev;
-  SHLO_TRY(current_device(&dev));
+  SHLO_TRY(calling_device(&dev));
   return launch_kv_append(*pool, *batch, k, k_token, k_head, v, v_token, v_head, dtype, (cudaStream_t)stream);
 }
 
@@ -365,7 +365,7 @@ int shlo_kv_gather_noalloc(const shlo_kv_pool *pool, const int32_t *tables, int6
                            void *stream) {
   if (!pool) return fail("kv_gather: null descriptor");
   Device *dev;
-  SHLO_TRY(current_device(&dev));
+  SHLO_TRY(calling_device(&dev));
   return launch_kv_gather(*pool, tables, table_stride, seqs, table_pages, seq, pos, n, k, k_token, k_head, v, v_token,
                           v_head, dtype, dev->sm_count, (cudaStream_t)stream);
 }

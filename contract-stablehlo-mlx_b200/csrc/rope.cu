@@ -269,7 +269,7 @@ int shlo_rope_noalloc(const void *x, int64_t x_token, int64_t x_head, const int3
                       void *y, int64_t y_token, int64_t y_head, int64_t tokens, int32_t heads, int32_t dim, int32_t rot,
                       uint8_t dtype, uint32_t flags, float factor, void *stream) {
   Device *dev;
-  SHLO_TRY(current_device(&dev));
+  SHLO_TRY(calling_device(&dev));
   RopeCall c{x, x_token, x_head, positions, phases, y, y_token, y_head, tokens, heads, dim, rot, dtype, flags, factor};
   return launch_rope(c, dev->sm_count, (cudaStream_t)stream);
 }

@@ -124,6 +124,12 @@ int current_device(Device **out) {
   return device_by_id(t_device, out);
 }
 
+int calling_device(Device **out) {
+  int id;
+  SHLO_CUDA(cudaGetDevice(&id));
+  return init_device(id, out);
+}
+
 int current_flavor() {
   int f = g_flavor.load();
   if (f < 0) {

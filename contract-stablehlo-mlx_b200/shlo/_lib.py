@@ -17,7 +17,7 @@ SYMBOLS = [
     "shlo_kernel_apply", "shlo_compile", "shlo_fn_free", "shlo_apply", "shlo_libm_erff_range",
     "shlo_count_nonzero", "shlo_current_stream", "shlo_launch_count", "shlo_device_ptr", "shlo_mul_mat_noalloc",
     "shlo_rope_phases", "shlo_rope_noalloc", "shlo_kv_append_noalloc", "shlo_kv_gather_noalloc",
-    "shlo_kv_attend_workspace", "shlo_kv_attend_noalloc",
+    "shlo_cuda_device", "shlo_kv_attend_workspace", "shlo_kv_attend_noalloc",
     "shlo_kv_new", "shlo_kv_free", "shlo_kv_storage", "shlo_kv_append", "shlo_kv_gather", "shlo_kv_attend",
     "shlo_test_attend_give_up",
 ]
@@ -123,6 +123,7 @@ def load() -> ctypes.CDLL:
     L.shlo_rope_noalloc.argtypes = [p, i64, i64, p, p, p, i64, i64, i64, i32, i32, i32, u8, ctypes.c_uint32, f32, p]
     L.shlo_kv_append_noalloc.argtypes = [pool, batch, p, i64, i64, p, i64, i64, u8, p]
     L.shlo_kv_gather_noalloc.argtypes = [pool, p, i64, i32, i32, p, p, i64, p, i64, i64, p, i64, i64, u8, p]
+    L.shlo_cuda_device.argtypes = []
     L.shlo_kv_attend_workspace.argtypes = [ctypes.POINTER(ctypes.c_size_t)]
     L.shlo_kv_attend_noalloc.argtypes = [pool, batch, p, i64, i64, i32, u8, f32, i32, i32, p, i64, i64, p, p,
                                          ctypes.c_size_t, p]

@@ -192,8 +192,9 @@ int shlo_mul_mat_noalloc(const float *w, const float *x, float *y, int64_t K, in
 /* ---- decoder operators (no counterpart in the reference, whose modules keep nothing between calls) ----
    Rotary positions, a paged key/value cache in 8 bits, and the attention that
    reads it, for hosts that generate token by token. The *_noalloc functions
-   work on caller-owned device memory of the current device, allocate nothing,
-   and queue their work on `stream` (a cudaStream_t; NULL is the default
+   work on caller-owned memory of the device that is current in CUDA
+   (cudaGetDevice, as for shlo_mul_mat_noalloc), allocate nothing, and queue
+   their work on `stream` (a cudaStream_t of that device; NULL is the default
    stream). Activations are float16 or float32 (`dtype`), given by a pointer and
    two strides in values, of a token and of a head; the values of a head are
    contiguous. Indices are int32 on the device. A host that has no memory of
@@ -258,7 +259,9 @@ int shlo_kv_gather_noalloc(const shlo_kv_pool *pool, const int32_t *tables, int6
                            int32_t table_pages, const int32_t *seq, const int32_t *pos, int64_t n, void *k,
                            int64_t k_token, int64_t k_head, void *v, int64_t v_token, int64_t v_head, uint8_t dtype,
                            void *stream);
-/* The bytes of workspace that an attention call needs on the current device. */
+/* The device that is current in CUDA on this thread (-1: none). */
+int shlo_cuda_device(void);
+/* The bytes of workspace that an attention call needs on that device. */
 int shlo_kv_attend_workspace(size_t *bytes);
 /* out = soft_max(scale q k^T) v over the cache, per row of the batch and query
    head; `heads` is a multiple of the cache's, consecutive ones sharing a

@@ -1,5 +1,9 @@
 """The decoder operators on the GPU where a batch or its addresses are unusual; the tolerances of
 tests/test_gpu_decode.py, whose cases these use."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -93,3 +97,28 @@ def test_a_cache_after_a_launch_that_gave_up():
         assert M.to_numpy(cache.attend(q, *batch, scale=0.125)).tobytes() == first.tobytes()
     finally:
         lib.shlo_test_attend_give_up(0)
+
+
+CHILD = r'''
+import sys
+sys.path[:0] = [%r, %r]
+import numpy as np, torch
+from shlo import decode as Dc
+x = torch.randn(4, 2, 16, device="cuda:0")
+out, pos = torch.empty_like(x), torch.zeros(4, dtype=torch.int32, device="cuda:0")
+phases = torch.from_numpy(Dc.rope_phases(16)[0]).cuda()
+Dc.rope_noalloc(x, pos, phases, out)
+torch.cuda.synchronize()
+assert Dc.load().shlo_cuda_device() == torch.cuda.current_device() == 0
+print("RESULT", bool(torch.equal(x, out)), Dc.attend_workspace() > 0)
+'''
+
+
+def test_the_callers_device_is_cudas():
+    """The entry points on caller-owned memory work on the device that is current in CUDA, whatever device the
+    library's own arrays would be on (here one that the machine does not have)."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    env = dict(os.environ, SHLO_DEVICE="63")
+    r = subprocess.run([sys.executable, "-c", CHILD % (root, os.path.join(root, "contract-stablehlo-mlx_b200"))],
+                       capture_output=True, text=True, timeout=200, env=env)
+    assert "RESULT True True" in r.stdout, r.stdout + r.stderr
