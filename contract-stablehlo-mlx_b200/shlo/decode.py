@@ -4,7 +4,8 @@ the attention that reads it, for hosts that generate token by token.
 The *_noalloc functions take device tensors of the caller's own -- objects with
 data_ptr(), shape, stride(), dtype, is_cuda, numel(), element_size() and is_contiguous(), as
 a torch.Tensor has them; nothing here imports torch -- and queue their work on `stream` (a cudaStream_t as
-an integer; 0 is the default stream). They allocate nothing. Every one is one call
+an integer; 0 is the default stream) of the device that is current in CUDA. A tensor of another device is refused,
+as far as it says where it lies (get_device()). They allocate nothing. Every one is one call
 of include/shlo_cuda.h, whose comments say what it computes; errors raise ShloError.
 """
 from __future__ import annotations
@@ -25,9 +26,22 @@ _F16, _F32, _I8, _I32, _I64 = M.dtF16, M.dtF32, M.dtI8, M.dtI32, M.dtI64
 _codes: dict = {}  # a dtype object seen before -> its code (None: not carried)
 
 
-def _code(x):
-    if not x.is_cuda:
-        raise ShloError("a tensor in host memory: the decoder operators take device memory")
+def _device(x, at):
+    """x lies on device `at` (None: on any)."""
+    try:
+        d = x.get_device()
+    except AttributeError:
+        d = at if x.is_cuda else -1
+    if d != at or at == -1:
+        if not x.is_cuda:
+            raise ShloError("a tensor in host memory: the decoder operators take device memory")
+        if at is not None:
+            raise ShloError("a tensor on device %d, but device %d is the current one or the other tensors'" % (d, at))
+    return d
+
+
+def _code(x, at):
+    _device(x, at)
     d = x.dtype
     try:
         return _codes[d]
@@ -47,9 +61,9 @@ def rope_phases(rot: int, base: float = 10000.0, scaling: str = "none", by: floa
     return out, f.value
 
 
-def _rows(x, what):
+def _rows(x, what, at):
     """A float [tokens, heads, dim] whose last axis is contiguous: (shape, strides, type code)."""
-    c, n, s = _code(x), x.shape, x.stride()
+    c, n, s = _code(x, at), x.shape, x.stride()
     if c != _F16 and c != _F32:
         raise ShloError("%s: %s not carried (float16 or float32)" % (what, x.dtype))
     if len(n) != 3:
@@ -59,20 +73,20 @@ def _rows(x, what):
     return n, s, c
 
 
-def _list(x, code, what):
+def _list(x, code, what, at):
     """A contiguous vector of a type: its length."""
     n = x.shape
-    if _code(x) != code or len(n) != 1:
+    if _code(x, at) != code or len(n) != 1:
         raise ShloError("%s: %s of rank %d, a vector of int%d expected" % (what, x.dtype, len(n), 32 if code == M.dtI32 else 64))
     if n[0] > 1 and x.stride()[0] != 1:
         raise ShloError("%s: the last axis is strided" % what)
     return n[0]
 
 
-def _tables(x, what):
+def _tables(x, what, at):
     """int32 [sequences, pages], rows at any distance: (shape, row stride)."""
     n, s = x.shape, x.stride()
-    if _code(x) != _I32 or len(n) != 2:
+    if _code(x, at) != _I32 or len(n) != 2:
         raise ShloError("%s: %s of rank %d, int32 of rank 2 expected" % (what, x.dtype, len(n)))
     if n[1] > 1 and s[1] != 1:
         raise ShloError("%s: the last axis is strided" % what)
@@ -81,40 +95,49 @@ def _tables(x, what):
 
 def rope_noalloc(x, positions, phases, out, *, interleaved=False, inverse=False, factor=1.0, stream=0):
     """x [tokens, heads, dim] turned by positions (int32 [tokens]) into out; phases: rope_phases' on the device."""
-    n, xs, dt = _rows(x, "rope: x")
-    m, ys, dy = _rows(out, "rope: out")
+    lib = load()
+    at = lib.shlo_cuda_device()
+    n, xs, dt = _rows(x, "rope: x", at)
+    m, ys, dy = _rows(out, "rope: out", at)
     if m != n or dy != dt:
         raise ShloError("rope: out is not x's shape and type")
     t, h, d = n
-    if _list(positions, _I32, "rope: positions") != t:
+    if _list(positions, _I32, "rope: positions", at) != t:
         raise ShloError("rope: %d positions for %d tokens" % (positions.shape[0], t))
-    check(load().shlo_rope_noalloc(x.data_ptr(), xs[0], xs[1], positions.data_ptr(), phases.data_ptr(), out.data_ptr(),
-                                   ys[0], ys[1], t, h, d, 2 * _list(phases, _I64, "rope: phases"), dt,
-                                   (1 if interleaved else 0) | (2 if inverse else 0), factor, stream))
+    check(lib.shlo_rope_noalloc(x.data_ptr(), xs[0], xs[1], positions.data_ptr(), phases.data_ptr(), out.data_ptr(),
+                                ys[0], ys[1], t, h, d, 2 * _list(phases, _I64, "rope: phases", at), dt,
+                                (1 if interleaved else 0) | (2 if inverse else 0), factor, stream))
 
 
 class Pool:
     """A paged cache over the caller's tensors: k and v int8 [pages, heads, page_tokens, head_dim] (any strides but
     the last axis's, the same for both), their scales float32 [pages, heads]. Holds on to the tensors."""
 
-    __slots__ = ("c", "keep")
+    __slots__ = ("c", "keep", "device")
 
     def __init__(self, k, v, k_scale, v_scale):
         n, m, s, z = k.shape, k_scale.shape, k.stride(), k_scale.stride()
-        if _code(k) != _I8 or _code(v) != _I8 or len(n) != 4:
+        at = self.device = _device(k, None)
+        if _code(k, at) != _I8 or _code(v, at) != _I8 or len(n) != 4:
             raise ShloError("cache: k and v are int8 [pages, heads, page_tokens, head_dim]")
         if v.shape != n or v.stride() != s or s[3] != 1:
             raise ShloError("cache: k and v differ in shape or strides, or their last axis is strided")
-        if _code(k_scale) != _F32 or _code(v_scale) != _F32 or m != n[:2] or v_scale.shape != m or v_scale.stride() != z:
+        if _code(k_scale, at) != _F32 or _code(v_scale, at) != _F32 or m != n[:2] or v_scale.shape != m or v_scale.stride() != z:
             raise ShloError("cache: the scales are not float32 [pages, heads] with the same strides")
         self.keep = (k, v, k_scale, v_scale)
         self.c = KvPool(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), n[0], s[0], s[1], s[2],
                         z[0], z[1], n[1], n[3], n[2])
 
 
-def _batch(starts, lens, tables, tokens):
-    (n, w), stride = _tables(tables, "batch: tables")
-    a, b = _list(starts, _I32, "batch: starts"), _list(lens, _I32, "batch: lens")
+    def check(self, at):
+        if self.device is not None and self.device != at:
+            raise ShloError("a cache on device %d, but device %d is the current one" % (self.device, at))
+        return self.c
+
+
+def _batch(starts, lens, tables, tokens, at):
+    (n, w), stride = _tables(tables, "batch: tables", at)
+    a, b = _list(starts, _I32, "batch: starts", at), _list(lens, _I32, "batch: lens", at)
     if a != n + 1 or b != n:
         raise ShloError("batch: %d starts and %d lengths for tables of %d sequences" % (a, b, n))
     return KvBatch(starts.data_ptr(), lens.data_ptr(), tables.data_ptr(), stride, n, w, tokens)
@@ -122,25 +145,29 @@ def _batch(starts, lens, tables, tokens):
 
 def append_noalloc(pool: Pool, k, v, starts, lens, tables, *, stream=0):
     """k and v [tokens, heads, dim] rounded into the pages of their sequences."""
-    n, ks, dt = _rows(k, "kv_append: k")
-    m, vs, dv = _rows(v, "kv_append: v")
-    c = pool.c
+    lib = load()
+    at = lib.shlo_cuda_device()
+    n, ks, dt = _rows(k, "kv_append: k", at)
+    m, vs, dv = _rows(v, "kv_append: v", at)
+    c = pool.check(at)
     if m != n or dv != dt or n[1] != c.heads or n[2] != c.head_dim:
         raise ShloError("kv_append: k and v are not [tokens, %d, %d] of one type" % (c.heads, c.head_dim))
-    check(load().shlo_kv_append_noalloc(c, _batch(starts, lens, tables, n[0]), k.data_ptr(), ks[0], ks[1], v.data_ptr(),
-                                        vs[0], vs[1], dt, stream))
+    check(lib.shlo_kv_append_noalloc(c, _batch(starts, lens, tables, n[0], at), k.data_ptr(), ks[0], ks[1], v.data_ptr(),
+                                     vs[0], vs[1], dt, stream))
 
 
 def gather_noalloc(pool: Pool, tables, seq, pos, k, v, *, stream=0):
     """The cache's values of tokens (seq[i], pos[i]) into k and v [n, heads, dim]."""
-    n, ks, dt = _rows(k, "kv_gather: k")
-    m, vs, dv = _rows(v, "kv_gather: v")
-    (seqs, width), stride = _tables(tables, "kv_gather: tables")
-    c, t = pool.c, _list(seq, _I32, "kv_gather: seq")
-    if _list(pos, _I32, "kv_gather: pos") != t or n != (t, c.heads, c.head_dim) or m != n or dv != dt:
+    lib = load()
+    at = lib.shlo_cuda_device()
+    n, ks, dt = _rows(k, "kv_gather: k", at)
+    m, vs, dv = _rows(v, "kv_gather: v", at)
+    (seqs, width), stride = _tables(tables, "kv_gather: tables", at)
+    c, t = pool.check(at), _list(seq, _I32, "kv_gather: seq", at)
+    if _list(pos, _I32, "kv_gather: pos", at) != t or n != (t, c.heads, c.head_dim) or m != n or dv != dt:
         raise ShloError("kv_gather: pos, k and v are not of %d tokens, %d heads of %d" % (t, c.heads, c.head_dim))
-    check(load().shlo_kv_gather_noalloc(c, tables.data_ptr(), stride, seqs, width, seq.data_ptr(), pos.data_ptr(), t,
-                                        k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], dt, stream))
+    check(lib.shlo_kv_gather_noalloc(c, tables.data_ptr(), stride, seqs, width, seq.data_ptr(), pos.data_ptr(), t,
+                                     k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], dt, stream))
 
 
 def attend_workspace() -> int:
@@ -153,24 +180,25 @@ def attend_workspace() -> int:
 def attend_noalloc(pool: Pool, q, starts, lens, tables, out, *, workspace, scale, lse=None, causal=True, window=0,
                    stream=0):
     """q [tokens, query heads, dim] against the cache into out (and lse, float32 [tokens, query heads])."""
-    n, qs, dt = _rows(q, "kv_attend: q")
-    m, os_, do = _rows(out, "kv_attend: out")
+    lib = load()
+    at = lib.shlo_cuda_device()
+    n, qs, dt = _rows(q, "kv_attend: q", at)
+    m, os_, do = _rows(out, "kv_attend: out", at)
     t, h, d = n
-    c = pool.c
+    c = pool.check(at)
     if d != c.head_dim:
         raise ShloError("kv_attend: queries of width %d, the cache's heads are %d wide" % (d, c.head_dim))
     if m != n or do != dt:
         raise ShloError("kv_attend: out is not q's shape and type")
     lp = None
-    if not workspace.is_cuda:
-        raise ShloError("kv_attend: the workspace is in host memory")
+    _device(workspace, at)
     if lse is not None:
-        if _code(lse) != _F32 or lse.shape != (t, h) or (t and h and not lse.is_contiguous()):
+        if _code(lse, at) != _F32 or lse.shape != (t, h) or (t and h and not lse.is_contiguous()):
             raise ShloError("kv_attend: lse is not a contiguous float32 [%d, %d]" % (t, h))
         lp = lse.data_ptr()
-    check(load().shlo_kv_attend_noalloc(c, _batch(starts, lens, tables, t), q.data_ptr(), qs[0], qs[1], h, dt, scale,
-                                        1 if causal else 0, window, out.data_ptr(), os_[0], os_[1], lp,
-                                        workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream))
+    check(lib.shlo_kv_attend_noalloc(c, _batch(starts, lens, tables, t, at), q.data_ptr(), qs[0], qs[1], h, dt, scale,
+                                     1 if causal else 0, window, out.data_ptr(), os_[0], os_[1], lp,
+                                     workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream))
 
 
 # ---- on arrays (mlx.Arr), in the library's own memory ----
