@@ -187,6 +187,8 @@ int launch_check(const char *what);
 extern std::atomic<uint64_t> g_launches;
 // Wait for all queued work of a device (bounded by SHLO_EVAL_TIMEOUT_S).
 int device_wait(Device *dev, const char *what);
+// What an earlier launch on the device reported, told once.
+int launch_error(Device *dev, const char *what);
 
 // The kernels of shlo_kernel_apply, by name (api.cu's table).
 enum KernelKind {

@@ -769,6 +769,7 @@ int shlo_kv_attend_noalloc(const shlo_kv_pool *pool, const shlo_kv_batch *batch,
   if (!pool || !batch) return fail("kv_attend: null descriptor");
   Device *dev;
   SHLO_TRY(calling_device(&dev));
+  SHLO_TRY(launch_error(dev, "kv_attend, an earlier call"));
   AttendCall c{*pool, *batch, q, q_token, q_head, out, out_token, out_head, lse, heads, dtype, scale, causal != 0, window,
                workspace, workspace_bytes, dev->pipe_err_dev};
   return launch_kv_attend(c, dev->sm_count, dev->id, (cudaStream_t)stream);

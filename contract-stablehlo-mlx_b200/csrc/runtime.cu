@@ -400,6 +400,14 @@ int make_contiguous(Arr *a, Arr **out) {
   return 0;
 }
 
+int launch_error(Device *dev, const char *what) {
+  volatile int *perr = dev->pipe_err_host;
+  if (!perr || !*perr) return 0;
+  *perr = 0;
+  return fail("%s: a launch on device %d gave up waiting for its own copies or products (the results "
+              "are not valid)", what, dev->id);
+}
+
 // Wait for all queued work on a device, bounded by SHLO_EVAL_TIMEOUT_S.
 static int wait_stream(Device *dev, cudaStream_t stream, const char *what) {
   static double limit = [] {
@@ -409,15 +417,7 @@ static int wait_stream(Device *dev, cudaStream_t stream, const char *what) {
   auto t0 = std::chrono::steady_clock::now();
   for (int spins = 0;; spins++) {
     cudaError_t e = cudaStreamQuery(stream);
-    if (e == cudaSuccess) {
-      volatile int *perr = dev->pipe_err_host;
-      if (perr && *perr) {
-        *perr = 0;
-        return fail("%s: a launch on device %d gave up waiting for its own copies or products (the results "
-                    "are not valid)", what, dev->id);
-      }
-      return 0;
-    }
+    if (e == cudaSuccess) return launch_error(dev, what);
     if (e != cudaErrorNotReady) return cuda_check(e, what);
     double dt = std::chrono::duration<double>(std::chrono::steady_clock::now() - t0).count();
     if (dt > limit) return fail("%s: device %d did not finish within %.0f s", what, dev->id, limit);

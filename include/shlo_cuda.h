@@ -271,8 +271,9 @@ int shlo_kv_attend_workspace(size_t *bytes);
    (float32 [tokens][heads], or NULL) is the logarithm of the sum of the
    exponentials of the scaled scores. The workspace must be zero before the
    first call that uses it; calls leave it ready for the next, on one stream at
-   a time, those that gave up a wait (which the library's next wait reports)
-   too. The same call gives the same bits. */
+   a time, those that gave up a wait too (which the library's next wait on the
+   device reports, or the next call: it does nothing else then). The same call
+   gives the same bits. */
 int shlo_kv_attend_noalloc(const shlo_kv_pool *pool, const shlo_kv_batch *batch, const void *q, int64_t q_token,
                            int64_t q_head, int32_t heads, uint8_t dtype, float scale, int32_t causal, int32_t window,
                            void *out, int64_t out_token, int64_t out_head, float *lse, void *workspace,

@@ -122,3 +122,23 @@ def test_the_callers_device_is_cudas():
     r = subprocess.run([sys.executable, "-c", CHILD % (root, os.path.join(root, "contract-stablehlo-mlx_b200"))],
                        capture_output=True, text=True, timeout=200, env=env)
     assert "RESULT True True" in r.stdout, r.stdout + r.stderr
+
+
+def test_a_launch_that_gave_up_is_told_by_the_next_call():
+    """Without the library's wait: the next call says so and does nothing, the one after it is right."""
+    c = Case("f16", 16, 1, 8, 64, [3000], [20])
+    work = torch.zeros(Dc.attend_workspace(), dtype=torch.uint8, device="cuda")
+    first = c.run(work=work)
+    lib = load()
+    try:
+        lib.shlo_test_attend_give_up(1)
+        c.run(work=work)
+    finally:
+        lib.shlo_test_attend_give_up(0)
+    torch.cuda.synchronize()
+    out = torch.full(c.q.shape, 9.0, dtype=torch.float16, device="cuda")
+    with pytest.raises(ShloError, match="gave up"):
+        c.run(work=work, out=out)
+    assert bool((out == 9.0).all())
+    again = c.run(work=work)
+    assert again[0].tobytes() == first[0].tobytes() and again[1].tobytes() == first[1].tobytes()
