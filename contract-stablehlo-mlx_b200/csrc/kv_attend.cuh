@@ -47,7 +47,7 @@ struct AttendArgs {
   int64_t above, upto;
   unsigned *counters;  // [2][kAttendMaxBlocks], zero between calls
   float *partials;     // [chunks][2][rows * (dim + 2)]
-  int *err;            // set by a launch that gave up a wait
+  int *err;            // 1: a launch gave up a wait; 2: the batch's starts descend
   unsigned give_up;    // every so many blocks of the tiles give up at once (0: none)
 };
 
@@ -223,7 +223,9 @@ __device__ __forceinline__ bool next_segment(const AttendArgs &a, const BatchArr
 // Lay out the line. All threads call it; NT threads, `sh` shared memory of NT +
 // 4 long longs, `copy` of `room` ints for the batch's arrays (each thread
 // searches them: from global memory every step of a search would wait for L2).
-// False: the block has no work.
+// False: the block has no work. Starts that descend would give the threads, which
+// find their sequences by a search, and the segments, which go on from one to the
+// next, lines that differ: such a batch has no work, and the host is told.
 template <int ROWS, int GRAN, int NT>
 __device__ bool schedule(const AttendArgs &a, int min_gran, long long *sh, int *copy, int room, BatchArrays &ba, Line &c) {
   ba.starts = a.batch.starts;
@@ -235,6 +237,8 @@ __device__ bool schedule(const AttendArgs &a, int min_gran, long long *sh, int *
     ba.starts = copy;
     ba.lens = copy + seqs + 1;
   }
+  int descends = 0;
+  for (int i = threadIdx.x; i < seqs; i += NT) descends |= ba.starts[i] > ba.starts[i + 1];
   const int chunk = (a.slots + NT - 1) / NT;
   const int s0 = min((int)threadIdx.x * chunk, a.slots), s1 = min(s0 + chunk, a.slots);
   long long mine = 0;
@@ -248,7 +252,10 @@ __device__ bool schedule(const AttendArgs &a, int min_gran, long long *sh, int *
     if (lane >= o) sum += v;
   }
   if (lane == 31) sh[warp] = sum;
-  __syncthreads();
+  if (__syncthreads_or(descends)) {
+    if (threadIdx.x == 0 && blockIdx.x == 0 && a.err) *a.err = 2;
+    return false;
+  }
   long long before = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < NT / 32; w++) {

@@ -402,8 +402,10 @@ int make_contiguous(Arr *a, Arr **out) {
 
 int launch_error(Device *dev, const char *what) {
   volatile int *perr = dev->pipe_err_host;
-  if (!perr || !*perr) return 0;
+  const int code = perr ? *perr : 0;
+  if (!code) return 0;
   *perr = 0;
+  if (code == 2) return fail("%s: a batch of an attention on device %d has starts that descend (nothing was computed)", what, dev->id);
   return fail("%s: a launch on device %d gave up waiting for its own copies or products (the results "
               "are not valid)", what, dev->id);
 }

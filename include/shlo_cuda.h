@@ -235,7 +235,8 @@ typedef struct {
 } shlo_kv_pool;
 /* A batch of sequences, all arrays on the device: sequence s has the rows
    starts[s] .. starts[s + 1] - 1 of the call's activations as its newest tokens
-   (starts[0] = 0, ascending; no rows is allowed), lens[s] tokens in all with
+   (ascending; no rows is allowed; an attention over starts that descend computes
+   nothing, and the library's next wait or its next call says so), lens[s] tokens in all with
    them, and page tables[s * table_stride + i] for its tokens
    i * page_tokens ... An entry outside the cache (-1, say) is a page it does
    not have. */

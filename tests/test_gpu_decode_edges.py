@@ -142,3 +142,22 @@ def test_a_launch_that_gave_up_is_told_by_the_next_call():
     assert bool((out == 9.0).all())
     again = c.run(work=work)
     assert again[0].tobytes() == first[0].tobytes() and again[1].tobytes() == first[1].tobytes()
+
+
+@pytest.mark.parametrize("kind", ["f16", "f32"])
+@pytest.mark.parametrize("starts", [[0, 30, 10, 60], [5, 0, 20, 40], [0, 20, 40, 39]])
+def test_starts_that_descend(kind, starts):
+    """Nothing is written, counters stay zero, the next call says what was wrong, and the one after it is right."""
+    c = Case(kind, 16, 2, 4, 64, [500, 200, 90], [30, 20, 10])
+    work = torch.zeros(Dc.attend_workspace(), dtype=torch.uint8, device="cuda")
+    first = c.run(work=work)
+    own, c.starts = c.starts, np.array(starts, np.int32)
+    out = torch.full(c.q.shape, 9.0, dtype=torch.from_numpy(c.q).dtype, device="cuda")
+    c.run(work=work, out=out)
+    assert bool((out == 9.0).all()) and int(work[:8192].to(torch.int32).sum()) == 0
+    c.starts = own
+    with pytest.raises(ShloError, match="descend"):
+        c.run(work=work)
+    again = c.run(work=work)
+    c.check(again)
+    assert again[0].tobytes() == first[0].tobytes() and again[1].tobytes() == first[1].tobytes()
