@@ -12,7 +12,8 @@ int k_rope(Device *dev, Arr *x, Arr *positions, Arr *phases, const uint32_t *p, 
   const int64_t T = p[0], H = p[1], D = p[2], rot = p[3];
   if (positions->dtype != kI32) return fail("shlo_rope: positions of %s, int32 expected", dtype_name(positions->dtype));
   if (phases->dtype != kI64) return fail("shlo_rope: phases of %s, int64 expected", dtype_name(phases->dtype));
-  if (H < 1 || D < 1 || T > 0x7fffffff || H > 0x7fffffff || D > 0x7fffffff || T * H > (int64_t)1 << 40)
+  // (products within 64 bits: the words are the caller's)
+  if (H < 1 || D < 1 || T > 0x7fffffff || H > 0x7fffffff || D > 0x7fffffff || T * H > ((int64_t)1 << 40) / D)
     return fail("shlo_rope: %lld tokens of %lld heads of %lld", (long long)T, (long long)H, (long long)D);
   if (numel(x) != T * H * D || numel(positions) != T || numel(phases) < rot / 2)
     return fail("shlo_rope: %lld values, %lld positions and %lld phases for [%lld, %lld, %lld] and %lld dimensions turned",

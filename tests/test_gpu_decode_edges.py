@@ -13,6 +13,7 @@ torch = pytest.importorskip("torch")
 
 from shlo import decode as Dc  # noqa: E402
 from shlo import mlx as M  # noqa: E402
+from shlo import run as Run  # noqa: E402
 from shlo._lib import ShloError, load  # noqa: E402
 from test_gpu_decode import Case, cuda  # noqa: E402
 
@@ -161,3 +162,14 @@ def test_starts_that_descend(kind, starts):
     again = c.run(work=work)
     c.check(again)
     assert again[0].tobytes() == first[0].tobytes() and again[1].tobytes() == first[1].tobytes()
+
+
+def test_rope_kernel_refuses_sizes_whose_product_wraps():
+    """Parameter words whose product is 2^64 plus the array's size."""
+    pos, phases = M.of_numpy(np.zeros(16, np.int32)), M.of_numpy(np.zeros(1, np.int64))
+    for t, h, d, n in ((16, 1 << 30, 1 << 30, 0), (5, 1 << 20, 1 << 30, 5), (16, 1 << 20, 1 << 21, 16)):
+        x = M.of_numpy(np.zeros(n, np.float32))
+        words = Run.params([t, h, d, 2, 0, 0x3F800000])
+        p = M.of_numpy(np.zeros(t, np.int32)) if t != 16 else pos
+        with pytest.raises(ShloError, match="tokens of"):
+            M.kernel_apply(Run.kernel("rope"), [x, p, phases, words], [[t, h, d]], bytes([M.dtF32]), [1, 1, 1], [64, 1, 1])
