@@ -85,7 +85,7 @@ __device__ __forceinline__ int row_hi(const AttendArgs &a, int keys, int pos) {
   return a.causal ? max(0, min(keys, pos + 1)) : keys;
 }
 __device__ __forceinline__ int row_lo(const AttendArgs &a, int pos) {
-  return a.window ? max(0, pos - a.window + 1) : 0;
+  return a.window && pos >= a.window ? pos - a.window + 1 : 0;  // (pos may be negative)
 }
 
 // The tile of a slot; returns its granules (0: the slot has no tile here).

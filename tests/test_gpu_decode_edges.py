@@ -173,3 +173,15 @@ def test_rope_kernel_refuses_sizes_whose_product_wraps():
         p = M.of_numpy(np.zeros(t, np.int32)) if t != 16 else pos
         with pytest.raises(ShloError, match="tokens of"):
             M.kernel_apply(Run.kernel("rope"), [x, p, phases, words], [[t, h, d]], bytes([M.dtF32]), [1, 1, 1], [64, 1, 1])
+
+
+@pytest.mark.parametrize("kind", ["f16", "f32"])
+@pytest.mark.parametrize("news", [[7, 1], [90, 3]])
+def test_the_widest_windows_and_rows_before_position_0(kind, news):
+    """A window of 2^31 - 1 is none, for rows before position 0 too (which see every key where nothing is causal)."""
+    c = Case(kind, 16, 2, 4, 64, [3, 40], news)
+    for window in (2 ** 31 - 1, 2 ** 31 - 2, 2 ** 31 - 100):
+        for causal in (False, True):
+            got, whole = c.run(causal, window), c.run(causal, 0)
+            c.check(whole, causal, 0)
+            assert got[0].tobytes() == whole[0].tobytes() and got[1].tobytes() == whole[1].tobytes()
