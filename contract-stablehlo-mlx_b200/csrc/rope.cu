@@ -151,6 +151,28 @@ void launch(const RopeArgs &a, bool inter, dim3 grid, size_t smem, cudaStream_t 
     k_rope<T, VEC, false><<<grid, kRopeThreads, smem, st>>>(a);
 }
 
+// Whether x and y have a value in common, y not being x itself (blocks then read
+// what others have written). Where their extents overlap they need the same
+// strides to have none: it comes down to one distance between rows.
+bool overlap(const RopeCall &c, size_t size) {
+  const int64_t off = ((intptr_t)c.y - (intptr_t)c.x) / (int64_t)size, T = c.tokens, H = c.heads, D = c.dim;
+  auto low = [](int64_t n, int64_t s) { return s < 0 ? (double)(n - 1) * s : 0.0; };
+  auto high = [](int64_t n, int64_t s) { return s > 0 ? (double)(n - 1) * s : 0.0; };
+  const double x0 = low(T, c.x_token) + low(H, c.x_head), x1 = high(T, c.x_token) + high(H, c.x_head) + D;
+  const double y0 = off + low(T, c.y_token) + low(H, c.y_head), y1 = off + high(T, c.y_token) + high(H, c.y_head) + D;
+  if (y1 <= x0 || x1 <= y0) return false;
+  if ((T > 1 && c.x_token != c.y_token) || (H > 1 && c.x_head != c.y_head)) return true;
+  const bool by_heads = H <= T;  // the shorter axis is gone through, the other solved for
+  const int64_t n1 = by_heads ? H : T, s1 = by_heads ? c.x_head : c.x_token;
+  const int64_t n2 = by_heads ? T : H, s2 = by_heads ? c.x_token : c.x_head;
+  for (int64_t i = 1 - n1; i < n1; i++) {
+    const int64_t r = off - i * s1, j0 = s2 && n2 > 1 ? r / s2 : 0;
+    for (int64_t j = j0 - 1; j <= j0 + 1; j++)
+      if (j > -n2 && j < n2 && llabs(r - j * s2) < D) return true;
+  }
+  return false;
+}
+
 }  // namespace
 
 int launch_rope(const RopeCall &c, int sms, cudaStream_t st) {
@@ -168,6 +190,7 @@ int launch_rope(const RopeCall &c, int sms, cudaStream_t st) {
   const bool same = c.x == c.y;
   if (same && (c.x_token != c.y_token || c.x_head != c.y_head))
     return fail("rope: x and y share storage with different strides");
+  if (!same && overlap(c, size)) return fail("rope: x and y overlap (y is x itself, or shares no value with it)");
   const int half = c.rot / 2, rest = same ? 0 : c.dim - c.rot;
   if (half == 0 && rest == 0) return 0;
   // The widest vector (16 bytes at most) that every offset is a multiple of.

@@ -212,7 +212,9 @@ int shlo_rope_phases(int32_t rot, double base, int32_t scaling, double by, doubl
                      int64_t *phases, float *factor);
 /* Turn the first `rot` of `dim` dimensions of x[tokens][heads][dim] by each
    token's position into y, the others copied:
-   (a, b) -> factor (a cos - b sin, b cos + a sin). y may be x itself. flags: 1
+   (a, b) -> factor (a cos - b sin, b cos + a sin). y may be x itself; else they
+   share no value, and have the same strides where one lies among the other's
+   rows. flags: 1
    pairs side by side (2i, 2i + 1) instead of half the part apart
    (i, i + rot / 2); 2 turned back (the gradient of the turn). Positions may be
    negative; angles are exact to 2^-32 turns at every position. */

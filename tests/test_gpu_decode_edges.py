@@ -185,3 +185,49 @@ def test_the_widest_windows_and_rows_before_position_0(kind, news):
             got, whole = c.run(causal, window), c.run(causal, 0)
             c.check(whole, causal, 0)
             assert got[0].tobytes() == whole[0].tobytes() and got[1].tobytes() == whole[1].tobytes()
+
+
+def test_rope_refuses_overlapping_storage():
+    """Views of one buffer, against their values' places counted one by one: what shares a value is refused, what does
+    not is right (in place too); only views of different strides inside each other's extent are refused untested."""
+    rng = np.random.default_rng(11)
+    buf = cuda(rng.standard_normal(700).astype(np.float32))
+    keep = buf.clone()
+    phases = cuda(Dc.rope_phases(4)[0])
+    taken = refused = 0
+    for _ in range(400):
+        T, H, D = (int(n) for n in rng.integers(1, 5, 3) + [0, 0, 3])
+        sh = int(rng.integers(D, 2 * D + 3)) if rng.integers(2) else int(rng.integers(T * D, T * D + 9))
+        st = int(rng.integers(H * sh, H * sh + 20)) if sh < T * D or T == 1 else int(rng.integers(D, sh // T + 1))
+        span = (T - 1) * st + (H - 1) * sh + D
+        if span > 300:
+            continue
+        same = bool(rng.integers(4))
+        tt, hh = (st, sh) if same else (st + int(rng.integers(3)), sh + int(rng.integers(3)))
+        ox = int(rng.integers(200))
+        oy = ox + int(rng.integers(-min(ox, span + 9), span + 9))
+        x, y = buf.as_strided((T, H, D), (st, sh, 1), ox), buf.as_strided((T, H, D), (tt, hh, 1), oy)
+        at = [{o + t * a + h * b + d for t in range(T) for h in range(H) for d in range(D)}
+              for o, a, b in ((ox, st, sh), (oy, tt, hh))]
+        alike = ox == oy and (st, sh) == (tt, hh)
+        # the same places by other strides of axes of one
+        shares = bool(at[0] & at[1]) and not alike
+        inside = max(at[0]) >= min(at[1]) and max(at[1]) >= min(at[0])
+        differ = (T > 1 and st != tt) or (H > 1 and sh != hh)
+        buf.copy_(keep)
+        pos = cuda(rng.integers(0, 99, T).astype(np.int32))
+        want = torch.empty(T, H, D, device="cuda")
+        Dc.rope_noalloc(x, pos, phases, want)
+        if shares or (inside and differ) or (ox == oy and not alike):
+            refused += 1
+            with pytest.raises(ShloError, match="overlap|share storage"):
+                Dc.rope_noalloc(x, pos, phases, y)
+            assert torch.equal(buf, keep)
+        else:
+            taken += 1
+            Dc.rope_noalloc(x, pos, phases, y)
+            assert torch.equal(y, want)
+            out = torch.ones(700, dtype=torch.bool)
+            out[sorted(at[1])] = False
+            assert torch.equal(buf.cpu()[out], keep.cpu()[out])
+    assert taken > 50 and refused > 50
