@@ -6,9 +6,11 @@
 //
 // Angles: a frequency is kept as a phase, the turns it makes per position as a
 // 64-bit fraction. position * phase wraps at whole turns, exactly, in integers;
-// its upper 32 bits are the signed fraction of a turn that sincospif takes. A
-// 32-bit product of position and frequency would be off by 0.06 rad at position
-// 10^6; this one by position * 2^-64 turns, and no 64-bit float is used.
+// its upper 32 bits are the signed fraction of a turn, which sincospif takes as a
+// binary32 number: 2^-26 turns off at most near half a turn, less nearer 0, and
+// the phase's own rounding adds position * 2^-65 (2^-34 at 2^31). A 32-bit product
+// of position and frequency would be off by 0.06 rad at position 10^6, and no
+// 64-bit float is used.
 //
 // Bound: bytes (each value read once and written once). A block computes the
 // cosines and sines of its tokens once, into shared memory, for all heads.

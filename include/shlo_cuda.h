@@ -214,10 +214,10 @@ int shlo_rope_phases(int32_t rot, double base, int32_t scaling, double by, doubl
    token's position into y, the others copied:
    (a, b) -> factor (a cos - b sin, b cos + a sin). y may be x itself; else they
    share no value, and have the same strides where one lies among the other's
-   rows. flags: 1
-   pairs side by side (2i, 2i + 1) instead of half the part apart
+   rows. flags: 1 pairs side by side (2i, 2i + 1) instead of half the part apart
    (i, i + rot / 2); 2 turned back (the gradient of the turn). Positions may be
-   negative; angles are exact to 2^-32 turns at every position. */
+   negative; an angle is within 2^-25 turns of position times frequency at every
+   position. */
 int shlo_rope_noalloc(const void *x, int64_t x_token, int64_t x_head, const int32_t *positions, const int64_t *phases,
                       void *y, int64_t y_token, int64_t y_head, int64_t tokens, int32_t heads, int32_t dim, int32_t rot,
                       uint8_t dtype, uint32_t flags, float factor, void *stream);

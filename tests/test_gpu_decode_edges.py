@@ -15,7 +15,7 @@ from shlo import decode as Dc  # noqa: E402
 from shlo import mlx as M  # noqa: E402
 from shlo import run as Run  # noqa: E402
 from shlo._lib import ShloError, load  # noqa: E402
-from test_gpu_decode import Case, cuda  # noqa: E402
+from test_gpu_decode import Case, cuda, rope_close  # noqa: E402
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -231,3 +231,27 @@ def test_rope_refuses_overlapping_storage():
             out[sorted(at[1])] = False
             assert torch.equal(buf.cpu()[out], keep.cpu()[out])
     assert taken > 50 and refused > 50
+
+
+@pytest.mark.parametrize("inverse", [False, True])
+def test_rope_angles_at_every_position(inverse):
+    """Positions over all of int32 against turns in exact integers, position * phase mod 2^64: the tolerance of small
+    positions (2^-20 of a pair's magnitude: 2^-26 turns are 2^-23.3 rad, and the sine's own error is less)."""
+    rng = np.random.default_rng(12)
+    T, D = 4000, 128
+    edge = [0, 1, -1, 2 ** 31 - 1, -2 ** 31, 2 ** 30, 2 ** 24 + 1]
+    pos = np.concatenate([edge, rng.integers(-2 ** 31, 2 ** 31, T - len(edge))]).astype(np.int32)
+    x = rng.standard_normal((T, 1, D)).astype(np.float32)
+    phases, _ = Dc.rope_phases(D, 500000.0)
+    out = torch.empty(T, 1, D, device="cuda")
+    Dc.rope_noalloc(cuda(x), cuda(pos), cuda(phases), out, inverse=inverse)
+    # the fraction of a turn, 53 bits of it, in [-1/2, 1/2)
+    whole = pos.astype(np.int64)[:, None].view(np.uint64) * phases.view(np.uint64)[None, :]
+    a = whole.view(np.int64).astype(np.float64) * 2.0 ** -63 * np.pi
+    c, s = np.cos(a)[:, None], np.sin(a)[:, None] * (-1 if inverse else 1)
+    lo, hi = x[..., :D // 2].astype(np.float64), x[..., D // 2:].astype(np.float64)
+    want = np.concatenate([lo * c - hi * s, hi * c + lo * s], -1)
+    rope_close(out.cpu().numpy(), want, x, np.zeros(D // 2), 1.0, False, "f32")
+    # the phases are those of the frequencies: 2^-65 turns a position each, and the 64-bit oracle's own 2^-52
+    freqs = 500000.0 ** (-2.0 * np.arange(D // 2) / D)
+    assert np.all(np.abs(phases.astype(np.float64) / 2.0 ** 64 * 2 * np.pi - freqs) <= 2.0 ** -48 * freqs + 2.0 ** -62)
