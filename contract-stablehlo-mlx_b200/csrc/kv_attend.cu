@@ -24,7 +24,10 @@
 // are not at one too) and the last blocks' ends. Two or four blocks an SM
 // measured 231 and 227 us for the first.
 //
-// Precision. Scores, maxima, sums and outputs are kept in 32 bits. The weights
+// Precision. Scores, maxima, sums and outputs are kept in 32 bits, outputs as
+// rounding adds of sixteen keys' products (sums that the matrix instructions
+// carry on lose up to 2^-23 of themselves each time, always downwards: 3e-4 over
+// 200000 keys; the adds cost 0.5 %). The weights
 // are rounded to float16 for the second product, as e^(s - m) (sv / largest sv
 // so far) 2^14: at most 2^14 and, since float16 reaches down to 2^-24, exact to
 // 2^-38 of the largest weight (of the largest value's scale among the keys of the
@@ -538,28 +541,20 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DP, NT>::PER_SM) k_kv_atten
           const uint32_t a23 = __byte_perm(x2, x3, 0x5140), b23 = __byte_perm(x2, x3, 0x7362);
           const uint32_t f0[4] = {half_pair<0x4140>(a01), half_pair<0x4342>(a01), half_pair<0x4140>(a23), half_pair<0x4342>(a23)};
           const uint32_t f1[4] = {half_pair<0x4140>(b01), half_pair<0x4342>(b01), half_pair<0x4140>(b23), half_pair<0x4342>(b23)};
-          if constexpr (TERMS == 1) {
+          // Over thousands of keys the instructions' cut-off bits would add up (they
+          // all point one way): sixteen keys' sums are added to O by rounding adds.
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-              mma16816(o[nt][2 * w], f0, pb[0][nt][0], pb[0][nt][1]);
-              mma16816(o[nt][2 * w + 1], f1, pb[0][nt][0], pb[0][nt][1]);
+          for (int nt = 0; nt < NT; nt++) {
+            float t0[4] = {}, t1[4] = {};
+#pragma unroll
+            for (int tm = TERMS - 1; tm >= 0; tm--) {
+              mma16816(t0, f0, pb[tm][nt][0], pb[tm][nt][1]);
+              mma16816(t1, f1, pb[tm][nt][0], pb[tm][nt][1]);
             }
-          } else {
-            // Over thousands of keys the instructions' cut-off bits would add up (they
-            // all point one way): sixteen keys' sums are added to O by rounding adds.
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-              float t0[4] = {}, t1[4] = {};
-#pragma unroll
-              for (int tm = TERMS - 1; tm >= 0; tm--) {
-                mma16816(t0, f0, pb[tm][nt][0], pb[tm][nt][1]);
-                mma16816(t1, f1, pb[tm][nt][0], pb[tm][nt][1]);
-              }
-#pragma unroll
-              for (int j = 0; j < 4; j++) {
-                o[nt][2 * w][j] += t0[j];
-                o[nt][2 * w + 1][j] += t1[j];
-              }
+            for (int j = 0; j < 4; j++) {
+              o[nt][2 * w][j] += t0[j];
+              o[nt][2 * w + 1][j] += t1[j];
             }
           }
         }

@@ -255,3 +255,38 @@ def test_rope_angles_at_every_position(inverse):
     # the phases are those of the frequencies: 2^-65 turns a position each, and the 64-bit oracle's own 2^-52
     freqs = 500000.0 ** (-2.0 * np.arange(D // 2) / D)
     assert np.all(np.abs(phases.astype(np.float64) / 2.0 ** 64 * 2 * np.pi - freqs) <= 2.0 ** -48 * freqs + 2.0 ** -62)
+
+
+def drift(kind, seqs, new, length, group=4, D=128, rows=4):
+    """The mean signed error, relative, of the newest tokens of some sequences that share one long run of pages, whose
+    values are all positive; against 64 bits, on the device."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    page = 256
+    pages = -(-length // page)
+
+    def ints(mean):
+        return (torch.randn(pages, 1, page, D, generator=g, device="cuda") * 20 + mean).round().clamp(-127, 127).to(torch.int8)
+    k, v, scale = ints(0), ints(60).abs_(), torch.full((pages, 1), 0.02, device="cuda")
+    tables = torch.arange(pages, dtype=torch.int32, device="cuda").expand(seqs, pages).contiguous()
+    starts, lens = torch.arange(seqs + 1, dtype=torch.int32, device="cuda") * new, torch.full((seqs,), length, dtype=torch.int32, device="cuda")
+    q = torch.randn(seqs * new, group, D, generator=g, device="cuda").to(torch.float16 if kind == "f16" else torch.float32)
+    out, work = torch.empty_like(q), torch.zeros(Dc.attend_workspace(), dtype=torch.uint8, device="cuda")
+    Dc.attend_noalloc(Dc.Pool(k, v, scale, scale), q, starts, lens, tables, out, scale=D ** -0.5, workspace=work)
+    kk, vv = (a.reshape(-1, D)[:length].double() * scale[0, 0].double() for a in (k, v))
+    errors = []
+    for s in range(0, seqs, seqs // rows):
+        at = s * new + new - 1
+        want = (q[at].double() @ kk.T * D ** -0.5).softmax(-1) @ vv
+        errors.append(((out[at].double() - want) / want).mean().item())
+    return float(np.mean(errors))
+
+
+@pytest.mark.parametrize("kind,bound", [("f16", 2.0 ** -13), ("f32", 2.0 ** -20)])
+def test_sums_over_long_units_do_not_drift(kind, bound):
+    """200 000 keys that no cut shares out among blocks (there are as many units as blocks). Errors that all point one
+    way show in the mean: a matrix instruction cuts up to 2^-23 of a sum off, so 3125 of them in a row 2^-11.4. What
+    may stay: the mean of 2048 results' roundings (2^-11 each, at random: 5 sigma are 2^-16; float32's 2^-24), and of
+    the weights' (at random over the keys), with room for the products of one stretch of 4096 keys (2^-15). A float32
+    call's weights and sums are rounded to 22 bits and more, at random: 2^-20 is several times a single rounding."""
+    blocks = 3 * torch.cuda.get_device_properties(0).multi_processor_count
+    assert abs(drift(kind, blocks, 1, 200000)) <= bound
