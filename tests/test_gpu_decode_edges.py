@@ -290,3 +290,9 @@ def test_sums_over_long_units_do_not_drift(kind, bound):
     call's weights and sums are rounded to 22 bits and more, at random: 2^-20 is several times a single rounding."""
     blocks = 3 * torch.cuda.get_device_properties(0).multi_processor_count
     assert abs(drift(kind, blocks, 1, 200000)) <= bound
+
+
+def test_tiles_sums_over_long_units_do_not_drift():
+    """The same bound for prompts: 64 new tokens of as many sequences as there are blocks, 12500 products a row."""
+    blocks = torch.cuda.get_device_properties(0).multi_processor_count
+    assert abs(drift("f16", blocks, 64, 200000)) <= 2.0 ** -13
