@@ -22,18 +22,19 @@
 // are the choice's cost: 2^-12 of each weight.
 //
 // The products cut up to 2^-23 of O off each time, always downwards: 1.2e-3 over
-// 200000 keys. So O is set aside every 4096 keys and the stretches are summed by
-// rounding adds (2e-5 stays), in the workspace, a row of 16 bytes a thread beside
-// its neighbours': 2.3 us a stretch. Rows of a thread's own, 512 bytes apart, took
-// 11; stretches of 8192 keys keep 5e-5 for 1 % less time.
+// 200000 keys. So O is set aside every 8192 keys and the stretches are summed by
+// rounding adds (5e-5 stays, a fifth of a float16 result's own rounding), in the
+// workspace, 16 bytes a thread beside its neighbours': 2.3 us a stretch. Rows of a
+// thread's own, 512 bytes apart, took 11; stretches of 4096 keys keep 2e-5, and a
+// prompt over 8192 keys then takes 420 us instead of 410.
 //
 // Bound: the softmax warps (2200 cycles of a tile's 3350: the exponentials, one
 // for 4 D flops, and what goes with them, on schedulers that the conversions
 // share), then a segment's beginning and end, which nothing overlaps (about 20
 // us; a block has a few). Measured on one B200, 32 query and 8 key/value heads of
-// 128: 512 new tokens of 4 sequences over 8192 keys (266 GFLOP) 404 us, 659
-// TFLOP/s; 4096 tokens on their own (137 GFLOP) 378 us, 364 TFLOP/s; prompts of
-// three sequences (207 GFLOP) 395 us. Measured and left: one block of 128 rows
+// 128: 512 new tokens of 4 sequences over 8192 keys (266 GFLOP) 410 us, 649
+// TFLOP/s; 4096 tokens on their own (137 GFLOP) 376 us, 366 TFLOP/s; prompts of
+// three sequences (207 GFLOP) 401 us. Measured and left: one block of 128 rows
 // twice on an SM, each converting for itself (346 TFLOP/s on the first case);
 // products issued in a fixed order (head-of-line waits: 599 us against 499);
 // descriptors as 64-bit sums (907 cycles to issue eight products against 541).
@@ -197,7 +198,7 @@ struct Tiles {
   static constexpr int GROUPS = KT / 16;
   static constexpr int META = 2 * GROUPS + 4;      // a tile's scales of keys and of values, its holes, whether the scores need care
   static constexpr int NM = 8;                     // such sets: those asked for (RS), converted (NS) and under the softmax
-  static constexpr int STRETCH = 4096 / KT;        // tiles whose products O sums up before it is set aside
+  static constexpr int STRETCH = 8192 / KT;        // tiles whose products O sums up before it is set aside
   static constexpr int BATCH = 1024;
   static constexpr int MISC = 256 + (THREADS + 4) * 8 + 64 + BATCH * 4 + NM * META * 4 + 64;
   static constexpr int BYTES = 1024 + RT * Q_BYTES + 2 * NS * K_BYTES + RS * K_BYTES + MISC;

@@ -286,7 +286,7 @@ def test_sums_over_long_units_do_not_drift(kind, bound):
     """200 000 keys that no cut shares out among blocks (there are as many units as blocks). Errors that all point one
     way show in the mean: a matrix instruction cuts up to 2^-23 of a sum off, so 3125 of them in a row 2^-11.4. What
     may stay: the mean of 2048 results' roundings (2^-11 each, at random: 5 sigma are 2^-16; float32's 2^-24), and of
-    the weights' (at random over the keys), with room for the products of one stretch of 4096 keys (2^-15). A float32
+    the weights' (at random over the keys), with room for the products of one stretch of 8192 keys (2^-14). A float32
     call's weights and sums are rounded to 22 bits and more, at random: 2^-20 is several times a single rounding."""
     blocks = 3 * torch.cuda.get_device_properties(0).multi_processor_count
     assert abs(drift(kind, blocks, 1, 200000)) <= bound
