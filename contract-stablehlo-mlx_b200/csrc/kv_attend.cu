@@ -744,7 +744,7 @@ extern "C" {
 
 int shlo_cuda_device(void) {
   int id;
-  return cudaGetDevice(&id) == cudaSuccess ? id : -1;
+  return cudaGetDevice(&id) == cudaSuccess ? id : -2;
 }
 
 int shlo_kv_attend_workspace(size_t *bytes) {

@@ -26,22 +26,20 @@ _F16, _F32, _I8, _I32, _I64 = M.dtF16, M.dtF32, M.dtI8, M.dtI32, M.dtI64
 _codes: dict = {}  # a dtype object seen before -> its code (None: not carried)
 
 
-def _device(x, at):
-    """x lies on device `at` (None: on any)."""
-    try:
-        d = x.get_device()
-    except AttributeError:
-        d = at if x.is_cuda else -1
-    if d != at or at == -1:
-        if not x.is_cuda:
-            raise ShloError("a tensor in host memory: the decoder operators take device memory")
-        if at is not None:
-            raise ShloError("a tensor on device %d, but device %d is the current one or the other tensors'" % (d, at))
-    return d
+def _elsewhere(x, at):
+    """x does not lie on device `at`, or does not say."""
+    if not x.is_cuda:
+        raise ShloError("a tensor in host memory: the decoder operators take device memory")
+    if at is not None and hasattr(x, "get_device"):
+        raise ShloError("a tensor on device %d, but device %d is the current one or the other tensors'" % (x.get_device(), at))
 
 
 def _code(x, at):
-    _device(x, at)
+    try:
+        if x.get_device() != at:
+            _elsewhere(x, at)
+    except AttributeError:
+        _elsewhere(x, at)
     d = x.dtype
     try:
         return _codes[d]
@@ -117,7 +115,9 @@ class Pool:
 
     def __init__(self, k, v, k_scale, v_scale):
         n, m, s, z = k.shape, k_scale.shape, k.stride(), k_scale.stride()
-        at = self.device = _device(k, None)
+        at = self.device = k.get_device() if hasattr(k, "get_device") else None
+        if not k.is_cuda:
+            _elsewhere(k, at)
         if _code(k, at) != _I8 or _code(v, at) != _I8 or len(n) != 4:
             raise ShloError("cache: k and v are int8 [pages, heads, page_tokens, head_dim]")
         if v.shape != n or v.stride() != s or s[3] != 1:
@@ -129,10 +129,9 @@ class Pool:
                         z[0], z[1], n[1], n[3], n[2])
 
 
-    def check(self, at):
-        if self.device is not None and self.device != at:
-            raise ShloError("a cache on device %d, but device %d is the current one" % (self.device, at))
-        return self.c
+def _pool(pool, at):
+    if pool.device is not None:
+        raise ShloError("a cache on device %d, but device %d is the current one" % (pool.device, at))
 
 
 def _batch(starts, lens, tables, tokens, at):
@@ -149,7 +148,9 @@ def append_noalloc(pool: Pool, k, v, starts, lens, tables, *, stream=0):
     at = lib.shlo_cuda_device()
     n, ks, dt = _rows(k, "kv_append: k", at)
     m, vs, dv = _rows(v, "kv_append: v", at)
-    c = pool.check(at)
+    c = pool.c
+    if pool.device != at:
+        _pool(pool, at)
     if m != n or dv != dt or n[1] != c.heads or n[2] != c.head_dim:
         raise ShloError("kv_append: k and v are not [tokens, %d, %d] of one type" % (c.heads, c.head_dim))
     check(lib.shlo_kv_append_noalloc(c, _batch(starts, lens, tables, n[0], at), k.data_ptr(), ks[0], ks[1], v.data_ptr(),
@@ -163,7 +164,9 @@ def gather_noalloc(pool: Pool, tables, seq, pos, k, v, *, stream=0):
     n, ks, dt = _rows(k, "kv_gather: k", at)
     m, vs, dv = _rows(v, "kv_gather: v", at)
     (seqs, width), stride = _tables(tables, "kv_gather: tables", at)
-    c, t = pool.check(at), _list(seq, _I32, "kv_gather: seq", at)
+    c, t = pool.c, _list(seq, _I32, "kv_gather: seq", at)
+    if pool.device != at:
+        _pool(pool, at)
     if _list(pos, _I32, "kv_gather: pos", at) != t or n != (t, c.heads, c.head_dim) or m != n or dv != dt:
         raise ShloError("kv_gather: pos, k and v are not of %d tokens, %d heads of %d" % (t, c.heads, c.head_dim))
     check(lib.shlo_kv_gather_noalloc(c, tables.data_ptr(), stride, seqs, width, seq.data_ptr(), pos.data_ptr(), t,
@@ -185,13 +188,19 @@ def attend_noalloc(pool: Pool, q, starts, lens, tables, out, *, workspace, scale
     n, qs, dt = _rows(q, "kv_attend: q", at)
     m, os_, do = _rows(out, "kv_attend: out", at)
     t, h, d = n
-    c = pool.check(at)
+    c = pool.c
+    if pool.device != at:
+        _pool(pool, at)
     if d != c.head_dim:
         raise ShloError("kv_attend: queries of width %d, the cache's heads are %d wide" % (d, c.head_dim))
     if m != n or do != dt:
         raise ShloError("kv_attend: out is not q's shape and type")
     lp = None
-    _device(workspace, at)
+    try:
+        if workspace.get_device() != at:
+            _elsewhere(workspace, at)
+    except AttributeError:
+        _elsewhere(workspace, at)
     if lse is not None:
         if _code(lse, at) != _F32 or lse.shape != (t, h) or (t and h and not lse.is_contiguous()):
             raise ShloError("kv_attend: lse is not a contiguous float32 [%d, %d]" % (t, h))

@@ -262,7 +262,8 @@ int shlo_kv_gather_noalloc(const shlo_kv_pool *pool, const int32_t *tables, int6
                            int32_t table_pages, const int32_t *seq, const int32_t *pos, int64_t n, void *k,
                            int64_t k_token, int64_t k_head, void *v, int64_t v_token, int64_t v_head, uint8_t dtype,
                            void *stream);
-/* The device that is current in CUDA on this thread (-1: none). */
+/* The device that is current in CUDA on this thread (-2: none; -1 is how many
+   libraries name host memory). */
 int shlo_cuda_device(void);
 /* The bytes of workspace that an attention call needs on that device. */
 int shlo_kv_attend_workspace(size_t *bytes);
