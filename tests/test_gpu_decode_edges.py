@@ -3,6 +3,7 @@ tests/test_gpu_decode.py, whose cases these use."""
 import os
 import subprocess
 import sys
+import threading
 
 import numpy as np
 import pytest
@@ -102,6 +103,7 @@ def test_a_cache_after_a_launch_that_gave_up():
 
 CHILD = r'''
 import sys
+import threading
 sys.path[:0] = [%r, %r]
 import numpy as np, torch
 from shlo import decode as Dc
@@ -296,3 +298,31 @@ def test_tiles_sums_over_long_units_do_not_drift():
     """The same bound for prompts: 64 new tokens of as many sequences as there are blocks, 12500 products a row."""
     blocks = torch.cuda.get_device_properties(0).multi_processor_count
     assert abs(drift("f16", blocks, 64, 200000)) <= 2.0 ** -13
+
+
+def test_threads_on_one_cache():
+    """Host threads that attend over one cache at once (and share the library's workspace): each gets its own bits."""
+    rng = np.random.default_rng(6)
+    n = 500
+    cache = Dc.Cache(32, 2, 64, 16)
+    kv = M.of_numpy(rng.standard_normal((n, 2, 64)).astype(np.float16))
+    whole = [M.of_numpy(a) for a in (np.array([0, n], np.int32), np.array([n], np.int32), np.arange(32, dtype=np.int32)[None])]
+    cache.append(kv, kv, *whole)
+    work = []
+    for t in (1, 3, 100, n):
+        q = M.of_numpy(rng.standard_normal((t, 8, 64)).astype(np.float16))
+        batch = [M.of_numpy(np.array([0, t], np.int32))] + whole[1:]
+        work.append((q, batch, M.to_numpy(cache.attend(q, *batch, scale=0.125)).tobytes()))
+    wrong = []
+
+    def run(q, batch, want):
+        M.set_device(0)
+        for _ in range(40):
+            if M.to_numpy(cache.attend(q, *batch, scale=0.125)).tobytes() != want:
+                wrong.append(len(want))
+    threads = [threading.Thread(target=run, args=w) for w in work * 2]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
