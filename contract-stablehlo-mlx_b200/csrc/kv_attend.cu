@@ -567,7 +567,6 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DP, NT>::PER_SM) k_kv_atten
     const bool more = next_segment<ROWS, GRAN>(a, ba, p, ns);
     if (more) pages = begin(ns, buf ^ 1);
 
-    const float unscale = vmax * 0x1p-14f;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -586,8 +585,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DP, NT>::PER_SM) k_kv_atten
         for (int w = 0; w < VW; w++) {
           const int d = VW == 2 ? 8 * g + 4 * w : 128 * (w / 4) + 16 * g + 4 * (w % 4);
           *reinterpret_cast<float4 *>(dst + d) =
-              make_float4(o[nt][2 * w][e] * unscale, o[nt][2 * w][2 + e] * unscale, o[nt][2 * w + 1][e] * unscale,
-                          o[nt][2 * w + 1][2 + e] * unscale);
+              make_float4(o[nt][2 * w][e] * 0x1p-14f * vmax, o[nt][2 * w][2 + e] * 0x1p-14f * vmax,
+                          o[nt][2 * w + 1][e] * 0x1p-14f * vmax, o[nt][2 * w + 1][2 + e] * 0x1p-14f * vmax);
         }
       }
     __syncthreads();

@@ -12,6 +12,7 @@ pytestmark = pytest.mark.gpu
 
 torch = pytest.importorskip("torch")
 
+import decode_oracle as O  # noqa: E402
 from shlo import decode as Dc  # noqa: E402
 from shlo import mlx as M  # noqa: E402
 from shlo import run as Run  # noqa: E402
@@ -326,3 +327,17 @@ def test_threads_on_one_cache():
     for t in threads:
         t.join()
     assert not wrong
+
+
+@pytest.mark.parametrize("exponent", [-125, -120, -113, -60, 100])
+def test_float32_values_of_every_size(exponent):
+    """Value scales near the ends of binary32's normal numbers: results keep their bits, relative to the row's largest
+    value (the stated bound without its absolute part)."""
+    c = Case("f32", 16, 2, 4, 64, [300, 64], [1, 2], seed=5)
+    c.cache.vs[:] = (np.random.default_rng(7).uniform(1, 2, c.cache.vs.shape) * 2.0 ** exponent).astype(np.float32)
+    want, wl, mag, vmax = O.attend(c.cache, c.q, c.starts, c.lens, c.tables, c.scale)
+    out, lse = c.run()
+    tol = (2 * 2.0 ** -20 * mag + 2.0 ** -18) * vmax
+    assert np.all(np.abs(out.astype(np.float64) - want) <= tol[..., None])
+    # and far inside it: 22-bit weights at random, 2^-21 of the largest value
+    assert np.sqrt(np.mean((out - want) ** 2)) <= 2.0 ** -21 * vmax.max()
