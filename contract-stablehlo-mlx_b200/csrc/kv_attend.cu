@@ -29,12 +29,12 @@
 // carry on lose up to 2^-23 of themselves each time, always downwards: 3e-4 over
 // 200000 keys; the adds cost 0.5 %). The weights
 // are rounded to float16 for the second product, as e^(s - m) (sv / largest sv
-// so far) 2^14: at most 2^14 and, since float16 reaches down to 2^-24, exact to
-// 2^-38 of the largest weight (of the largest value's scale among the keys of the
-// tile of rows: a page whose scale is 2^28 times a row's others costs that row's
-// bits). For float32 queries q and the weights are split
-// into two float16 terms each (22 bits), q after scaling each row by a power of
-// two to below 2^14.
+// so far, rounded down to a power of two) 2^14: below 2^15 and, since float16
+// reaches down to 2^-24, exact to 2^-38 of the largest weight (of the largest
+// value's scale among the keys of the tile of rows: a page whose scale is 2^28
+// times a row's others costs that row's bits). For float32 queries q and the
+// weights are split into two float16 terms each (22 bits), q after scaling each
+// row by a power of two to below 2^14.
 #include "kv_attend.cuh"
 
 namespace shlo {
@@ -329,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DP, NT>::PER_SM) k_kv_atten
       m[nt][0] = m[nt][1] = -INFINITY;
       l[nt][0] = l[nt][1] = 0.0f;
     }
-    float ksl = 0.0f, ratio_l = 0.0f;  // of the lane's tile: keys' scale, 2^14 values' scale / largest so far
+    float ksl = 0.0f, ratio_l = 0.0f;  // of the lane's tile: keys' scale, 2^14 values' scale / vmax
     uint32_t holes = 0;
     int pages_next = -1, slot = 0;  // slot: of the piece that comes next
     const int key0 = first_key(sg);
@@ -351,6 +351,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DP, NT>::PER_SM) k_kv_atten
         float top = finite ? fmaxf(vmax, fabsf(vs)) : vmax;
 #pragma unroll
         for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+        // (a power of two, so that 2^-14 of it is exact where it is no normal number)
+        top = top == 0.0f ? 0.0f : fmaxf(__uint_as_float(__float_as_uint(top) & 0x7f800000u), 0x1p-126f);
         if (top != vmax) {
           const float f = __fdiv_rn(vmax, top);
 #pragma unroll
@@ -567,6 +569,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DP, NT>::PER_SM) k_kv_atten
     const bool more = next_segment<ROWS, GRAN>(a, ba, p, ns);
     if (more) pages = begin(ns, buf ^ 1);
 
+    const float unscale = vmax * 0x1p-14f;
 #pragma unroll
     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -585,8 +588,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, DP, NT>::PER_SM) k_kv_atten
         for (int w = 0; w < VW; w++) {
           const int d = VW == 2 ? 8 * g + 4 * w : 128 * (w / 4) + 16 * g + 4 * (w % 4);
           *reinterpret_cast<float4 *>(dst + d) =
-              make_float4(o[nt][2 * w][e] * 0x1p-14f * vmax, o[nt][2 * w][2 + e] * 0x1p-14f * vmax,
-                          o[nt][2 * w + 1][e] * 0x1p-14f * vmax, o[nt][2 * w + 1][2 + e] * 0x1p-14f * vmax);
+              make_float4(o[nt][2 * w][e] * unscale, o[nt][2 * w][2 + e] * unscale, o[nt][2 * w + 1][e] * unscale,
+                          o[nt][2 * w + 1][2 + e] * unscale);
         }
       }
     __syncthreads();
