@@ -16,8 +16,8 @@
 // tile may be taken in any order, so each lane reads 16 contiguous bytes.
 //
 // Measured on one B200, 128-wide heads, four query heads to a key/value head,
-// float16: 64 sequences x 8192 keys (1.07 GB) 218 us, 4.93 TB/s; 64 ragged ones
-// (505 MB) 118 us; two of 150 to 200 thousand keys (343 MB) 88 us; one of 256
+// float16: 64 sequences x 8192 keys (1.07 GB) 219 us, 4.91 TB/s; 64 ragged ones
+// (505 MB) 119 us; two of 150 to 200 thousand keys (343 MB) 89 us; one of 256
 // keys 12 us. A loop without the products takes as long: the rest over the bytes
 // is the start (the line, the first pages and pieces, 8 us), a block's cuts
 // between units (8 us each, which the SM's other blocks cover as long as they
@@ -726,6 +726,13 @@ int launch_kv_attend(const AttendCall &c, int sms, int device, cudaStream_t st) 
   // Tiles of 8 rows where the sequences have 8 or fewer on average, else 16. Above
   // 16, float16 sequences of more than 16 rows go to the tiles of 128 (in which a
   // 16-row tile would cost as much as a full one), in a launch of their own.
+  // Measured with 32 sequences of 4096 keys and 8 key/value heads, us here and in
+  // the tiles: 128 wide, 24 rows 150 and 165, 32 rows 152 and 166, 48 rows 215 and
+  // 168, 256 rows 1028 and 265; 64 wide, 32 rows 100 and 142, 48 rows 146 and 142;
+  // 256 wide, 20 rows 324 and 260. So 16 is the crossing of the widest heads, and
+  // sends rows of 17 to 47 of narrower ones to the tiles 10 to 55 % early. The
+  // average hides one prompt among single tokens: 128 tokens (512 rows) among 64 of
+  // 2048 keys 200 us, 200 tokens, in the tiles, 180.
   const int64_t rows = (int64_t)c.batch.tokens * group;
   const int nt = rows <= (int64_t)8 * c.batch.seqs ? 1 : 2;
   if (c.dtype == kF16 && rows > (int64_t)16 * c.batch.seqs) {

@@ -26,15 +26,15 @@
 // rounding adds (5e-5 stays, a fifth of a float16 result's own rounding), in the
 // workspace, 16 bytes a thread beside its neighbours': 2.3 us a stretch. Rows of a
 // thread's own, 512 bytes apart, took 11; stretches of 4096 keys keep 2e-5, and a
-// prompt over 8192 keys then takes 420 us instead of 410.
+// prompt over 8192 keys then takes 420 us instead of 414.
 //
 // Bound: the softmax warps (2200 cycles of a tile's 3350: the exponentials, one
 // for 4 D flops, and what goes with them, on schedulers that the conversions
 // share), then a segment's beginning and end, which nothing overlaps (about 20
 // us; a block has a few). Measured on one B200, 32 query and 8 key/value heads of
-// 128: 512 new tokens of 4 sequences over 8192 keys (266 GFLOP) 410 us, 649
-// TFLOP/s; 4096 tokens on their own (137 GFLOP) 376 us, 366 TFLOP/s; prompts of
-// three sequences (207 GFLOP) 401 us. Measured and left: one block of 128 rows
+// 128: 512 new tokens of 4 sequences over 8192 keys (266 GFLOP) 414 us, 643
+// TFLOP/s; 4096 tokens on their own (137 GFLOP) 384 us, 358 TFLOP/s; prompts of
+// three sequences (207 GFLOP) 404 us. Measured and left: one block of 128 rows
 // twice on an SM, each converting for itself (346 TFLOP/s on the first case);
 // products issued in a fixed order (head-of-line waits: 599 us against 499);
 // descriptors as 64-bit sums (907 cycles to issue eight products against 541).

@@ -16,7 +16,7 @@
 // cosines and sines of its tokens once, into shared memory, for all heads.
 // Measured on one B200: 16384 tokens x 40 heads x 128, float16 (336 MB) 55.3 us,
 // 6.07 TB/s (0.93 of a copy's rate); 24001 x 12 x 80 float32, 32 dimensions turned
-// in interleaved pairs (184 MB) 33.5 us, 5.50 TB/s; 16 x 40 x 128 4.1 us, a launch.
+// in interleaved pairs (184 MB) 34.4 us, 5.36 TB/s; 16 x 40 x 128 4.1 us, a launch.
 #include <cmath>
 
 #include "decode.cuh"

@@ -238,8 +238,8 @@ typedef struct {
 /* A batch of sequences, all arrays on the device: sequence s has the rows
    starts[s] .. starts[s + 1] - 1 of the call's activations as its newest tokens
    (ascending; no rows is allowed; an attention over starts that descend computes
-   nothing, and the library's next wait or its next call says so), lens[s] tokens in all with
-   them, and page tables[s * table_stride + i] for its tokens
+   nothing, and the library's next wait or its next call says so), lens[s] tokens
+   in all with them, and page tables[s * table_stride + i] for its tokens
    i * page_tokens ... An entry outside the cache (-1, say) is a page it does
    not have. */
 typedef struct {
@@ -273,11 +273,11 @@ int shlo_kv_attend_workspace(size_t *bytes);
    tokens t < lens, with `causal` t <= p, with `window` > 0 t > p - window, in
    pages that its table has. A row that sees none gives 0, and -inf in lse. lse
    (float32 [tokens][heads], or NULL) is the logarithm of the sum of the
-   exponentials of the scaled scores. The workspace must be zero before the
-   first call that uses it; calls leave it ready for the next, on one stream at
-   a time, those that gave up a wait too (which the library's next wait on the
-   device reports, or the next call: it does nothing else then). The same call
-   gives the same bits. */
+   exponentials of the scaled scores. out shares no memory with q. The workspace
+   must be zero before the first call that uses it; calls leave it ready for the
+   next, on one stream at a time, those that gave up a wait too (which the
+   library's next wait on the device reports, or the next call: it does nothing
+   else then). The same call gives the same bits. */
 int shlo_kv_attend_noalloc(const shlo_kv_pool *pool, const shlo_kv_batch *batch, const void *q, int64_t q_token,
                            int64_t q_head, int32_t heads, uint8_t dtype, float scale, int32_t causal, int32_t window,
                            void *out, int64_t out_token, int64_t out_head, float *lse, void *workspace,
