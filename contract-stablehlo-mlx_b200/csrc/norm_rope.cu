@@ -1,0 +1,524 @@
+// The norm of queries and keys for each head, with the position rotation in the
+// same pass, and its gradient. A head x of D values becomes
+//   n = x / sqrt(mean(x^2) + eps),   z = n w,   y = turn(z, position),
+// where w is the queries' weight for the first q_heads heads and the keys' for
+// the others, and turn is rope.cu's (pairs of the first `rot` dimensions, the
+// angles' arithmetic too). Of dy:
+//   dz = turn(dy, -position),  dw = sum of dz n over tokens and heads,
+//   g = dz w,   dx = (g - n mean(g n)) / sqrt(mean(x^2) + eps).
+//
+// Bound: bytes (each value read once and written once). A group of 1 to 32 lanes
+// holds a head in registers; it keeps one token and goes over heads, so that its
+// pairs' cosines and sines, and the weight, stay in registers too. A group's next
+// head is asked for before the one in hand is worked on.
+#include <algorithm>
+#include <cmath>
+
+#include "decode.cuh"
+
+namespace shlo {
+
+namespace {
+
+constexpr int kThreads = 256;
+
+struct NormArgs {
+  const void *x, *dy;
+  void *y;  // dx in the backward pass
+  const int32_t *pos;
+  const int64_t *phases;
+  const void *wq, *wk;
+  int64_t xt, xh, gt, gh, yt, yh;  // token and head strides, in values (g: dy's)
+  int64_t tokens;
+  int heads, q_heads, dim, rot;
+  int lanes_log;  // lanes a group
+  int nt_log;     // tokens a block (at a time)
+  int hb;         // forward: heads a block
+  int parts_q;    // backward: blockIdx.y below this: query heads, hb_q a block; from there on key heads, hb_k a block
+  int hb_q, hb_k;
+  float eps, factor;
+  bool w_half;
+  float *partials;  // backward: [gridDim.y][gridDim.x][dim], nullptr without the weights' gradients
+};
+
+template <int BYTES> struct Raw;
+template <> struct Raw<16> { using T = uint4; };
+template <> struct Raw<8> { using T = uint2; };
+template <> struct Raw<4> { using T = uint32_t; };
+template <> struct Raw<2> { using T = uint16_t; };
+
+__device__ __forceinline__ float to_f32(__half h) { return __half2float(h); }
+__device__ __forceinline__ float to_f32(float f) { return f; }
+__device__ __forceinline__ void of_f32(__half &d, float f) { d = __float2half_rn(f); }
+__device__ __forceinline__ void of_f32(float &d, float f) { d = f; }
+
+// A lane's part of a head: NS slots of two vectors of VEC values. The first
+// rot / 2 / VEC slots of a head hold pairs (the vectors half the part apart, or
+// side by side); the others two vectors of the part that is not turned, the last
+// of which may have one only.
+template <typename T, int VEC, int NS> struct Part {
+  T v[NS][2][VEC];
+};
+template <int NS> struct Places {
+  int o[NS], o2[NS];  // -1: none
+  bool pair[NS];
+};
+
+template <int VEC, int NS, bool INTER>
+__device__ __forceinline__ void places(const NormArgs &a, int lane, Places<NS> &p) {
+  const int half = a.rot / 2, ru = half / VEC, cv = (a.dim - a.rot) / VEC;
+#pragma unroll
+  for (int s = 0; s < NS; s++) {
+    const int u = lane + (s << a.lanes_log), c = 2 * (u - ru);
+    p.pair[s] = u < ru;
+    p.o[s] = u < ru ? (INTER ? 2 * VEC : VEC) * u : c < cv ? a.rot + c * VEC : -1;
+    p.o2[s] = u < ru ? p.o[s] + (INTER ? VEC : half) : c + 1 < cv ? a.rot + (c + 1) * VEC : -1;
+  }
+}
+template <typename T, int VEC, int NS>
+__device__ __forceinline__ void load_part(const T *x, const Places<NS> &p, Part<T, VEC, NS> &r) {
+  using R = typename Raw<VEC * sizeof(T)>::T;
+#pragma unroll
+  for (int s = 0; s < NS; s++) {
+    if (p.o[s] >= 0) *reinterpret_cast<R *>(r.v[s][0]) = *reinterpret_cast<const R *>(x + p.o[s]);
+    if (p.o2[s] >= 0) *reinterpret_cast<R *>(r.v[s][1]) = *reinterpret_cast<const R *>(x + p.o2[s]);
+  }
+}
+template <typename T, int VEC, int NS>
+__device__ __forceinline__ void store_part(T *y, const Places<NS> &p, const Part<T, VEC, NS> &r) {
+  using R = typename Raw<VEC * sizeof(T)>::T;
+#pragma unroll
+  for (int s = 0; s < NS; s++) {
+    if (p.o[s] >= 0) *reinterpret_cast<R *>(y + p.o[s]) = *reinterpret_cast<const R *>(r.v[s][0]);
+    if (p.o2[s] >= 0) *reinterpret_cast<R *>(y + p.o2[s]) = *reinterpret_cast<const R *>(r.v[s][1]);
+  }
+}
+template <typename T, int VEC, int NS>
+__device__ __forceinline__ void clear_part(Part<T, VEC, NS> &r) {
+#pragma unroll
+  for (int s = 0; s < NS; s++)
+#pragma unroll
+    for (int k = 0; k < 2; k++)
+#pragma unroll
+      for (int j = 0; j < VEC; j++) of_f32(r.v[s][k][j], 0.0f);
+}
+// The two values of pair j of a slot.
+template <int VEC, bool INTER, typename V> __device__ __forceinline__ V &first(V (&v)[2][VEC], int j) { return INTER ? v[(2 * j) / VEC][(2 * j) % VEC] : v[0][j]; }
+template <int VEC, bool INTER, typename V> __device__ __forceinline__ V &second(V (&v)[2][VEC], int j) { return INTER ? v[(2 * j + 1) / VEC][(2 * j + 1) % VEC] : v[1][j]; }
+
+__device__ __forceinline__ float group_sum(float v, int lanes_log) {
+  for (int i = 0; i < lanes_log; i++) v += __shfl_xor_sync(~0u, v, 1 << i);
+  return v;
+}
+
+// Squares of 32-bit values can leave the range where the values themselves are
+// well inside it: such a head is scaled by a power of two first. Returns the scale.
+__device__ __forceinline__ float safe_scale(float ss, float eps) {
+  if (!(ss < 0x1p120f)) return 0x1p-80f;
+  if (ss < 0x1p-80f && eps < 0x1p-80f) return 0x1p66f;
+  return 1.0f;
+}
+
+// BACK: the gradient. A block goes over tiles of 2^nt_log tokens, one in the
+// forward pass, for the heads of its part.
+template <typename T, int VEC, int NS, bool INTER, bool BACK>
+__global__ void __launch_bounds__(kThreads) k_norm_rope(const NormArgs a) {
+  extern __shared__ float sh[];  // cosines, sines: [token][half] each; backward: the block's sums in their place
+  const int half = a.rot / 2, nt = 1 << a.nt_log;
+  float *const cs = sh, *const sn = sh + nt * half;
+  const int lane = threadIdx.x & ((1 << a.lanes_log) - 1), group = threadIdx.x >> a.lanes_log;
+  const int groups = kThreads >> a.lanes_log;
+  // A block of the backward pass has heads of one weight, whose sums it keeps.
+  const bool back_keys = BACK && (int)blockIdx.y >= a.parts_q;
+  const int h0 = !BACK ? blockIdx.y * a.hb : back_keys ? a.q_heads + (blockIdx.y - a.parts_q) * a.hb_k : blockIdx.y * a.hb_q;
+  const int h1 = !BACK ? min(h0 + a.hb, a.heads) : back_keys ? min(h0 + a.hb_k, a.heads) : min(h0 + a.hb_q, a.q_heads);
+  Places<NS> at;
+  places<VEC, NS, INTER>(a, lane, at);
+  float w[NS][2][VEC];
+  int has = -1;  // whose weight w is: 0 the queries', 1 the keys'
+  auto weigh = [&](int keys) {
+    if (keys == has) return;
+    has = keys;
+    const void *const wp = keys ? a.wk : a.wq;
+#pragma unroll
+    for (int s = 0; s < NS; s++)
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        const int o = k ? at.o2[s] : at.o[s];
+#pragma unroll
+        for (int j = 0; j < VEC; j++)
+          w[s][k][j] = o < 0 ? 0.0f : !wp ? 1.0f : a.w_half ? __half2float(static_cast<const __half *>(wp)[o + j]) : static_cast<const float *>(wp)[o + j];
+      }
+  };
+  float dw[BACK ? NS : 1][2][VEC];
+  if (BACK) {
+#pragma unroll
+    for (int s = 0; s < NS; s++)
+#pragma unroll
+      for (int j = 0; j < VEC; j++) dw[s][0][j] = dw[s][1][j] = 0.0f;
+  }
+  const float inv_dim = 1.0f / a.dim;
+  const int t = group & (nt - 1), h_first = h0 + (group >> a.nt_log), h_step = max(groups >> a.nt_log, 1);
+  const int64_t tiles = (a.tokens + nt - 1) >> a.nt_log;
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int64_t t0 = tile << a.nt_log;
+    const bool mine = t0 + t < a.tokens;
+    const T *const x = static_cast<const T *>(a.x) + (t0 + t) * a.xt;
+    const T *const g = static_cast<const T *>(a.dy) + (BACK ? (t0 + t) * a.gt : 0);
+    T *const y = static_cast<T *>(a.y) + (t0 + t) * a.yt;
+    // (the loads need nothing of the angles: they go out first)
+    Part<T, VEC, NS> next, next_g;
+    clear_part(next);
+    if (BACK) clear_part(next_g);
+    if (mine && h_first < h1) {
+      load_part(x + h_first * a.xh, at, next);
+      if (BACK) load_part(g + h_first * a.gh, at, next_g);
+    }
+    if (BACK && tile != (int64_t)blockIdx.x) __syncthreads();
+    for (int i = threadIdx.x; i < nt * half; i += kThreads) {
+      const int tt = i / half, p = i - tt * half;
+      if (t0 + tt < a.tokens) {
+        const int64_t turns = (int64_t)((uint64_t)(int64_t)a.pos[t0 + tt] * (uint64_t)a.phases[p]) >> 32;
+        float s, c;
+        sincospif((float)turns * 0x1p-31f, &s, &c);
+        cs[i] = c * a.factor;
+        sn[i] = (BACK ? -s : s) * a.factor;
+      }
+    }
+    __syncthreads();
+    float c[NS][VEC], s_[NS][VEC];
+#pragma unroll
+    for (int s = 0; s < NS; s++)
+#pragma unroll
+      for (int j = 0; j < VEC; j++) {
+        const int p = (lane + (s << a.lanes_log)) * VEC + j;
+        c[s][j] = at.pair[s] && mine ? cs[t * half + p] : 1.0f;
+        s_[s][j] = at.pair[s] && mine ? sn[t * half + p] : 0.0f;
+      }
+    // (a warp's groups take the same number of turns: its shuffles name all lanes)
+    for (int h = h_first - (group >> a.nt_log); h < h1; h += h_step) {
+      const int hh = h + (group >> a.nt_log);
+      const bool there = mine && hh < h1;
+      weigh(BACK ? back_keys : hh >= a.q_heads);
+      Part<T, VEC, NS> in = next, in_g = next_g;
+      if (mine && hh + h_step < h1) {
+        load_part(x + (hh + h_step) * a.xh, at, next);
+        if (BACK) load_part(g + (hh + h_step) * a.gh, at, next_g);
+      }
+      float v[NS][2][VEC], ss = 0.0f;
+#pragma unroll
+      for (int s = 0; s < NS; s++)
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+          for (int j = 0; j < VEC; j++) {
+            v[s][k][j] = to_f32(in.v[s][k][j]);
+            ss = __fmaf_rn(v[s][k][j], v[s][k][j], ss);
+          }
+      ss = group_sum(ss, a.lanes_log);
+      float scale = 1.0f, eps = a.eps;
+      if (sizeof(T) == 4) {
+        scale = safe_scale(ss, eps);
+        if (__any_sync(~0u, scale != 1.0f)) {
+          eps = eps * scale * scale;  // (scale^2 itself has no place in 32 bits)
+          ss = 0.0f;
+#pragma unroll
+          for (int s = 0; s < NS; s++)
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+              for (int j = 0; j < VEC; j++) {
+                v[s][k][j] *= scale;
+                ss = __fmaf_rn(v[s][k][j], v[s][k][j], ss);
+              }
+          ss = group_sum(ss, a.lanes_log);
+        }
+      }
+      const float inv = __frsqrt_rn(__fmaf_rn(ss, inv_dim, eps));
+      Part<T, VEC, NS> out;
+      if (!BACK) {
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+#pragma unroll
+          for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) v[s][k][j] = v[s][k][j] * inv * w[s][k][j];
+          if (at.pair[s]) {
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+              const float p = first<VEC, INTER>(v[s], j), q = second<VEC, INTER>(v[s], j);
+              first<VEC, INTER>(v[s], j) = __fmaf_rn(p, c[s][j], -(q * s_[s][j]));
+              second<VEC, INTER>(v[s], j) = __fmaf_rn(q, c[s][j], p * s_[s][j]);
+            }
+          }
+        }
+      } else {
+        float d[NS][2][VEC], gn = 0.0f;
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+#pragma unroll
+          for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) d[s][k][j] = to_f32(in_g.v[s][k][j]);
+          if (at.pair[s]) {
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+              const float p = first<VEC, INTER>(d[s], j), q = second<VEC, INTER>(d[s], j);
+              first<VEC, INTER>(d[s], j) = __fmaf_rn(p, c[s][j], -(q * s_[s][j]));
+              second<VEC, INTER>(d[s], j) = __fmaf_rn(q, c[s][j], p * s_[s][j]);
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) {
+              v[s][k][j] *= inv;
+              if (there) dw[s][k][j] = __fmaf_rn(d[s][k][j], v[s][k][j], dw[s][k][j]);
+              d[s][k][j] *= w[s][k][j];
+              gn = __fmaf_rn(d[s][k][j], v[s][k][j], gn);
+            }
+        }
+        gn = group_sum(gn, a.lanes_log) * inv_dim;
+#pragma unroll
+        for (int s = 0; s < NS; s++)
+#pragma unroll
+          for (int k = 0; k < 2; k++)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) v[s][k][j] = __fmaf_rn(-v[s][k][j], gn, d[s][k][j]) * inv * scale;
+      }
+#pragma unroll
+      for (int s = 0; s < NS; s++)
+#pragma unroll
+        for (int k = 0; k < 2; k++)
+#pragma unroll
+          for (int j = 0; j < VEC; j++) of_f32(out.v[s][k][j], v[s][k][j]);
+      if (there) store_part(y + hh * a.yh, at, out);
+    }
+  }
+  if (BACK && a.partials) {
+    // The block's sums: groups one after the other, each adding to the block's row.
+    __syncthreads();
+    const int L = 1 << a.lanes_log;
+#pragma unroll
+    for (int s = 0; s < NS; s++)
+#pragma unroll
+      for (int k = 0; k < 2; k++)
+#pragma unroll
+        for (int j = 0; j < VEC; j++)
+          for (int i = L; i < 32; i *= 2) dw[s][k][j] += __shfl_xor_sync(~0u, dw[s][k][j], i);
+    const int warp = threadIdx.x / 32, wl = threadIdx.x % 32;
+    if (wl < L) {
+#pragma unroll
+      for (int s = 0; s < NS; s++)
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const int o = k ? at.o2[s] : at.o[s];
+          if (o >= 0)
+#pragma unroll
+            for (int j = 0; j < VEC; j++) sh[warp * a.dim + o + j] = dw[s][k][j];
+        }
+    }
+    __syncthreads();
+    float *const to = a.partials + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * a.dim;
+    for (int i = threadIdx.x; i < a.dim; i += kThreads) {
+      float sum = 0.0f;
+      for (int k = 0; k < kThreads / 32; k++) sum += sh[k * a.dim + i];
+      to[i] = sum;
+    }
+  }
+}
+
+// The blocks' sums of a weight's gradient, added in one order: blockIdx.y 0 the
+// queries' rows [0, rows_q), 1 the keys' behind them. 32 dimensions a block.
+__global__ void __launch_bounds__(1024) k_norm_rope_dw(const float *partials, int rows_q, int rows_k, int dim, float *dq, float *dk) {
+  __shared__ float sums[32][33];
+  const int c = threadIdx.x % 32, r = threadIdx.x / 32, i = blockIdx.x * 32 + c;
+  const float *const from = partials + (blockIdx.y ? (int64_t)rows_q * dim : 0);
+  float *const to = blockIdx.y ? dk : dq;
+  const int rows = blockIdx.y ? rows_k : rows_q;
+  if (!to) return;
+  float sum = 0.0f;
+  if (i < dim)
+    for (int k = r; k < rows; k += 32) sum += from[(int64_t)k * dim + i];
+  sums[r][c] = sum;
+  __syncthreads();
+  if (r == 0 && i < dim) {
+    sum = 0.0f;
+    for (int k = 0; k < 32; k++) sum += sums[k][c];
+    to[i] = sum;
+  }
+}
+
+template <typename T, int VEC, int NS>
+int launch(const NormArgs &a, bool inter, bool back, dim3 grid, size_t smem, cudaStream_t st) {
+  if (back) {
+    if (inter) k_norm_rope<T, VEC, NS, true, true><<<grid, kThreads, smem, st>>>(a);
+    else k_norm_rope<T, VEC, NS, false, true><<<grid, kThreads, smem, st>>>(a);
+  } else {
+    if (inter) k_norm_rope<T, VEC, NS, true, false><<<grid, kThreads, smem, st>>>(a);
+    else k_norm_rope<T, VEC, NS, false, false><<<grid, kThreads, smem, st>>>(a);
+  }
+  return launch_check(back ? "norm_rope_grad" : "norm_rope");
+}
+
+// Blocks of the backward pass: their sums go to the workspace.
+constexpr int kBackBlocksPerSm = 4;
+int back_blocks(int sms) { return sms * kBackBlocksPerSm; }
+
+}  // namespace
+
+size_t norm_rope_work_bytes(int sms) { return (size_t)(back_blocks(sms) + 2) * 512 * sizeof(float); }
+
+int launch_norm_rope(const NormRopeCall &c, int sms, cudaStream_t st) {
+  const bool back = c.dy != nullptr;
+  const char *const what = back ? "norm_rope_grad" : "norm_rope";
+  if (c.dtype != kF16 && c.dtype != kF32) return fail("%s: %s not carried (float16 or float32)", what, dtype_name(c.dtype));
+  if (c.weight_dtype != kF16 && c.weight_dtype != kF32) return fail("%s: weights of %s not carried (float16 or float32)", what, dtype_name(c.weight_dtype));
+  if (c.tokens < 0 || c.heads < 1 || c.dim < 1 || c.dim > 512)
+    return fail("%s: %lld tokens, %d heads of %d (1 to 512)", what, (long long)c.tokens, c.heads, c.dim);
+  if (c.q_heads < 0 || c.q_heads > c.heads) return fail("%s: %d query heads of %d", what, c.q_heads, c.heads);
+  if (c.rot < 0 || c.rot > c.dim || c.rot % 2) return fail("%s: %d of %d dimensions turned (an even number)", what, c.rot, c.dim);
+  if (c.flags & ~1u) return fail("%s: flags 0x%x", what, c.flags);
+  if (!(c.eps > 0.0f) || !std::isfinite(c.eps)) return fail("%s: eps %g (finite, above 0)", what, c.eps);
+  if (c.tokens > 0x7fffffff) return fail("%s: %lld tokens, at most 2^31 - 1", what, (long long)c.tokens);
+  const size_t size = dtype_size(c.dtype), wsize = dtype_size(c.weight_dtype);
+  const bool sums = back && (c.dq_weight || c.dk_weight);
+  if ((uintptr_t)c.dq_weight % 4 || (uintptr_t)c.dk_weight % 4 || (uintptr_t)c.work % 4) return fail("%s: misaligned gradient or workspace", what);
+  if (sums && (!c.work || c.work_bytes < norm_rope_work_bytes(sms)))
+    return fail("%s: a workspace of %zu bytes, %zu needed", what, c.work ? c.work_bytes : 0, norm_rope_work_bytes(sms));
+  if (c.tokens == 0) {
+    if (c.dq_weight) SHLO_CUDA(cudaMemsetAsync(c.dq_weight, 0, c.dim * sizeof(float), st));
+    if (c.dk_weight) SHLO_CUDA(cudaMemsetAsync(c.dk_weight, 0, c.dim * sizeof(float), st));
+    return 0;
+  }
+  if (!c.x || !c.y || (c.rot && (!c.positions || !c.phases))) return fail("%s: null pointer", what);
+  if (((uintptr_t)c.x | (uintptr_t)c.y | (uintptr_t)c.dy) % size) return fail("%s: an operand is not aligned to its type", what);
+  if (((uintptr_t)c.q_weight | (uintptr_t)c.k_weight) % wsize) return fail("%s: a weight is not aligned to its type", what);
+  if ((uintptr_t)c.positions % 4 || (uintptr_t)c.phases % 8) return fail("%s: misaligned positions or phases", what);
+  SHLO_TRY(check_in_place(c.x, c.x_token, c.x_head, c.y, c.y_token, c.y_head, c.tokens, c.heads, c.dim, size, what, "x", back ? "dx" : "y"));
+  if (back)
+    SHLO_TRY(check_in_place(c.dy, c.dy_token, c.dy_head, c.y, c.y_token, c.y_head, c.tokens, c.heads, c.dim, size, what, "dy", "dx"));
+  // The widest vector (16 bytes at most) that every offset is a multiple of.
+  const int half = c.rot / 2, rest = c.dim - c.rot;
+  int vec = (int)(16 / size);
+  const bool strided_h = c.heads > 1, strided_t = c.tokens > 1;
+  auto fits = [&](int v) {
+    auto row = [&](const void *p, int64_t token, int64_t head) {
+      return (uintptr_t)p % (v * size) == 0 && (!strided_t || token % v == 0) && (!strided_h || head % v == 0);
+    };
+    return half % v == 0 && rest % v == 0 && row(c.x, c.x_token, c.x_head) && row(c.y, c.y_token, c.y_head) && (!back || row(c.dy, c.dy_token, c.dy_head));
+  };
+  while (vec > 1 && !fits(vec)) vec /= 2;
+  const int units = half / vec + (rest / vec + 1) / 2;
+  const int slots = c.dtype == kF32 && vec == 4 && units <= 32 ? 1 : 8 / vec;
+  NormArgs a;
+  a.x = c.x; a.dy = c.dy; a.y = c.y; a.pos = c.positions; a.phases = c.phases; a.wq = c.q_weight; a.wk = c.k_weight;
+  a.xt = c.x_token; a.xh = c.x_head; a.gt = c.dy_token; a.gh = c.dy_head; a.yt = c.y_token; a.yh = c.y_head;
+  a.tokens = c.tokens; a.heads = c.heads; a.q_heads = c.q_heads; a.dim = c.dim; a.rot = c.rot;
+  a.eps = c.eps; a.factor = c.factor; a.w_half = c.weight_dtype == kF16;
+  a.partials = sums ? (float *)c.work : nullptr;
+  a.lanes_log = 0;
+  while (a.lanes_log < 5 && (1 << a.lanes_log) < units) a.lanes_log++;
+  // A block's tokens: a group a token where that leaves every SM blocks; then its
+  // heads are shared among blocks while there are fewer than two a SM.
+  const int groups = kThreads >> a.lanes_log, hq = c.q_heads, hk = c.heads - c.q_heads;
+  a.nt_log = 0;
+  while ((2 << a.nt_log) <= groups && a.nt_log < 3 && (c.tokens >> (a.nt_log + 1)) >= 4 * sms) a.nt_log++;
+  const int64_t tiles = (c.tokens + (1 << a.nt_log) - 1) >> a.nt_log;
+  const int step = std::max(1, groups >> a.nt_log);
+  dim3 grid((unsigned)tiles, 1);
+  int parts = 1, parts_k = 0;
+  a.hb = a.hb_q = a.hb_k = 1;
+  a.parts_q = 0;
+  if (!back) {
+    while (tiles * parts < 2 * sms && parts < (c.heads + step - 1) / step) parts++;
+    a.hb = (c.heads + parts - 1) / parts;
+    grid.y = (c.heads + a.hb - 1) / a.hb;
+  } else {
+    // Parts of about the same number of heads, of one weight each, and more of
+    // them while there are fewer blocks than the SMs take.
+    int hb = hq && hk ? std::min(hq, hk) : c.heads;
+    while (hb > step && tiles * ((hq + hb - 1) / hb + (hk + hb - 1) / hb) < back_blocks(sms)) hb = std::max(step, hb / 2);
+    while ((hq + hb - 1) / hb + (hk + hb - 1) / hb > back_blocks(sms)) hb *= 2;
+    a.hb_q = a.hb_k = hb;
+    a.parts_q = (hq + hb - 1) / hb;
+    parts_k = (hk + hb - 1) / hb;
+    grid.y = a.parts_q + parts_k;
+    grid.x = (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, back_blocks(sms) / grid.y));
+  }
+  size_t smem = (size_t)(1 << a.nt_log) * half * 2 * sizeof(float);
+  if (back) smem = std::max(smem, (size_t)(kThreads / 32) * c.dim * sizeof(float));
+  const bool inter = (c.flags & 1) != 0;
+  if (c.dtype == kF16) {
+    switch (vec) {
+      case 8: SHLO_TRY((launch<__half, 8, 1>(a, inter, back, grid, smem, st))); break;
+      case 4: SHLO_TRY((launch<__half, 4, 2>(a, inter, back, grid, smem, st))); break;
+      case 2: SHLO_TRY((launch<__half, 2, 4>(a, inter, back, grid, smem, st))); break;
+      default: SHLO_TRY((launch<__half, 1, 8>(a, inter, back, grid, smem, st))); break;
+    }
+  } else {
+    switch (vec) {
+      case 4:
+        if (slots == 1) SHLO_TRY((launch<float, 4, 1>(a, inter, back, grid, smem, st)));
+        else SHLO_TRY((launch<float, 4, 2>(a, inter, back, grid, smem, st)));
+        break;
+      case 2: SHLO_TRY((launch<float, 2, 4>(a, inter, back, grid, smem, st))); break;
+      default: SHLO_TRY((launch<float, 1, 8>(a, inter, back, grid, smem, st))); break;
+    }
+  }
+  if (!sums) return 0;
+  k_norm_rope_dw<<<dim3((c.dim + 31) / 32, 2), 1024, 0, st>>>(a.partials, a.parts_q * (int)grid.x, parts_k * (int)grid.x, c.dim, c.dq_weight, c.dk_weight);
+  return launch_check("norm_rope_grad");
+}
+
+}  // namespace shlo
+
+using namespace shlo;
+
+extern "C" {
+
+int shlo_norm_rope_noalloc(const void *x, int64_t x_token, int64_t x_head, const int32_t *positions, const int64_t *phases,
+                           const void *q_weight, const void *k_weight, uint8_t weight_dtype, int32_t q_heads, float eps,
+                           void *y, int64_t y_token, int64_t y_head, int64_t tokens, int32_t heads, int32_t dim, int32_t rot,
+                           uint8_t dtype, uint32_t flags, float factor, void *stream) {
+  Device *dev;
+  SHLO_TRY(calling_device(&dev));
+  NormRopeCall c = {};
+  c.x = x; c.x_token = x_token; c.x_head = x_head;
+  c.positions = positions; c.phases = phases;
+  c.q_weight = q_weight; c.k_weight = k_weight; c.weight_dtype = weight_dtype; c.q_heads = q_heads; c.eps = eps;
+  c.y = y; c.y_token = y_token; c.y_head = y_head;
+  c.tokens = tokens; c.heads = heads; c.dim = dim; c.rot = rot; c.dtype = dtype; c.flags = flags; c.factor = factor;
+  return launch_norm_rope(c, dev->sm_count, (cudaStream_t)stream);
+}
+
+int shlo_norm_rope_workspace(size_t *bytes) {
+  if (!bytes) return fail("norm_rope_workspace: null pointer");
+  Device *dev;
+  SHLO_TRY(calling_device(&dev));
+  *bytes = norm_rope_work_bytes(dev->sm_count);
+  return 0;
+}
+
+int shlo_norm_rope_grad_noalloc(const void *x, int64_t x_token, int64_t x_head, const void *dy, int64_t dy_token, int64_t dy_head,
+                                const int32_t *positions, const int64_t *phases, const void *q_weight, const void *k_weight,
+                                uint8_t weight_dtype, int32_t q_heads, float eps, void *dx, int64_t dx_token, int64_t dx_head,
+                                float *dq_weight, float *dk_weight, int64_t tokens, int32_t heads, int32_t dim, int32_t rot,
+                                uint8_t dtype, uint32_t flags, float factor, void *workspace, size_t workspace_bytes, void *stream) {
+  if (!dy && tokens) return fail("norm_rope_grad: null pointer");
+  Device *dev;
+  SHLO_TRY(calling_device(&dev));
+  NormRopeCall c = {};
+  c.x = x; c.x_token = x_token; c.x_head = x_head;
+  c.dy = dy ? dy : x; c.dy_token = dy_token; c.dy_head = dy_head;
+  if (!c.dy) c.dy = "";  // (no tokens: nothing is read)
+  c.positions = positions; c.phases = phases;
+  c.q_weight = q_weight; c.k_weight = k_weight; c.weight_dtype = weight_dtype; c.q_heads = q_heads; c.eps = eps;
+  c.y = dx; c.y_token = dx_token; c.y_head = dx_head;
+  c.dq_weight = dq_weight; c.dk_weight = dk_weight;
+  c.tokens = tokens; c.heads = heads; c.dim = dim; c.rot = rot; c.dtype = dtype; c.flags = flags; c.factor = factor;
+  c.work = workspace; c.work_bytes = workspace_bytes;
+  return launch_norm_rope(c, dev->sm_count, (cudaStream_t)stream);
+}
+
+}  // extern "C"

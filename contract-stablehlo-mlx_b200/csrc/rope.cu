@@ -156,17 +156,18 @@ void launch(const RopeArgs &a, bool inter, dim3 grid, size_t smem, cudaStream_t 
 // Whether x and y have a value in common, y not being x itself (blocks then read
 // what others have written). Where their extents overlap they need the same
 // strides to have none: it comes down to one distance between rows.
-bool overlap(const RopeCall &c, size_t size) {
-  const int64_t off = ((intptr_t)c.y - (intptr_t)c.x) / (int64_t)size, T = c.tokens, H = c.heads, D = c.dim;
+bool overlap(const void *x, int64_t x_token, int64_t x_head, const void *y, int64_t y_token, int64_t y_head, int64_t T, int64_t H,
+             int64_t D, size_t size) {
+  const int64_t off = ((intptr_t)y - (intptr_t)x) / (int64_t)size;
   auto low = [](int64_t n, int64_t s) { return s < 0 ? (double)(n - 1) * s : 0.0; };
   auto high = [](int64_t n, int64_t s) { return s > 0 ? (double)(n - 1) * s : 0.0; };
-  const double x0 = low(T, c.x_token) + low(H, c.x_head), x1 = high(T, c.x_token) + high(H, c.x_head) + D;
-  const double y0 = off + low(T, c.y_token) + low(H, c.y_head), y1 = off + high(T, c.y_token) + high(H, c.y_head) + D;
+  const double x0 = low(T, x_token) + low(H, x_head), x1 = high(T, x_token) + high(H, x_head) + D;
+  const double y0 = off + low(T, y_token) + low(H, y_head), y1 = off + high(T, y_token) + high(H, y_head) + D;
   if (y1 <= x0 || x1 <= y0) return false;
-  if ((T > 1 && c.x_token != c.y_token) || (H > 1 && c.x_head != c.y_head)) return true;
+  if ((T > 1 && x_token != y_token) || (H > 1 && x_head != y_head)) return true;
   const bool by_heads = H <= T;  // the shorter axis is gone through, the other solved for
-  const int64_t n1 = by_heads ? H : T, s1 = by_heads ? c.x_head : c.x_token;
-  const int64_t n2 = by_heads ? T : H, s2 = by_heads ? c.x_token : c.x_head;
+  const int64_t n1 = by_heads ? H : T, s1 = by_heads ? x_head : x_token;
+  const int64_t n2 = by_heads ? T : H, s2 = by_heads ? x_token : x_head;
   for (int64_t i = 1 - n1; i < n1; i++) {
     const int64_t r = off - i * s1, j0 = s2 && n2 > 1 ? r / s2 : 0;
     for (int64_t j = j0 - 1; j <= j0 + 1; j++)
@@ -176,6 +177,15 @@ bool overlap(const RopeCall &c, size_t size) {
 }
 
 }  // namespace
+
+int check_in_place(const void *x, int64_t x_token, int64_t x_head, const void *y, int64_t y_token, int64_t y_head, int64_t tokens,
+                   int64_t heads, int64_t dim, size_t size, const char *what, const char *x_name, const char *y_name) {
+  const bool same = x == y;
+  if (same && (x_token != y_token || x_head != y_head)) return fail("%s: %s and %s share storage with different strides", what, x_name, y_name);
+  if (!same && overlap(x, x_token, x_head, y, y_token, y_head, tokens, heads, dim, size))
+    return fail("%s: %s and %s overlap (%s is %s itself, or shares no value with it)", what, x_name, y_name, y_name, x_name);
+  return 0;
+}
 
 int launch_rope(const RopeCall &c, int sms, cudaStream_t st) {
   if (c.dtype != kF16 && c.dtype != kF32) return fail("rope: %s not carried (float16 or float32)", dtype_name(c.dtype));
@@ -190,9 +200,7 @@ int launch_rope(const RopeCall &c, int sms, cudaStream_t st) {
   if (((uintptr_t)c.x | (uintptr_t)c.y) % size) return fail("rope: x or y is not aligned to its type");
   if ((uintptr_t)c.positions % 4 || (uintptr_t)c.phases % 8) return fail("rope: misaligned positions or phases");
   const bool same = c.x == c.y;
-  if (same && (c.x_token != c.y_token || c.x_head != c.y_head))
-    return fail("rope: x and y share storage with different strides");
-  if (!same && overlap(c, size)) return fail("rope: x and y overlap (y is x itself, or shares no value with it)");
+  SHLO_TRY(check_in_place(c.x, c.x_token, c.x_head, c.y, c.y_token, c.y_head, c.tokens, c.heads, c.dim, size, "rope", "x", "y"));
   const int half = c.rot / 2, rest = same ? 0 : c.dim - c.rot;
   if (half == 0 && rest == 0) return 0;
   // The widest vector (16 bytes at most) that every offset is a multiple of.

@@ -20,6 +20,9 @@ SYMBOLS = [
     "shlo_cuda_device", "shlo_kv_attend_workspace", "shlo_kv_attend_noalloc",
     "shlo_kv_new", "shlo_kv_free", "shlo_kv_storage", "shlo_kv_append", "shlo_kv_gather", "shlo_kv_attend",
     "shlo_test_attend_give_up",
+    "shlo_norm_rope_noalloc", "shlo_norm_rope_workspace", "shlo_norm_rope_grad_noalloc", "shlo_quantise_rows_noalloc",
+    "shlo_mul_mat8_noalloc", "shlo_linear8_workspace", "shlo_linear8_noalloc", "shlo_beam_workspace",
+    "shlo_beam_select_noalloc", "shlo_kv_fork_noalloc",
 ]
 
 
@@ -124,6 +127,18 @@ def load() -> ctypes.CDLL:
     L.shlo_kv_append_noalloc.argtypes = [pool, batch, p, i64, i64, p, i64, i64, u8, p]
     L.shlo_kv_gather_noalloc.argtypes = [pool, p, i64, i32, i32, p, p, i64, p, i64, i64, p, i64, i64, u8, p]
     L.shlo_cuda_device.argtypes = []
+    u32, size, sizep = ctypes.c_uint32, ctypes.c_size_t, ctypes.POINTER(ctypes.c_size_t)
+    L.shlo_norm_rope_noalloc.argtypes = [p, i64, i64, p, p, p, p, u8, i32, f32, p, i64, i64, i64, i32, i32, i32, u8, u32, f32, p]
+    L.shlo_norm_rope_workspace.argtypes = [sizep]
+    L.shlo_norm_rope_grad_noalloc.argtypes = [p, i64, i64, p, i64, i64, p, p, p, p, u8, i32, f32, p, i64, i64, p, p, i64, i32,
+                                              i32, i32, u8, u32, f32, p, size, p]
+    L.shlo_quantise_rows_noalloc.argtypes = [p, i64, i64, i32, u8, p, i64, p, p]
+    L.shlo_mul_mat8_noalloc.argtypes = [p, i64, p, p, i64, p, p, p, i64, i64, i32, i32, u8, p]
+    L.shlo_linear8_workspace.argtypes = [i64, i32, sizep]
+    L.shlo_linear8_noalloc.argtypes = [p, i64, u8, p, i64, p, p, p, i64, i64, i32, i32, u8, p, size, p]
+    L.shlo_beam_workspace.argtypes = [i32, i32, i32, i32, sizep]
+    L.shlo_beam_select_noalloc.argtypes = [p, i64, p, p, i32, i32, i32, i32, i32, u8, p, p, p, p, size, p]
+    L.shlo_kv_fork_noalloc.argtypes = [pool, p, i64, p, i32, i32, p, p, i32, p, i64, p, p]
     L.shlo_kv_attend_workspace.argtypes = [ctypes.POINTER(ctypes.c_size_t)]
     L.shlo_kv_attend_noalloc.argtypes = [pool, batch, p, i64, i64, i32, u8, f32, i32, i32, p, i64, i64, p, p,
                                          ctypes.c_size_t, p]

@@ -1,5 +1,6 @@
-"""The decoder operators: rotary positions, the paged key/value cache in 8 bits and
-the attention that reads it, for hosts that generate token by token.
+"""The decoder operators: rotary positions (with the norm of queries and keys), the
+paged key/value cache in 8 bits and the attention that reads it, products in 8-bit
+integers, and beam search, for hosts that generate token by token.
 
 The *_noalloc functions take device tensors of the caller's own -- objects with
 data_ptr(), shape, stride(), dtype, is_cuda, numel(), element_size() and is_contiguous(), as
@@ -89,6 +90,18 @@ def _tables(x, what, at):
     if n[1] > 1 and s[1] != 1:
         raise ShloError("%s: the last axis is strided" % what)
     return n, s[0]
+
+
+def _workspace(x, at):
+    """A workspace's pointer and its bytes."""
+    if x is None:
+        return None, 0
+    try:
+        if x.get_device() != at:
+            _elsewhere(x, at)
+    except AttributeError:
+        _elsewhere(x, at)
+    return x.data_ptr(), x.numel() * x.element_size()
 
 
 def rope_noalloc(x, positions, phases, out, *, interleaved=False, inverse=False, factor=1.0, stream=0):
@@ -208,6 +221,205 @@ def attend_noalloc(pool: Pool, q, starts, lens, tables, out, *, workspace, scale
     check(lib.shlo_kv_attend_noalloc(c, _batch(starts, lens, tables, t, at), q.data_ptr(), qs[0], qs[1], h, dt, scale,
                                      1 if causal else 0, window, out.data_ptr(), os_[0], os_[1], lp,
                                      workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream))
+
+
+def _weights(q_weight, k_weight, q_heads, h, d, what, at):
+    """The two weights' pointers and their type."""
+    if not 0 <= q_heads <= h:
+        raise ShloError("%s: %d query heads of %d" % (what, q_heads, h))
+    code, ptr = _F32, [None, None]
+    for i, w in enumerate((q_weight, k_weight)):
+        if w is None:
+            continue
+        c = _code(w, at)
+        if c != _F16 and c != _F32 or tuple(w.shape) != (d,) or (d > 1 and w.stride()[0] != 1):
+            raise ShloError("%s: a weight is not a contiguous float16 or float32 [%d]" % (what, d))
+        if i and ptr[0] is not None and c != code:
+            raise ShloError("%s: weights of two types" % what)
+        code, ptr[i] = c, w.data_ptr()
+    return ptr[0], ptr[1], code
+
+
+def norm_rope_noalloc(x, positions, phases, out, *, q_heads, q_weight, k_weight, eps, interleaved=False, factor=1.0,
+                      stream=0):
+    """x [tokens, heads, dim], each head normed (by the root of its mean square), weighted -- the first q_heads by
+    q_weight, the others by k_weight, [dim], None for ones -- and turned by positions into out."""
+    lib = load()
+    at = lib.shlo_cuda_device()
+    n, xs, dt = _rows(x, "norm_rope: x", at)
+    m, ys, dy = _rows(out, "norm_rope: out", at)
+    if m != n or dy != dt:
+        raise ShloError("norm_rope: out is not x's shape and type")
+    t, h, d = n
+    if _list(positions, _I32, "norm_rope: positions", at) != t:
+        raise ShloError("norm_rope: %d positions for %d tokens" % (positions.shape[0], t))
+    wq, wk, dw = _weights(q_weight, k_weight, q_heads, h, d, "norm_rope", at)
+    check(lib.shlo_norm_rope_noalloc(x.data_ptr(), xs[0], xs[1], positions.data_ptr(), phases.data_ptr(), wq, wk, dw,
+                                     q_heads, eps, out.data_ptr(), ys[0], ys[1], t, h, d,
+                                     2 * _list(phases, _I64, "norm_rope: phases", at), dt, 1 if interleaved else 0, factor,
+                                     stream))
+
+
+def norm_rope_workspace() -> int:
+    """Bytes of the workspace that norm_rope_grad_noalloc needs on the current device."""
+    n = ctypes.c_size_t()
+    check(load().shlo_norm_rope_workspace(ctypes.byref(n)))
+    return n.value
+
+
+def norm_rope_grad_noalloc(x, dy, positions, phases, dx, dq_weight=None, dk_weight=None, *, q_heads, q_weight, k_weight,
+                           eps, workspace=None, interleaved=False, factor=1.0, stream=0):
+    """The gradient of norm_rope_noalloc: of its output dy, into dx and the weights' (float32 [dim], None where they are
+    not asked for)."""
+    lib = load()
+    at = lib.shlo_cuda_device()
+    n, xs, dt = _rows(x, "norm_rope_grad: x", at)
+    m, gs, dg = _rows(dy, "norm_rope_grad: dy", at)
+    o, ys, do = _rows(dx, "norm_rope_grad: dx", at)
+    if m != n or dg != dt or o != n or do != dt:
+        raise ShloError("norm_rope_grad: dy or dx is not x's shape and type")
+    t, h, d = n
+    if _list(positions, _I32, "norm_rope_grad: positions", at) != t:
+        raise ShloError("norm_rope_grad: %d positions for %d tokens" % (positions.shape[0], t))
+    wq, wk, dw = _weights(q_weight, k_weight, q_heads, h, d, "norm_rope_grad", at)
+    sums = [None, None]
+    for i, w in enumerate((dq_weight, dk_weight)):
+        if w is not None:
+            if _code(w, at) != _F32 or tuple(w.shape) != (d,) or (d > 1 and w.stride()[0] != 1):
+                raise ShloError("norm_rope_grad: a weight's gradient is not a contiguous float32 [%d]" % d)
+            sums[i] = w.data_ptr()
+    wp, wn = _workspace(workspace, at)
+    check(lib.shlo_norm_rope_grad_noalloc(x.data_ptr(), xs[0], xs[1], dy.data_ptr(), gs[0], gs[1], positions.data_ptr(),
+                                          phases.data_ptr(), wq, wk, dw, q_heads, eps, dx.data_ptr(), ys[0], ys[1],
+                                          sums[0], sums[1], t, h, d, 2 * _list(phases, _I64, "norm_rope_grad: phases", at),
+                                          dt, 1 if interleaved else 0, factor, wp, wn, stream))
+
+
+# ---- products in 8-bit integers ----
+
+def _matrix(x, codes, what, at):
+    """[rows, n] whose last axis is contiguous, of one of the types: (rows, n, row stride, type code)."""
+    c, n, s = _code(x, at), x.shape, x.stride()
+    if c not in codes or len(n) != 2:
+        raise ShloError("%s: %s of rank %d not carried" % (what, x.dtype, len(n)))
+    if n[1] > 1 and s[1] != 1:
+        raise ShloError("%s: the last axis is strided" % what)
+    return n[0], n[1], s[0], c
+
+
+def _scales(x, n, what, at):
+    if _code(x, at) != _F32 or tuple(x.shape) != (n,) or (n > 1 and x.stride()[0] != 1):
+        raise ShloError("%s is not a contiguous float32 [%d]" % (what, n))
+    return x.data_ptr()
+
+
+def quantise_rows_noalloc(x, q, scale, *, stream=0):
+    """x [rows, n] rounded to int8 row by row into q, by scale (float32 [rows]); weights [channels, n] too."""
+    lib = load()
+    at = lib.shlo_cuda_device()
+    r, n, xs, dt = _matrix(x, (_F16, _F32), "quantise_rows: x", at)
+    rq, nq, qs, _ = _matrix(q, (_I8,), "quantise_rows: q", at)
+    if (rq, nq) != (r, n):
+        raise ShloError("quantise_rows: q is not x's shape")
+    if r > 1 and qs < n:
+        raise ShloError("quantise_rows: rows of q overlap")
+    check(lib.shlo_quantise_rows_noalloc(x.data_ptr(), xs, r, n, dt, q.data_ptr(), qs, _scales(scale, r, "quantise_rows: scale", at),
+                                         stream))
+
+
+def _product(n, w, w_scale, rows, out, bias, what, at):
+    m, nw, ws, _ = _matrix(w, (_I8,), what + ": w", at)
+    ro, mo, ys, dt = _matrix(out, (_F16, _F32), what + ": out", at)
+    if nw != n or ro != rows or mo != m:
+        raise ShloError("%s: [%d, %d] by weights [%d, %d] into [%d, %d]" % (what, rows, n, m, nw, ro, mo))
+    if rows > 1 and ys < m:
+        raise ShloError("%s: rows of out overlap" % what)
+    return (w.data_ptr(), ws, _scales(w_scale, m, what + ": w_scale", at),
+            None if bias is None else _scales(bias, m, what + ": bias", at), out.data_ptr(), ys, rows, n, m, dt)
+
+
+def mul_mat8_noalloc(x, x_scale, w, w_scale, out, *, bias=None, stream=0):
+    """x int8 [rows, n] by weights int8 [channels, n], times both scales, + bias (float32 [channels]) into out
+    (float16 or float32 [rows, channels]). Rows of x and w begin on multiples of 16 bytes."""
+    lib = load()
+    at = lib.shlo_cuda_device()
+    r, n, xs, _ = _matrix(x, (_I8,), "mul_mat8: x", at)
+    check(lib.shlo_mul_mat8_noalloc(x.data_ptr(), xs, _scales(x_scale, r, "mul_mat8: x_scale", at),
+                                    *_product(n, w, w_scale, r, out, bias, "mul_mat8", at), stream))
+
+
+def linear8_workspace(rows: int, n: int) -> int:
+    """Bytes of the workspace that linear8_noalloc needs for so many rows of n values."""
+    b = ctypes.c_size_t()
+    check(load().shlo_linear8_workspace(rows, n, ctypes.byref(b)))
+    return b.value
+
+
+def linear8_noalloc(x, w, w_scale, out, *, workspace, bias=None, stream=0):
+    """x [rows, n] (float16 or float32) rounded to 8 bits row by row, by weights int8 [channels, n] as mul_mat8_noalloc."""
+    lib = load()
+    at = lib.shlo_cuda_device()
+    r, n, xs, dt = _matrix(x, (_F16, _F32), "linear8: x", at)
+    wp, wn = _workspace(workspace, at)
+    check(lib.shlo_linear8_noalloc(x.data_ptr(), xs, dt, *_product(n, w, w_scale, r, out, bias, "linear8", at), wp, wn, stream))
+
+
+# ---- beam search ----
+
+def _grid(x, code, shape, what, at):
+    if _code(x, at) != code or tuple(x.shape) != shape or not x.is_contiguous():
+        raise ShloError("%s is not a contiguous %s [%d, %d]" % ((what, "float32" if code == _F32 else "int32") + shape))
+    return x.data_ptr()
+
+
+def beam_workspace(seqs: int, beams: int, keep: int, vocab: int) -> int:
+    """Bytes of the workspace that beam_select_noalloc needs."""
+    n = ctypes.c_size_t()
+    check(load().shlo_beam_workspace(seqs, beams, keep, vocab, ctypes.byref(n)))
+    return n.value
+
+
+def beam_select_noalloc(logits, scores, next_scores, parents, tokens, *, workspace, ended=None, end_token=-1, stream=0):
+    """The best continuations of every sequence's beams: logits [seqs * beams, vocab], scores float32 [seqs, beams] ->
+    next_scores float32, parents (rows of the logits) and tokens int32, each [seqs, keep]. ended int32 [seqs, beams]."""
+    lib = load()
+    at = lib.shlo_cuda_device()
+    rows, vocab, stride, dt = _matrix(logits, (_F16, _F32), "beam_select: logits", at)
+    if len(scores.shape) != 2 or len(next_scores.shape) != 2:
+        raise ShloError("beam_select: scores and next_scores are of rank 2")
+    (seqs, beams), keep = scores.shape, next_scores.shape[1]
+    if rows != seqs * beams:
+        raise ShloError("beam_select: %d rows of logits for %d sequences of %d beams" % (rows, seqs, beams))
+    wp, wn = _workspace(workspace, at)
+    check(lib.shlo_beam_select_noalloc(
+        logits.data_ptr(), stride, _grid(scores, _F32, (seqs, beams), "beam_select: scores", at),
+        None if ended is None else _grid(ended, _I32, (seqs, beams), "beam_select: ended", at), end_token, seqs, beams, keep,
+        vocab, dt, _grid(next_scores, _F32, (seqs, keep), "beam_select: next_scores", at),
+        _grid(parents, _I32, (seqs, keep), "beam_select: parents", at),
+        _grid(tokens, _I32, (seqs, keep), "beam_select: tokens", at), wp, wn, stream))
+
+
+def fork_noalloc(pool: Pool, tables, lens, parents, fresh, out_tables, out_lens, *, stream=0):
+    """Row r of the new tables and lengths goes on from row parents[r] (-1: none) of the old ones; a last page that is
+    not full is copied into page fresh[r] for all but the first row that continues its owner."""
+    lib = load()
+    at = lib.shlo_cuda_device()
+    (rows, width), stride = _tables(tables, "kv_fork: tables", at)
+    (news, w), ostride = _tables(out_tables, "kv_fork: out_tables", at)
+    if pool.device != at:
+        _pool(pool, at)
+    # (a selection's parents come as [sequences, beams])
+    flat = parents.shape if len(parents.shape) == 1 else (parents.shape[0] * parents.shape[1],) if parents.is_contiguous() else (-1,)
+    if _code(parents, at) != _I32 or flat[0] != news or (len(parents.shape) == 1 and news > 1 and parents.stride()[0] != 1):
+        raise ShloError("kv_fork: parents are not int32 of %d rows" % news)
+    if w != width or _list(lens, _I32, "kv_fork: lens", at) != rows or _list(fresh, _I32, "kv_fork: fresh", at) != news or \
+            _list(out_lens, _I32, "kv_fork: out_lens", at) != news:
+        raise ShloError("kv_fork: lens, fresh, out_tables and out_lens are not of %d rows continued by %d, tables of %d pages"
+                        % (rows, news, width))
+    if news > 1 and ostride < width:
+        raise ShloError("kv_fork: rows of out_tables overlap")
+    check(lib.shlo_kv_fork_noalloc(pool.c, tables.data_ptr(), stride, lens.data_ptr(), rows, width, parents.data_ptr(),
+                                   fresh.data_ptr(), news, out_tables.data_ptr(), ostride, out_lens.data_ptr(), stream))
 
 
 # ---- on arrays (mlx.Arr), in the library's own memory ----

@@ -190,8 +190,8 @@ int shlo_mul_mat_noalloc(const float *w, const float *x, float *y, int64_t K, in
                          int64_t w_batch_stride, void *stream);
 
 /* ---- decoder operators (no counterpart in the reference, whose modules keep nothing between calls) ----
-   Rotary positions, a paged key/value cache in 8 bits, and the attention that
-   reads it, for hosts that generate token by token. The *_noalloc functions
+   Rotary positions, a paged key/value cache in 8 bits, the attention that reads
+   it, products in 8 bits and beam search, for hosts that generate token by token. The *_noalloc functions
    work on caller-owned memory of the device that is current in CUDA
    (cudaGetDevice, as for shlo_mul_mat_noalloc), allocate nothing, and queue
    their work on `stream` (a cudaStream_t of that device; NULL is the default
@@ -221,6 +221,67 @@ int shlo_rope_phases(int32_t rot, double base, int32_t scaling, double by, doubl
 int shlo_rope_noalloc(const void *x, int64_t x_token, int64_t x_head, const int32_t *positions, const int64_t *phases,
                       void *y, int64_t y_token, int64_t y_head, int64_t tokens, int32_t heads, int32_t dim, int32_t rot,
                       uint8_t dtype, uint32_t flags, float factor, void *stream);
+
+/* The norm of queries and keys for each head with the rotation in the same pass:
+   y = turn(n w), n = x / sqrt(mean of x^2 over the head's dim values + eps), the
+   turn shlo_rope_noalloc's (flags: 1 alone). The first q_heads heads have the
+   weight q_weight [dim], the others k_weight [dim] (float16 or float32,
+   `weight_dtype`; NULL: ones). dim up to 512; y as shlo_rope_noalloc's. */
+int shlo_norm_rope_noalloc(const void *x, int64_t x_token, int64_t x_head, const int32_t *positions, const int64_t *phases,
+                           const void *q_weight, const void *k_weight, uint8_t weight_dtype, int32_t q_heads, float eps,
+                           void *y, int64_t y_token, int64_t y_head, int64_t tokens, int32_t heads, int32_t dim, int32_t rot,
+                           uint8_t dtype, uint32_t flags, float factor, void *stream);
+/* The bytes of workspace that its gradient needs on the current device. */
+int shlo_norm_rope_workspace(size_t *bytes);
+/* Its gradient: dx of x's type from dy of the same type (dx may be x or dy itself;
+   else it shares no value with them), and the weights' (float32 [dim], overwritten;
+   NULL: not asked for), sums over all tokens and their heads. The workspace holds
+   nothing between calls (NULL without the weights' gradients); calls that may run
+   at once have one each. The same call gives the same bits. */
+int shlo_norm_rope_grad_noalloc(const void *x, int64_t x_token, int64_t x_head, const void *dy, int64_t dy_token, int64_t dy_head,
+                                const int32_t *positions, const int64_t *phases, const void *q_weight, const void *k_weight,
+                                uint8_t weight_dtype, int32_t q_heads, float eps, void *dx, int64_t dx_token, int64_t dx_head,
+                                float *dq_weight, float *dk_weight, int64_t tokens, int32_t heads, int32_t dim, int32_t rot,
+                                uint8_t dtype, uint32_t flags, float factor, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Products in 8-bit integers with a scale for each row of both sides. Rows of n
+   float16 or float32 values (x_row values apart) as q [rows][n] (q_row bytes apart)
+   and scale [rows]: q = 127 x / top to the nearest whole number (of two the even
+   one), scale = top / 127, top the row's largest magnitude. A row of zeros has
+   scale 0; one with a value that is not finite zeros and scale NaN. Weights
+   [channels][n] are laid out by the same call. */
+int shlo_quantise_rows_noalloc(const void *x, int64_t x_row, int64_t rows, int32_t n, uint8_t dtype, int8_t *q, int64_t q_row,
+                               float *scale, void *stream);
+/* y[r][c] = (sum over i < n of x[r][i] w[c][i]) x_scale[r] w_scale[c] + bias[c], for
+   `rows` rows and m channels; y of `dtype`, y_row values apart, bias float32 [m] or
+   NULL. The sum is exact (32-bit integers; n up to 131071). x and w begin on
+   16-byte boundaries and have rows a multiple of 16 bytes apart; what lies between
+   rows is not read. y shares no memory with the operands. */
+int shlo_mul_mat8_noalloc(const int8_t *x, int64_t x_row, const float *x_scale, const int8_t *w, int64_t w_row, const float *w_scale,
+                          const float *bias, void *y, int64_t y_row, int64_t rows, int32_t n, int32_t m, uint8_t dtype, void *stream);
+/* Both: activations of `x_dtype`, rounded row by row into the workspace (begins on a
+   16-byte boundary; it holds nothing between calls; calls that may run at once have
+   one each), against weights in 8 bits. */
+int shlo_linear8_workspace(int64_t rows, int32_t n, size_t *bytes);
+int shlo_linear8_noalloc(const void *x, int64_t x_row, uint8_t x_dtype, const int8_t *w, int64_t w_row, const float *w_scale,
+                         const float *bias, void *y, int64_t y_row, int64_t rows, int32_t n, int32_t m, uint8_t y_dtype,
+                         void *workspace, size_t workspace_bytes, void *stream);
+
+/* Beam search's selection. Row seq * beams + b of the logits [seqs * beams][vocab]
+   (row values apart, float16 or float32) is beam b's of sequence seq; the beam goes
+   on with token t at scores[seq][b] + logit[t] - log(sum of e^logit). Of every
+   sequence the `keep` best in descending order (of equal ones the lowest beam, then
+   the lowest token first): their scores into next, the rows that they continue into
+   parents, their tokens, each [seqs][keep]. A beam with ended[seq][b] != 0 (int32,
+   or NULL) goes on with end_token alone, at its score. What is masked (-inf), and a
+   row whose logits hold a NaN or +inf, gives nothing to choose from; where less than
+   `keep` is there, the rest has score -inf, parent -1 and token -1. Up to 64 beams
+   and 64 kept, a vocabulary of up to 2^20. The workspace (8-byte boundary) holds
+   nothing between calls; calls that may run at once have one each. */
+int shlo_beam_workspace(int32_t seqs, int32_t beams, int32_t keep, int32_t vocab, size_t *bytes);
+int shlo_beam_select_noalloc(const void *logits, int64_t row, const float *scores, const int32_t *ended, int32_t end_token,
+                             int32_t seqs, int32_t beams, int32_t keep, int32_t vocab, uint8_t dtype, float *next,
+                             int32_t *parents, int32_t *tokens, void *workspace, size_t workspace_bytes, void *stream);
 
 /* A paged cache: `pages` pages of `page_tokens` tokens (16, 32, 64, 128 or 256)
    for `heads` key/value heads of `head_dim` values (a multiple of 16, up to
@@ -262,6 +323,17 @@ int shlo_kv_gather_noalloc(const shlo_kv_pool *pool, const int32_t *tables, int6
                            int32_t table_pages, const int32_t *seq, const int32_t *pos, int64_t n, void *k,
                            int64_t k_token, int64_t k_head, void *v, int64_t v_token, int64_t v_head, uint8_t dtype,
                            void *stream);
+/* Rows that go on as other rows, as a beam search's: new row r (of `news`, up to
+   65536) gets the length and the pages of row parents[r] of `rows` (outside them: no
+   tokens, no pages). Full pages are shared. A last page that is not full stays with
+   the first new row that continues its owner; for each later one its tokens and
+   scales are copied into page fresh[r], which no row holds, and that is its last
+   page. fresh[r] is not read otherwise. Entries behind a row's last page become -1.
+   out_tables and out_lens share no memory with tables and lens. A host that keeps
+   one table for several caches makes the call for each of them. */
+int shlo_kv_fork_noalloc(const shlo_kv_pool *pool, const int32_t *tables, int64_t table_stride, const int32_t *lens, int32_t rows,
+                         int32_t table_pages, const int32_t *parents, const int32_t *fresh, int32_t news, int32_t *out_tables,
+                         int64_t out_stride, int32_t *out_lens, void *stream);
 /* The device that is current in CUDA on this thread (-2: none; -1 is how many
    libraries name host memory). */
 int shlo_cuda_device(void);
