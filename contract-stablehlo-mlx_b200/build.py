@@ -24,7 +24,7 @@ LIB = os.path.join(LIB_DIR, "libshlo_cuda.so")
 SOURCES = ["mul_mat_tm_split1.cu", "mul_mat_tm_split2.cu", "mul_mat_tm_split4.cu", "mul_mat_tm_split8.cu",
            "mul_mat_tm_split16.cu", "mul_mat_short.cu", "mul_mat_seg.cu",
            "ggml_kernels.cu", "attention.cu", "rope.cu", "kv_cache.cu", "kv_attend.cu", "kv_attend_tiles.cu",
-           "norm_rope.cu", "linear8.cu", "beam.cu", "kv_fork.cu", "decode_arrays.cu", "runtime.cu", "elementwise.cu", "api.cu", "fusion.cu"]
+           "norm_rope.cu", "linear8.cu", "linear8_tiles.cu", "beam.cu", "kv_fork.cu", "decode_arrays.cu", "runtime.cu", "elementwise.cu", "api.cu", "fusion.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

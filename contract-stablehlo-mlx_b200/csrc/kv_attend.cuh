@@ -53,8 +53,6 @@ struct AttendArgs {
   unsigned give_up;    // every so many blocks of the tiles give up at once (0: none)
 };
 
-constexpr uint64_t kWaitLimitNs = 2000000000ull;
-
 constexpr int kAttendMaxBlocks = 1024;
 // Partials joined at once: what a join's factors take in shared memory bounds it.
 template <int ROWS> constexpr int kJoin = ROWS >= 128 ? 32 : 64;

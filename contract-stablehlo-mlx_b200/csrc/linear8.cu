@@ -59,47 +59,6 @@ __global__ void __launch_bounds__(kQuantThreads) k_quantise_rows(const T *x, int
   for (int i = n + threadIdx.x; i < fill; i += kQuantThreads) q[i] = 0;
 }
 
-// 64 channels by 32 rows a block, 32 values of both at a time; a thread has 4 by 2 sums.
-__global__ void __launch_bounds__(256) k_mul_mat8(const Mm8Call c) {
-  __shared__ int ws[64][9], xs[32][9];
-  const int64_t c0 = (int64_t)blockIdx.x * 64, r0 = (int64_t)blockIdx.y * 32;
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  int acc[2][4] = {};
-  auto four = [&](const int8_t *p, int at) {
-    uint32_t v = 0;
-#pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (at + j < c.n) v |= (uint32_t)(uint8_t)p[at + j] << (8 * j);
-    return (int)v;
-  };
-  for (int k = 0; k < c.n; k += 32) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < 96 * 8; i += 256) {
-      const int r = i / 8, at = k + i % 8 * 4;
-      if (r < 64) ws[r][i % 8] = c0 + r < c.m ? four(c.w + (c0 + r) * c.w_row, at) : 0;
-      else xs[r - 64][i % 8] = r0 + r - 64 < c.rows ? four(c.x + (r0 + r - 64) * c.x_row, at) : 0;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-#pragma unroll
-      for (int a = 0; a < 2; a++)
-#pragma unroll
-        for (int b = 0; b < 4; b++) acc[a][b] = __dp4a(xs[ty + 16 * a][i], ws[tx + 16 * b][i], acc[a][b]);
-  }
-#pragma unroll
-  for (int a = 0; a < 2; a++)
-#pragma unroll
-    for (int b = 0; b < 4; b++) {
-      const int64_t r = r0 + ty + 16 * a, ch = c0 + tx + 16 * b;
-      if (r >= c.rows || ch >= c.m) continue;
-      float v = (float)acc[a][b] * c.x_scale[r] * c.w_scale[ch];
-      if (c.bias) v += c.bias[ch];
-      if (c.dtype == kF16) static_cast<__half *>(c.y)[r * c.y_row + ch] = __float2half_rn(v);
-      else static_cast<float *>(c.y)[r * c.y_row + ch] = v;
-    }
-}
-
 }  // namespace
 
 int launch_quantise_rows(const void *x, int64_t x_row, uint8_t dtype, int64_t rows, int32_t n, int8_t *q, int64_t q_row, float *scale,
@@ -145,8 +104,7 @@ int launch_mul_mat8(const Mm8Call &c, int sms, cudaStream_t st) {
   if ((uintptr_t)c.x % 16 || (c.rows > 1 && (c.x_row % 16 || c.x_row < c.n)))
     return fail("mul_mat8: rows of x begin on multiples of 16 bytes and do not overlap (a distance of %lld for %d values)", (long long)c.x_row, c.n);
   if ((uintptr_t)c.x_scale % 4) return fail("mul_mat8: an operand is not aligned to its type");
-  k_mul_mat8<<<dim3((c.m + 63) / 64, (unsigned)((c.rows + 31) / 32)), 256, 0, st>>>(c);
-  return launch_check("mul_mat8");
+  return launch_mul_mat8_tiles(c, sms, st);
 }
 
 // Rows of int8 at distances of a multiple of 16 bytes, then their scales.
@@ -185,6 +143,7 @@ int shlo_mul_mat8_noalloc(const int8_t *x, int64_t x_row, const float *x_scale, 
                           const float *bias, void *y, int64_t y_row, int64_t rows, int32_t n, int32_t m, uint8_t dtype, void *stream) {
   Device *dev;
   SHLO_TRY(calling_device(&dev));
+  SHLO_TRY(launch_error(dev, "mul_mat8, an earlier call"));
   Mm8Call c{x, x_row, x_scale, w, w_row, w_scale, bias, y, y_row, rows, n, m, dtype, dev->pipe_err_dev};
   return launch_mul_mat8(c, dev->sm_count, (cudaStream_t)stream);
 }
@@ -201,6 +160,7 @@ int shlo_linear8_noalloc(const void *x, int64_t x_row, uint8_t x_dtype, const in
                          void *workspace, size_t workspace_bytes, void *stream) {
   Device *dev;
   SHLO_TRY(calling_device(&dev));
+  SHLO_TRY(launch_error(dev, "linear8, an earlier call"));
   Mm8Call c{nullptr, 0, nullptr, w, w_row, w_scale, bias, y, y_row, rows, n, m, y_dtype, dev->pipe_err_dev};
   return launch_linear8(c, x, x_row, x_dtype, workspace, workspace_bytes, dev->sm_count, (cudaStream_t)stream);
 }

@@ -67,7 +67,7 @@ def quantise(x):
 
 def mul_mat8(x, xs, w, ws, bias=None, dtype=np.float32):
     """The stated binary32 operations, in order."""
-    acc = x.astype(np.int64) @ w.astype(np.int64).T
+    acc = x.astype(np.float64) @ w.astype(np.float64).T  # whole numbers below 2^53
     with np.errstate(over="ignore", invalid="ignore"):
         y = acc.astype(np.float32) * xs[:, None] * ws[None, :]
         if bias is not None:

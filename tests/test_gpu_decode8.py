@@ -255,7 +255,7 @@ def weights(rng, m, n):
 @pytest.mark.parametrize("r,n,m", [(1, 1, 1), (1, 512, 768), (1, 4097, 130), (2, 16, 64), (3, 100, 1000), (5, 2000, 129), (8, 640, 257),
                                    (16, 1024, 4096), (17, 515, 300), (24, 4096, 515), (33, 31, 33), (64, 8192, 384), (65, 777, 1001),
                                    (130, 1300, 200), (257, 129, 640), (300, 512, 2050), (1000, 260, 1111), (2, 131071, 3),
-                                   (700, 1999, 2049)])
+                                   (700, 1999, 2049), (2300, 1000, 2700), (100, 200, 40000)])
 def test_linear8(kind, r, n, m):
     rng = np.random.default_rng(r * 31 + n)
     x, (w, ws) = activations(rng, r, n, kind), weights(rng, m, n)
