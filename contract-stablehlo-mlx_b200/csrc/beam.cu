@@ -3,19 +3,26 @@
 //   score[beam] + logit - log(sum over the vocabulary of e^logit),
 // in descending order, of equal ones the lowest beam first, then the lowest token.
 //
-// Two kernels. The first gives a block a segment of a row, which it reads once
-// into registers: the segment's largest logit, the sum of e^(logit - largest), and
-// its `keep` largest logits, in order. The second joins a sequence's segments: a
-// row's sum, then its segments' lists merged one continuation at a time.
+// Two kernels. The first gives a block a part of a row, which it reads once, a stretch
+// of registers at a time: each thread's largest logit so far and the sum of
+// e^(logit - largest), and the part's `keep` largest logits, of which the first
+// stretch gives a border that few of the later ones pass. The second joins a
+// sequence's parts: a row's sum, then its parts' lists.
 //
 // Two beams' continuations may lie closer together than binary32 tells apart, and
-// the order between them is part of the result: the exponentials are a polynomial
-// that is right to 2^-25 at each term and unbiased, eight of them are added in
-// binary32 and all else in 64 bits. A row's logarithm is then off by 2^-23 at most
-// and, where several logits matter, by 10^-8.
+// the order between them is part of the result. A term of the sum is ex2.approx's,
+// within 2^-22, eight of them are added in binary32 and the rest in 64 bits; the
+// terms of the candidates, which are most of a peaked row's sum, are replaced by a
+// polynomial's, right to 2^-24. What is left is 2^-22 of the light terms' share, and
+// averages out where they are many.
 //
-// Bound: bytes (each logit read once); the first kernel's 10 instructions a logit
-// are next.
+// Bound: bytes (each logit read once), then the first kernel's ten instructions a
+// logit. Measured on one B200: 64 sequences of 8 beams over 128256 float16 logits (125
+// MB) 47 us; 5 of 32 over 50257 float32 logits, 64 kept 38 us; one of 4 over 32001 10
+// us. Measured and left: the polynomial for every term (64 us on the first case: the
+// heavy half of the FMA pipe), a part of one stretch each (73 us: every one searches
+// for its border), borders by halving over lists in memory (67 us for the second case's
+// join alone).
 #include <algorithm>
 #include <cmath>
 
@@ -27,9 +34,12 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxKeep = 64, kMaxBeams = 64;
-constexpr int kRoom = 256;  // candidates that a segment ranks at once
+constexpr int kRoom = 512;  // candidates of a part at a time
+constexpr int kGroup = 4;   // stretches whose candidates are looked at together: 1, 1, 2, 4, 4, ...
 constexpr int kJoin = 256;  // the second kernel's threads
-constexpr int kPicked = 512;  // candidates that it ranks at once
+constexpr int kPicked = 512;  // candidates that it ranks
+constexpr int kSteps = 7;     // entries 2^j - 1 < kMaxKeep of a list
+static_assert(1 << (kSteps - 1) <= kMaxKeep, "entries of a list");
 
 struct BeamArgs {
   const void *z;
@@ -38,10 +48,10 @@ struct BeamArgs {
   const int32_t *ended;
   float *next;
   int32_t *parents, *tokens;
-  uint64_t *best;  // [rows][segs][keep]: ordered logit above, ~token below; 0: none
-  double *sum;     // [rows][segs]
-  float *top;      // [rows][segs]: NaN: a value that is not a number, or infinity
-  int vocab, beams, keep, segs, seg, end_token;
+  uint64_t *best;  // [rows][parts][keep]: ordered logit above, ~token below; 0: none
+  double *sum;     // [rows][parts]
+  float *top;      // [rows][parts]: what the sum counts from; NaN: a value that is not a number, or infinity
+  int vocab, beams, keep, parts, part, end_token;  // part: logits a part
   int group;  // lanes: 256 / group is at least keep
 };
 
@@ -60,16 +70,17 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+__device__ __forceinline__ uint32_t bits(float x) { return __float_as_uint(x); }
+__device__ __forceinline__ uint32_t bits(__half x) { return __half_as_ushort(x); }
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
-// e^d for -87 <= d <= 0: d = i ln 2 + r (ln 2 in two parts, the first of 15 bits, so
-// that its products are exact), e^r = 1 + r + r^2 g(r), g of degree 4 fitted to the
-// smallest largest relative error (2^-28, 3 10^-10 on average).
-__device__ __forceinline__ float2 exp_below(float2 d) {
+// e^d for -87 <= d <= 87: d = i ln 2 + r (ln 2 rounded: 2.7 10^-9 of d), e^r = 1 + r +
+// r^2 g(r), g of degree 4 fitted to the smallest largest relative error (2^-28,
+// 3 10^-10 on average).
+__device__ __forceinline__ float2 exp_near(float2 d) {
   const float2 m = __ffma2_rn(d, both(0x1.715476p+0f), both(12582912.0f));
   const float2 i = __fadd2_rn(m, both(-12582912.0f));
-  float2 r = __ffma2_rn(i, both(-0x1.62e4p-1f), d);
-  r = __ffma2_rn(i, both(-0x1.7f7d1cp-20f), r);
+  const float2 r = __ffma2_rn(i, both(-0x1.62e430p-1f), d);
   float2 g = both(0x1.6a23d0p-10f);
   g = __ffma2_rn(g, r, both(0x1.123a20p-7f));
   g = __ffma2_rn(g, r, both(0x1.5558f2p-5f));
@@ -82,6 +93,15 @@ __device__ __forceinline__ float2 exp_below(float2 d) {
   return g;
 }
 
+// The same within 2^-22, and 0 for -infinity: 2^(d log2(e)), the product in two parts.
+__device__ __forceinline__ float2 exp_fast(float2 d) {
+  const float2 t = __ffma2_rn(d, both(0x1.4ae0c0p-26f), __fmul2_rn(d, both(0x1.715476p+0f)));
+  float2 e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+  return e;
+}
+
 // What a type's vectors of 16 bytes need: the largest of their values (NaN where
 // one is), their values less the largest of all, the values themselves.
 template <typename T> struct Vec;
@@ -92,13 +112,12 @@ template <> struct Vec<__half> {
     const __half2 m = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
     return max_nan(__low2float(m), __high2float(m));
   }
-  // (what is more than 80 below adds 10^-35: it is kept there, for e^d's range)
   static __device__ __forceinline__ float2 below(const uint4 &v, int pair, float top) {
     const __half2 h = reinterpret_cast<const __half2 *>(&v)[pair];
     float2 d;
     asm("add.rn.f32.f16 %0, %1, %2;" : "=f"(d.x) : "h"(__half_as_ushort(__low2half(h))), "f"(-top));
     asm("add.rn.f32.f16 %0, %1, %2;" : "=f"(d.y) : "h"(__half_as_ushort(__high2half(h))), "f"(-top));
-    return make_float2(fmaxf(d.x, -80.0f), fmaxf(d.y, -80.0f));
+    return d;
   }
   static __device__ __forceinline__ float value(const uint4 &v, int i) { return __half2float(reinterpret_cast<const __half *>(&v)[i]); }
   static __device__ __half neg_inf() { return __ushort_as_half(0xfc00); }
@@ -110,8 +129,7 @@ template <> struct Vec<float> {
   }
   static __device__ __forceinline__ float2 below(const uint4 &v, int pair, float top) {
     const float *f = reinterpret_cast<const float *>(&v) + 2 * pair;
-    const float2 d = __fadd2_rn(make_float2(f[0], f[1]), both(-top));
-    return make_float2(fmaxf(d.x, -80.0f), fmaxf(d.y, -80.0f));
+    return __fadd2_rn(make_float2(f[0], f[1]), both(-top));
   }
   static __device__ __forceinline__ float value(const uint4 &v, int i) { return reinterpret_cast<const float *>(&v)[i]; }
   static __device__ float neg_inf() { return -INFINITY; }
@@ -120,24 +138,27 @@ template <> struct Vec<float> {
 // (four blocks on an SM: the waits for the logits and between the warps of one
 // are the others' work)
 template <typename T, int NV>
-__global__ void __launch_bounds__(kThreads, 4) k_beam_segments(const BeamArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) k_beam_parts(const BeamArgs a) {
   using V = Vec<T>;
-  constexpr int W = V::W;  // values a vector
+  constexpr int W = V::W;                    // values a vector
+  constexpr int STRETCH = NV * kThreads * W;
   __shared__ float tops[kWarps], lows[kWarps];
   __shared__ double sums[kWarps];
   __shared__ uint64_t found[kRoom];
   __shared__ int count;
-  const int row = blockIdx.y, s = blockIdx.x, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  __shared__ uint32_t least_shared;
+  const int row = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   if (a.ended && a.ended[row]) return;  // it goes on with one token, whatever its logits
   const T *const z = static_cast<const T *>(a.z) + row * a.row;
-  const int lo = s * a.seg;
-  // Vector i of this thread. Which logits it has does not depend on where the row
-  // lies, so that equal rows have equal sums; where it begins between two 16-byte
-  // boundaries it is cut from two of memory's vectors.
+  const int begin = blockIdx.x * a.part, end = min(begin + a.part, a.vocab);
+  // Vector i of this thread in the stretch from lo on. Which logits it has does not
+  // depend on where the row lies, so that equal rows have equal sums; where it begins
+  // between two 16-byte boundaries it is cut from two of memory's vectors.
   const int past = (int)((uintptr_t)z & 15);
-  auto load = [&](int i) -> uint4 {
+  auto load = [&](int lo, int i) -> uint4 {
     const int at = lo + (i * kThreads + threadIdx.x) * W, off = past / (int)sizeof(T);
     if (past == 0 && at + W <= a.vocab) return __ldg(reinterpret_cast<const uint4 *>(z + at));
+    if (sizeof(T) == 4 && at + W <= a.vocab) return make_uint4(bits(z[at]), bits(z[at + 1]), bits(z[at + 2]), bits(z[at + 3]));
     if (past && at >= off && at - off + 2 * W <= a.vocab) {
       const uint4 p = __ldg(reinterpret_cast<const uint4 *>(z + (at - off))), q = __ldg(reinterpret_cast<const uint4 *>(z + (at - off) + W));
       const int sh = past % 4 * 8;
@@ -158,160 +179,269 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_segments(const BeamArgs a)
     memcpy(&r, e, 16);
     return r;
   };
-  uint4 v[NV];
+  auto token = [&](int lo, int i, int j) { return lo + (i * kThreads + (int)threadIdx.x) * W + j; };
+
+  // (every logit -infinity where `from` is)
+  auto exps = [&](const uint4 (&v)[NV], float from) {
+    const float zero = from > -INFINITY ? from : 0.0f;
+    double sum = 0.0;
 #pragma unroll
-  for (int i = 0; i < NV; i++) v[i] = load(i);
+    for (int i = 0; i < NV; i++) {
+      float2 e[W / 2];
+#pragma unroll
+      for (int j = 0; j < W / 2; j++) e[j] = exp_fast(V::below(v[i], j, zero));
+#pragma unroll
+      for (int j = W / 4; j; j /= 2)
+#pragma unroll
+        for (int l = 0; l < j; l++) e[l] = __fadd2_rn(e[l], e[l + j]);
+      sum += (double)(e[0].x + e[0].y);
+    }
+    return sum;
+  };
+  // Candidates threadIdx.x / per (and, above kThreads of them, threadIdx.x + kThreads),
+  // and how many are above them (none of a thread's: kRoom); `per` lanes count for one.
+  auto rank = [&](int n, uint64_t (&k)[2]) {
+    const int per = n <= kThreads / 4 ? 4 : n <= kThreads / 2 ? 2 : 1, at = (int)threadIdx.x / per, off = (int)threadIdx.x % per;
+    int2 above = make_int2(0, 0);
+    k[0] = at < n ? found[at] : 0;
+    k[1] = at + kThreads < n ? found[at + kThreads] : 0;
+    if (n <= kThreads)
+      for (int j = off; j < n; j += per) above.x += found[j] > k[0];
+    else
+      for (int j = 0; j < n; j++) {
+        const uint64_t o = found[j];
+        above.x += o > k[0];
+        above.y += o > k[1];
+      }
+    for (int i = 1; i < per; i *= 2) above.x += __shfl_xor_sync(~0u, above.x, i);
+    if (at >= n || off) above.x = kRoom;
+    if (at + kThreads >= n || per > 1) above.y = kRoom;
+    return above;
+  };
+  // The next stretch is on its way to shared memory while one is worked on; a thread
+  // reads there what it asked for itself.
+  __shared__ uint4 ahead[NV * kThreads];
+  int asked = -1;
+  double sum = 0.0;        // the sum of e^(logit - from) over this thread's logits,
+  float from = -INFINITY;  // the first stretch's largest
+  bool odd = false;        // whether one is not a number, or infinity,
+  bool far = false;        // or too far above `from`
+  uint32_t least = 0;     // candidates are the logits that reach this, in order
+  int n = 0;              // candidates so far
   if (threadIdx.x == 0) count = 0;
-  auto token = [&](int i, int j) { return lo + (i * kThreads + (int)threadIdx.x) * W + j; };
+  for (int lo = begin; lo < end;) {
+    const bool first = lo == begin;
+    const int group = lo, group_end = min(end, lo + (first ? 1 : min((lo - begin) / STRETCH, kGroup)) * STRETCH);
+    bool some = false;
+    for (; lo < group_end; lo += STRETCH) {
+      uint4 v[NV];
+      if (lo == asked) {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < NV; i++) v[i] = ahead[i * kThreads + threadIdx.x];
+      } else {
+#pragma unroll
+        for (int i = 0; i < NV; i++) v[i] = load(lo, i);
+      }
+      if (past == 0 && lo + STRETCH < end && lo + 2 * STRETCH <= a.vocab) {
+        asked = lo + STRETCH;
+        const uint4 *const p = reinterpret_cast<const uint4 *>(z + asked) + threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(ahead + i * kThreads + threadIdx.x)), "l"(p + i * kThreads) : "memory");
+      }
+      float tops_of[NV], mine = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        tops_of[i] = V::top(v[i]);
+        mine = max_nan(mine, tops_of[i]);
+      }
+      odd = odd || !(mine < INFINITY);
+      const uint32_t key = ordered(mine);
+      if (first) {
+        // A border that at least `keep` threads' largest logits reach, and few more: from
+        // the smallest of the largest of `group` lanes each, as many groups as are kept,
+        // by halving between two borders. (Where fewer threads have any logit above
+        // -infinity, all of those are candidates.)
+        float top = mine, low = mine;
+#pragma unroll
+        for (int i = 1; i < 32; i *= 2) {
+          top = fmaxf(top, __shfl_xor_sync(~0u, top, i));
+          const float o = __shfl_xor_sync(~0u, low, i);
+          low = i < a.group ? fmaxf(low, o) : fminf(low, o);
+        }
+        if (lane == 0) tops[warp] = top, lows[warp] = low;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kWarps; i++) {
+          top = fmaxf(top, tops[i]);
+          low = fminf(low, lows[i]);
+        }
+        from = top;
+        uint32_t over = ordered(top) + 1;
+        least = low > -INFINITY ? ordered(low) : kNegInf + 1;
+        int have = __syncthreads_count(key >= least);
+        if (have >= a.keep)
+          while (have > a.keep + 8 && over - least > 1 && over > least) {
+            const uint32_t mid = least + (over - least) / 2;
+            const int m = __syncthreads_count(key >= mid);
+            if (m >= a.keep) least = mid, have = m;
+            else over = mid;
+          }
+      }
 
-  // The largest logit, and the smallest of the largest of `group` lanes each: as many
-  // groups as are kept, so that at least so many threads' largest reach it.
-  float mine = -INFINITY;
+      far = far || mine > from + 60.0f;
+      sum += exps(v, from);
+
+      if (key >= least) {
+        some = true;
+        const float border = of_ordered(least);
+        unsigned which = 0;
 #pragma unroll
-  for (int i = 0; i < NV; i++) mine = max_nan(mine, V::top(v[i]));
-  float top = mine, low = mine;
+        for (int i = 0; i < NV; i++) which |= (tops_of[i] >= border) << i;
+        for (; which; which &= which - 1) {
+          const int i = __ffs(which) - 1;
+          uint4 w = v[0];
 #pragma unroll
-  for (int i = 1; i < 32; i *= 2) {
-    top = max_nan(top, __shfl_xor_sync(~0u, top, i));
-    const float o = __shfl_xor_sync(~0u, low, i);
-    low = i < a.group ? fmaxf(low, o) : fminf(low, o);
+          for (int j = 1; j < NV; j++)
+            if (i == j) w = v[j];
+#pragma unroll
+          for (int j = 0; j < W; j++)
+            if (V::value(w, j) >= border) {
+              const int k = atomicAdd(&count, 1);
+              if (k < kRoom) found[k] = (uint64_t)ordered(V::value(w, j)) << 32 | (uint32_t)~token(lo, i, j);
+            }
+        }
+      }
+    }
+    if (!__syncthreads_or(some)) continue;
+    const int before = n;
+    n = count;
+    __syncthreads();
+    if (n > kRoom) {
+      // More of them than there is room for (many equal ones, or rows that rise): the
+      // exact border of these stretches, and which of the logits that equal it.
+      auto counted = [&](uint32_t t, uint32_t last) {  // logits above t, and those at t whose ~token is at least last
+        int c = 0;
+        for (int at = group; at < group_end; at += STRETCH)
+#pragma unroll 1
+          for (int i = 0; i < NV; i++) {
+            const uint4 w = load(at, i);
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+              const uint32_t u = ordered(V::value(w, j));
+              if (u > t || (u == t && (uint32_t)~token(at, i, j) >= last)) c++;
+            }
+          }
+        c = __reduce_add_sync(~0u, c);
+        __syncthreads();
+        if (lane == 0) tops[warp] = __int_as_float(c);
+        __syncthreads();
+        c = 0;
+#pragma unroll
+        for (int i = 0; i < kWarps; i++) c += __float_as_int(tops[i]);
+        return c;
+      };
+      uint32_t t0 = least, t1 = 0xff800001u;  // enough reach t0; t1 is above all numbers
+      while (t1 - t0 > 1) {
+        const uint32_t mid = t0 + (t1 - t0) / 2;
+        if (counted(mid, 0) >= a.keep) t0 = mid;
+        else t1 = mid;
+      }
+      uint32_t l0 = 0, l1 = 0xffffffffu;  // enough at or above l0
+      while (l1 - l0 > 1) {
+        const uint32_t mid = l0 + (l1 - l0) / 2;
+        if (counted(t0, mid) >= a.keep) l0 = mid;
+        else l1 = mid;
+      }
+      __syncthreads();
+      if (threadIdx.x == 0) count = before;
+      __syncthreads();
+      for (int at = group; at < group_end; at += STRETCH)
+#pragma unroll 1
+        for (int i = 0; i < NV; i++) {
+          const uint4 w = load(at, i);
+#pragma unroll
+          for (int j = 0; j < W; j++) {
+            const uint32_t u = ordered(V::value(w, j)), last = ~token(at, i, j);
+            if (u > t0 || (u == t0 && last >= l0)) found[atomicAdd(&count, 1)] = (uint64_t)u << 32 | last;
+          }
+        }
+      __syncthreads();
+      n = count;
+      __syncthreads();
+    }
+    // The best of them, in order; later stretches' candidates are above the last (of
+    // equal ones the earlier is better).
+    if (n >= a.keep) {
+      uint64_t k[2];
+      const int2 above = rank(n, k);
+      __syncthreads();
+      if (above.x < a.keep) found[above.x] = k[0];
+      if (above.y < a.keep) found[above.y] = k[1];
+      if (above.x == a.keep - 1) least_shared = (uint32_t)(k[0] >> 32) + 1, count = a.keep;
+      if (above.y == a.keep - 1) least_shared = (uint32_t)(k[1] >> 32) + 1, count = a.keep;
+      __syncthreads();
+      least = least_shared;
+      n = a.keep;
+    }
   }
-  if (lane == 0) tops[warp] = top, lows[warp] = low;
-  __syncthreads();
+
+  // A row whose first stretch is far below what follows (or masked) is added up once
+  // more, from its largest.
+  if (__syncthreads_or(far)) {
+    float most = -INFINITY;
+    for (int lo = begin; lo < end; lo += STRETCH)
+#pragma unroll 1
+      for (int i = 0; i < NV; i++) most = fmaxf(most, V::top(load(lo, i)));
 #pragma unroll
-  for (int i = 0; i < kWarps; i++) {
-    top = max_nan(top, tops[i]);
-    low = fminf(low, lows[i]);
+    for (int i = 16; i; i /= 2) most = fmaxf(most, __shfl_xor_sync(~0u, most, i));
+    if (lane == 0) tops[warp] = most;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kWarps; i++) most = fmaxf(most, tops[i]);
+    from = most;
+    sum = 0.0;
+    for (int lo = begin; lo < end; lo += STRETCH) {
+      uint4 v[NV];
+#pragma unroll
+      for (int i = 0; i < NV; i++) v[i] = load(lo, i);
+      sum += exps(v, from);
+    }
   }
-  const int64_t place = (int64_t)row * a.segs + s;
+  const int64_t place = (int64_t)row * a.parts + blockIdx.x;
   uint64_t *const best = a.best + place * a.keep;
-  if (!(top < INFINITY) || top == -INFINITY) {  // nothing to choose from
-    if (threadIdx.x == 0) {
-      a.top[place] = top == -INFINITY ? top : __uint_as_float(0x7fc00000u);
-      a.sum[place] = 0.0;
-    }
-    for (int i = threadIdx.x; i < a.keep; i += kThreads) best[i] = 0;
-    return;
+  if (n == a.keep) {  // (in order already)
+    if ((int)threadIdx.x < n) best[threadIdx.x] = found[threadIdx.x];
+  } else {
+    uint64_t k[2];
+    const int above = rank(n, k).x;  // (fewer than keep: one a thread)
+    if (above < a.keep) best[above] = k[0];
   }
-
-  // A border that at least `keep` threads' largest logits reach, and few more: found
-  // by halving between two borders. (Where fewer threads than `keep` have any logit
-  // above -infinity, all of them are candidates, or the exact border below is found.)
-  uint32_t under = low > -INFINITY ? ordered(low) : kNegInf + 1, over = ordered(top) + 1;
-  const uint32_t key = ordered(mine);
-  int have = __syncthreads_count(key >= under);
-  if (have >= a.keep)
-    while (have > 2 * a.keep && over - under > 1) {
-      const uint32_t mid = under + (over - under) / 2;
-      const int n = __syncthreads_count(key >= mid);
-      if (n >= a.keep) under = mid, have = n;
-      else over = mid;
-    }
-
-  double sum = 0.0;
-#pragma unroll
-  for (int i = 0; i < NV; i++) {
-    float2 e[W / 2];
-#pragma unroll
-    for (int j = 0; j < W / 2; j++) e[j] = exp_below(V::below(v[i], j, top));
-#pragma unroll
-    for (int j = W / 4; j; j /= 2)
-#pragma unroll
-      for (int l = 0; l < j; l++) e[l] = __fadd2_rn(e[l], e[l + j]);
-    sum += (double)(e[0].x + e[0].y);
+  for (int i = n + threadIdx.x; i < a.keep; i += kThreads) best[i] = 0;
+  // The part's sum, the candidates' terms by the polynomial.
+  if ((int)threadIdx.x < n) {
+    const float d = of_ordered((uint32_t)(found[threadIdx.x] >> 32)) - from;
+    sum += (double)exp_near(make_float2(fmaxf(d, -80.0f), 0.0f)).x - (double)exp_fast(make_float2(d, 0.0f)).x;
   }
 #pragma unroll
   for (int i = 16; i; i /= 2) sum += __shfl_xor_sync(~0u, sum, i);
   if (lane == 0) sums[warp] = sum;
-  if (key >= under) {
-    const float border = of_ordered(under);
-    unsigned which = 0;
-#pragma unroll
-    for (int i = 0; i < NV; i++) which |= (V::top(v[i]) >= border) << i;
-    for (; which; which &= which - 1) {  // (read again, from L2: few threads have any)
-      const int i = __ffs(which) - 1;
-      const uint4 w = load(i);
-#pragma unroll
-      for (int j = 0; j < W; j++)
-        if (V::value(w, j) >= border) {
-          const int n = atomicAdd(&count, 1);
-          if (n < kRoom) found[n] = (uint64_t)ordered(V::value(w, j)) << 32 | (uint32_t)~token(i, j);
-        }
-    }
-  }
-  __syncthreads();
+  odd = __syncthreads_or(odd);
   if (threadIdx.x == 0) {
     double all = 0.0;
 #pragma unroll
     for (int i = 0; i < kWarps; i++) all += sums[i];
     a.sum[place] = all;
-    a.top[place] = top;
+    a.top[place] = odd ? __uint_as_float(0x7fc00000u) : from;
   }
-  int n = count;
-  if (n > kRoom) {
-    // More of them than there is room for (many equal ones, or few threads that
-    // hold most): the exact border, and which of those that equal it.
-    auto counted = [&](uint32_t t, uint32_t last) {  // logits above t, and those at t whose ~token is at least last
-      int c = 0;
-#pragma unroll 1
-      for (int i = 0; i < NV; i++) {
-        const uint4 w = load(i);
-#pragma unroll
-        for (int j = 0; j < W; j++) {
-          const uint32_t u = ordered(V::value(w, j));
-          if (u > t || (u == t && (uint32_t)~token(i, j) >= last)) c++;
-        }
-      }
-      c = __reduce_add_sync(~0u, c);
-      __syncthreads();
-      if (lane == 0) tops[warp] = __int_as_float(c);
-      __syncthreads();
-      c = 0;
-#pragma unroll
-      for (int i = 0; i < kWarps; i++) c += __float_as_int(tops[i]);
-      return c;
-    };
-    uint32_t t0 = under, t1 = ordered(top) + 1;  // enough reach t0; t1 is above all
-    while (t1 - t0 > 1) {
-      const uint32_t mid = t0 + (t1 - t0) / 2;
-      if (counted(mid, 0) >= a.keep) t0 = mid;
-      else t1 = mid;
-    }
-    uint32_t l0 = 0, l1 = 0xffffffffu;  // enough at or above l0
-    while (l1 - l0 > 1) {
-      const uint32_t mid = l0 + (l1 - l0) / 2;
-      if (counted(t0, mid) >= a.keep) l0 = mid;
-      else l1 = mid;
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) count = 0;
-    __syncthreads();
-#pragma unroll 1
-    for (int i = 0; i < NV; i++) {
-      const uint4 w = load(i);
-#pragma unroll
-      for (int j = 0; j < W; j++) {
-        const uint32_t u = ordered(V::value(w, j)), last = ~token(i, j);
-        if (u > t0 || (u == t0 && last >= l0)) found[atomicAdd(&count, 1)] = (uint64_t)u << 32 | last;
-      }
-    }
-    __syncthreads();
-    n = count;
-  }
-  for (int i = threadIdx.x; i < n; i += kThreads) {
-    const uint64_t k = found[i];
-    int above = 0;
-    for (int j = 0; j < n; j++) above += found[j] > k;
-    if (above < a.keep) best[above] = k;
-  }
-  for (int i = n + threadIdx.x; i < a.keep; i += kThreads) best[i] = 0;
 }
 
-// A sequence a block. A list is a segment's of one beam, in descending order; a
-// thread has lists threadIdx.x, + kJoin, ... Of the threads' best heads the
-// keep-th best is a border: what reaches it is a handful of each list's entries,
-// which are ranked against each other. Where they are too many (or too few lists
-// have a head), the best of all heads is taken `keep` times instead.
+// A sequence a block. A list is a part's of one beam, in descending order; a
+// thread has lists threadIdx.x, + kJoin, ... From entries 0, 1, 3, 7, ... of each list
+// follows a border that at least `keep` entries reach, and few more; those are ranked
+// against each other. Where too many are equal, the best of all heads is taken `keep`
+// times instead.
 __global__ void __launch_bounds__(kJoin) k_beam_join(const BeamArgs a) {
   extern __shared__ unsigned char at_list[];  // of a list: how many of its entries are taken
   // Of a beam: its score less the logarithm of its row's sum (NaN: none to choose
@@ -324,42 +454,55 @@ __global__ void __launch_bounds__(kJoin) k_beam_join(const BeamArgs a) {
   __shared__ uint64_t key_of[kPicked];
   __shared__ int list_of[kPicked];
   __shared__ int picked;
-  __shared__ double border;
-  const int seq = blockIdx.x, lists = a.beams * a.segs, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const int seq = blockIdx.x, lists = a.beams * a.parts, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const double none = -INFINITY;
-  cudaGridDependencySynchronize();  // (it may begin before the segments are done)
-  for (int b = warp; b < a.beams; b += kJoin / 32) {
+  cudaGridDependencySynchronize();  // (it may begin before the parts are done)
+  // (entries 0, 1, 3, 7, ... of a thread's first list are on their way meanwhile)
+  uint64_t some[kSteps];
+#pragma unroll
+  for (int j = 0; j < kSteps; j++)
+    some[j] = (int)threadIdx.x < lists && (1 << j) <= a.keep ? a.best[((int64_t)seq * lists + threadIdx.x) * a.keep + (1 << j) - 1] : 0;
+  // A few lanes a beam: all beams at once.
+  int lanes = 32;
+  while (lanes * a.beams > kJoin) lanes /= 2;
+  {
+    const int b = threadIdx.x / lanes;
     const int64_t row = (int64_t)seq * a.beams + b;
-    const double score = (double)a.scores[row];
-    const bool end = a.ended && a.ended[row];
+    const bool there = b < a.beams, end = there && a.ended && a.ended[row];
+    const double score = there ? (double)a.scores[row] : 0.0;
     float top = -INFINITY;
     double sum = 0.0;
-    if (!end) {
-      for (int s = lane; s < a.segs; s += 32) top = max_nan(top, a.top[row * a.segs + s]);
-      for (int i = 16; i; i /= 2) top = max_nan(top, __shfl_xor_sync(~0u, top, i));
-      if (top > -INFINITY)
-        for (int s = lane; s < a.segs; s += 32) {
-          const float t = a.top[row * a.segs + s];
-          if (t > -INFINITY) sum += a.sum[row * a.segs + s] * exp((double)t - (double)top);
-        }
-      for (int i = 16; i; i /= 2) sum += __shfl_xor_sync(~0u, sum, i);
-    }
-    if (lane == 0) {
-      base[b] = end ? score : top > -INFINITY ? score - log(sum) : __longlong_as_double(0x7ff8000000000000ll);
-      top_of[b] = top;
+    if (there && !end)
+      for (int s = threadIdx.x % lanes; s < a.parts; s += lanes) {
+        const float t = a.top[row * a.parts + s];
+        const double part = a.sum[row * a.parts + s];
+        const float m = max_nan(top, t);
+        if (m > -INFINITY) sum = (top > -INFINITY ? sum * exp((double)top - (double)m) : 0.0) + (t > -INFINITY ? part * exp((double)t - (double)m) : 0.0);
+        top = m;
+      }
+    float m = top;
+    for (int i = 1; i < lanes; i *= 2) m = max_nan(m, __shfl_xor_sync(~0u, m, i));
+    sum = top > -INFINITY ? sum * exp((double)top - (double)m) : 0.0;
+    for (int i = 1; i < lanes; i *= 2) sum += __shfl_xor_sync(~0u, sum, i);
+    if (there && threadIdx.x % lanes == 0) {
+      base[b] = end ? score : m > -INFINITY ? score - log(sum) : __longlong_as_double(0x7ff8000000000000ll);
+      top_of[b] = m;
       ended[b] = end;
     }
   }
   for (int i = threadIdx.x; i < lists; i += kJoin) at_list[i] = 0;
-  if (threadIdx.x == 0) picked = 0, border = none;
+  if (threadIdx.x == 0) picked = 0;
   __syncthreads();
-  // Entry `at` of list l: its key, 0 behind the last, and its total.
+  // A list is named by its beam (the upper half) and its number. Entry `at` of it: its
+  // key, 0 behind the last, and its total.
+  auto named = [&](int l) { return l / a.parts << 16 | l; };
   auto entry = [&](int l, int at, double &t) -> uint64_t {
-    const int b = l / a.segs, s = l - b * a.segs;
+    const int b = l >> 16;
+    l &= 0xffff;
     t = base[b];
-    if (ended[b]) return s == 0 && at == 0 && t > none ? ~0ull : 0;
+    if (ended[b]) return l == b * a.parts && at == 0 && t > none ? ~0ull : 0;
     if (at >= a.keep || !(t > none)) return 0;
-    const uint64_t k = a.best[(((int64_t)seq * a.beams + b) * a.segs + s) * a.keep + at];
+    const uint64_t k = a.best[((int64_t)seq * lists + l) * a.keep + at];
     t += (double)of_ordered((uint32_t)(k >> 32)) - (double)top_of[b];
     return t > none ? k : 0;
   };
@@ -368,13 +511,12 @@ __global__ void __launch_bounds__(kJoin) k_beam_join(const BeamArgs a) {
     if (l2 < 0) return false;
     if (l < 0) return true;
     if (t != t2) return t2 > t;
-    const int b = l / a.segs, b2 = l2 / a.segs;
-    return b != b2 ? b2 < b : k2 > k;
+    return l >> 16 != l2 >> 16 ? l2 >> 16 < l >> 16 : k2 > k;
   };
   auto write = [&](int i, double t, uint64_t k, int l) {
     const int64_t to = (int64_t)seq * a.keep + i;
     a.next[to] = l < 0 ? -INFINITY : (float)t;
-    a.parents[to] = l < 0 ? -1 : seq * a.beams + l / a.segs;
+    a.parents[to] = l < 0 ? -1 : seq * a.beams + (l >> 16);
     a.tokens[to] = l < 0 ? -1 : k == ~0ull ? a.end_token : (int32_t)~(uint32_t)k;
   };
   // The best of this thread's heads.
@@ -387,38 +529,111 @@ __global__ void __launch_bounds__(kJoin) k_beam_join(const BeamArgs a) {
     key = 0;
     for (int l = threadIdx.x; l < lists; l += kJoin) {
       double t;
-      const uint64_t k = entry(l, at_list[l], t);
-      if (k && better(total, key, list, t, k, l)) total = t, key = k, list = l;
+      const int name = named(l);
+      const uint64_t k = entry(name, at_list[l], t);
+      if (k && better(total, key, list, t, k, name)) total = t, key = k, list = name;
     }
   };
-  offer();
-
-  total_of[threadIdx.x] = total;
-  __syncthreads();
-  int above = 0;
-  for (int i = 0; i < kJoin; i++) above += total_of[i] > total || (total_of[i] == total && i < (int)threadIdx.x);
-  if (above == a.keep - 1) border = total;  // (-infinity where fewer threads have a head)
-  __syncthreads();
-  const double least = border;
-  if (list >= 0)
-    for (int l = threadIdx.x; l < lists; l += kJoin)
-      for (int at = 0;; at += 4) {
-        double t[4];
-        uint64_t k[4];
+  // The totals of those entries; none: -infinity.
+  double reached[kSteps];
 #pragma unroll
-        for (int j = 0; j < 4; j++) k[j] = entry(l, at + j, t[j]);
-        bool on = true;
+  for (int j = 0; j < kSteps; j++) {
+    const int b = min((int)threadIdx.x / a.parts, a.beams - 1);
+    if (ended[b]) reached[j] = j == 0 && (int)threadIdx.x < lists && threadIdx.x % a.parts == 0 ? base[b] : none;
+    else reached[j] = some[j] ? base[b] + ((double)of_ordered((uint32_t)(some[j] >> 32)) - (double)top_of[b]) : none;
+    if (!(reached[j] > none)) reached[j] = none;
+  }
+  // How many entries reach each of eight borders at least: of a list whose entry
+  // 2^j - 1 does, 2^j; so that less than twice as many do (and as many lists more).
+  // Returns the last border that `keep` reach (and how many do), 8 for none; borders
+  // descend.
+  auto first_enough = [&](const double (&t)[8], int &c) {
+    int m[8];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          on = on && k[j] && t[j] >= least;
-          if (on) {
-            const int n = atomicAdd(&picked, 1);
-            if (n < kPicked) total_of[n] = t[j], key_of[n] = k[j], list_of[n] = l;
-            else on = false;
-          }
-        }
-        if (!on) break;
+    for (int i = 0; i < 8; i++) {
+      m[i] = 0;
+#pragma unroll
+      for (int j = 0; j < kSteps; j++) m[i] += reached[j] >= t[i] ? (1 << j) - (1 << j >> 1) : 0;
+    }
+    for (int l = threadIdx.x + kJoin; l < lists; l += kJoin) {
+      const int name = named(l);
+      for (int j = 0; j < kSteps && 1 << j <= a.keep; j++) {
+        double u;
+        if (!entry(name, (1 << j) - 1, u)) break;
+        for (int i = 0; i < 8; i++) m[i] += u >= t[i] ? (1 << j) - (1 << j >> 1) : 0;
       }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      m[i] = __reduce_add_sync(~0u, m[i]);
+      if (lane == i) list_of[warp * 8 + i] = m[i];
+    }
+    __syncthreads();
+    int got = 0;
+    if (lane < 8)
+      for (int i = 0; i < kJoin / 32; i++) got += list_of[i * 8 + lane];
+    const unsigned enough = __ballot_sync(~0u, lane < 8 && got >= a.keep);
+    const int at = enough ? __ffs(enough) - 1 : 8;
+    if (at < 8) c = __shfl_sync(~0u, got, at);
+    __syncthreads();
+    return at;
+  };
+  // A border that `keep` entries reach, and few more: some way below the best, then
+  // by eighths of what is left.
+  double best = reached[0];
+  for (int l = threadIdx.x + kJoin; l < lists; l += kJoin) {
+    double t;
+    if (entry(named(l), 0, t)) best = fmax(best, t);
+  }
+  for (int i = 16; i; i /= 2) best = fmax(best, __shfl_xor_sync(~0u, best, i));
+  if (lane == 0) total_of[warp] = best;
+  __syncthreads();
+  for (int i = 0; i < kJoin / 32; i++) best = fmax(best, total_of[i]);
+  double near = best, far = none;  // (too few reach `near`, enough reach `far`)
+  if (best > none) {
+    int c = 0;
+    double t[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) t[i] = best - (double)(1 << (i < 6 ? i : 2 * i - 5));  // 1, 2, 4, ... 32, 128, 512
+    const int at = first_enough(t, c);
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      if (i == at) far = t[i];
+      if (i < at) near = t[i];
+    }
+    for (int k = 0; k < 4 && far > none && c > a.keep + a.keep / 2 + 8; k++) {
+      const double by = (far - near) / 9.0;
+#pragma unroll
+      for (int i = 0; i < 8; i++) t[i] = near + by * (i + 1);
+      const int at = first_enough(t, c);
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        if (i == at) far = t[i];
+        if (i < at) near = t[i];
+      }
+    }
+  }
+  const double least = far;  // (-infinity: all there are)
+  for (int l = threadIdx.x; l < lists; l += kJoin) {
+    const int name = named(l);
+    for (int at = 0;; at += 4) {
+      double t[4];
+      uint64_t k[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) k[j] = entry(name, at + j, t[j]);
+      bool on = true;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        on = on && k[j] && t[j] >= least;
+        if (on) {
+          const int i = atomicAdd(&picked, 1);
+          if (i < kPicked) total_of[i] = t[j], key_of[i] = k[j], list_of[i] = name;
+          else on = false;
+        }
+      }
+      if (!on) break;
+    }
+  }
   __syncthreads();
   const int n = picked;
   if (n <= kPicked) {
@@ -437,6 +652,7 @@ __global__ void __launch_bounds__(kJoin) k_beam_join(const BeamArgs a) {
     return;
   }
 
+  offer();
   for (int i = 0; i < a.keep; i++) {
     double t = total;
     uint64_t k = key;
@@ -453,31 +669,47 @@ __global__ void __launch_bounds__(kJoin) k_beam_join(const BeamArgs a) {
     for (int j = 0; j < kJoin / 32; j++)
       if (better(t, k, l, total_of[j], key_of[j], list_of[j])) t = total_of[j], k = key_of[j], l = list_of[j];
     if (threadIdx.x == 0) write(i, t, k, l);
-    if (l >= 0 && l % kJoin == (int)threadIdx.x) {
-      at_list[l]++;
+    if (l >= 0 && (l & 0xffff) % kJoin == (int)threadIdx.x) {
+      at_list[l & 0xffff]++;
       offer();
     }
   }
 }
 
-// The segments of a row: a block's registers hold `nv` vectors a thread, fewer where
-// the segments would leave SMs without work.
-int segments(int vocab, size_t size, int nv) {
-  const int seg = nv * kThreads * (16 / (int)size);
-  return (vocab + seg - 1) / seg;
-}
-int vectors(int64_t rows, int vocab, size_t size, int sms) {
-  int nv = size == 2 ? 4 : 8;
-  while (nv > 1 && rows * segments(vocab, size, nv) < 2 * sms) nv /= 2;
-  return nv;
+// How a row is cut: stretches of `nv` vectors a thread, `turns` of them a part.
+struct Cut {
+  int nv, stretch, turns, parts;
+};
+Cut cut(int64_t rows, int vocab, size_t size, int sms) {
+  Cut c;
+  auto stretches = [&](int nv) {
+    c.stretch = nv * kThreads * (16 / (int)size);
+    return (vocab + c.stretch - 1) / c.stretch;
+  };
+  // Shorter stretches where they would leave SMs without work.
+  c.nv = size == 2 ? 4 : 8;
+  while (c.nv > 1 && rows * stretches(c.nv) < 2 * sms) c.nv /= 2;
+  const int n = stretches(c.nv);
+  // Turns of blocks, four an SM, by the stretches of each, the first of which costs
+  // two: its border has to be found. (512 rows of 128256: 47 us at 8 and 16 stretches a
+  // part, 53 at 4, 73 at 1; 160 rows of 50257: 38 us at 1, 47 at 2, 60 at 7.)
+  const int64_t slots = 4 * (int64_t)sms;
+  int64_t least = INT64_MAX;
+  c.turns = 1;
+  for (int t = 1; t <= n; t++) {
+    const int64_t cost = (rows * ((n + t - 1) / t) + slots - 1) / slots * (t + 1);
+    if (cost < least) least = cost, c.turns = t;
+  }
+  c.parts = (n + c.turns - 1) / c.turns;
+  return c;
 }
 
 }  // namespace
 
-// The room for both types: float32's segments are the shorter ones.
+// (float32's shortest stretches are the most parts that a row can have)
 size_t beam_work_bytes(int64_t rows, int32_t keep, int32_t vocab) {
-  const int64_t segs = segments(vocab, 4, 1);
-  return (size_t)(rows * segs * (8 * (int64_t)keep + 12) + 16);
+  const int64_t parts = (vocab + 4 * kThreads - 1) / (4 * kThreads);
+  return (size_t)(rows * parts * (8 * (int64_t)keep + 12) + 16);
 }
 
 int launch_beam_select(const BeamCall &c, int sms, cudaStream_t st) {
@@ -495,33 +727,33 @@ int launch_beam_select(const BeamCall &c, int sms, cudaStream_t st) {
   const size_t need = beam_work_bytes(rows, c.keep, c.vocab);
   if (!c.work || c.work_bytes < need) return fail("beam_select: a workspace of %zu bytes, %zu needed", c.work ? c.work_bytes : 0, need);
   if ((uintptr_t)c.work % 8) return fail("beam_select: misaligned workspace");
-  const int nv = vectors(rows, c.vocab, size, sms);
+  const Cut how = cut(rows, c.vocab, size, sms);
   BeamArgs a;
   a.z = c.logits; a.row = c.row; a.scores = c.scores; a.ended = c.ended; a.next = c.next; a.parents = c.parents; a.tokens = c.tokens;
   a.vocab = c.vocab; a.beams = c.beams; a.keep = c.keep; a.end_token = c.end_token;
   a.group = 32;
   while (a.group > 1 && kThreads / a.group < c.keep) a.group /= 2;
-  a.seg = nv * kThreads * (16 / (int)size);
-  a.segs = segments(c.vocab, size, nv);
+  a.part = how.stretch * how.turns;
+  a.parts = how.parts;
   a.best = (uint64_t *)c.work;
-  a.sum = (double *)(a.best + rows * a.segs * c.keep);
-  a.top = (float *)(a.sum + rows * a.segs);
-  const dim3 grid((unsigned)a.segs, (unsigned)rows);
+  a.sum = (double *)(a.best + rows * a.parts * c.keep);
+  a.top = (float *)(a.sum + rows * a.parts);
+  const dim3 grid((unsigned)a.parts, (unsigned)rows);
   if (c.dtype == kF16) {
-    if (nv == 4) k_beam_segments<__half, 4><<<grid, kThreads, 0, st>>>(a);
-    else if (nv == 2) k_beam_segments<__half, 2><<<grid, kThreads, 0, st>>>(a);
-    else k_beam_segments<__half, 1><<<grid, kThreads, 0, st>>>(a);
+    if (how.nv == 4) k_beam_parts<__half, 4><<<grid, kThreads, 0, st>>>(a);
+    else if (how.nv == 2) k_beam_parts<__half, 2><<<grid, kThreads, 0, st>>>(a);
+    else k_beam_parts<__half, 1><<<grid, kThreads, 0, st>>>(a);
   } else {
-    if (nv == 8) k_beam_segments<float, 8><<<grid, kThreads, 0, st>>>(a);
-    else if (nv == 4) k_beam_segments<float, 4><<<grid, kThreads, 0, st>>>(a);
-    else if (nv == 2) k_beam_segments<float, 2><<<grid, kThreads, 0, st>>>(a);
-    else k_beam_segments<float, 1><<<grid, kThreads, 0, st>>>(a);
+    if (how.nv == 8) k_beam_parts<float, 8><<<grid, kThreads, 0, st>>>(a);
+    else if (how.nv == 4) k_beam_parts<float, 4><<<grid, kThreads, 0, st>>>(a);
+    else if (how.nv == 2) k_beam_parts<float, 2><<<grid, kThreads, 0, st>>>(a);
+    else k_beam_parts<float, 1><<<grid, kThreads, 0, st>>>(a);
   }
   SHLO_TRY(launch_check("beam_select"));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)c.seqs);
   cfg.blockDim = dim3(kJoin);
-  cfg.dynamicSmemBytes = (size_t)c.beams * a.segs;
+  cfg.dynamicSmemBytes = (size_t)c.beams * a.parts;
   cfg.stream = st;
   cudaLaunchAttribute early;
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
