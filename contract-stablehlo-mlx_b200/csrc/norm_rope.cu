@@ -33,12 +33,10 @@ struct NormArgs {
   int heads, q_heads, dim, rot;
   int lanes_log;  // lanes a group
   int nt_log;     // tokens a block (at a time)
-  int hb;         // forward: heads a block
-  int parts_q;    // backward: blockIdx.y below this: query heads, hb_q a block; from there on key heads, hb_k a block
-  int hb_q, hb_k;
+  int hb;         // heads a block
   float eps, factor;
-  bool w_half;
-  float *partials;  // backward: [gridDim.y][gridDim.x][dim], nullptr without the weights' gradients
+  bool w_half, w_wide;  // the weights' type, and whether they allow wide loads
+  float *partials;      // backward: [blocks][2][dim], nullptr without the weights' gradients
 };
 
 template <int BYTES> struct Raw;
@@ -119,27 +117,75 @@ __device__ __forceinline__ float safe_scale(float ss, float eps) {
   return 1.0f;
 }
 
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 neg(float2 x) { return make_float2(-x.x, -x.y); }
+
+// A part as pairs (a, b), two of them in a register pair. (Where a slot is not
+// turned, its pairs' sine is 0.)
+template <typename T, int VEC, int NS, bool INTER>
+__device__ __forceinline__ void pairs(Part<T, VEC, NS> &r, float2 (&a)[NS * VEC / 2], float2 (&b)[NS * VEC / 2]) {
+#pragma unroll
+  for (int i = 0; i < NS * VEC / 2; i++) {
+    constexpr int V = VEC;
+    const int p = 2 * i, q = 2 * i + 1;
+    a[i] = make_float2(to_f32(first<V, INTER>(r.v[p / V], p % V)), to_f32(first<V, INTER>(r.v[q / V], q % V)));
+    b[i] = make_float2(to_f32(second<V, INTER>(r.v[p / V], p % V)), to_f32(second<V, INTER>(r.v[q / V], q % V)));
+  }
+}
+template <typename T, int VEC, int NS, bool INTER>
+__device__ __forceinline__ void unpairs(const float2 (&a)[NS * VEC / 2], const float2 (&b)[NS * VEC / 2], Part<T, VEC, NS> &r) {
+#pragma unroll
+  for (int i = 0; i < NS * VEC / 2; i++) {
+    constexpr int V = VEC;
+    const int p = 2 * i, q = 2 * i + 1;
+    of_f32(first<V, INTER>(r.v[p / V], p % V), a[i].x);
+    of_f32(first<V, INTER>(r.v[q / V], q % V), a[i].y);
+    of_f32(second<V, INTER>(r.v[p / V], p % V), b[i].x);
+    of_f32(second<V, INTER>(r.v[q / V], q % V), b[i].y);
+  }
+}
+
 // BACK: the gradient. A block goes over tiles of 2^nt_log tokens, one in the
 // forward pass, for the heads of its part.
 template <typename T, int VEC, int NS, bool INTER, bool BACK>
-__global__ void __launch_bounds__(kThreads) k_norm_rope(const NormArgs a) {
-  extern __shared__ float sh[];  // cosines, sines: [token][half] each; backward: the block's sums in their place
+__global__ void __launch_bounds__(kThreads, NS * VEC > 8 || (BACK && sizeof(T) == 2) ? 2 : 3) k_norm_rope(const NormArgs a) {
+  // Backward: 2 P pairs a thread; then the cosines and sines, [token][half] each, and at
+  // the end the block's sums, [warp][dim], in their place.
+  extern __shared__ float2 sh[];
+  constexpr int P = NS * VEC / 2;
   const int half = a.rot / 2, nt = 1 << a.nt_log;
-  float *const cs = sh, *const sn = sh + nt * half;
+  float *const cs = reinterpret_cast<float *>(sh + (BACK ? 2 * P * kThreads : 0)), *const sn = cs + nt * half;
   const int lane = threadIdx.x & ((1 << a.lanes_log) - 1), group = threadIdx.x >> a.lanes_log;
   const int groups = kThreads >> a.lanes_log;
-  // A block of the backward pass has heads of one weight, whose sums it keeps.
-  const bool back_keys = BACK && (int)blockIdx.y >= a.parts_q;
-  const int h0 = !BACK ? blockIdx.y * a.hb : back_keys ? a.q_heads + (blockIdx.y - a.parts_q) * a.hb_k : blockIdx.y * a.hb_q;
-  const int h1 = !BACK ? min(h0 + a.hb, a.heads) : back_keys ? min(h0 + a.hb_k, a.heads) : min(h0 + a.hb_q, a.q_heads);
+  const int h0 = blockIdx.y * a.hb, h1 = min(h0 + a.hb, a.heads);
   Places<NS> at;
   places<VEC, NS, INTER>(a, lane, at);
-  float w[NS][2][VEC];
-  int has = -1;  // whose weight w is: 0 the queries', 1 the keys'
-  auto weigh = [&](int keys) {
-    if (keys == has) return;
-    has = keys;
+  auto weight = [&](bool keys, float2 (&wa)[P], float2 (&wb)[P]) {
     const void *const wp = keys ? a.wk : a.wq;
+    Part<float, VEC, NS> w;
+    Part<__half, VEC, NS> wh;
+    clear_part(w);
+    if (wp && a.w_wide) {
+      if (a.w_half) {
+        clear_part(wh);
+        load_part(static_cast<const __half *>(wp), at, wh);
+        pairs<__half, VEC, NS, INTER>(wh, wa, wb);
+        return;
+      }
+      constexpr int V = VEC < 4 ? VEC : 4;
+      using R = typename Raw<V * sizeof(float)>::T;
+#pragma unroll
+      for (int s = 0; s < NS; s++)
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const int o = k ? at.o2[s] : at.o[s];
+#pragma unroll
+          for (int j = 0; j < VEC; j += V)
+            if (o >= 0) *reinterpret_cast<R *>(&w.v[s][k][j]) = *reinterpret_cast<const R *>(static_cast<const float *>(wp) + o + j);
+        }
+      pairs<float, VEC, NS, INTER>(w, wa, wb);
+      return;
+    }
 #pragma unroll
     for (int s = 0; s < NS; s++)
 #pragma unroll
@@ -147,32 +193,66 @@ __global__ void __launch_bounds__(kThreads) k_norm_rope(const NormArgs a) {
         const int o = k ? at.o2[s] : at.o[s];
 #pragma unroll
         for (int j = 0; j < VEC; j++)
-          w[s][k][j] = o < 0 ? 0.0f : !wp ? 1.0f : a.w_half ? __half2float(static_cast<const __half *>(wp)[o + j]) : static_cast<const float *>(wp)[o + j];
+          if (o >= 0) w.v[s][k][j] = !wp ? 1.0f : a.w_half ? __half2float(static_cast<const __half *>(wp)[o + j]) : static_cast<const float *>(wp)[o + j];
       }
+    pairs<float, VEC, NS, INTER>(w, wa, wb);
   };
-  float dw[BACK ? NS : 1][2][VEC];
-  if (BACK) {
-#pragma unroll
-    for (int s = 0; s < NS; s++)
-#pragma unroll
-      for (int j = 0; j < VEC; j++) dw[s][0][j] = dw[s][1][j] = 0.0f;
-  }
-  const float inv_dim = 1.0f / a.dim;
   const int t = group & (nt - 1), h_first = h0 + (group >> a.nt_log), h_step = max(groups >> a.nt_log, 1);
+  // Of a token's pairs (shared memory's, and none where a slot is not turned): the cosines and sines.
+  auto turn = [&](float2 (&c)[P], float2 (&s)[P]) {
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+      float cc[2], ss[2];
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const int p = 2 * i + j, slot = p / VEC, unit = lane + (slot << a.lanes_log);
+        cc[j] = at.pair[slot] ? cs[t * half + unit * VEC + p % VEC] : 1.0f;
+        ss[j] = at.pair[slot] ? sn[t * half + unit * VEC + p % VEC] : 0.0f;
+      }
+      c[i] = make_float2(cc[0], cc[1]);
+      s[i] = make_float2(ss[0], ss[1]);
+    }
+  };
+  // Backward: a weight, and the sums of its gradient; the other weight's sums lie in
+  // shared memory meanwhile.
+  float2 dwa[BACK ? P : 1], dwb[BACK ? P : 1], wa[BACK ? P : 1], wb[BACK ? P : 1];
+  float2 *const other = sh + threadIdx.x;
+  int has = -1;  // whose weight is in registers: 0 the queries', 1 the keys'
+  if constexpr (BACK) {
+#pragma unroll
+    for (int i = 0; i < P; i++) {
+      dwa[i] = dwb[i] = both(0.0f);
+      other[2 * i * kThreads] = other[(2 * i + 1) * kThreads] = both(0.0f);
+    }
+  }
+  auto swap = [&]() {
+    if constexpr (BACK) {
+#pragma unroll
+      for (int i = 0; i < P; i++) {
+        const float2 p = other[2 * i * kThreads], q = other[(2 * i + 1) * kThreads];
+        other[2 * i * kThreads] = dwa[i];
+        other[(2 * i + 1) * kThreads] = dwb[i];
+        dwa[i] = p;
+        dwb[i] = q;
+      }
+    }
+  };
+  const float inv_dim = 1.0f / a.dim;
   const int64_t tiles = (a.tokens + nt - 1) >> a.nt_log;
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int64_t t0 = tile << a.nt_log;
     const bool mine = t0 + t < a.tokens;
-    const T *const x = static_cast<const T *>(a.x) + (t0 + t) * a.xt;
-    const T *const g = static_cast<const T *>(a.dy) + (BACK ? (t0 + t) * a.gt : 0);
-    T *const y = static_cast<T *>(a.y) + (t0 + t) * a.yt;
+    const T *x = static_cast<const T *>(a.x) + (t0 + t) * a.xt + h_first * a.xh;
+    const T *g = BACK ? static_cast<const T *>(a.dy) + (t0 + t) * a.gt + h_first * a.gh : nullptr;
+    T *y = static_cast<T *>(a.y) + (t0 + t) * a.yt + h_first * a.yh;
+    const int64_t x_step = h_step * a.xh, g_step = h_step * a.gh, y_step = h_step * a.yh;
     // (the loads need nothing of the angles: they go out first)
     Part<T, VEC, NS> next, next_g;
     clear_part(next);
     if (BACK) clear_part(next_g);
     if (mine && h_first < h1) {
-      load_part(x + h_first * a.xh, at, next);
-      if (BACK) load_part(g + h_first * a.gh, at, next_g);
+      load_part(x, at, next);
+      if (BACK) load_part(g, at, next_g);
     }
     if (BACK && tile != (int64_t)blockIdx.x) __syncthreads();
     for (int i = threadIdx.x; i < nt * half; i += kThreads) {
@@ -182,170 +262,162 @@ __global__ void __launch_bounds__(kThreads) k_norm_rope(const NormArgs a) {
         float s, c;
         sincospif((float)turns * 0x1p-31f, &s, &c);
         cs[i] = c * a.factor;
-        sn[i] = (BACK ? -s : s) * a.factor;
+        sn[i] = s * a.factor;
       }
     }
     __syncthreads();
-    float c[NS][VEC], s_[NS][VEC];
-#pragma unroll
-    for (int s = 0; s < NS; s++)
-#pragma unroll
-      for (int j = 0; j < VEC; j++) {
-        const int p = (lane + (s << a.lanes_log)) * VEC + j;
-        c[s][j] = at.pair[s] && mine ? cs[t * half + p] : 1.0f;
-        s_[s][j] = at.pair[s] && mine ? sn[t * half + p] : 0.0f;
-      }
+    // Forward: what a pair's two results take of its two values, weight and turn in
+    // one: (a, b) -> (a ca - b sb, b cb + a sa). Backward: the turn.
+    float2 ca[P], sa[P], cb[BACK ? 1 : P], sb[BACK ? 1 : P];
+    if constexpr (BACK) turn(ca, sa);
+    else has = -1;
     // (a warp's groups take the same number of turns: its shuffles name all lanes)
-    for (int h = h_first - (group >> a.nt_log); h < h1; h += h_step) {
+    for (int h = h0; h < h1; h += h_step) {
       const int hh = h + (group >> a.nt_log);
       const bool there = mine && hh < h1;
-      weigh(BACK ? back_keys : hh >= a.q_heads);
-      Part<T, VEC, NS> in = next, in_g = next_g;
-      if (mine && hh + h_step < h1) {
-        load_part(x + (hh + h_step) * a.xh, at, next);
-        if (BACK) load_part(g + (hh + h_step) * a.gh, at, next_g);
-      }
-      float v[NS][2][VEC], ss = 0.0f;
+      if (has != (int)(hh >= a.q_heads)) {
+        if (BACK && has >= 0) swap();
+        has = hh >= a.q_heads;
+        if constexpr (BACK) {
+          weight(has, wa, wb);
+        } else {
+          float2 c[P], s[P], u[P], v[P];
+          turn(c, s);
+          weight(has, u, v);
 #pragma unroll
-      for (int s = 0; s < NS; s++)
-#pragma unroll
-        for (int k = 0; k < 2; k++)
-#pragma unroll
-          for (int j = 0; j < VEC; j++) {
-            v[s][k][j] = to_f32(in.v[s][k][j]);
-            ss = __fmaf_rn(v[s][k][j], v[s][k][j], ss);
+          for (int i = 0; i < P; i++) {
+            ca[i] = __fmul2_rn(u[i], c[i]);
+            sa[i] = __fmul2_rn(u[i], s[i]);
+            cb[i] = __fmul2_rn(v[i], c[i]);
+            sb[i] = __fmul2_rn(v[i], s[i]);
           }
-      ss = group_sum(ss, a.lanes_log);
-      float scale = 1.0f, eps = a.eps;
+        }
+      }
+      float2 xa[P], xb[P], sum = both(0.0f);
+      pairs<T, VEC, NS, INTER>(next, xa, xb);
+      Part<T, VEC, NS> in_g;
+      if (BACK) in_g = next_g;
+      if (mine && hh + h_step < h1) {
+        load_part(x + x_step, at, next);
+        if (BACK) load_part(g + g_step, at, next_g);
+      }
+#pragma unroll
+      for (int i = 0; i < P; i++) sum = __ffma2_rn(xb[i], xb[i], __ffma2_rn(xa[i], xa[i], sum));
+      float ss = group_sum(sum.x + sum.y, a.lanes_log), scale = 1.0f, eps = a.eps;
       if (sizeof(T) == 4) {
         scale = safe_scale(ss, eps);
         if (__any_sync(~0u, scale != 1.0f)) {
           eps = eps * scale * scale;  // (scale^2 itself has no place in 32 bits)
-          ss = 0.0f;
+          sum = both(0.0f);
 #pragma unroll
-          for (int s = 0; s < NS; s++)
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-#pragma unroll
-              for (int j = 0; j < VEC; j++) {
-                v[s][k][j] *= scale;
-                ss = __fmaf_rn(v[s][k][j], v[s][k][j], ss);
-              }
-          ss = group_sum(ss, a.lanes_log);
+          for (int i = 0; i < P; i++) {
+            xa[i] = __fmul2_rn(xa[i], both(scale));
+            xb[i] = __fmul2_rn(xb[i], both(scale));
+            sum = __ffma2_rn(xb[i], xb[i], __ffma2_rn(xa[i], xa[i], sum));
+          }
+          ss = group_sum(sum.x + sum.y, a.lanes_log);
         }
       }
-      const float inv = __frsqrt_rn(__fmaf_rn(ss, inv_dim, eps));
-      Part<T, VEC, NS> out;
-      if (!BACK) {
+      // (2^-22 is enough where the result has 11 bits)
+      const float inv = sizeof(T) == 2 ? rsqrtf(__fmaf_rn(ss, inv_dim, eps)) : __frsqrt_rn(__fmaf_rn(ss, inv_dim, eps));
+      float2 ya[P], yb[P];
+      if constexpr (!BACK) {
 #pragma unroll
-        for (int s = 0; s < NS; s++) {
-#pragma unroll
-          for (int k = 0; k < 2; k++)
-#pragma unroll
-            for (int j = 0; j < VEC; j++) v[s][k][j] = v[s][k][j] * inv * w[s][k][j];
-          if (at.pair[s]) {
-#pragma unroll
-            for (int j = 0; j < VEC; j++) {
-              const float p = first<VEC, INTER>(v[s], j), q = second<VEC, INTER>(v[s], j);
-              first<VEC, INTER>(v[s], j) = __fmaf_rn(p, c[s][j], -(q * s_[s][j]));
-              second<VEC, INTER>(v[s], j) = __fmaf_rn(q, c[s][j], p * s_[s][j]);
-            }
-          }
+        for (int i = 0; i < P; i++) {
+          const float2 p = __fmul2_rn(xa[i], both(inv)), q = __fmul2_rn(xb[i], both(inv));
+          ya[i] = __ffma2_rn(p, ca[i], neg(__fmul2_rn(q, sb[i])));
+          yb[i] = __ffma2_rn(q, cb[i], __fmul2_rn(p, sa[i]));
         }
       } else {
-        float d[NS][2][VEC], gn = 0.0f;
+        float2 ga[P], gb[P], dot = both(0.0f);
+        pairs<T, VEC, NS, INTER>(in_g, ga, gb);
 #pragma unroll
-        for (int s = 0; s < NS; s++) {
-#pragma unroll
-          for (int k = 0; k < 2; k++)
-#pragma unroll
-            for (int j = 0; j < VEC; j++) d[s][k][j] = to_f32(in_g.v[s][k][j]);
-          if (at.pair[s]) {
-#pragma unroll
-            for (int j = 0; j < VEC; j++) {
-              const float p = first<VEC, INTER>(d[s], j), q = second<VEC, INTER>(d[s], j);
-              first<VEC, INTER>(d[s], j) = __fmaf_rn(p, c[s][j], -(q * s_[s][j]));
-              second<VEC, INTER>(d[s], j) = __fmaf_rn(q, c[s][j], p * s_[s][j]);
-            }
+        for (int i = 0; i < P; i++) {
+          xa[i] = __fmul2_rn(xa[i], both(inv));
+          xb[i] = __fmul2_rn(xb[i], both(inv));
+          // turned back
+          const float2 p = __ffma2_rn(ga[i], ca[i], __fmul2_rn(gb[i], sa[i]));
+          const float2 q = __ffma2_rn(gb[i], ca[i], neg(__fmul2_rn(ga[i], sa[i])));
+          if (there) {
+            dwa[i] = __ffma2_rn(p, xa[i], dwa[i]);
+            dwb[i] = __ffma2_rn(q, xb[i], dwb[i]);
           }
-#pragma unroll
-          for (int k = 0; k < 2; k++)
-#pragma unroll
-            for (int j = 0; j < VEC; j++) {
-              v[s][k][j] *= inv;
-              if (there) dw[s][k][j] = __fmaf_rn(d[s][k][j], v[s][k][j], dw[s][k][j]);
-              d[s][k][j] *= w[s][k][j];
-              gn = __fmaf_rn(d[s][k][j], v[s][k][j], gn);
-            }
+          ga[i] = __fmul2_rn(p, wa[i]);
+          gb[i] = __fmul2_rn(q, wb[i]);
+          dot = __ffma2_rn(gb[i], xb[i], __ffma2_rn(ga[i], xa[i], dot));
         }
-        gn = group_sum(gn, a.lanes_log) * inv_dim;
+        const float gn = -(group_sum(dot.x + dot.y, a.lanes_log) * inv_dim);
 #pragma unroll
-        for (int s = 0; s < NS; s++)
-#pragma unroll
-          for (int k = 0; k < 2; k++)
-#pragma unroll
-            for (int j = 0; j < VEC; j++) v[s][k][j] = __fmaf_rn(-v[s][k][j], gn, d[s][k][j]) * inv * scale;
+        for (int i = 0; i < P; i++) {
+          ya[i] = __fmul2_rn(__ffma2_rn(xa[i], both(gn), ga[i]), both(inv));
+          yb[i] = __fmul2_rn(__ffma2_rn(xb[i], both(gn), gb[i]), both(inv));
+          if (sizeof(T) == 4) {
+            ya[i] = __fmul2_rn(ya[i], both(scale));
+            yb[i] = __fmul2_rn(yb[i], both(scale));
+          }
+        }
       }
-#pragma unroll
-      for (int s = 0; s < NS; s++)
-#pragma unroll
-        for (int k = 0; k < 2; k++)
-#pragma unroll
-          for (int j = 0; j < VEC; j++) of_f32(out.v[s][k][j], v[s][k][j]);
-      if (there) store_part(y + hh * a.yh, at, out);
+      Part<T, VEC, NS> out;
+      unpairs<T, VEC, NS, INTER>(ya, yb, out);
+      if (there) store_part(y, at, out);
+      x += x_step;
+      y += y_step;
+      if (BACK) g += g_step;
     }
   }
-  if (BACK && a.partials) {
-    // The block's sums: groups one after the other, each adding to the block's row.
+  if constexpr (BACK) {
+    if (!a.partials) return;
+    // The block's sums, of one weight and then of the other: a warp's groups, then the
+    // warps one after the other.
+    const int L = 1 << a.lanes_log, warp = threadIdx.x / 32, wl = threadIdx.x % 32;
+    // (the first round stores the queries')
+    if (has == 1) swap();
+    float *const rows = cs;
     __syncthreads();
-    const int L = 1 << a.lanes_log;
-#pragma unroll
-    for (int s = 0; s < NS; s++)
-#pragma unroll
-      for (int k = 0; k < 2; k++)
-#pragma unroll
-        for (int j = 0; j < VEC; j++)
-          for (int i = L; i < 32; i *= 2) dw[s][k][j] += __shfl_xor_sync(~0u, dw[s][k][j], i);
-    const int warp = threadIdx.x / 32, wl = threadIdx.x % 32;
-    if (wl < L) {
+    for (int k0 = 0; k0 < 2; k0++) {
+      Part<float, VEC, NS> d;
+      unpairs<float, VEC, NS, INTER>(dwa, dwb, d);
 #pragma unroll
       for (int s = 0; s < NS; s++)
 #pragma unroll
         for (int k = 0; k < 2; k++) {
           const int o = k ? at.o2[s] : at.o[s];
-          if (o >= 0)
 #pragma unroll
-            for (int j = 0; j < VEC; j++) sh[warp * a.dim + o + j] = dw[s][k][j];
+          for (int j = 0; j < VEC; j++) {
+            float v = d.v[s][k][j];
+            for (int i = L; i < 32; i *= 2) v += __shfl_xor_sync(~0u, v, i);
+            if (wl < L && o >= 0) rows[warp * a.dim + o + j] = v;
+          }
         }
-    }
-    __syncthreads();
-    float *const to = a.partials + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * a.dim;
-    for (int i = threadIdx.x; i < a.dim; i += kThreads) {
-      float sum = 0.0f;
-      for (int k = 0; k < kThreads / 32; k++) sum += sh[k * a.dim + i];
-      to[i] = sum;
+      __syncthreads();
+      float *const to = a.partials + (((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + k0) * a.dim;
+      for (int i = threadIdx.x; i < a.dim; i += kThreads) {
+        double sum = 0.0;
+        for (int k = 0; k < kThreads / 32; k++) sum += rows[k * a.dim + i];
+        to[i] = (float)sum;
+      }
+      __syncthreads();
+      swap();
     }
   }
 }
 
 // The blocks' sums of a weight's gradient, added in one order: blockIdx.y 0 the
-// queries' rows [0, rows_q), 1 the keys' behind them. 32 dimensions a block.
-__global__ void __launch_bounds__(1024) k_norm_rope_dw(const float *partials, int rows_q, int rows_k, int dim, float *dq, float *dk) {
-  __shared__ float sums[32][33];
+// queries', 1 the keys'. 32 dimensions a block.
+__global__ void __launch_bounds__(1024) k_norm_rope_dw(const float *partials, int blocks, int dim, float *dq, float *dk) {
+  __shared__ double sums[32][33];
   const int c = threadIdx.x % 32, r = threadIdx.x / 32, i = blockIdx.x * 32 + c;
-  const float *const from = partials + (blockIdx.y ? (int64_t)rows_q * dim : 0);
   float *const to = blockIdx.y ? dk : dq;
-  const int rows = blockIdx.y ? rows_k : rows_q;
   if (!to) return;
-  float sum = 0.0f;
+  double sum = 0.0;
   if (i < dim)
-    for (int k = r; k < rows; k += 32) sum += from[(int64_t)k * dim + i];
+    for (int k = r; k < blocks; k += 32) sum += partials[((int64_t)k * 2 + blockIdx.y) * dim + i];
   sums[r][c] = sum;
   __syncthreads();
   if (r == 0 && i < dim) {
-    sum = 0.0f;
+    sum = 0.0;
     for (int k = 0; k < 32; k++) sum += sums[k][c];
-    to[i] = sum;
+    to[i] = (float)sum;
   }
 }
 
@@ -362,12 +434,12 @@ int launch(const NormArgs &a, bool inter, bool back, dim3 grid, size_t smem, cud
 }
 
 // Blocks of the backward pass: their sums go to the workspace.
-constexpr int kBackBlocksPerSm = 4;
+constexpr int kBackBlocksPerSm = 3;
 int back_blocks(int sms) { return sms * kBackBlocksPerSm; }
 
 }  // namespace
 
-size_t norm_rope_work_bytes(int sms) { return (size_t)(back_blocks(sms) + 2) * 512 * sizeof(float); }
+size_t norm_rope_work_bytes(int sms) { return (size_t)back_blocks(sms) * 2 * 512 * sizeof(float); }
 
 int launch_norm_rope(const NormRopeCall &c, int sms, cudaStream_t st) {
   const bool back = c.dy != nullptr;
@@ -419,35 +491,25 @@ int launch_norm_rope(const NormRopeCall &c, int sms, cudaStream_t st) {
   a.partials = sums ? (float *)c.work : nullptr;
   a.lanes_log = 0;
   while (a.lanes_log < 5 && (1 << a.lanes_log) < units) a.lanes_log++;
-  // A block's tokens: a group a token where that leaves every SM blocks; then its
-  // heads are shared among blocks while there are fewer than two a SM.
-  const int groups = kThreads >> a.lanes_log, hq = c.q_heads, hk = c.heads - c.q_heads;
+  // A block's tokens, as long as every SM gets blocks; then its heads are shared among
+  // blocks while there are fewer than two a SM.
+  const int groups = kThreads >> a.lanes_log;
   a.nt_log = 0;
   while ((2 << a.nt_log) <= groups && a.nt_log < 3 && (c.tokens >> (a.nt_log + 1)) >= 4 * sms) a.nt_log++;
   const int64_t tiles = (c.tokens + (1 << a.nt_log) - 1) >> a.nt_log;
   const int step = std::max(1, groups >> a.nt_log);
-  dim3 grid((unsigned)tiles, 1);
-  int parts = 1, parts_k = 0;
-  a.hb = a.hb_q = a.hb_k = 1;
-  a.parts_q = 0;
-  if (!back) {
-    while (tiles * parts < 2 * sms && parts < (c.heads + step - 1) / step) parts++;
-    a.hb = (c.heads + parts - 1) / parts;
-    grid.y = (c.heads + a.hb - 1) / a.hb;
-  } else {
-    // Parts of about the same number of heads, of one weight each, and more of
-    // them while there are fewer blocks than the SMs take.
-    int hb = hq && hk ? std::min(hq, hk) : c.heads;
-    while (hb > step && tiles * ((hq + hb - 1) / hb + (hk + hb - 1) / hb) < back_blocks(sms)) hb = std::max(step, hb / 2);
-    while ((hq + hb - 1) / hb + (hk + hb - 1) / hb > back_blocks(sms)) hb *= 2;
-    a.hb_q = a.hb_k = hb;
-    a.parts_q = (hq + hb - 1) / hb;
-    parts_k = (hk + hb - 1) / hb;
-    grid.y = a.parts_q + parts_k;
-    grid.x = (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, back_blocks(sms) / grid.y));
-  }
+  int parts = 1;
+  while (tiles * parts < 2 * sms && parts < (c.heads + step - 1) / step) parts++;
+  a.hb = (c.heads + parts - 1) / parts;
+  dim3 grid((unsigned)tiles, (unsigned)((c.heads + a.hb - 1) / a.hb));
+  // The backward pass has as many blocks as run at once (of float16, two an SM), each
+  // with a row of sums.
+  if (back) grid.x = (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, (c.dtype == kF16 ? 2 * sms : back_blocks(sms)) / grid.y));
   size_t smem = (size_t)(1 << a.nt_log) * half * 2 * sizeof(float);
-  if (back) smem = std::max(smem, (size_t)(kThreads / 32) * c.dim * sizeof(float));
+  if (back) smem = std::max(smem, (size_t)(kThreads / 32) * c.dim * sizeof(float)) + (size_t)slots * vec * kThreads * sizeof(float2);
+  a.w_wide = true;
+  for (const void *w : {c.q_weight, c.k_weight})
+    if ((uintptr_t)w % (vec * wsize > 16 ? 16 : vec * wsize)) a.w_wide = false;
   const bool inter = (c.flags & 1) != 0;
   if (c.dtype == kF16) {
     switch (vec) {
@@ -467,7 +529,7 @@ int launch_norm_rope(const NormRopeCall &c, int sms, cudaStream_t st) {
     }
   }
   if (!sums) return 0;
-  k_norm_rope_dw<<<dim3((c.dim + 31) / 32, 2), 1024, 0, st>>>(a.partials, a.parts_q * (int)grid.x, parts_k * (int)grid.x, c.dim, c.dq_weight, c.dk_weight);
+  k_norm_rope_dw<<<dim3((c.dim + 31) / 32, 2), 1024, 0, st>>>(a.partials, (int)(grid.x * grid.y), c.dim, c.dq_weight, c.dk_weight);
   return launch_check("norm_rope_grad");
 }
 

@@ -395,6 +395,25 @@ def test_beam_select_ties(kind):
 
 
 @pytest.mark.parametrize("kind", ["f16", "f32"])
+def test_beam_select_long_rows(kind):
+    """Rows that a block goes over in several turns: rising ones (each turn's candidates are more than there is room
+    for), ones whose beginning is masked or far below what follows, falling ones, flat ones."""
+    rng = np.random.default_rng(9)
+    seqs, beams, v = 64, 8, 41003
+    z = rng.standard_normal((seqs * beams, v)).astype(NP[kind])
+    z[:64] = np.sort(z[:64], axis=1)
+    z[64:128, :30000] = -np.inf
+    z[128:192, :9000] -= 200
+    z[192:200] = z[192:200, ::-1]
+    z[200:208, :] = 1
+    z[208:216, 20000:] += 90
+    z[216:224, ::2] = -np.inf
+    scores = -rng.random((seqs, beams)).astype(np.float32)
+    for keep in (8, 64):
+        same(select(z, scores, keep, kind), O8.beam(z, scores, keep))
+
+
+@pytest.mark.parametrize("kind", ["f16", "f32"])
 def test_beam_select_strides(kind):
     """Rows at any distance and offset: vectors of 16 bytes begin inside of them."""
     rng = np.random.default_rng(4)
