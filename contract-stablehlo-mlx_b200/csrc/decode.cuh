@@ -68,8 +68,9 @@ struct Mm8Call {
 // `fill`: zeros behind a row's last value up to a multiple of 16.
 int launch_quantise_rows(const void *x, int64_t x_row, uint8_t dtype, int64_t rows, int32_t n, int8_t *q, int64_t q_row, float *scale,
                          bool fill, const char *what, cudaStream_t st);
-int launch_mul_mat8(const Mm8Call &c, int sms, cudaStream_t st);
-int launch_mul_mat8_tiles(const Mm8Call &c, int sms, cudaStream_t st);  // (arguments checked)
+// `after_rows`: the launch before it on the stream is the one that rounds its x.
+int launch_mul_mat8(const Mm8Call &c, bool after_rows, int sms, cudaStream_t st);
+int launch_mul_mat8_tiles(const Mm8Call &c, bool after_rows, int sms, cudaStream_t st);  // (arguments checked)
 size_t linear8_work_bytes(int64_t rows, int32_t n);
 int launch_linear8(const Mm8Call &c, const void *x, int64_t x_row, uint8_t x_dtype, void *work, size_t work_bytes, int sms, cudaStream_t st);
 

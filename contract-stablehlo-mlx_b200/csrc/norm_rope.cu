@@ -7,10 +7,16 @@
 //   dz = turn(dy, -position),  dw = sum of dz n over tokens and heads,
 //   g = dz w,   dx = (g - n mean(g n)) / sqrt(mean(x^2) + eps).
 //
-// Bound: bytes (each value read once and written once). A group of 1 to 32 lanes
-// holds a head in registers; it keeps one token and goes over heads, so that its
-// pairs' cosines and sines, and the weight, stay in registers too. A group's next
-// head is asked for before the one in hand is worked on.
+// Bound: bytes (each value read once and written once), and close behind them the
+// instructions. A group of 1 to 32 lanes holds a head in registers; it keeps one token
+// and goes over heads, so that its pairs' cosines and sines, and the weight, stay in
+// registers too (forward: their products); heads to come are asked for ahead, four of
+// them forward and one backward. Two pairs go through each packed instruction.
+// Measured on one B200: 16384 tokens x 40 heads x 128, float16 (336 MB) 62 us, 5.4 TB/s
+// (rope.cu alone 55); the gradient of 24001 x 12 x 80 float32, 32 dimensions turned in
+// interleaved pairs (277 MB) 80 us, 3.5 TB/s: 330 instructions a group's head, and
+// lanes without values (10 units of 4 on 16 lanes). Measured and left there: four
+// blocks an SM (125 us, registers to memory) and two (91 us), no head ahead (88 us).
 #include <algorithm>
 #include <cmath>
 
@@ -21,6 +27,7 @@ namespace shlo {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kBackBlocksPerSm = 3;  // float32's backward pass (float16's needs the registers of two)
 
 struct NormArgs {
   const void *x, *dy;
@@ -148,11 +155,11 @@ __device__ __forceinline__ void unpairs(const float2 (&a)[NS * VEC / 2], const f
 // BACK: the gradient. A block goes over tiles of 2^nt_log tokens, one in the
 // forward pass, for the heads of its part.
 template <typename T, int VEC, int NS, bool INTER, bool BACK>
-__global__ void __launch_bounds__(kThreads, NS * VEC > 8 || (BACK && sizeof(T) == 2) ? 2 : 3) k_norm_rope(const NormArgs a) {
+__global__ void __launch_bounds__(kThreads, BACK && sizeof(T) == 4 ? kBackBlocksPerSm : 2) k_norm_rope(const NormArgs a) {
   // Backward: 2 P pairs a thread; then the cosines and sines, [token][half] each, and at
   // the end the block's sums, [warp][dim], in their place.
   extern __shared__ float2 sh[];
-  constexpr int P = NS * VEC / 2;
+  constexpr int P = NS * VEC / 2, AHEAD = BACK ? 1 : 4;  // heads asked for beside the one in hand
   const int half = a.rot / 2, nt = 1 << a.nt_log;
   float *const cs = reinterpret_cast<float *>(sh + (BACK ? 2 * P * kThreads : 0)), *const sn = cs + nt * half;
   const int lane = threadIdx.x & ((1 << a.lanes_log) - 1), group = threadIdx.x >> a.lanes_log;
@@ -198,19 +205,26 @@ __global__ void __launch_bounds__(kThreads, NS * VEC > 8 || (BACK && sizeof(T) =
     pairs<float, VEC, NS, INTER>(w, wa, wb);
   };
   const int t = group & (nt - 1), h_first = h0 + (group >> a.nt_log), h_step = max(groups >> a.nt_log, 1);
-  // Of a token's pairs (shared memory's, and none where a slot is not turned): the cosines and sines.
+  // Of a token's pairs the cosines and sines from shared memory, none where a slot is
+  // not turned.
   auto turn = [&](float2 (&c)[P], float2 (&s)[P]) {
+    constexpr int V = VEC < 4 ? VEC : 4;
+    using R = typename Raw<V * sizeof(float)>::T;
+    float cc[2 * P], ss[2 * P];
+#pragma unroll
+    for (int i = 0; i < 2 * P; i += V) {
+      const int slot = i / VEC, p = t * half + (lane + (slot << a.lanes_log)) * VEC + i % VEC;
+#pragma unroll
+      for (int j = 0; j < V; j++) cc[i + j] = 1.0f, ss[i + j] = 0.0f;
+      if (at.pair[slot]) {
+        *reinterpret_cast<R *>(cc + i) = *reinterpret_cast<const R *>(cs + p);
+        *reinterpret_cast<R *>(ss + i) = *reinterpret_cast<const R *>(sn + p);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < P; i++) {
-      float cc[2], ss[2];
-#pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const int p = 2 * i + j, slot = p / VEC, unit = lane + (slot << a.lanes_log);
-        cc[j] = at.pair[slot] ? cs[t * half + unit * VEC + p % VEC] : 1.0f;
-        ss[j] = at.pair[slot] ? sn[t * half + unit * VEC + p % VEC] : 0.0f;
-      }
-      c[i] = make_float2(cc[0], cc[1]);
-      s[i] = make_float2(ss[0], ss[1]);
+      c[i] = make_float2(cc[2 * i], cc[2 * i + 1]);
+      s[i] = make_float2(ss[2 * i], ss[2 * i + 1]);
     }
   };
   // Backward: a weight, and the sums of its gradient; the other weight's sums lie in
@@ -247,12 +261,15 @@ __global__ void __launch_bounds__(kThreads, NS * VEC > 8 || (BACK && sizeof(T) =
     T *y = static_cast<T *>(a.y) + (t0 + t) * a.yt + h_first * a.yh;
     const int64_t x_step = h_step * a.xh, g_step = h_step * a.gh, y_step = h_step * a.yh;
     // (the loads need nothing of the angles: they go out first)
-    Part<T, VEC, NS> next, next_g;
-    clear_part(next);
-    if (BACK) clear_part(next_g);
-    if (mine && h_first < h1) {
-      load_part(x, at, next);
-      if (BACK) load_part(g, at, next_g);
+    Part<T, VEC, NS> next[AHEAD], next_g[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) {
+      clear_part(next[i]);
+      if (BACK) clear_part(next_g[i]);
+      if (mine && h_first + i * h_step < h1) {
+        load_part(x + i * x_step, at, next[i]);
+        if (BACK) load_part(g + i * g_step, at, next_g[i]);
+      }
     }
     if (BACK && tile != (int64_t)blockIdx.x) __syncthreads();
     for (int i = threadIdx.x; i < nt * half; i += kThreads) {
@@ -267,102 +284,111 @@ __global__ void __launch_bounds__(kThreads, NS * VEC > 8 || (BACK && sizeof(T) =
     }
     __syncthreads();
     // Forward: what a pair's two results take of its two values, weight and turn in
-    // one: (a, b) -> (a ca - b sb, b cb + a sa). Backward: the turn.
-    float2 ca[P], sa[P], cb[BACK ? 1 : P], sb[BACK ? 1 : P];
-    if constexpr (BACK) turn(ca, sa);
-    else has = -1;
+    // one: (a, b) -> (a ca + b sb, b cb + a sa). Backward: the turn, its sine negated too.
+    float2 ca[P], sa[P], cb[BACK ? 1 : P], sb[P];
+    if constexpr (BACK) {
+      turn(ca, sa);
+#pragma unroll
+      for (int i = 0; i < P; i++) sb[i] = neg(sa[i]);
+    } else {
+      has = -1;
+    }
     // (a warp's groups take the same number of turns: its shuffles name all lanes)
-    for (int h = h0; h < h1; h += h_step) {
-      const int hh = h + (group >> a.nt_log);
-      const bool there = mine && hh < h1;
-      if (has != (int)(hh >= a.q_heads)) {
-        if (BACK && has >= 0) swap();
-        has = hh >= a.q_heads;
-        if constexpr (BACK) {
-          weight(has, wa, wb);
+    for (int h = h0; h < h1; h += AHEAD * h_step) {
+#pragma unroll
+      for (int ahead = 0; ahead < AHEAD; ahead++) {
+        if (AHEAD > 1 && h + ahead * h_step >= h1) break;
+        const int hh = h + ahead * h_step + (group >> a.nt_log);
+        const bool there = mine && hh < h1;
+        if (has != (int)(hh >= a.q_heads)) {
+          if (BACK && has >= 0) swap();
+          has = hh >= a.q_heads;
+          if constexpr (BACK) {
+            weight(has, wa, wb);
+          } else {
+            float2 c[P], s[P], u[P], v[P];
+            turn(c, s);
+            weight(has, u, v);
+#pragma unroll
+            for (int i = 0; i < P; i++) {
+              ca[i] = __fmul2_rn(u[i], c[i]);
+              sa[i] = __fmul2_rn(u[i], s[i]);
+              cb[i] = __fmul2_rn(v[i], c[i]);
+              sb[i] = __fmul2_rn(v[i], neg(s[i]));
+            }
+          }
+        }
+        float2 xa[P], xb[P], sum = both(0.0f);
+        pairs<T, VEC, NS, INTER>(next[ahead], xa, xb);
+        Part<T, VEC, NS> in_g;
+        if (BACK) in_g = next_g[ahead];
+        if (mine && hh + AHEAD * h_step < h1) {
+          load_part(x + AHEAD * x_step, at, next[ahead]);
+          if (BACK) load_part(g + AHEAD * g_step, at, next_g[ahead]);
+        }
+#pragma unroll
+        for (int i = 0; i < P; i++) sum = __ffma2_rn(xb[i], xb[i], __ffma2_rn(xa[i], xa[i], sum));
+        float ss = group_sum(sum.x + sum.y, a.lanes_log), scale = 1.0f, eps = a.eps;
+        if (sizeof(T) == 4) {
+          scale = safe_scale(ss, eps);
+          if (__any_sync(~0u, scale != 1.0f)) {
+            eps = eps * scale * scale;  // (scale^2 itself has no place in 32 bits)
+            sum = both(0.0f);
+#pragma unroll
+            for (int i = 0; i < P; i++) {
+              xa[i] = __fmul2_rn(xa[i], both(scale));
+              xb[i] = __fmul2_rn(xb[i], both(scale));
+              sum = __ffma2_rn(xb[i], xb[i], __ffma2_rn(xa[i], xa[i], sum));
+            }
+            ss = group_sum(sum.x + sum.y, a.lanes_log);
+          }
+        }
+        // (2^-22 is enough where the result has 11 bits)
+        const float inv = sizeof(T) == 2 ? rsqrtf(__fmaf_rn(ss, inv_dim, eps)) : __frsqrt_rn(__fmaf_rn(ss, inv_dim, eps));
+        float2 ya[P], yb[P];
+        if constexpr (!BACK) {
+#pragma unroll
+          for (int i = 0; i < P; i++) {
+            const float2 p = __fmul2_rn(xa[i], both(inv)), q = __fmul2_rn(xb[i], both(inv));
+            ya[i] = __ffma2_rn(q, sb[i], __fmul2_rn(p, ca[i]));
+            yb[i] = __ffma2_rn(q, cb[i], __fmul2_rn(p, sa[i]));
+          }
         } else {
-          float2 c[P], s[P], u[P], v[P];
-          turn(c, s);
-          weight(has, u, v);
+          float2 ga[P], gb[P], dot = both(0.0f);
+          pairs<T, VEC, NS, INTER>(in_g, ga, gb);
 #pragma unroll
           for (int i = 0; i < P; i++) {
-            ca[i] = __fmul2_rn(u[i], c[i]);
-            sa[i] = __fmul2_rn(u[i], s[i]);
-            cb[i] = __fmul2_rn(v[i], c[i]);
-            sb[i] = __fmul2_rn(v[i], s[i]);
+            xa[i] = __fmul2_rn(xa[i], both(inv));
+            xb[i] = __fmul2_rn(xb[i], both(inv));
+            // turned back
+            const float2 p = __ffma2_rn(ga[i], ca[i], __fmul2_rn(gb[i], sa[i]));
+            const float2 q = __ffma2_rn(ga[i], sb[i], __fmul2_rn(gb[i], ca[i]));
+            if (there) {
+              dwa[i] = __ffma2_rn(p, xa[i], dwa[i]);
+              dwb[i] = __ffma2_rn(q, xb[i], dwb[i]);
+            }
+            ga[i] = __fmul2_rn(p, wa[i]);
+            gb[i] = __fmul2_rn(q, wb[i]);
+            dot = __ffma2_rn(gb[i], xb[i], __ffma2_rn(ga[i], xa[i], dot));
           }
-        }
-      }
-      float2 xa[P], xb[P], sum = both(0.0f);
-      pairs<T, VEC, NS, INTER>(next, xa, xb);
-      Part<T, VEC, NS> in_g;
-      if (BACK) in_g = next_g;
-      if (mine && hh + h_step < h1) {
-        load_part(x + x_step, at, next);
-        if (BACK) load_part(g + g_step, at, next_g);
-      }
-#pragma unroll
-      for (int i = 0; i < P; i++) sum = __ffma2_rn(xb[i], xb[i], __ffma2_rn(xa[i], xa[i], sum));
-      float ss = group_sum(sum.x + sum.y, a.lanes_log), scale = 1.0f, eps = a.eps;
-      if (sizeof(T) == 4) {
-        scale = safe_scale(ss, eps);
-        if (__any_sync(~0u, scale != 1.0f)) {
-          eps = eps * scale * scale;  // (scale^2 itself has no place in 32 bits)
-          sum = both(0.0f);
+          const float gn = -(group_sum(dot.x + dot.y, a.lanes_log) * inv_dim);
 #pragma unroll
           for (int i = 0; i < P; i++) {
-            xa[i] = __fmul2_rn(xa[i], both(scale));
-            xb[i] = __fmul2_rn(xb[i], both(scale));
-            sum = __ffma2_rn(xb[i], xb[i], __ffma2_rn(xa[i], xa[i], sum));
+            ya[i] = __fmul2_rn(__ffma2_rn(xa[i], both(gn), ga[i]), both(inv));
+            yb[i] = __fmul2_rn(__ffma2_rn(xb[i], both(gn), gb[i]), both(inv));
+            if (sizeof(T) == 4) {
+              ya[i] = __fmul2_rn(ya[i], both(scale));
+              yb[i] = __fmul2_rn(yb[i], both(scale));
+            }
           }
-          ss = group_sum(sum.x + sum.y, a.lanes_log);
         }
+        Part<T, VEC, NS> out;
+        unpairs<T, VEC, NS, INTER>(ya, yb, out);
+        if (there) store_part(y, at, out);
+        x += x_step;
+        y += y_step;
+        if (BACK) g += g_step;
       }
-      // (2^-22 is enough where the result has 11 bits)
-      const float inv = sizeof(T) == 2 ? rsqrtf(__fmaf_rn(ss, inv_dim, eps)) : __frsqrt_rn(__fmaf_rn(ss, inv_dim, eps));
-      float2 ya[P], yb[P];
-      if constexpr (!BACK) {
-#pragma unroll
-        for (int i = 0; i < P; i++) {
-          const float2 p = __fmul2_rn(xa[i], both(inv)), q = __fmul2_rn(xb[i], both(inv));
-          ya[i] = __ffma2_rn(p, ca[i], neg(__fmul2_rn(q, sb[i])));
-          yb[i] = __ffma2_rn(q, cb[i], __fmul2_rn(p, sa[i]));
-        }
-      } else {
-        float2 ga[P], gb[P], dot = both(0.0f);
-        pairs<T, VEC, NS, INTER>(in_g, ga, gb);
-#pragma unroll
-        for (int i = 0; i < P; i++) {
-          xa[i] = __fmul2_rn(xa[i], both(inv));
-          xb[i] = __fmul2_rn(xb[i], both(inv));
-          // turned back
-          const float2 p = __ffma2_rn(ga[i], ca[i], __fmul2_rn(gb[i], sa[i]));
-          const float2 q = __ffma2_rn(gb[i], ca[i], neg(__fmul2_rn(ga[i], sa[i])));
-          if (there) {
-            dwa[i] = __ffma2_rn(p, xa[i], dwa[i]);
-            dwb[i] = __ffma2_rn(q, xb[i], dwb[i]);
-          }
-          ga[i] = __fmul2_rn(p, wa[i]);
-          gb[i] = __fmul2_rn(q, wb[i]);
-          dot = __ffma2_rn(gb[i], xb[i], __ffma2_rn(ga[i], xa[i], dot));
-        }
-        const float gn = -(group_sum(dot.x + dot.y, a.lanes_log) * inv_dim);
-#pragma unroll
-        for (int i = 0; i < P; i++) {
-          ya[i] = __fmul2_rn(__ffma2_rn(xa[i], both(gn), ga[i]), both(inv));
-          yb[i] = __fmul2_rn(__ffma2_rn(xb[i], both(gn), gb[i]), both(inv));
-          if (sizeof(T) == 4) {
-            ya[i] = __fmul2_rn(ya[i], both(scale));
-            yb[i] = __fmul2_rn(yb[i], both(scale));
-          }
-        }
-      }
-      Part<T, VEC, NS> out;
-      unpairs<T, VEC, NS, INTER>(ya, yb, out);
-      if (there) store_part(y, at, out);
-      x += x_step;
-      y += y_step;
-      if (BACK) g += g_step;
     }
   }
   if constexpr (BACK) {
@@ -434,7 +460,6 @@ int launch(const NormArgs &a, bool inter, bool back, dim3 grid, size_t smem, cud
 }
 
 // Blocks of the backward pass: their sums go to the workspace.
-constexpr int kBackBlocksPerSm = 3;
 int back_blocks(int sms) { return sms * kBackBlocksPerSm; }
 
 }  // namespace
