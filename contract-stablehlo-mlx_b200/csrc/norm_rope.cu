@@ -43,7 +43,7 @@ struct NormArgs {
   int hb;         // heads a block
   float eps, factor;
   bool w_half, w_wide;  // the weights' type, and whether they allow wide loads
-  float *partials;      // backward: [blocks][2][dim], nullptr without the weights' gradients
+  double *partials;     // backward: [blocks][2][dim], nullptr without the weights' gradients
 };
 
 template <int BYTES> struct Raw;
@@ -156,12 +156,12 @@ __device__ __forceinline__ void unpairs(const float2 (&a)[NS * VEC / 2], const f
 // forward pass, for the heads of its part.
 template <typename T, int VEC, int NS, bool INTER, bool BACK>
 __global__ void __launch_bounds__(kThreads, BACK && sizeof(T) == 4 ? kBackBlocksPerSm : 2) k_norm_rope(const NormArgs a) {
-  // Backward: 2 P pairs a thread; then the cosines and sines, [token][half] each, and at
+  // Backward: 8 P sums a thread; then the cosines and sines, [token][half] each, and at
   // the end the block's sums, [warp][dim], in their place.
-  extern __shared__ float2 sh[];
+  extern __shared__ double sh[];
   constexpr int P = NS * VEC / 2, AHEAD = BACK ? 1 : 4;  // heads asked for beside the one in hand
   const int half = a.rot / 2, nt = 1 << a.nt_log;
-  float *const cs = reinterpret_cast<float *>(sh + (BACK ? 2 * P * kThreads : 0)), *const sn = cs + nt * half;
+  float *const cs = reinterpret_cast<float *>(sh + (BACK ? 8 * P * kThreads : 0)), *const sn = cs + nt * half;
   const int lane = threadIdx.x & ((1 << a.lanes_log) - 1), group = threadIdx.x >> a.lanes_log;
   const int groups = kThreads >> a.lanes_log;
   const int h0 = blockIdx.y * a.hb, h1 = min(h0 + a.hb, a.heads);
@@ -227,27 +227,27 @@ __global__ void __launch_bounds__(kThreads, BACK && sizeof(T) == 4 ? kBackBlocks
       s[i] = make_float2(ss[2 * i], ss[2 * i + 1]);
     }
   };
-  // Backward: a weight, and the sums of its gradient; the other weight's sums lie in
-  // shared memory meanwhile.
+  // Backward: a weight, and the sums of its gradient over a few heads; then they go to
+  // the thread's sums in 64 bits, [weight][4 P], in shared memory.
   float2 dwa[BACK ? P : 1], dwb[BACK ? P : 1], wa[BACK ? P : 1], wb[BACK ? P : 1];
-  float2 *const other = sh + threadIdx.x;
+  double *const sums = reinterpret_cast<double *>(sh) + threadIdx.x;
   int has = -1;  // whose weight is in registers: 0 the queries', 1 the keys'
   if constexpr (BACK) {
 #pragma unroll
-    for (int i = 0; i < P; i++) {
-      dwa[i] = dwb[i] = both(0.0f);
-      other[2 * i * kThreads] = other[(2 * i + 1) * kThreads] = both(0.0f);
-    }
+    for (int i = 0; i < P; i++) dwa[i] = dwb[i] = both(0.0f);
+#pragma unroll
+    for (int i = 0; i < 8 * P; i++) sums[i * kThreads] = 0.0;
   }
-  auto swap = [&]() {
+  auto flush = [&]() {
     if constexpr (BACK) {
+      double *const to = sums + has * 4 * P * kThreads;
 #pragma unroll
       for (int i = 0; i < P; i++) {
-        const float2 p = other[2 * i * kThreads], q = other[(2 * i + 1) * kThreads];
-        other[2 * i * kThreads] = dwa[i];
-        other[(2 * i + 1) * kThreads] = dwb[i];
-        dwa[i] = p;
-        dwb[i] = q;
+        to[(4 * i) * kThreads] += (double)dwa[i].x;
+        to[(4 * i + 1) * kThreads] += (double)dwa[i].y;
+        to[(4 * i + 2) * kThreads] += (double)dwb[i].x;
+        to[(4 * i + 3) * kThreads] += (double)dwb[i].y;
+        dwa[i] = dwb[i] = both(0.0f);
       }
     }
   };
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, BACK && sizeof(T) == 4 ? kBackBlocks
         const int hh = h + ahead * h_step + (group >> a.nt_log);
         const bool there = mine && hh < h1;
         if (has != (int)(hh >= a.q_heads)) {
-          if (BACK && has >= 0) swap();
+          if (BACK && has >= 0) flush();
           has = hh >= a.q_heads;
           if constexpr (BACK) {
             weight(has, wa, wb);
@@ -396,41 +396,35 @@ __global__ void __launch_bounds__(kThreads, BACK && sizeof(T) == 4 ? kBackBlocks
     // The block's sums, of one weight and then of the other: a warp's groups, then the
     // warps one after the other.
     const int L = 1 << a.lanes_log, warp = threadIdx.x / 32, wl = threadIdx.x % 32;
-    // (the first round stores the queries')
-    if (has == 1) swap();
-    float *const rows = cs;
-    __syncthreads();
+    if (has >= 0) flush();
+    double *const rows = reinterpret_cast<double *>(cs);
     for (int k0 = 0; k0 < 2; k0++) {
-      Part<float, VEC, NS> d;
-      unpairs<float, VEC, NS, INTER>(dwa, dwb, d);
+      __syncthreads();
 #pragma unroll
-      for (int s = 0; s < NS; s++)
+      for (int p = 0; p < 2 * P; p++)
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
+        for (int q = 0; q < 2; q++) {  // pair p's first and second value
+          constexpr int V = VEC;
+          const int s = p / V, j = p % V, k = INTER ? (2 * j + q) / V : q, at_j = INTER ? (2 * j + q) % V : j;
           const int o = k ? at.o2[s] : at.o[s];
-#pragma unroll
-          for (int j = 0; j < VEC; j++) {
-            float v = d.v[s][k][j];
-            for (int i = L; i < 32; i *= 2) v += __shfl_xor_sync(~0u, v, i);
-            if (wl < L && o >= 0) rows[warp * a.dim + o + j] = v;
-          }
+          double v = sums[(k0 * 4 * P + p / 2 * 4 + 2 * q + p % 2) * kThreads];
+          for (int i = L; i < 32; i *= 2) v += __shfl_xor_sync(~0u, v, i);
+          if (wl < L && o >= 0) rows[warp * a.dim + o + at_j] = v;
         }
       __syncthreads();
-      float *const to = a.partials + (((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + k0) * a.dim;
+      double *const to = a.partials + (((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + k0) * a.dim;
       for (int i = threadIdx.x; i < a.dim; i += kThreads) {
         double sum = 0.0;
         for (int k = 0; k < kThreads / 32; k++) sum += rows[k * a.dim + i];
-        to[i] = (float)sum;
+        to[i] = sum;
       }
-      __syncthreads();
-      swap();
     }
   }
 }
 
 // The blocks' sums of a weight's gradient, added in one order: blockIdx.y 0 the
 // queries', 1 the keys'. 32 dimensions a block.
-__global__ void __launch_bounds__(1024) k_norm_rope_dw(const float *partials, int blocks, int dim, float *dq, float *dk) {
+__global__ void __launch_bounds__(1024) k_norm_rope_dw(const double *partials, int blocks, int dim, float *dq, float *dk) {
   __shared__ double sums[32][33];
   const int c = threadIdx.x % 32, r = threadIdx.x / 32, i = blockIdx.x * 32 + c;
   float *const to = blockIdx.y ? dk : dq;
@@ -449,13 +443,18 @@ __global__ void __launch_bounds__(1024) k_norm_rope_dw(const float *partials, in
 
 template <typename T, int VEC, int NS>
 int launch(const NormArgs &a, bool inter, bool back, dim3 grid, size_t smem, cudaStream_t st) {
-  if (back) {
-    if (inter) k_norm_rope<T, VEC, NS, true, true><<<grid, kThreads, smem, st>>>(a);
-    else k_norm_rope<T, VEC, NS, false, true><<<grid, kThreads, smem, st>>>(a);
-  } else {
-    if (inter) k_norm_rope<T, VEC, NS, true, false><<<grid, kThreads, smem, st>>>(a);
-    else k_norm_rope<T, VEC, NS, false, false><<<grid, kThreads, smem, st>>>(a);
+  const auto kernel = back ? inter ? k_norm_rope<T, VEC, NS, true, true> : k_norm_rope<T, VEC, NS, false, true>
+                           : inter ? k_norm_rope<T, VEC, NS, true, false> : k_norm_rope<T, VEC, NS, false, false>;
+  if (smem > 48 * 1024) {
+    static std::atomic<uint64_t> set[2]{};
+    int device;
+    SHLO_CUDA(cudaGetDevice(&device));
+    if (device >= 64 || !(set[inter].load(std::memory_order_relaxed) >> device & 1)) {
+      SHLO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 112 * 1024));
+      if (device < 64) set[inter].fetch_or(1ull << device);
+    }
   }
+  kernel<<<grid, kThreads, smem, st>>>(a);
   return launch_check(back ? "norm_rope_grad" : "norm_rope");
 }
 
@@ -464,7 +463,7 @@ int back_blocks(int sms) { return sms * kBackBlocksPerSm; }
 
 }  // namespace
 
-size_t norm_rope_work_bytes(int sms) { return (size_t)back_blocks(sms) * 2 * 512 * sizeof(float); }
+size_t norm_rope_work_bytes(int sms) { return (size_t)back_blocks(sms) * 2 * 512 * sizeof(double); }
 
 int launch_norm_rope(const NormRopeCall &c, int sms, cudaStream_t st) {
   const bool back = c.dy != nullptr;
@@ -480,7 +479,7 @@ int launch_norm_rope(const NormRopeCall &c, int sms, cudaStream_t st) {
   if (c.tokens > 0x7fffffff) return fail("%s: %lld tokens, at most 2^31 - 1", what, (long long)c.tokens);
   const size_t size = dtype_size(c.dtype), wsize = dtype_size(c.weight_dtype);
   const bool sums = back && (c.dq_weight || c.dk_weight);
-  if ((uintptr_t)c.dq_weight % 4 || (uintptr_t)c.dk_weight % 4 || (uintptr_t)c.work % 4) return fail("%s: misaligned gradient or workspace", what);
+  if ((uintptr_t)c.dq_weight % 4 || (uintptr_t)c.dk_weight % 4 || (sums && (uintptr_t)c.work % 8)) return fail("%s: misaligned gradient or workspace", what);
   if (sums && (!c.work || c.work_bytes < norm_rope_work_bytes(sms)))
     return fail("%s: a workspace of %zu bytes, %zu needed", what, c.work ? c.work_bytes : 0, norm_rope_work_bytes(sms));
   if (c.tokens == 0) {
@@ -513,7 +512,7 @@ int launch_norm_rope(const NormRopeCall &c, int sms, cudaStream_t st) {
   a.xt = c.x_token; a.xh = c.x_head; a.gt = c.dy_token; a.gh = c.dy_head; a.yt = c.y_token; a.yh = c.y_head;
   a.tokens = c.tokens; a.heads = c.heads; a.q_heads = c.q_heads; a.dim = c.dim; a.rot = c.rot;
   a.eps = c.eps; a.factor = c.factor; a.w_half = c.weight_dtype == kF16;
-  a.partials = sums ? (float *)c.work : nullptr;
+  a.partials = sums ? (double *)c.work : nullptr;
   a.lanes_log = 0;
   while (a.lanes_log < 5 && (1 << a.lanes_log) < units) a.lanes_log++;
   // A block's tokens, as long as every SM gets blocks; then its heads are shared among
@@ -531,7 +530,7 @@ int launch_norm_rope(const NormRopeCall &c, int sms, cudaStream_t st) {
   // with a row of sums.
   if (back) grid.x = (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, (c.dtype == kF16 ? 2 * sms : back_blocks(sms)) / grid.y));
   size_t smem = (size_t)(1 << a.nt_log) * half * 2 * sizeof(float);
-  if (back) smem = std::max(smem, (size_t)(kThreads / 32) * c.dim * sizeof(float)) + (size_t)slots * vec * kThreads * sizeof(float2);
+  if (back) smem = std::max(smem, (size_t)(kThreads / 32) * c.dim * sizeof(double)) + (size_t)slots * vec * 4 * kThreads * sizeof(double);
   a.w_wide = true;
   for (const void *w : {c.q_weight, c.k_weight})
     if ((uintptr_t)w % (vec * wsize > 16 ? 16 : vec * wsize)) a.w_wide = false;
