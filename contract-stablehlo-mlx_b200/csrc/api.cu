@@ -45,6 +45,8 @@ const KernelInfo kKernels[] = {
     {"shlo_attention", KK_ATTENTION, 4, 3, 5, kF32},      // q, k, v, p = [B, S, H, width, scale bits]
     // Rotary positions (float16 or float32, the result of x's type):
     {"shlo_rope", KK_ROPE, 4, 3, 6, kNumDTypes},          // x, positions, phases, p = [T, H, D, rot, flags, factor bits]
+    // x, positions, phases, the queries' and the keys' weight, p = [the six of shlo_rope, query heads, eps bits]
+    {"shlo_norm_rope", KK_NORM_ROPE, 6, 5, 8, kNumDTypes},
 };
 
 }  // namespace
@@ -284,7 +286,7 @@ int shlo_kernel_apply(shlo_kernel k, const shlo_arr *inputs, int n_inputs, const
   Device *dev;
   SHLO_TRY(arr_device(inputs[0], &dev));
   // The kernels index flat row-major buffers (c/smlx_shim.c:292-293).
-  Arr *in[5] = {nullptr, nullptr, nullptr, nullptr, nullptr};
+  Arr *in[6] = {};
   int rc = 0;
   for (int i = 0; i < n_inputs && !rc; i++) {
     if (i == ki.param_index) continue;
@@ -326,6 +328,7 @@ int shlo_kernel_apply(shlo_kernel k, const shlo_arr *inputs, int n_inputs, const
       case KK_NORM_AFFINE: rc = k_norm_affine(dev, in[0], p, in[1], in[2], &o); break;
       case KK_ATTENTION: rc = k_attention(dev, in[0], in[1], in[2], p, &o); break;
       case KK_ROPE: rc = k_rope(dev, in[0], in[1], in[2], p, &o); break;
+      case KK_NORM_ROPE: rc = k_norm_rope(dev, in[0], in[1], in[2], in[3], in[4], p, &o); break;
     }
   }
   for (Arr *a : in)

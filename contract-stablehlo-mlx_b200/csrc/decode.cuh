@@ -48,6 +48,8 @@ struct NormRopeCall {
   size_t work_bytes;
 };
 size_t norm_rope_work_bytes(int sms);
+// A call's operands from arrays, without its result; p: the "shlo_norm_rope" kernel's words.
+int norm_rope_call(const char *what, Arr *x, Arr *positions, Arr *phases, Arr *q_weight, Arr *k_weight, const uint32_t *p, NormRopeCall *c);
 int launch_norm_rope(const NormRopeCall &c, int sms, cudaStream_t st);
 
 // Products in 8-bit integers (linear8.cu, linear8_tiles.cu): y = x w^T, scaled.

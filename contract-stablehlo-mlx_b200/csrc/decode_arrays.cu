@@ -32,6 +32,58 @@ int k_rope(Device *dev, Arr *x, Arr *positions, Arr *phases, const uint32_t *p, 
   return 0;
 }
 
+// "shlo_norm_rope": x [T][H][D], positions int32 [T], phases int64 [rot / 2], the
+// queries' and the keys' weight [D], p = [T, H, D, rot, flags, factor bits, query
+// heads, eps bits]; the result is of x's type.
+int k_norm_rope(Device *dev, Arr *x, Arr *positions, Arr *phases, Arr *q_weight, Arr *k_weight, const uint32_t *p, Arr **out) {
+  NormRopeCall c = {};
+  SHLO_TRY(norm_rope_call("shlo_norm_rope", x, positions, phases, q_weight, k_weight, p, &c));
+  const int64_t shape[3] = {p[0], p[1], p[2]};
+  Arr *o;
+  SHLO_TRY(new_array(dev, x->dtype, shape, 3, &o));
+  c.y = data_ptr(o);
+  c.y_token = c.x_token;
+  c.y_head = c.x_head;
+  if (launch_norm_rope(c, dev->sm_count, dev->stream)) {
+    shlo_release(o);
+    return 1;
+  }
+  *out = o;
+  return 0;
+}
+
+int norm_rope_call(const char *what, Arr *x, Arr *positions, Arr *phases, Arr *q_weight, Arr *k_weight, const uint32_t *p, NormRopeCall *c) {
+  const int64_t T = p[0], H = p[1], D = p[2], rot = p[3];
+  if (positions->dtype != kI32) return fail("%s: positions of %s, int32 expected", what, dtype_name(positions->dtype));
+  if (phases->dtype != kI64) return fail("%s: phases of %s, int64 expected", what, dtype_name(phases->dtype));
+  if (H < 1 || D < 1 || T > 0x7fffffff || H > 0x7fffffff || D > 512 || T * H > ((int64_t)1 << 40) / D)
+    return fail("%s: %lld tokens of %lld heads of %lld", what, (long long)T, (long long)H, (long long)D);
+  if (numel(x) != T * H * D || numel(positions) != T || numel(phases) < rot / 2)
+    return fail("%s: %lld values, %lld positions and %lld phases for [%lld, %lld, %lld] and %lld dimensions turned", what,
+                (long long)numel(x), (long long)numel(positions), (long long)numel(phases), (long long)T, (long long)H,
+                (long long)D, (long long)rot);
+  if (numel(q_weight) != D || numel(k_weight) != D || q_weight->dtype != k_weight->dtype)
+    return fail("%s: the weights are not of %lld values of one type", what, (long long)D);
+  c->x = data_ptr(x);
+  c->x_token = H * D;
+  c->x_head = D;
+  c->positions = (const int32_t *)data_ptr(positions);
+  c->phases = (const int64_t *)data_ptr(phases);
+  c->q_weight = data_ptr(q_weight);
+  c->k_weight = data_ptr(k_weight);
+  c->weight_dtype = q_weight->dtype;
+  c->q_heads = (int32_t)p[6];
+  c->eps = bitsf_host(p[7]);
+  c->tokens = T;
+  c->heads = (int32_t)H;
+  c->dim = (int32_t)D;
+  c->rot = (int32_t)rot;
+  c->dtype = x->dtype;
+  c->flags = p[4];
+  c->factor = bitsf_host(p[5]);
+  return 0;
+}
+
 namespace {
 
 // The attention's workspace, one a device: all of a device's work is on its stream.
@@ -70,6 +122,9 @@ struct shlo_kv_s {
 };
 
 namespace {
+
+// The op log's names of what is read here (those of elementwise.cu and runtime.cu are below 30).
+enum { OT_NORM_ROPE_GRAD = 30, OT_QUANTISE_ROWS, OT_LINEAR8, OT_BEAM_SELECT };
 
 // References that are dropped at the end of a call.
 struct Held {
@@ -117,6 +172,35 @@ int ints_of(shlo_kv kv, Arr *a, int ndim, const char *what, const char *name, He
   SHLO_TRY(make_contiguous(a, out));
   held.arrays.push_back(*out);
   return 0;
+}
+
+// Row-major copies where they are needed, held to one device.
+int whole(Device *dev, Arr *a, const char *what, const char *name, Held &held, Arr **out) {
+  if (!a) return fail("%s: %s is null", what, name);
+  if (numel(a) && (!a->buf || a->buf->dev != dev)) return fail("%s: %s is on another device", what, name);
+  SHLO_TRY(make_contiguous(a, out));
+  held.arrays.push_back(*out);
+  return 0;
+}
+int shaped(Arr *a, uint8_t dtype, std::initializer_list<int64_t> shape, const char *what, const char *name) {
+  bool same = a->dtype == dtype && a->ndim == (int)shape.size();
+  int i = 0;
+  for (int64_t n : shape) {
+    same = same && a->shape[i] == n;
+    i++;
+  }
+  if (!same) return fail("%s: %s is %s of rank %d, or of another shape", what, name, dtype_name(a->dtype), a->ndim);
+  return 0;
+}
+int made(Device *dev, uint8_t dtype, std::initializer_list<int64_t> shape, Held &held, Arr **out) {
+  std::vector<int64_t> n(shape);
+  SHLO_TRY(new_array(dev, dtype, n.data(), (int)n.size(), out));
+  held.arrays.push_back(*out);
+  return 0;
+}
+void give(Arr *a, shlo_arr *out) {
+  shlo_retain(a);
+  *out = a;
 }
 
 int batch_of(shlo_kv kv, Arr *starts, Arr *lens, Arr *tables, int64_t tokens, const char *what, Held &held, shlo_kv_batch *b) {
@@ -266,6 +350,180 @@ int shlo_kv_attend(shlo_kv kv, shlo_arr q, shlo_arr starts, shlo_arr lens, shlo_
     shlo_retain(l);
     *lse = l;
   }
+  return 0;
+}
+
+int shlo_kv_fork(shlo_kv kv, shlo_arr tables, shlo_arr lens, shlo_arr parents, shlo_arr fresh, shlo_arr *out_tables, shlo_arr *out_lens) {
+  SHLO_TRY(usable(kv, "kv_fork"));
+  if (!out_tables || !out_lens) return fail("kv_fork: null pointer");
+  Held held;
+  Arr *t, *l, *p, *f, *ot, *ol;
+  SHLO_TRY(ints_of(kv, tables, 2, "kv_fork", "tables", held, &t));
+  SHLO_TRY(ints_of(kv, lens, 1, "kv_fork", "lens", held, &l));
+  SHLO_TRY(ints_of(kv, parents, 1, "kv_fork", "parents", held, &p));
+  SHLO_TRY(ints_of(kv, fresh, 1, "kv_fork", "fresh", held, &f));
+  const int64_t rows = t->shape[0], width = t->shape[1], news = p->shape[0];
+  if (l->shape[0] != rows || f->shape[0] != news || rows > 0x7fffffff || news > 65536 || width > (1 << 22))
+    return fail("kv_fork: %lld lengths for tables of %lld rows of %lld pages, %lld fresh pages for %lld rows", (long long)l->shape[0],
+                (long long)rows, (long long)width, (long long)f->shape[0], (long long)news);
+  SHLO_TRY(made(kv->dev, kI32, {news, width}, held, &ot));
+  SHLO_TRY(made(kv->dev, kI32, {news}, held, &ol));
+  ForkCall c{kv->pool, (const int32_t *)data_ptr(t), (const int32_t *)data_ptr(l), width, (const int32_t *)data_ptr(p),
+             (const int32_t *)data_ptr(f), (int32_t *)data_ptr(ot), (int32_t *)data_ptr(ol), width, (int32_t)rows, (int32_t)news, (int32_t)width};
+  SHLO_TRY(launch_kv_fork(c, kv->dev->stream));
+  give(ot, out_tables);
+  give(ol, out_lens);
+  return 0;
+}
+
+int shlo_norm_rope_grad(shlo_arr x, shlo_arr dy, shlo_arr positions, shlo_arr phases, shlo_arr q_weight, shlo_arr k_weight,
+                        int32_t q_heads, float eps, uint32_t flags, float factor, shlo_arr *dx, shlo_arr *dq_weight, shlo_arr *dk_weight) {
+  const char *const what = "norm_rope_grad";
+  if (!x || !dx || !dq_weight || !dk_weight) return fail("%s: null pointer", what);
+  Arr *const ins[6] = {x, dy, positions, phases, q_weight, k_weight};
+  for (Arr *a : ins)
+    if (!a) return fail("%s: null array", what);
+  TraceScope ts(TK_OTHER, OT_NORM_ROPE_GRAD, nullptr, 0, ins, 6);
+  Device *dev;
+  SHLO_TRY(arr_device(x, &dev));
+  Held held;
+  Arr *a[6];
+  static const char *const names[6] = {"x", "dy", "positions", "phases", "q_weight", "k_weight"};
+  for (int i = 0; i < 6; i++) SHLO_TRY(whole(dev, ins[i], what, names[i], held, &a[i]));
+  if (x->ndim != 3 || phases->ndim != 1) return fail("%s: x is not [tokens, heads, dim], or phases are no vector", what);
+  SHLO_TRY(shaped(dy, x->dtype, {x->shape[0], x->shape[1], x->shape[2]}, what, "dy"));
+  if (x->shape[0] > 0x7fffffff || x->shape[1] > 0x7fffffff || x->shape[2] > 512) return fail("%s: x is too large", what);
+  uint32_t p[8] = {(uint32_t)x->shape[0], (uint32_t)x->shape[1], (uint32_t)x->shape[2], (uint32_t)(2 * phases->shape[0]), flags, 0, (uint32_t)q_heads, 0};
+  memcpy(&p[5], &factor, 4);
+  memcpy(&p[7], &eps, 4);
+  NormRopeCall c = {};
+  SHLO_TRY(norm_rope_call(what, a[0], a[2], a[3], a[4], a[5], p, &c));
+  Arr *o, *q, *k, *w;
+  SHLO_TRY(made(dev, x->dtype, {x->shape[0], x->shape[1], x->shape[2]}, held, &o));
+  SHLO_TRY(made(dev, kF32, {c.dim}, held, &q));
+  SHLO_TRY(made(dev, kF32, {c.dim}, held, &k));
+  const size_t bytes = norm_rope_work_bytes(dev->sm_count);
+  SHLO_TRY(made(dev, kU8, {(int64_t)bytes}, held, &w));
+  c.dy = c.tokens ? data_ptr(a[1]) : (const void *)"";
+  c.dy_token = c.x_token;
+  c.dy_head = c.x_head;
+  c.y = data_ptr(o);
+  c.y_token = c.x_token;
+  c.y_head = c.x_head;
+  c.dq_weight = (float *)data_ptr(q);
+  c.dk_weight = (float *)data_ptr(k);
+  c.work = data_ptr(w);
+  c.work_bytes = bytes;
+  SHLO_TRY(launch_norm_rope(c, dev->sm_count, dev->stream));
+  give(o, dx);
+  give(q, dq_weight);
+  give(k, dk_weight);
+  ts.done(nullptr);
+  return 0;
+}
+
+int shlo_quantise_rows(shlo_arr x, shlo_arr *q, shlo_arr *scale) {
+  const char *const what = "quantise_rows";
+  if (!x || !q || !scale) return fail("%s: null pointer", what);
+  TraceScope ts(TK_OTHER, OT_QUANTISE_ROWS, nullptr, 0, &x, 1);
+  Device *dev;
+  SHLO_TRY(arr_device(x, &dev));
+  Held held;
+  Arr *a, *o, *s;
+  SHLO_TRY(whole(dev, x, what, "x", held, &a));
+  if (x->ndim != 2 || x->shape[1] < 1 || x->shape[1] > 0x7fffff00) return fail("%s: x is not [rows, values]", what);
+  const int64_t rows = x->shape[0], n = x->shape[1], row = (n + 15) / 16 * 16;
+  SHLO_TRY(made(dev, kI8, {rows, row}, held, &o));
+  SHLO_TRY(made(dev, kF32, {rows}, held, &s));
+  SHLO_TRY(launch_quantise_rows(data_ptr(a), n, x->dtype, rows, (int32_t)n, (int8_t *)data_ptr(o), row, (float *)data_ptr(s), true, what, dev->stream));
+  give(o, q);
+  give(s, scale);
+  ts.done(nullptr);
+  return 0;
+}
+
+int shlo_linear8(shlo_arr x, shlo_arr x_scale, shlo_arr w, shlo_arr w_scale, shlo_arr bias, uint8_t dtype, shlo_arr *out) {
+  const char *const what = "linear8";
+  if (!x || !w || !w_scale || !out) return fail("%s: null pointer", what);
+  Arr *ins[5] = {x, w, w_scale, nullptr, nullptr};
+  int n_ins = 3;
+  if (x_scale) ins[n_ins++] = x_scale;
+  if (bias) ins[n_ins++] = bias;
+  TraceScope ts(TK_OTHER, OT_LINEAR8, nullptr, 0, ins, n_ins);
+  Device *dev;
+  SHLO_TRY(arr_device(x, &dev));
+  Held held;
+  Arr *a, *b, *s, *o, *e = nullptr;
+  SHLO_TRY(whole(dev, x, what, "x", held, &a));
+  SHLO_TRY(whole(dev, w, what, "w", held, &b));
+  SHLO_TRY(whole(dev, w_scale, what, "w_scale", held, &s));
+  if (x->ndim != 2 || w->ndim != 2 || w->dtype != kI8) return fail("%s: x is not [rows, values], or w not int8 [channels, values]", what);
+  const int64_t rows = x->shape[0], n = x->shape[1], m = w->shape[0], row = (n + 15) / 16 * 16;
+  if (n < 1 || n > 131071 || m < 1 || m > 0x7fffffff || rows > (1 << 28)) return fail("%s: %lld rows, %lld channels of %lld values", what, (long long)rows, (long long)m, (long long)n);
+  if (w->shape[1] != row) return fail("%s: rows of w of %lld values, x's %lld and zeros up to a multiple of 16 expected", what, (long long)w->shape[1], (long long)n);
+  SHLO_TRY(shaped(w_scale, kF32, {m}, what, "w_scale"));
+  if (bias) {
+    SHLO_TRY(whole(dev, bias, what, "bias", held, &e));
+    SHLO_TRY(shaped(bias, kF32, {m}, what, "bias"));
+  }
+  SHLO_TRY(made(dev, dtype, {rows, m}, held, &o));
+  Mm8Call c{nullptr, 0, nullptr, (const int8_t *)data_ptr(b), row, (const float *)data_ptr(s), e ? (const float *)data_ptr(e) : nullptr,
+            data_ptr(o), m, rows, (int32_t)n, (int32_t)m, dtype, dev->pipe_err_dev};
+  if (x->dtype == kI8) {
+    if (!x_scale) return fail("%s: x of int8 without its scales", what);
+    if (n != row) return fail("%s: rows of x of %lld values, a multiple of 16 expected", what, (long long)n);
+    Arr *t;
+    SHLO_TRY(whole(dev, x_scale, what, "x_scale", held, &t));
+    SHLO_TRY(shaped(x_scale, kF32, {rows}, what, "x_scale"));
+    c.x = (const int8_t *)data_ptr(a);
+    c.x_row = row;
+    c.x_scale = (const float *)data_ptr(t);
+    SHLO_TRY(launch_mul_mat8(c, false, dev->sm_count, dev->stream));
+  } else {
+    if (x_scale) return fail("%s: scales of rows that are not int8", what);
+    const size_t bytes = linear8_work_bytes(rows, (int32_t)n);
+    Arr *t;
+    SHLO_TRY(made(dev, kU8, {(int64_t)bytes}, held, &t));
+    SHLO_TRY(launch_linear8(c, data_ptr(a), n, x->dtype, data_ptr(t), bytes, dev->sm_count, dev->stream));
+  }
+  give(o, out);
+  ts.done(o);
+  return 0;
+}
+
+int shlo_beam_select(shlo_arr logits, shlo_arr scores, shlo_arr ended, int32_t end_token, int32_t keep, shlo_arr *next, shlo_arr *parents,
+                     shlo_arr *tokens) {
+  const char *const what = "beam_select";
+  if (!logits || !scores || !next || !parents || !tokens) return fail("%s: null pointer", what);
+  Arr *ins[3] = {logits, scores, ended};
+  TraceScope ts(TK_OTHER, OT_BEAM_SELECT, nullptr, 0, ins, ended ? 3 : 2);
+  Device *dev;
+  SHLO_TRY(arr_device(logits, &dev));
+  Held held;
+  Arr *z, *s, *e = nullptr, *o, *p, *t, *w;
+  SHLO_TRY(whole(dev, logits, what, "logits", held, &z));
+  SHLO_TRY(whole(dev, scores, what, "scores", held, &s));
+  if (logits->ndim != 2 || scores->ndim != 2 || scores->dtype != kF32 || scores->shape[0] * scores->shape[1] != logits->shape[0])
+    return fail("%s: logits are not [sequences * beams, vocabulary] of scores float32 [sequences, beams]", what);
+  const int64_t seqs = scores->shape[0], beams = scores->shape[1], vocab = logits->shape[1];
+  if (seqs > 65535 || beams > 65535 || vocab > 0x7fffffff) return fail("%s: %lld sequences of %lld beams over %lld", what, (long long)seqs, (long long)beams, (long long)vocab);
+  if (ended) {
+    SHLO_TRY(whole(dev, ended, what, "ended", held, &e));
+    SHLO_TRY(shaped(ended, kI32, {seqs, beams}, what, "ended"));
+  }
+  size_t bytes;
+  SHLO_TRY(shlo_beam_workspace((int32_t)seqs, (int32_t)beams, keep, (int32_t)vocab, &bytes));
+  SHLO_TRY(made(dev, kF32, {seqs, keep}, held, &o));
+  SHLO_TRY(made(dev, kI32, {seqs, keep}, held, &p));
+  SHLO_TRY(made(dev, kI32, {seqs, keep}, held, &t));
+  SHLO_TRY(made(dev, kU8, {(int64_t)bytes}, held, &w));
+  BeamCall c{data_ptr(z), vocab, (const float *)data_ptr(s), e ? (const int32_t *)data_ptr(e) : nullptr, end_token, (int32_t)seqs, (int32_t)beams,
+             keep, (int32_t)vocab, logits->dtype, (float *)data_ptr(o), (int32_t *)data_ptr(p), (int32_t *)data_ptr(t), data_ptr(w), bytes};
+  SHLO_TRY(launch_beam_select(c, dev->sm_count, dev->stream));
+  give(o, next);
+  give(p, parents);
+  give(t, tokens);
+  ts.done(nullptr);
   return 0;
 }
 

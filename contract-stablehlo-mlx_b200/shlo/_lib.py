@@ -22,7 +22,8 @@ SYMBOLS = [
     "shlo_test_attend_give_up",
     "shlo_norm_rope_noalloc", "shlo_norm_rope_workspace", "shlo_norm_rope_grad_noalloc", "shlo_quantise_rows_noalloc",
     "shlo_mul_mat8_noalloc", "shlo_linear8_workspace", "shlo_linear8_noalloc", "shlo_beam_workspace",
-    "shlo_beam_select_noalloc", "shlo_kv_fork_noalloc",
+    "shlo_beam_select_noalloc", "shlo_kv_fork_noalloc", "shlo_kv_fork", "shlo_norm_rope_grad", "shlo_quantise_rows",
+    "shlo_linear8", "shlo_beam_select",
 ]
 
 
@@ -142,6 +143,12 @@ def load() -> ctypes.CDLL:
     L.shlo_kv_attend_workspace.argtypes = [ctypes.POINTER(ctypes.c_size_t)]
     L.shlo_kv_attend_noalloc.argtypes = [pool, batch, p, i64, i64, i32, u8, f32, i32, i32, p, i64, i64, p, p,
                                          ctypes.c_size_t, p]
+    outp = ctypes.POINTER(p)
+    L.shlo_kv_fork.argtypes = [p, c_arr, c_arr, c_arr, c_arr, outp, outp]
+    L.shlo_norm_rope_grad.argtypes = [c_arr] * 6 + [i32, f32, u32, f32, outp, outp, outp]
+    L.shlo_quantise_rows.argtypes = [c_arr, outp, outp]
+    L.shlo_linear8.argtypes = [c_arr, c_arr, c_arr, c_arr, c_arr, u8, outp]
+    L.shlo_beam_select.argtypes = [c_arr, c_arr, c_arr, i32, i32, outp, outp, outp]
     L.shlo_kv_new.argtypes = [i64, i32, i32, i32, ctypes.POINTER(p)]
     L.shlo_kv_free.argtypes = [p]
     L.shlo_kv_free.restype = None

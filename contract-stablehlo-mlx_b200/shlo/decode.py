@@ -424,14 +424,65 @@ def fork_noalloc(pool: Pool, tables, lens, parents, fresh, out_tables, out_lens,
 
 # ---- on arrays (mlx.Arr), in the library's own memory ----
 
+def _bits(x: float) -> int:
+    return int(np.array([x], np.float32).view(np.uint32)[0])
+
+
 def rope(x: M.Arr, positions: M.Arr, phases: M.Arr, *, interleaved=False, inverse=False, factor=1.0) -> M.Arr:
     """x [tokens, heads, dim] turned by positions (int32 [tokens]); phases: rope_phases' as an int64 array. May be
     called inside a compiled function."""
     t, h, d = M.shape(x)
     words = [t, h, d, 2 * M.shape(phases)[0], (1 if interleaved else 0) | (2 if inverse else 0),
-             int(np.array([factor], np.float32).view(np.uint32)[0])]
+             _bits(factor)]
     return M.kernel_apply(Run.kernel("rope"), [x, positions, phases, Run.params(words)], [[t, h, d]],
                           bytes([M.dtype(x)]), [max(t, 1), 1, 1], [64, 1, 1])[0]
+
+
+def norm_rope(x: M.Arr, positions: M.Arr, phases: M.Arr, q_weight: M.Arr, k_weight: M.Arr, *, q_heads: int, eps: float,
+              interleaved=False, factor=1.0) -> M.Arr:
+    """x [tokens, heads, dim], each head normed, weighted (the first q_heads by q_weight, the others by k_weight, [dim])
+    and turned by positions. May be called inside a compiled function, as may what follows up to Cache."""
+    t, h, d = M.shape(x)
+    words = [t, h, d, 2 * M.shape(phases)[0], 1 if interleaved else 0, _bits(factor), q_heads, _bits(eps)]
+    return M.kernel_apply(Run.kernel("norm_rope"), [x, positions, phases, q_weight, k_weight, Run.params(words)], [[t, h, d]],
+                          bytes([M.dtype(x)]), [max(t, 1), 1, 1], [64, 1, 1])[0]
+
+
+def _outs(n):
+    return [ctypes.c_void_p() for _ in range(n)]
+
+
+def norm_rope_grad(x: M.Arr, dy: M.Arr, positions: M.Arr, phases: M.Arr, q_weight: M.Arr, k_weight: M.Arr, *, q_heads: int,
+                   eps: float, interleaved=False, factor=1.0):
+    """(dx, dq_weight, dk_weight) of norm_rope."""
+    o = _outs(3)
+    check(load().shlo_norm_rope_grad(x.h, dy.h, positions.h, phases.h, q_weight.h, k_weight.h, q_heads, eps,
+                                     1 if interleaved else 0, factor, *[ctypes.byref(a) for a in o]))
+    return tuple(M.Arr(a.value) for a in o)
+
+
+def quantise_rows(x: M.Arr):
+    """(q int8 [rows, n and zeros up to a multiple of 16], scale float32 [rows]) of x [rows, n]."""
+    o = _outs(2)
+    check(load().shlo_quantise_rows(x.h, *[ctypes.byref(a) for a in o]))
+    return tuple(M.Arr(a.value) for a in o)
+
+
+def linear8(x: M.Arr, w: M.Arr, w_scale: M.Arr, *, x_scale: M.Arr | None = None, bias: M.Arr | None = None,
+            dtype: int = M.dtF32) -> M.Arr:
+    """x [rows, n] (float, or quantise_rows' with x_scale) by weights (quantise_rows' of [channels, n])."""
+    o = ctypes.c_void_p()
+    check(load().shlo_linear8(x.h, x_scale.h if x_scale else None, w.h, w_scale.h, bias.h if bias else None, dtype,
+                              ctypes.byref(o)))
+    return M.Arr(o.value)
+
+
+def beam_select(logits: M.Arr, scores: M.Arr, keep: int, *, ended: M.Arr | None = None, end_token=-1):
+    """(scores, parents, tokens) [sequences, keep] of logits [sequences * beams, vocabulary], scores [sequences, beams]."""
+    o = _outs(3)
+    check(load().shlo_beam_select(logits.h, scores.h, ended.h if ended else None, end_token, keep,
+                                  *[ctypes.byref(a) for a in o]))
+    return tuple(M.Arr(a.value) for a in o)
 
 
 class Cache:
@@ -467,6 +518,12 @@ class Cache:
         k, v = ctypes.c_void_p(), ctypes.c_void_p()
         check(load().shlo_kv_gather(self.h, tables.h, seq.h, pos.h, dtype, ctypes.byref(k), ctypes.byref(v)))
         return M.Arr(k.value), M.Arr(v.value)
+
+    def fork(self, tables: M.Arr, lens: M.Arr, parents: M.Arr, fresh: M.Arr):
+        """(tables, lens) of the rows that go on from parents; shared last pages are copied into fresh ones."""
+        t, l = ctypes.c_void_p(), ctypes.c_void_p()
+        check(load().shlo_kv_fork(self.h, tables.h, lens.h, parents.h, fresh.h, ctypes.byref(t), ctypes.byref(l)))
+        return M.Arr(t.value), M.Arr(l.value)
 
     def attend(self, q: M.Arr, starts: M.Arr, lens: M.Arr, tables: M.Arr, *, scale: float, causal=True, window=0,
                lse=False):

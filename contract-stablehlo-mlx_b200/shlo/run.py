@@ -37,6 +37,7 @@ FUSED = {
     "norm_affine": (["x", "gamma", "beta", "p"], ["y"]),
     "attention": (["q", "k", "v", "p"], ["y"]),
     "rope": (["x", "positions", "phases", "p"], ["y"]),
+    "norm_rope": (["x", "positions", "phases", "qWeight", "kWeight", "p"], ["y"]),
 }
 EP_BIAS, EP_BIAS_LHS, EP_RES, EP_RES_LHS, EP_GELU = 1, 2, 4, 8, 16
 

@@ -376,10 +376,32 @@ int shlo_kv_storage(shlo_kv kv, shlo_kv_pool *pool);
 int shlo_kv_append(shlo_kv kv, shlo_arr k, shlo_arr v, shlo_arr starts, shlo_arr lens, shlo_arr tables);
 /* New arrays [n, heads, head_dim] of `dtype`. */
 int shlo_kv_gather(shlo_kv kv, shlo_arr tables, shlo_arr seq, shlo_arr pos, uint8_t dtype, shlo_arr *k, shlo_arr *v);
+/* The tables [news, table pages] and lengths [news] of the rows that go on from
+   parents (int32 [news]) of tables and lens; fresh int32 [news]. */
+int shlo_kv_fork(shlo_kv kv, shlo_arr tables, shlo_arr lens, shlo_arr parents, shlo_arr fresh, shlo_arr *out_tables, shlo_arr *out_lens);
 /* A new array of q's shape and type, and of the logarithms [tokens, query heads]
    where `lse` is not NULL; rows that no sequence has are 0. */
 int shlo_kv_attend(shlo_kv kv, shlo_arr q, shlo_arr starts, shlo_arr lens, shlo_arr tables, float scale, int32_t causal,
                    int32_t window, shlo_arr *out, shlo_arr *lse);
+
+/* The norm with rotation is the kernel "shlo_norm_rope": inputs x [T, H, D], positions
+   int32 [T], phases int64 [rot / 2], the two weights [D] of one type, and the words [T,
+   H, D, rot, flags, factor bits, query heads, eps bits]. What follows may be called
+   inside a compiled function too. Its gradient: new arrays of x's shape and type, and
+   float32 [D] of each weight. */
+int shlo_norm_rope_grad(shlo_arr x, shlo_arr dy, shlo_arr positions, shlo_arr phases, shlo_arr q_weight, shlo_arr k_weight,
+                        int32_t q_heads, float eps, uint32_t flags, float factor, shlo_arr *dx, shlo_arr *dq_weight, shlo_arr *dk_weight);
+/* x [rows, n] as int8 [rows, n and zeros up to a multiple of 16] and float32 [rows]. */
+int shlo_quantise_rows(shlo_arr x, shlo_arr *q, shlo_arr *scale);
+/* A new array [rows, channels] of `dtype`: x [rows, n] of float16 or float32 (x_scale
+   NULL), or int8 with its scales, both as shlo_quantise_rows makes them, by w int8
+   [channels, n and zeros up to a multiple of 16] and w_scale float32 [channels]; bias
+   float32 [channels] or NULL. */
+int shlo_linear8(shlo_arr x, shlo_arr x_scale, shlo_arr w, shlo_arr w_scale, shlo_arr bias, uint8_t dtype, shlo_arr *out);
+/* logits [sequences * beams, vocabulary], scores float32 [sequences, beams], ended int32
+   of the same shape or NULL: new arrays [sequences, keep]. */
+int shlo_beam_select(shlo_arr logits, shlo_arr scores, shlo_arr ended, int32_t end_token, int32_t keep, shlo_arr *next,
+                     shlo_arr *parents, shlo_arr *tokens);
 
 /* ---- test-driver helpers (Mlx.lean:69-73) ---- */
 
