@@ -725,8 +725,8 @@ int launch_beam_select(const BeamCall &c, int sms, cudaStream_t st) {
   if ((uintptr_t)c.logits % size || ((uintptr_t)c.scores | (uintptr_t)c.ended | (uintptr_t)c.next | (uintptr_t)c.parents | (uintptr_t)c.tokens) % 4)
     return fail("beam_select: an operand is not aligned to its type");
   const size_t need = beam_work_bytes(rows, c.keep, c.vocab);
-  if (!c.work || c.work_bytes < need) return fail("beam_select: a workspace of %zu bytes, %zu needed", c.work ? c.work_bytes : 0, need);
-  if ((uintptr_t)c.work % 8) return fail("beam_select: misaligned workspace");
+  if (!c.workspace || c.workspace_bytes < need) return fail("beam_select: a workspace of %zu bytes, %zu needed", c.workspace ? c.workspace_bytes : 0, need);
+  if ((uintptr_t)c.workspace % 8) return fail("beam_select: misaligned workspace");
   const Cut how = cut(rows, c.vocab, size, sms);
   BeamArgs a;
   a.z = c.logits; a.row = c.row; a.scores = c.scores; a.ended = c.ended; a.next = c.next; a.parents = c.parents; a.tokens = c.tokens;
@@ -735,7 +735,7 @@ int launch_beam_select(const BeamCall &c, int sms, cudaStream_t st) {
   while (a.group > 1 && kThreads / a.group < c.keep) a.group /= 2;
   a.part = how.stretch * how.turns;
   a.parts = how.parts;
-  a.best = (uint64_t *)c.work;
+  a.best = (uint64_t *)c.workspace;
   a.sum = (double *)(a.best + rows * a.parts * c.keep);
   a.top = (float *)(a.sum + rows * a.parts);
   const dim3 grid((unsigned)a.parts, (unsigned)rows);
@@ -778,13 +778,11 @@ int shlo_beam_workspace(int32_t seqs, int32_t beams, int32_t keep, int32_t vocab
   return 0;
 }
 
-int shlo_beam_select_noalloc(const void *logits, int64_t row, const float *scores, const int32_t *ended, int32_t end_token,
-                             int32_t seqs, int32_t beams, int32_t keep, int32_t vocab, uint8_t dtype, float *next,
-                             int32_t *parents, int32_t *tokens, void *workspace, size_t workspace_bytes, void *stream) {
+int shlo_beam_select_noalloc(const shlo_beam_args *args, void *stream) {
+  if (!args) return fail("beam_select: null arguments");
   Device *dev;
   SHLO_TRY(calling_device(&dev));
-  BeamCall c{logits, row, scores, ended, end_token, seqs, beams, keep, vocab, dtype, next, parents, tokens, workspace, workspace_bytes};
-  return launch_beam_select(c, dev->sm_count, (cudaStream_t)stream);
+  return launch_beam_select(*args, dev->sm_count, (cudaStream_t)stream);
 }
 
 }  // extern "C"

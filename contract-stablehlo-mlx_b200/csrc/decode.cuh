@@ -25,71 +25,27 @@ int launch_rope(const RopeCall &c, int sms, cudaStream_t st);
 int check_in_place(const void *x, int64_t x_token, int64_t x_head, const void *y, int64_t y_token, int64_t y_head, int64_t tokens,
                    int64_t heads, int64_t dim, size_t size, const char *what, const char *x_name, const char *y_name);
 
-struct NormRopeCall {
-  const void *x;
-  int64_t x_token, x_head;
-  const void *dy;  // nullptr: the forward pass
-  int64_t dy_token, dy_head;
-  const int32_t *positions;
-  const int64_t *phases;
-  const void *q_weight, *k_weight;  // nullptr: ones
-  uint8_t weight_dtype;
-  int32_t q_heads;
-  float eps;
-  void *y;  // dx in the backward pass
-  int64_t y_token, y_head;
-  float *dq_weight, *dk_weight;  // nullptr: not asked for
-  int64_t tokens;
-  int32_t heads, dim, rot;
-  uint8_t dtype;
-  uint32_t flags;
-  float factor;
-  void *work;
-  size_t work_bytes;
-};
+// (dy: the gradient)
+using NormRopeCall = shlo_norm_rope_args;
 size_t norm_rope_work_bytes(int sms);
 // A call's operands from arrays, without its result; p: the "shlo_norm_rope" kernel's words.
 int norm_rope_call(const char *what, Arr *x, Arr *positions, Arr *phases, Arr *q_weight, Arr *k_weight, const uint32_t *p, NormRopeCall *c);
-int launch_norm_rope(const NormRopeCall &c, int sms, cudaStream_t st);
+int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st);
 
 // Products in 8-bit integers (linear8.cu, linear8_tiles.cu): y = x w^T, scaled.
-struct Mm8Call {
-  const int8_t *x;
-  int64_t x_row;  // bytes
-  const float *x_scale;
-  const int8_t *w;
-  int64_t w_row;
-  const float *w_scale, *bias;  // (no bias: nullptr)
-  void *y;
-  int64_t y_row;  // values
-  int64_t rows;
-  int32_t n, m;   // values a row, channels
-  uint8_t dtype;  // y's
-  int *err;       // the device's word for launches that gave up a wait
-};
+using Mm8Call = shlo_mul_mat8_args;
 // `fill`: zeros behind a row's last value up to a multiple of 16.
 int launch_quantise_rows(const void *x, int64_t x_row, uint8_t dtype, int64_t rows, int32_t n, int8_t *q, int64_t q_row, float *scale,
                          bool fill, const char *what, cudaStream_t st);
-// `after_rows`: the launch before it on the stream is the one that rounds its x.
-int launch_mul_mat8(const Mm8Call &c, bool after_rows, int sms, cudaStream_t st);
-int launch_mul_mat8_tiles(const Mm8Call &c, bool after_rows, int sms, cudaStream_t st);  // (arguments checked)
+// `after_rows`: the launch before it on the stream is the one that rounds its x. `err`:
+// the device's word for launches that gave up a wait.
+int launch_mul_mat8(const Mm8Call &c, bool after_rows, int *err, int sms, cudaStream_t st);
+int launch_mul_mat8_tiles(const Mm8Call &c, bool after_rows, int *err, int sms, cudaStream_t st);  // (arguments checked)
 size_t linear8_work_bytes(int64_t rows, int32_t n);
-int launch_linear8(const Mm8Call &c, const void *x, int64_t x_row, uint8_t x_dtype, void *work, size_t work_bytes, int sms, cudaStream_t st);
+int launch_linear8(const Mm8Call &c, int *err, int sms, cudaStream_t st);
 
 // Beam search (beam.cu).
-struct BeamCall {
-  const void *logits;  // [seqs * beams][vocab]
-  int64_t row;         // values between rows
-  const float *scores; // [seqs][beams]
-  const int32_t *ended;  // nullptr: none has
-  int32_t end_token;
-  int32_t seqs, beams, keep, vocab;
-  uint8_t dtype;
-  float *next;  // [seqs][keep], as are the two below
-  int32_t *parents, *tokens;
-  void *work;
-  size_t work_bytes;
-};
+using BeamCall = shlo_beam_args;
 size_t beam_work_bytes(int64_t rows, int32_t keep, int32_t vocab);
 int launch_beam_select(const BeamCall &c, int sms, cudaStream_t st);
 
@@ -103,16 +59,7 @@ int launch_kv_gather(const shlo_kv_pool &p, const int32_t *tables, int64_t table
                      int32_t table_pages, const int32_t *seq, const int32_t *pos, int64_t n, void *k, int64_t k_token,
                      int64_t k_head, void *v, int64_t v_token, int64_t v_head, uint8_t dtype, int sms, cudaStream_t st);
 
-struct ForkCall {
-  shlo_kv_pool pool;
-  const int32_t *tables, *lens;  // of `rows` rows
-  int64_t table_stride;
-  const int32_t *parents, *fresh;  // of `news` rows
-  int32_t *out_tables, *out_lens;
-  int64_t out_stride;
-  int32_t rows, news, table_pages;
-};
-int launch_kv_fork(const ForkCall &c, cudaStream_t st);
+int launch_kv_fork(const shlo_kv_pool &p, const shlo_kv_fork_args &c, cudaStream_t st);
 
 struct AttendCall {
   shlo_kv_pool pool;

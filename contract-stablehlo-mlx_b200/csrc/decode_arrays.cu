@@ -44,7 +44,7 @@ int k_norm_rope(Device *dev, Arr *x, Arr *positions, Arr *phases, Arr *q_weight,
   c.y = data_ptr(o);
   c.y_token = c.x_token;
   c.y_head = c.x_head;
-  if (launch_norm_rope(c, dev->sm_count, dev->stream)) {
+  if (launch_norm_rope(c, false, dev->sm_count, dev->stream)) {
     shlo_release(o);
     return 1;
   }
@@ -368,9 +368,10 @@ int shlo_kv_fork(shlo_kv kv, shlo_arr tables, shlo_arr lens, shlo_arr parents, s
                 (long long)rows, (long long)width, (long long)f->shape[0], (long long)news);
   SHLO_TRY(made(kv->dev, kI32, {news, width}, held, &ot));
   SHLO_TRY(made(kv->dev, kI32, {news}, held, &ol));
-  ForkCall c{kv->pool, (const int32_t *)data_ptr(t), (const int32_t *)data_ptr(l), width, (const int32_t *)data_ptr(p),
-             (const int32_t *)data_ptr(f), (int32_t *)data_ptr(ot), (int32_t *)data_ptr(ol), width, (int32_t)rows, (int32_t)news, (int32_t)width};
-  SHLO_TRY(launch_kv_fork(c, kv->dev->stream));
+  const shlo_kv_fork_args c{(const int32_t *)data_ptr(t), (const int32_t *)data_ptr(l), width, (const int32_t *)data_ptr(p),
+                            (const int32_t *)data_ptr(f), (int32_t *)data_ptr(ot), (int32_t *)data_ptr(ol), width, (int32_t)rows,
+                            (int32_t)news, (int32_t)width};
+  SHLO_TRY(launch_kv_fork(kv->pool, c, kv->dev->stream));
   give(ot, out_tables);
   give(ol, out_lens);
   return 0;
@@ -404,7 +405,7 @@ int shlo_norm_rope_grad(shlo_arr x, shlo_arr dy, shlo_arr positions, shlo_arr ph
   SHLO_TRY(made(dev, kF32, {c.dim}, held, &k));
   const size_t bytes = norm_rope_work_bytes(dev->sm_count);
   SHLO_TRY(made(dev, kU8, {(int64_t)bytes}, held, &w));
-  c.dy = c.tokens ? data_ptr(a[1]) : (const void *)"";
+  c.dy = data_ptr(a[1]);
   c.dy_token = c.x_token;
   c.dy_head = c.x_head;
   c.y = data_ptr(o);
@@ -412,9 +413,9 @@ int shlo_norm_rope_grad(shlo_arr x, shlo_arr dy, shlo_arr positions, shlo_arr ph
   c.y_head = c.x_head;
   c.dq_weight = (float *)data_ptr(q);
   c.dk_weight = (float *)data_ptr(k);
-  c.work = data_ptr(w);
-  c.work_bytes = bytes;
-  SHLO_TRY(launch_norm_rope(c, dev->sm_count, dev->stream));
+  c.workspace = data_ptr(w);
+  c.workspace_bytes = bytes;
+  SHLO_TRY(launch_norm_rope(c, true, dev->sm_count, dev->stream));
   give(o, dx);
   give(q, dq_weight);
   give(k, dk_weight);
@@ -467,24 +468,27 @@ int shlo_linear8(shlo_arr x, shlo_arr x_scale, shlo_arr w, shlo_arr w_scale, shl
     SHLO_TRY(shaped(bias, kF32, {m}, what, "bias"));
   }
   SHLO_TRY(made(dev, dtype, {rows, m}, held, &o));
-  Mm8Call c{nullptr, 0, nullptr, (const int8_t *)data_ptr(b), row, (const float *)data_ptr(s), e ? (const float *)data_ptr(e) : nullptr,
-            data_ptr(o), m, rows, (int32_t)n, (int32_t)m, dtype, dev->pipe_err_dev};
+  Mm8Call c = {};
+  c.x = data_ptr(a); c.x_row = n; c.x_dtype = x->dtype;
+  c.w = (const int8_t *)data_ptr(b); c.w_row = row; c.w_scale = (const float *)data_ptr(s);
+  c.bias = e ? (const float *)data_ptr(e) : nullptr;
+  c.y = data_ptr(o); c.y_row = m; c.dtype = dtype;
+  c.rows = rows; c.n = (int32_t)n; c.m = (int32_t)m;
   if (x->dtype == kI8) {
     if (!x_scale) return fail("%s: x of int8 without its scales", what);
     if (n != row) return fail("%s: rows of x of %lld values, a multiple of 16 expected", what, (long long)n);
     Arr *t;
     SHLO_TRY(whole(dev, x_scale, what, "x_scale", held, &t));
     SHLO_TRY(shaped(x_scale, kF32, {rows}, what, "x_scale"));
-    c.x = (const int8_t *)data_ptr(a);
-    c.x_row = row;
     c.x_scale = (const float *)data_ptr(t);
-    SHLO_TRY(launch_mul_mat8(c, false, dev->sm_count, dev->stream));
+    SHLO_TRY(launch_mul_mat8(c, false, dev->pipe_err_dev, dev->sm_count, dev->stream));
   } else {
     if (x_scale) return fail("%s: scales of rows that are not int8", what);
-    const size_t bytes = linear8_work_bytes(rows, (int32_t)n);
+    c.workspace_bytes = linear8_work_bytes(rows, (int32_t)n);
     Arr *t;
-    SHLO_TRY(made(dev, kU8, {(int64_t)bytes}, held, &t));
-    SHLO_TRY(launch_linear8(c, data_ptr(a), n, x->dtype, data_ptr(t), bytes, dev->sm_count, dev->stream));
+    SHLO_TRY(made(dev, kU8, {(int64_t)c.workspace_bytes}, held, &t));
+    c.workspace = data_ptr(t);
+    SHLO_TRY(launch_linear8(c, dev->pipe_err_dev, dev->sm_count, dev->stream));
   }
   give(o, out);
   ts.done(o);
@@ -517,8 +521,12 @@ int shlo_beam_select(shlo_arr logits, shlo_arr scores, shlo_arr ended, int32_t e
   SHLO_TRY(made(dev, kI32, {seqs, keep}, held, &p));
   SHLO_TRY(made(dev, kI32, {seqs, keep}, held, &t));
   SHLO_TRY(made(dev, kU8, {(int64_t)bytes}, held, &w));
-  BeamCall c{data_ptr(z), vocab, (const float *)data_ptr(s), e ? (const int32_t *)data_ptr(e) : nullptr, end_token, (int32_t)seqs, (int32_t)beams,
-             keep, (int32_t)vocab, logits->dtype, (float *)data_ptr(o), (int32_t *)data_ptr(p), (int32_t *)data_ptr(t), data_ptr(w), bytes};
+  BeamCall c = {};
+  c.logits = data_ptr(z); c.row = vocab; c.dtype = logits->dtype;
+  c.scores = (const float *)data_ptr(s); c.ended = e ? (const int32_t *)data_ptr(e) : nullptr; c.end_token = end_token;
+  c.next = (float *)data_ptr(o); c.parents = (int32_t *)data_ptr(p); c.tokens = (int32_t *)data_ptr(t);
+  c.workspace = data_ptr(w); c.workspace_bytes = bytes;
+  c.seqs = (int32_t)seqs; c.beams = (int32_t)beams; c.keep = keep; c.vocab = (int32_t)vocab;
   SHLO_TRY(launch_beam_select(c, dev->sm_count, dev->stream));
   give(o, next);
   give(p, parents);

@@ -15,6 +15,10 @@ namespace {
 
 constexpr int kForkThreads = 128;
 
+struct ForkCall : shlo_kv_fork_args {
+  shlo_kv_pool pool;
+};
+
 __global__ void __launch_bounds__(kForkThreads) k_kv_fork(const ForkCall a) {
   const int r = blockIdx.x, parent = __ldg(a.parents + r), PT = a.pool.page_tokens;
   const bool live = parent >= 0 && parent < a.rows;
@@ -80,7 +84,10 @@ __global__ void __launch_bounds__(kForkThreads) k_kv_fork(const ForkCall a) {
 
 }  // namespace
 
-int launch_kv_fork(const ForkCall &c, cudaStream_t st) {
+int launch_kv_fork(const shlo_kv_pool &p, const shlo_kv_fork_args &args, cudaStream_t st) {
+  ForkCall c;
+  static_cast<shlo_kv_fork_args &>(c) = args;
+  c.pool = p;
   SHLO_TRY(check_pool(&c.pool, "kv_fork"));
   if (c.rows < 0 || c.news < 0 || c.news > 65536 || c.table_pages < 0 || c.table_pages > (1 << 22))
     return fail("kv_fork: %d rows continued by %d (at most 65536), tables of %d pages (at most 2^22)", c.rows, c.news, c.table_pages);
@@ -101,14 +108,11 @@ using namespace shlo;
 
 extern "C" {
 
-int shlo_kv_fork_noalloc(const shlo_kv_pool *pool, const int32_t *tables, int64_t table_stride, const int32_t *lens, int32_t rows,
-                         int32_t table_pages, const int32_t *parents, const int32_t *fresh, int32_t news, int32_t *out_tables,
-                         int64_t out_stride, int32_t *out_lens, void *stream) {
-  if (!pool) return fail("kv_fork: null descriptor");
+int shlo_kv_fork_noalloc(const shlo_kv_pool *pool, const shlo_kv_fork_args *args, void *stream) {
+  if (!pool || !args) return fail("kv_fork: null descriptor");
   Device *dev;
   SHLO_TRY(calling_device(&dev));
-  ForkCall c{*pool, tables, lens, table_stride, parents, fresh, out_tables, out_lens, out_stride, rows, news, table_pages};
-  return launch_kv_fork(c, (cudaStream_t)stream);
+  return launch_kv_fork(*pool, *args, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -182,8 +182,9 @@ void launch_rows(const T *x, int64_t x_row, int64_t rows, int n, int8_t *q, int6
 int launch_quantise_rows(const void *x, int64_t x_row, uint8_t dtype, int64_t rows, int32_t n, int8_t *q, int64_t q_row, float *scale,
                          bool fill, const char *what, cudaStream_t st) {
   if (dtype != kF16 && dtype != kF32) return fail("%s: %s not carried (float16 or float32)", what, dtype_name(dtype));
-  if (rows < 0 || rows > 0x7fffffff || n < 1) return fail("%s: %lld rows of %d values", what, (long long)rows, n);
+  if (rows < 0 || rows > 0x7fffffff || n < 1 || n > (1 << 30)) return fail("%s: %lld rows of %d values (up to 2^30)", what, (long long)rows, n);
   if (rows == 0) return 0;
+  if (rows > 1 && q_row < n) return fail("%s: rows of q overlap", what);
   if (!x || !q || !scale) return fail("%s: null pointer", what);
   const size_t size = dtype_size(dtype);
   if ((uintptr_t)x % size || (uintptr_t)scale % 4) return fail("%s: an operand is not aligned to its type", what);
@@ -208,37 +209,39 @@ static int check_mul_mat8(const Mm8Call &c, const char *what) {
   if (!c.w || !c.w_scale || !c.y) return fail("%s: null pointer", what);
   if ((uintptr_t)c.w % 16 || (c.m > 1 && (c.w_row % 16 || c.w_row < c.n)))
     return fail("%s: rows of w begin on multiples of 16 bytes and do not overlap (a distance of %lld for %d values)", what, (long long)c.w_row, c.n);
+  if (c.rows > 1 && c.y_row < c.m) return fail("%s: rows of the result overlap", what);
   if ((uintptr_t)c.w_scale % 4 || (uintptr_t)c.bias % 4 || (uintptr_t)c.y % dtype_size(c.dtype)) return fail("%s: an operand is not aligned to its type", what);
   return 0;
 }
 
-int launch_mul_mat8(const Mm8Call &c, bool after_rows, int sms, cudaStream_t st) {
+int launch_mul_mat8(const Mm8Call &c, bool after_rows, int *err, int sms, cudaStream_t st) {
   SHLO_TRY(check_mul_mat8(c, "mul_mat8"));
   if (c.rows == 0) return 0;
   if (!c.x || !c.x_scale) return fail("mul_mat8: null pointer");
   if ((uintptr_t)c.x % 16 || (c.rows > 1 && (c.x_row % 16 || c.x_row < c.n)))
     return fail("mul_mat8: rows of x begin on multiples of 16 bytes and do not overlap (a distance of %lld for %d values)", (long long)c.x_row, c.n);
   if ((uintptr_t)c.x_scale % 4) return fail("mul_mat8: an operand is not aligned to its type");
-  return launch_mul_mat8_tiles(c, after_rows, sms, st);
+  return launch_mul_mat8_tiles(c, after_rows, err, sms, st);
 }
 
 // Rows of int8 at distances of a multiple of 16 bytes, then their scales.
 static int64_t quantised_row(int32_t n) { return ((int64_t)n + 15) / 16 * 16; }
 size_t linear8_work_bytes(int64_t rows, int32_t n) { return (size_t)rows * (quantised_row(n) + 4) + 16; }
 
-int launch_linear8(const Mm8Call &call, const void *x, int64_t x_row, uint8_t x_dtype, void *work, size_t work_bytes, int sms, cudaStream_t st) {
+int launch_linear8(const Mm8Call &call, int *err, int sms, cudaStream_t st) {
   Mm8Call c = call;
   SHLO_TRY(check_mul_mat8(c, "linear8"));
-  if (x_dtype != kF16 && x_dtype != kF32) return fail("linear8: %s not carried (float16 or float32)", dtype_name(x_dtype));
+  if (c.x_dtype != kF16 && c.x_dtype != kF32) return fail("linear8: %s not carried (float16 or float32)", dtype_name(c.x_dtype));
   if (c.rows == 0) return 0;
-  if (!work || work_bytes < linear8_work_bytes(c.rows, c.n))
-    return fail("linear8: a workspace of %zu bytes, %zu needed", work ? work_bytes : 0, linear8_work_bytes(c.rows, c.n));
-  if ((uintptr_t)work % 16) return fail("linear8: the workspace does not begin on a multiple of 16 bytes");
+  int8_t *const q = (int8_t *)c.workspace;
+  if (!q || c.workspace_bytes < linear8_work_bytes(c.rows, c.n))
+    return fail("linear8: a workspace of %zu bytes, %zu needed", q ? c.workspace_bytes : 0, linear8_work_bytes(c.rows, c.n));
+  if ((uintptr_t)q % 16) return fail("linear8: the workspace does not begin on a multiple of 16 bytes");
+  c.x = q;
   c.x_row = quantised_row(c.n);
-  c.x = (const int8_t *)work;
-  c.x_scale = (const float *)((const int8_t *)work + c.rows * c.x_row);
-  SHLO_TRY(launch_quantise_rows(x, x_row, x_dtype, c.rows, c.n, (int8_t *)work, c.x_row, (float *)c.x_scale, false, "linear8", st));
-  return launch_mul_mat8(c, true, sms, st);
+  c.x_scale = (const float *)(q + c.rows * c.x_row);
+  SHLO_TRY(launch_quantise_rows(call.x, call.x_row, c.x_dtype, c.rows, c.n, q, c.x_row, (float *)c.x_scale, false, "linear8", st));
+  return launch_mul_mat8(c, true, err, sms, st);
 }
 
 }  // namespace shlo
@@ -254,13 +257,12 @@ int shlo_quantise_rows_noalloc(const void *x, int64_t x_row, int64_t rows, int32
   return launch_quantise_rows(x, x_row, dtype, rows, n, q, q_row, scale, false, "quantise_rows", (cudaStream_t)stream);
 }
 
-int shlo_mul_mat8_noalloc(const int8_t *x, int64_t x_row, const float *x_scale, const int8_t *w, int64_t w_row, const float *w_scale,
-                          const float *bias, void *y, int64_t y_row, int64_t rows, int32_t n, int32_t m, uint8_t dtype, void *stream) {
+int shlo_mul_mat8_noalloc(const shlo_mul_mat8_args *args, void *stream) {
+  if (!args) return fail("mul_mat8: null arguments");
   Device *dev;
   SHLO_TRY(calling_device(&dev));
   SHLO_TRY(launch_error(dev, "mul_mat8, an earlier call"));
-  Mm8Call c{x, x_row, x_scale, w, w_row, w_scale, bias, y, y_row, rows, n, m, dtype, dev->pipe_err_dev};
-  return launch_mul_mat8(c, false, dev->sm_count, (cudaStream_t)stream);
+  return launch_mul_mat8(*args, false, dev->pipe_err_dev, dev->sm_count, (cudaStream_t)stream);
 }
 
 int shlo_linear8_workspace(int64_t rows, int32_t n, size_t *bytes) {
@@ -270,14 +272,12 @@ int shlo_linear8_workspace(int64_t rows, int32_t n, size_t *bytes) {
   return 0;
 }
 
-int shlo_linear8_noalloc(const void *x, int64_t x_row, uint8_t x_dtype, const int8_t *w, int64_t w_row, const float *w_scale,
-                         const float *bias, void *y, int64_t y_row, int64_t rows, int32_t n, int32_t m, uint8_t y_dtype,
-                         void *workspace, size_t workspace_bytes, void *stream) {
+int shlo_linear8_noalloc(const shlo_mul_mat8_args *args, void *stream) {
+  if (!args) return fail("linear8: null arguments");
   Device *dev;
   SHLO_TRY(calling_device(&dev));
   SHLO_TRY(launch_error(dev, "linear8, an earlier call"));
-  Mm8Call c{nullptr, 0, nullptr, w, w_row, w_scale, bias, y, y_row, rows, n, m, y_dtype, dev->pipe_err_dev};
-  return launch_linear8(c, x, x_row, x_dtype, workspace, workspace_bytes, dev->sm_count, (cudaStream_t)stream);
+  return launch_linear8(*args, dev->pipe_err_dev, dev->sm_count, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -366,7 +366,7 @@ int encode(CUtensorMap *map, const int8_t *p, int64_t row, int64_t rows, int n, 
 }
 
 template <int N, int CG, typename Y>
-int launch(const Mm8Call &c, int ch, int splits, bool after_rows, int sms, cudaStream_t st) {
+int launch(const Mm8Call &c, int ch, int splits, bool after_rows, int *err, int sms, cudaStream_t st) {
   using S = Tile<N, CG>;
   TileArgs a;
   a.x_scale = c.x_scale; a.w_scale = c.w_scale; a.bias = c.bias; a.y = c.y; a.y_row = c.y_row; a.rows = c.rows;
@@ -374,17 +374,19 @@ int launch(const Mm8Call &c, int ch, int splits, bool after_rows, int sms, cudaS
   a.kblocks = (c.n + kK - 1) / kK;
   a.ch = CG == 2 ? 128 : ch;
   a.ch_tiles = (c.m + a.ch * CG - 1) / (a.ch * CG);
-  a.tiles = a.ch_tiles * (int)((c.rows + N - 1) / N);
+  const int64_t tiles = (int64_t)a.ch_tiles * ((c.rows + N - 1) / N);
+  if (tiles > (1 << 30)) return fail("mul_mat8: %lld rows by %d channels", (long long)c.rows, c.m);
+  a.tiles = (int)tiles;
   a.splits = splits;
   a.after_rows = after_rows;
-  a.err = c.err;
+  a.err = err;
   a.stage_bytes = a.ch * kK + S::B_BYTES;
   const int beyond = (128 - a.ch) * kK;  // what the products read behind the last stage's weights
   a.stages = std::min(kMaxStages, (S::ROOM - 1024 - beyond) / a.stage_bytes);
   const int bytes = 1024 + beyond + std::max(a.stages * a.stage_bytes, splits > 1 ? N * 512 : 0);
   CUtensorMap wmap, xmap;
   SHLO_TRY(encode(&wmap, c.w, c.w_row, c.m, c.n, a.ch));
-  SHLO_TRY(encode(&xmap, c.x, c.x_row, c.rows, c.n, N / CG));
+  SHLO_TRY(encode(&xmap, (const int8_t *)c.x, c.x_row, c.rows, c.n, N / CG));
   const auto kernel = k_mul_mat8_tiles<N, CG, Y>;
   static std::atomic<uint64_t> set{0};
   int device;
@@ -456,21 +458,21 @@ Shape choose(const Mm8Call &c, int sms) {
 }
 
 template <typename Y>
-int launch_for(const Mm8Call &c, bool after_rows, int sms, cudaStream_t st) {
+int launch_for(const Mm8Call &c, bool after_rows, int *err, int sms, cudaStream_t st) {
   const Shape s = choose(c, sms);
   switch (s.n) {
-    case 16: return launch<16, 1, Y>(c, s.ch, s.splits, after_rows, sms, st);
-    case 32: return launch<32, 1, Y>(c, s.ch, s.splits, after_rows, sms, st);
-    case 64: return launch<64, 1, Y>(c, s.ch, s.splits, after_rows, sms, st);
-    case 128: return launch<128, 1, Y>(c, s.ch, s.splits, after_rows, sms, st);
-    default: return launch<256, 2, Y>(c, 128, 1, after_rows, sms, st);
+    case 16: return launch<16, 1, Y>(c, s.ch, s.splits, after_rows, err, sms, st);
+    case 32: return launch<32, 1, Y>(c, s.ch, s.splits, after_rows, err, sms, st);
+    case 64: return launch<64, 1, Y>(c, s.ch, s.splits, after_rows, err, sms, st);
+    case 128: return launch<128, 1, Y>(c, s.ch, s.splits, after_rows, err, sms, st);
+    default: return launch<256, 2, Y>(c, 128, 1, after_rows, err, sms, st);
   }
 }
 
 }  // namespace
 
-int launch_mul_mat8_tiles(const Mm8Call &c, bool after_rows, int sms, cudaStream_t st) {
-  return c.dtype == kF16 ? launch_for<__half>(c, after_rows, sms, st) : launch_for<float>(c, after_rows, sms, st);
+int launch_mul_mat8_tiles(const Mm8Call &c, bool after_rows, int *err, int sms, cudaStream_t st) {
+  return c.dtype == kF16 ? launch_for<__half>(c, after_rows, err, sms, st) : launch_for<float>(c, after_rows, err, sms, st);
 }
 
 }  // namespace shlo

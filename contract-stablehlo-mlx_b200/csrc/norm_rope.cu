@@ -465,8 +465,7 @@ int back_blocks(int sms) { return sms * kBackBlocksPerSm; }
 
 size_t norm_rope_work_bytes(int sms) { return (size_t)back_blocks(sms) * 2 * 512 * sizeof(double); }
 
-int launch_norm_rope(const NormRopeCall &c, int sms, cudaStream_t st) {
-  const bool back = c.dy != nullptr;
+int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st) {
   const char *const what = back ? "norm_rope_grad" : "norm_rope";
   if (c.dtype != kF16 && c.dtype != kF32) return fail("%s: %s not carried (float16 or float32)", what, dtype_name(c.dtype));
   if (c.weight_dtype != kF16 && c.weight_dtype != kF32) return fail("%s: weights of %s not carried (float16 or float32)", what, dtype_name(c.weight_dtype));
@@ -479,16 +478,18 @@ int launch_norm_rope(const NormRopeCall &c, int sms, cudaStream_t st) {
   if (c.tokens > 0x7fffffff) return fail("%s: %lld tokens, at most 2^31 - 1", what, (long long)c.tokens);
   const size_t size = dtype_size(c.dtype), wsize = dtype_size(c.weight_dtype);
   const bool sums = back && (c.dq_weight || c.dk_weight);
-  if ((uintptr_t)c.dq_weight % 4 || (uintptr_t)c.dk_weight % 4 || (sums && (uintptr_t)c.work % 8)) return fail("%s: misaligned gradient or workspace", what);
-  if (sums && (!c.work || c.work_bytes < norm_rope_work_bytes(sms)))
-    return fail("%s: a workspace of %zu bytes, %zu needed", what, c.work ? c.work_bytes : 0, norm_rope_work_bytes(sms));
+  if ((uintptr_t)c.dq_weight % 4 || (uintptr_t)c.dk_weight % 4 || (sums && (uintptr_t)c.workspace % 8)) return fail("%s: misaligned gradient or workspace", what);
+  if (sums && (!c.workspace || c.workspace_bytes < norm_rope_work_bytes(sms)))
+    return fail("%s: a workspace of %zu bytes, %zu needed", what, c.workspace ? c.workspace_bytes : 0, norm_rope_work_bytes(sms));
   if (c.tokens == 0) {
     if (c.dq_weight) SHLO_CUDA(cudaMemsetAsync(c.dq_weight, 0, c.dim * sizeof(float), st));
     if (c.dk_weight) SHLO_CUDA(cudaMemsetAsync(c.dk_weight, 0, c.dim * sizeof(float), st));
     return 0;
   }
-  if (!c.x || !c.y || (c.rot && (!c.positions || !c.phases))) return fail("%s: null pointer", what);
-  if (((uintptr_t)c.x | (uintptr_t)c.y | (uintptr_t)c.dy) % size) return fail("%s: an operand is not aligned to its type", what);
+  if (!c.x || !c.y || (back && !c.dy) || (c.rot && (!c.positions || !c.phases))) return fail("%s: null pointer", what);
+  if ((c.tokens > 1 && llabs(c.y_token) < c.dim) || (c.heads > 1 && llabs(c.y_head) < c.dim))
+    return fail("%s: rows of %s overlap", what, back ? "dx" : "y");
+  if (((uintptr_t)c.x | (uintptr_t)c.y | (back ? (uintptr_t)c.dy : 0)) % size) return fail("%s: an operand is not aligned to its type", what);
   if (((uintptr_t)c.q_weight | (uintptr_t)c.k_weight) % wsize) return fail("%s: a weight is not aligned to its type", what);
   if ((uintptr_t)c.positions % 4 || (uintptr_t)c.phases % 8) return fail("%s: misaligned positions or phases", what);
   SHLO_TRY(check_in_place(c.x, c.x_token, c.x_head, c.y, c.y_token, c.y_head, c.tokens, c.heads, c.dim, size, what, "x", back ? "dx" : "y"));
@@ -512,7 +513,7 @@ int launch_norm_rope(const NormRopeCall &c, int sms, cudaStream_t st) {
   a.xt = c.x_token; a.xh = c.x_head; a.gt = c.dy_token; a.gh = c.dy_head; a.yt = c.y_token; a.yh = c.y_head;
   a.tokens = c.tokens; a.heads = c.heads; a.q_heads = c.q_heads; a.dim = c.dim; a.rot = c.rot;
   a.eps = c.eps; a.factor = c.factor; a.w_half = c.weight_dtype == kF16;
-  a.partials = sums ? (double *)c.work : nullptr;
+  a.partials = sums ? (double *)c.workspace : nullptr;
   a.lanes_log = 0;
   while (a.lanes_log < 5 && (1 << a.lanes_log) < units) a.lanes_log++;
   // A block's tokens, as long as every SM gets blocks; then its heads are shared among
@@ -563,19 +564,11 @@ using namespace shlo;
 
 extern "C" {
 
-int shlo_norm_rope_noalloc(const void *x, int64_t x_token, int64_t x_head, const int32_t *positions, const int64_t *phases,
-                           const void *q_weight, const void *k_weight, uint8_t weight_dtype, int32_t q_heads, float eps,
-                           void *y, int64_t y_token, int64_t y_head, int64_t tokens, int32_t heads, int32_t dim, int32_t rot,
-                           uint8_t dtype, uint32_t flags, float factor, void *stream) {
+int shlo_norm_rope_noalloc(const shlo_norm_rope_args *args, void *stream) {
+  if (!args) return fail("norm_rope: null arguments");
   Device *dev;
   SHLO_TRY(calling_device(&dev));
-  NormRopeCall c = {};
-  c.x = x; c.x_token = x_token; c.x_head = x_head;
-  c.positions = positions; c.phases = phases;
-  c.q_weight = q_weight; c.k_weight = k_weight; c.weight_dtype = weight_dtype; c.q_heads = q_heads; c.eps = eps;
-  c.y = y; c.y_token = y_token; c.y_head = y_head;
-  c.tokens = tokens; c.heads = heads; c.dim = dim; c.rot = rot; c.dtype = dtype; c.flags = flags; c.factor = factor;
-  return launch_norm_rope(c, dev->sm_count, (cudaStream_t)stream);
+  return launch_norm_rope(*args, false, dev->sm_count, (cudaStream_t)stream);
 }
 
 int shlo_norm_rope_workspace(size_t *bytes) {
@@ -586,25 +579,11 @@ int shlo_norm_rope_workspace(size_t *bytes) {
   return 0;
 }
 
-int shlo_norm_rope_grad_noalloc(const void *x, int64_t x_token, int64_t x_head, const void *dy, int64_t dy_token, int64_t dy_head,
-                                const int32_t *positions, const int64_t *phases, const void *q_weight, const void *k_weight,
-                                uint8_t weight_dtype, int32_t q_heads, float eps, void *dx, int64_t dx_token, int64_t dx_head,
-                                float *dq_weight, float *dk_weight, int64_t tokens, int32_t heads, int32_t dim, int32_t rot,
-                                uint8_t dtype, uint32_t flags, float factor, void *workspace, size_t workspace_bytes, void *stream) {
-  if (!dy && tokens) return fail("norm_rope_grad: null pointer");
+int shlo_norm_rope_grad_noalloc(const shlo_norm_rope_args *args, void *stream) {
+  if (!args) return fail("norm_rope_grad: null arguments");
   Device *dev;
   SHLO_TRY(calling_device(&dev));
-  NormRopeCall c = {};
-  c.x = x; c.x_token = x_token; c.x_head = x_head;
-  c.dy = dy ? dy : x; c.dy_token = dy_token; c.dy_head = dy_head;
-  if (!c.dy) c.dy = "";  // (no tokens: nothing is read)
-  c.positions = positions; c.phases = phases;
-  c.q_weight = q_weight; c.k_weight = k_weight; c.weight_dtype = weight_dtype; c.q_heads = q_heads; c.eps = eps;
-  c.y = dx; c.y_token = dx_token; c.y_head = dx_head;
-  c.dq_weight = dq_weight; c.dk_weight = dk_weight;
-  c.tokens = tokens; c.heads = heads; c.dim = dim; c.rot = rot; c.dtype = dtype; c.flags = flags; c.factor = factor;
-  c.work = workspace; c.work_bytes = workspace_bytes;
-  return launch_norm_rope(c, dev->sm_count, (cudaStream_t)stream);
+  return launch_norm_rope(*args, true, dev->sm_count, (cudaStream_t)stream);
 }
 
 }  // extern "C"

@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 PKG = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 LIB_PATH = os.environ.get("SHLO_CUDA_LIB", os.path.join(PKG, "lib", "libshlo_cuda.so"))
@@ -55,6 +56,12 @@ class KvBatch(ctypes.Structure):
                 ("table_stride", ctypes.c_int64), ("seqs", ctypes.c_int32), ("table_pages", ctypes.c_int32),
                 ("tokens", ctypes.c_int32)]
 
+
+# The descriptors of include/shlo_cuda.h that a call fills anew, in their fields' order (native alignment).
+NORM_ROPE_ARGS = struct.Struct("PqqPPPPPqqPqqPPPNqiiiiffIBB")
+MUL_MAT8_ARGS = struct.Struct("PqPPqPPPqPNqiiBB")
+BEAM_ARGS = struct.Struct("PqPPPPPPNiiiiiB")
+KV_FORK_ARGS = struct.Struct("PPqPPPPqiii")
 
 _lib = None
 
@@ -129,17 +136,14 @@ def load() -> ctypes.CDLL:
     L.shlo_kv_gather_noalloc.argtypes = [pool, p, i64, i32, i32, p, p, i64, p, i64, i64, p, i64, i64, u8, p]
     L.shlo_cuda_device.argtypes = []
     u32, size, sizep = ctypes.c_uint32, ctypes.c_size_t, ctypes.POINTER(ctypes.c_size_t)
-    L.shlo_norm_rope_noalloc.argtypes = [p, i64, i64, p, p, p, p, u8, i32, f32, p, i64, i64, i64, i32, i32, i32, u8, u32, f32, p]
+    packed = ctypes.c_char_p  # (a descriptor's bytes: one conversion a call, where fields as arguments take one each)
+    for name in ("norm_rope", "norm_rope_grad", "mul_mat8", "linear8", "beam_select"):
+        getattr(L, "shlo_%s_noalloc" % name).argtypes = [packed, p]
     L.shlo_norm_rope_workspace.argtypes = [sizep]
-    L.shlo_norm_rope_grad_noalloc.argtypes = [p, i64, i64, p, i64, i64, p, p, p, p, u8, i32, f32, p, i64, i64, p, p, i64, i32,
-                                              i32, i32, u8, u32, f32, p, size, p]
     L.shlo_quantise_rows_noalloc.argtypes = [p, i64, i64, i32, u8, p, i64, p, p]
-    L.shlo_mul_mat8_noalloc.argtypes = [p, i64, p, p, i64, p, p, p, i64, i64, i32, i32, u8, p]
     L.shlo_linear8_workspace.argtypes = [i64, i32, sizep]
-    L.shlo_linear8_noalloc.argtypes = [p, i64, u8, p, i64, p, p, p, i64, i64, i32, i32, u8, p, size, p]
     L.shlo_beam_workspace.argtypes = [i32, i32, i32, i32, sizep]
-    L.shlo_beam_select_noalloc.argtypes = [p, i64, p, p, i32, i32, i32, i32, i32, u8, p, p, p, p, size, p]
-    L.shlo_kv_fork_noalloc.argtypes = [pool, p, i64, p, i32, i32, p, p, i32, p, i64, p, p]
+    L.shlo_kv_fork_noalloc.argtypes = [pool, packed, p]
     L.shlo_kv_attend_workspace.argtypes = [ctypes.POINTER(ctypes.c_size_t)]
     L.shlo_kv_attend_noalloc.argtypes = [pool, batch, p, i64, i64, i32, u8, f32, i32, i32, p, i64, i64, p, p,
                                          ctypes.c_size_t, p]

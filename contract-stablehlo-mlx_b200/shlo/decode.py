@@ -12,12 +12,16 @@ of include/shlo_cuda.h, whose comments say what it computes; errors raise ShloEr
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import numpy as np
 
 from . import mlx as M
 from . import run as Run
-from ._lib import KvBatch, KvPool, ShloError, check, load
+from ._lib import BEAM_ARGS, KV_FORK_ARGS, MUL_MAT8_ARGS, NORM_ROPE_ARGS, KvBatch, KvPool, ShloError, check, load
+
+_UNPACKED = (struct.error, OverflowError)  # a number that a descriptor's field does not hold
+_norm_rope, _mul_mat8, _beam, _fork = NORM_ROPE_ARGS.pack, MUL_MAT8_ARGS.pack, BEAM_ARGS.pack, KV_FORK_ARGS.pack
 
 SCALINGS = {"none": 0, "linear": 1, "base": 2, "ramp": 3, "blend": 4}
 
@@ -95,7 +99,7 @@ def _tables(x, what, at):
 def _workspace(x, at):
     """A workspace's pointer and its bytes."""
     if x is None:
-        return None, 0
+        return 0, 0
     try:
         if x.get_device() != at:
             _elsewhere(x, at)
@@ -227,17 +231,22 @@ def _weights(q_weight, k_weight, q_heads, h, d, what, at):
     """The two weights' pointers and their type."""
     if not 0 <= q_heads <= h:
         raise ShloError("%s: %d query heads of %d" % (what, q_heads, h))
-    code, ptr = _F32, [None, None]
-    for i, w in enumerate((q_weight, k_weight)):
-        if w is None:
-            continue
-        c = _code(w, at)
-        if c != _F16 and c != _F32 or tuple(w.shape) != (d,) or (d > 1 and w.stride()[0] != 1):
-            raise ShloError("%s: a weight is not a contiguous float16 or float32 [%d]" % (what, d))
-        if i and ptr[0] is not None and c != code:
+    code, q, k = _F32, 0, 0
+    if q_weight is not None:
+        code, q = _vector(q_weight, d, what + ": q_weight", at)
+    if k_weight is not None:
+        c, k = _vector(k_weight, d, what + ": k_weight", at)
+        if q and c != code:
             raise ShloError("%s: weights of two types" % what)
-        code, ptr[i] = c, w.data_ptr()
-    return ptr[0], ptr[1], code
+        code = c
+    return q, k, code
+
+
+def _vector(w, d, what, at):
+    c = _code(w, at)
+    if c != _F16 and c != _F32 or w.shape != (d,) or (d > 1 and w.stride()[0] != 1):
+        raise ShloError("%s is not a contiguous float16 or float32 [%d]" % (what, d))
+    return c, w.data_ptr()
 
 
 def norm_rope_noalloc(x, positions, phases, out, *, q_heads, q_weight, k_weight, eps, interleaved=False, factor=1.0,
@@ -254,10 +263,14 @@ def norm_rope_noalloc(x, positions, phases, out, *, q_heads, q_weight, k_weight,
     if _list(positions, _I32, "norm_rope: positions", at) != t:
         raise ShloError("norm_rope: %d positions for %d tokens" % (positions.shape[0], t))
     wq, wk, dw = _weights(q_weight, k_weight, q_heads, h, d, "norm_rope", at)
-    check(lib.shlo_norm_rope_noalloc(x.data_ptr(), xs[0], xs[1], positions.data_ptr(), phases.data_ptr(), wq, wk, dw,
-                                     q_heads, eps, out.data_ptr(), ys[0], ys[1], t, h, d,
-                                     2 * _list(phases, _I64, "norm_rope: phases", at), dt, 1 if interleaved else 0, factor,
-                                     stream))
+    try:
+        if lib.shlo_norm_rope_noalloc(
+                _norm_rope(x.data_ptr(), xs[0], xs[1], positions.data_ptr(), phases.data_ptr(), wq, wk, out.data_ptr(), ys[0],
+                           ys[1], 0, 0, 0, 0, 0, 0, 0, t, h, d, 2 * _list(phases, _I64, "norm_rope: phases", at), q_heads, eps,
+                           factor, 1 if interleaved else 0, dt, dw), stream):
+            check(1)
+    except _UNPACKED as e:
+        raise ShloError("norm_rope: %s" % e) from None
 
 
 def norm_rope_workspace() -> int:
@@ -282,17 +295,22 @@ def norm_rope_grad_noalloc(x, dy, positions, phases, dx, dq_weight=None, dk_weig
     if _list(positions, _I32, "norm_rope_grad: positions", at) != t:
         raise ShloError("norm_rope_grad: %d positions for %d tokens" % (positions.shape[0], t))
     wq, wk, dw = _weights(q_weight, k_weight, q_heads, h, d, "norm_rope_grad", at)
-    sums = [None, None]
+    sums = [0, 0]
     for i, w in enumerate((dq_weight, dk_weight)):
         if w is not None:
-            if _code(w, at) != _F32 or tuple(w.shape) != (d,) or (d > 1 and w.stride()[0] != 1):
+            if _code(w, at) != _F32 or w.shape != (d,) or (d > 1 and w.stride()[0] != 1):
                 raise ShloError("norm_rope_grad: a weight's gradient is not a contiguous float32 [%d]" % d)
             sums[i] = w.data_ptr()
     wp, wn = _workspace(workspace, at)
-    check(lib.shlo_norm_rope_grad_noalloc(x.data_ptr(), xs[0], xs[1], dy.data_ptr(), gs[0], gs[1], positions.data_ptr(),
-                                          phases.data_ptr(), wq, wk, dw, q_heads, eps, dx.data_ptr(), ys[0], ys[1],
-                                          sums[0], sums[1], t, h, d, 2 * _list(phases, _I64, "norm_rope_grad: phases", at),
-                                          dt, 1 if interleaved else 0, factor, wp, wn, stream))
+    try:
+        if lib.shlo_norm_rope_grad_noalloc(
+                _norm_rope(x.data_ptr(), xs[0], xs[1], positions.data_ptr(), phases.data_ptr(), wq, wk, dx.data_ptr(), ys[0],
+                           ys[1], dy.data_ptr(), gs[0], gs[1], sums[0], sums[1], wp, wn, t, h, d,
+                           2 * _list(phases, _I64, "norm_rope_grad: phases", at), q_heads, eps, factor, 1 if interleaved else 0,
+                           dt, dw), stream):
+            check(1)
+    except _UNPACKED as e:
+        raise ShloError("norm_rope_grad: %s" % e) from None
 
 
 # ---- products in 8-bit integers ----
@@ -308,7 +326,7 @@ def _matrix(x, codes, what, at):
 
 
 def _scales(x, n, what, at):
-    if _code(x, at) != _F32 or tuple(x.shape) != (n,) or (n > 1 and x.stride()[0] != 1):
+    if _code(x, at) != _F32 or x.shape != (n,) or (n > 1 and x.stride()[0] != 1):
         raise ShloError("%s is not a contiguous float32 [%d]" % (what, n))
     return x.data_ptr()
 
@@ -327,15 +345,20 @@ def quantise_rows_noalloc(x, q, scale, *, stream=0):
                                          stream))
 
 
-def _product(n, w, w_scale, rows, out, bias, what, at):
+def _product(entry, x, xs, x_scale, r, n, x_dtype, w, w_scale, out, bias, wp, wn, what, at, stream):
     m, nw, ws, _ = _matrix(w, (_I8,), what + ": w", at)
     ro, mo, ys, dt = _matrix(out, (_F16, _F32), what + ": out", at)
-    if nw != n or ro != rows or mo != m:
-        raise ShloError("%s: [%d, %d] by weights [%d, %d] into [%d, %d]" % (what, rows, n, m, nw, ro, mo))
-    if rows > 1 and ys < m:
+    if nw != n or ro != r or mo != m:
+        raise ShloError("%s: [%d, %d] by weights [%d, %d] into [%d, %d]" % (what, r, n, m, nw, ro, mo))
+    if r > 1 and ys < m:
         raise ShloError("%s: rows of out overlap" % what)
-    return (w.data_ptr(), ws, _scales(w_scale, m, what + ": w_scale", at),
-            None if bias is None else _scales(bias, m, what + ": bias", at), out.data_ptr(), ys, rows, n, m, dt)
+    try:
+        if entry(_mul_mat8(x.data_ptr(), xs, x_scale, w.data_ptr(), ws, _scales(w_scale, m, what + ": w_scale", at),
+                           0 if bias is None else _scales(bias, m, what + ": bias", at), out.data_ptr(), ys, wp, wn, r, n, m, dt,
+                           x_dtype), stream):
+            check(1)
+    except _UNPACKED as e:
+        raise ShloError("%s: %s" % (what, e)) from None
 
 
 def mul_mat8_noalloc(x, x_scale, w, w_scale, out, *, bias=None, stream=0):
@@ -344,8 +367,8 @@ def mul_mat8_noalloc(x, x_scale, w, w_scale, out, *, bias=None, stream=0):
     lib = load()
     at = lib.shlo_cuda_device()
     r, n, xs, _ = _matrix(x, (_I8,), "mul_mat8: x", at)
-    check(lib.shlo_mul_mat8_noalloc(x.data_ptr(), xs, _scales(x_scale, r, "mul_mat8: x_scale", at),
-                                    *_product(n, w, w_scale, r, out, bias, "mul_mat8", at), stream))
+    _product(lib.shlo_mul_mat8_noalloc, x, xs, _scales(x_scale, r, "mul_mat8: x_scale", at), r, n, _I8, w, w_scale, out, bias, 0,
+             0, "mul_mat8", at, stream)
 
 
 def linear8_workspace(rows: int, n: int) -> int:
@@ -361,13 +384,13 @@ def linear8_noalloc(x, w, w_scale, out, *, workspace, bias=None, stream=0):
     at = lib.shlo_cuda_device()
     r, n, xs, dt = _matrix(x, (_F16, _F32), "linear8: x", at)
     wp, wn = _workspace(workspace, at)
-    check(lib.shlo_linear8_noalloc(x.data_ptr(), xs, dt, *_product(n, w, w_scale, r, out, bias, "linear8", at), wp, wn, stream))
+    _product(lib.shlo_linear8_noalloc, x, xs, 0, r, n, dt, w, w_scale, out, bias, wp, wn, "linear8", at, stream)
 
 
 # ---- beam search ----
 
 def _grid(x, code, shape, what, at):
-    if _code(x, at) != code or tuple(x.shape) != shape or not x.is_contiguous():
+    if _code(x, at) != code or x.shape != shape or not x.is_contiguous():
         raise ShloError("%s is not a contiguous %s [%d, %d]" % ((what, "float32" if code == _F32 else "int32") + shape))
     return x.data_ptr()
 
@@ -391,12 +414,17 @@ def beam_select_noalloc(logits, scores, next_scores, parents, tokens, *, workspa
     if rows != seqs * beams:
         raise ShloError("beam_select: %d rows of logits for %d sequences of %d beams" % (rows, seqs, beams))
     wp, wn = _workspace(workspace, at)
-    check(lib.shlo_beam_select_noalloc(
-        logits.data_ptr(), stride, _grid(scores, _F32, (seqs, beams), "beam_select: scores", at),
-        None if ended is None else _grid(ended, _I32, (seqs, beams), "beam_select: ended", at), end_token, seqs, beams, keep,
-        vocab, dt, _grid(next_scores, _F32, (seqs, keep), "beam_select: next_scores", at),
-        _grid(parents, _I32, (seqs, keep), "beam_select: parents", at),
-        _grid(tokens, _I32, (seqs, keep), "beam_select: tokens", at), wp, wn, stream))
+    try:
+        if lib.shlo_beam_select_noalloc(
+                _beam(logits.data_ptr(), stride, _grid(scores, _F32, (seqs, beams), "beam_select: scores", at),
+                      0 if ended is None else _grid(ended, _I32, (seqs, beams), "beam_select: ended", at),
+                      _grid(next_scores, _F32, (seqs, keep), "beam_select: next_scores", at),
+                      _grid(parents, _I32, (seqs, keep), "beam_select: parents", at),
+                      _grid(tokens, _I32, (seqs, keep), "beam_select: tokens", at), wp, wn, seqs, beams, keep, vocab, end_token, dt),
+                stream):
+            check(1)
+    except _UNPACKED as e:
+        raise ShloError("beam_select: %s" % e) from None
 
 
 def fork_noalloc(pool: Pool, tables, lens, parents, fresh, out_tables, out_lens, *, stream=0):
@@ -418,8 +446,10 @@ def fork_noalloc(pool: Pool, tables, lens, parents, fresh, out_tables, out_lens,
                         % (rows, news, width))
     if news > 1 and ostride < width:
         raise ShloError("kv_fork: rows of out_tables overlap")
-    check(lib.shlo_kv_fork_noalloc(pool.c, tables.data_ptr(), stride, lens.data_ptr(), rows, width, parents.data_ptr(),
-                                   fresh.data_ptr(), news, out_tables.data_ptr(), ostride, out_lens.data_ptr(), stream))
+    if lib.shlo_kv_fork_noalloc(
+            pool.c, _fork(tables.data_ptr(), lens.data_ptr(), stride, parents.data_ptr(), fresh.data_ptr(), out_tables.data_ptr(),
+                          out_lens.data_ptr(), ostride, rows, news, width), stream):
+        check(1)
 
 
 # ---- on arrays (mlx.Arr), in the library's own memory ----

@@ -145,6 +145,8 @@ class Decoder:
         cfg = self.cfg
         if not cfg.vocab:
             raise ShloError("decoder: search needs a vocabulary")
+        if len(prompt) == 0 or not all(0 <= t < cfg.vocab for t in prompt):
+            raise ShloError("decoder: a prompt is one token or more of a vocabulary of %d" % cfg.vocab)
         s, y = self.start(self.embed[np.asarray(prompt)])
         rows, texts, scores, y = [s], [[]], np.zeros((1, 1), np.float32), y[-1:]
         ended = np.zeros((1, 1), np.int32)

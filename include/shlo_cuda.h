@@ -226,23 +226,37 @@ int shlo_rope_noalloc(const void *x, int64_t x_token, int64_t x_head, const int3
    y = turn(n w), n = x / sqrt(mean of x^2 over the head's dim values + eps), the
    turn shlo_rope_noalloc's (flags: 1 alone). The first q_heads heads have the
    weight q_weight [dim], the others k_weight [dim] (float16 or float32,
-   `weight_dtype`; NULL: ones). dim up to 512; y as shlo_rope_noalloc's. */
-int shlo_norm_rope_noalloc(const void *x, int64_t x_token, int64_t x_head, const int32_t *positions, const int64_t *phases,
-                           const void *q_weight, const void *k_weight, uint8_t weight_dtype, int32_t q_heads, float eps,
-                           void *y, int64_t y_token, int64_t y_head, int64_t tokens, int32_t heads, int32_t dim, int32_t rot,
-                           uint8_t dtype, uint32_t flags, float factor, void *stream);
+   `weight_dtype`; NULL: ones). dim up to 512; y as shlo_rope_noalloc's. Strides
+   are in values. */
+typedef struct {
+	const void *x;
+	int64_t x_token, x_head;
+	const int32_t *positions;
+	const int64_t *phases;
+	const void *q_weight, *k_weight;
+	void *y; /* the gradient: dx */
+	int64_t y_token, y_head;
+	/* Of the gradient alone: of y, and of the weights (float32 [dim], overwritten; NULL: not asked for). */
+	const void *dy;
+	int64_t dy_token, dy_head;
+	float *dq_weight, *dk_weight;
+	void *workspace;
+	size_t workspace_bytes;
+	int64_t tokens;
+	int32_t heads, dim, rot, q_heads;
+	float eps, factor;
+	uint32_t flags;
+	uint8_t dtype, weight_dtype;
+} shlo_norm_rope_args;
+int shlo_norm_rope_noalloc(const shlo_norm_rope_args *args, void *stream);
 /* The bytes of workspace that its gradient needs on the current device. */
 int shlo_norm_rope_workspace(size_t *bytes);
 /* Its gradient: dx of x's type from dy of the same type (dx may be x or dy itself;
-   else it shares no value with them), and the weights' (float32 [dim], overwritten;
-   NULL: not asked for), sums over all tokens and their heads. The workspace holds
-   nothing between calls (NULL without the weights' gradients); calls that may run
-   at once have one each. The same call gives the same bits. */
-int shlo_norm_rope_grad_noalloc(const void *x, int64_t x_token, int64_t x_head, const void *dy, int64_t dy_token, int64_t dy_head,
-                                const int32_t *positions, const int64_t *phases, const void *q_weight, const void *k_weight,
-                                uint8_t weight_dtype, int32_t q_heads, float eps, void *dx, int64_t dx_token, int64_t dx_head,
-                                float *dq_weight, float *dk_weight, int64_t tokens, int32_t heads, int32_t dim, int32_t rot,
-                                uint8_t dtype, uint32_t flags, float factor, void *workspace, size_t workspace_bytes, void *stream);
+   else it shares no value with them), and the weights', sums over all tokens and
+   their heads. The workspace (8-byte boundary) holds nothing between calls (NULL
+   without the weights' gradients); calls that may run at once have one each. The
+   same call gives the same bits. */
+int shlo_norm_rope_grad_noalloc(const shlo_norm_rope_args *args, void *stream);
 
 /* Products in 8-bit integers with a scale for each row of both sides. Rows of n
    float16 or float32 values (x_row values apart) as q [rows][n] (q_row bytes apart)
@@ -254,21 +268,34 @@ int shlo_quantise_rows_noalloc(const void *x, int64_t x_row, int64_t rows, int32
                                float *scale, void *stream);
 /* y[r][c] = (sum over i < n of x[r][i] w[c][i]) x_scale[r] w_scale[c] + bias[c], for
    `rows` rows and m channels; y of `dtype`, y_row values apart, bias float32 [m] or
-   NULL. The sum is exact (32-bit integers; n up to 131071). x and w begin on
-   16-byte boundaries and have rows a multiple of 16 bytes apart; what lies between
-   rows is not read. y shares no memory with the operands. */
-int shlo_mul_mat8_noalloc(const int8_t *x, int64_t x_row, const float *x_scale, const int8_t *w, int64_t w_row, const float *w_scale,
-                          const float *bias, void *y, int64_t y_row, int64_t rows, int32_t n, int32_t m, uint8_t dtype, void *stream);
-/* Both: activations of `x_dtype`, rounded row by row into the workspace (begins on a
+   NULL. The sum is exact (32-bit integers; n up to 131071). w begins on a 16-byte
+   boundary and has rows a multiple of 16 bytes apart; what lies between rows is not
+   read. y shares no memory with the operands. */
+typedef struct {
+	const void *x;
+	int64_t x_row; /* in values */
+	const float *x_scale;
+	const int8_t *w;
+	int64_t w_row; /* in bytes */
+	const float *w_scale, *bias;
+	void *y;
+	int64_t y_row;
+	void *workspace;
+	size_t workspace_bytes;
+	int64_t rows;
+	int32_t n, m;
+	uint8_t dtype, x_dtype;
+} shlo_mul_mat8_args;
+/* Of x in int8 with its scales, laid out as w is (no workspace; x_dtype is not read). */
+int shlo_mul_mat8_noalloc(const shlo_mul_mat8_args *args, void *stream);
+/* Of activations of `x_dtype`, rounded row by row into the workspace (begins on a
    16-byte boundary; it holds nothing between calls; calls that may run at once have
-   one each), against weights in 8 bits. */
+   one each; x_scale is not read). */
 int shlo_linear8_workspace(int64_t rows, int32_t n, size_t *bytes);
-int shlo_linear8_noalloc(const void *x, int64_t x_row, uint8_t x_dtype, const int8_t *w, int64_t w_row, const float *w_scale,
-                         const float *bias, void *y, int64_t y_row, int64_t rows, int32_t n, int32_t m, uint8_t y_dtype,
-                         void *workspace, size_t workspace_bytes, void *stream);
+int shlo_linear8_noalloc(const shlo_mul_mat8_args *args, void *stream);
 
 /* Beam search's selection. Row seq * beams + b of the logits [seqs * beams][vocab]
-   (row values apart, float16 or float32) is beam b's of sequence seq; the beam goes
+   (`row` values apart, float16 or float32) is beam b's of sequence seq; the beam goes
    on with token t at scores[seq][b] + logit[t] - log(sum of e^logit). Of every
    sequence the `keep` best in descending order (of equal ones the lowest beam, then
    the lowest token first): their scores into next, the rows that they continue into
@@ -278,10 +305,20 @@ int shlo_linear8_noalloc(const void *x, int64_t x_row, uint8_t x_dtype, const in
    `keep` is there, the rest has score -inf, parent -1 and token -1. Up to 64 beams
    and 64 kept, a vocabulary of up to 2^20. The workspace (8-byte boundary) holds
    nothing between calls; calls that may run at once have one each. */
+typedef struct {
+	const void *logits;
+	int64_t row;
+	const float *scores;
+	const int32_t *ended;
+	float *next;
+	int32_t *parents, *tokens;
+	void *workspace;
+	size_t workspace_bytes;
+	int32_t seqs, beams, keep, vocab, end_token;
+	uint8_t dtype;
+} shlo_beam_args;
 int shlo_beam_workspace(int32_t seqs, int32_t beams, int32_t keep, int32_t vocab, size_t *bytes);
-int shlo_beam_select_noalloc(const void *logits, int64_t row, const float *scores, const int32_t *ended, int32_t end_token,
-                             int32_t seqs, int32_t beams, int32_t keep, int32_t vocab, uint8_t dtype, float *next,
-                             int32_t *parents, int32_t *tokens, void *workspace, size_t workspace_bytes, void *stream);
+int shlo_beam_select_noalloc(const shlo_beam_args *args, void *stream);
 
 /* A paged cache: `pages` pages of `page_tokens` tokens (16, 32, 64, 128 or 256)
    for `heads` key/value heads of `head_dim` values (a multiple of 16, up to
@@ -331,9 +368,15 @@ int shlo_kv_gather_noalloc(const shlo_kv_pool *pool, const int32_t *tables, int6
    page. fresh[r] is not read otherwise. Entries behind a row's last page become -1.
    out_tables and out_lens share no memory with tables and lens. A host that keeps
    one table for several caches makes the call for each of them. */
-int shlo_kv_fork_noalloc(const shlo_kv_pool *pool, const int32_t *tables, int64_t table_stride, const int32_t *lens, int32_t rows,
-                         int32_t table_pages, const int32_t *parents, const int32_t *fresh, int32_t news, int32_t *out_tables,
-                         int64_t out_stride, int32_t *out_lens, void *stream);
+typedef struct {
+	const int32_t *tables, *lens; /* [rows][table_pages], table_stride apart; [rows] */
+	int64_t table_stride;
+	const int32_t *parents, *fresh; /* [news] */
+	int32_t *out_tables, *out_lens; /* [news][table_pages], out_stride apart; [news] */
+	int64_t out_stride;
+	int32_t rows, news, table_pages;
+} shlo_kv_fork_args;
+int shlo_kv_fork_noalloc(const shlo_kv_pool *pool, const shlo_kv_fork_args *args, void *stream);
 /* The device that is current in CUDA on this thread (-2: none; -1 is how many
    libraries name host memory). */
 int shlo_cuda_device(void);

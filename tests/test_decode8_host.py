@@ -101,6 +101,14 @@ def test_refusals(calls, at, change):
     assert calls == ENTRIES[:at]
 
 
+def test_numbers_that_no_field_holds(calls):
+    t = operands()
+    for end in (1 << 40, -1 << 31 << 1):
+        with pytest.raises(ShloError, match="beam_select"):
+            Dc.beam_select_noalloc(t["z"], t["scores"], t["next"], t["parents"], t["tokens"], workspace=t["work"], end_token=end)
+    assert calls == []
+
+
 def test_workspace_sizes():
     assert Dc.linear8_workspace(3, 5) >= 3 * 16 + 3 * 4
     assert Dc.beam_workspace(2, 4, 8, 50000) >= 2 * 4 * 8 * 8
@@ -117,3 +125,29 @@ def test_the_oracles_ties():
     """Halves of a step go to the even whole number."""
     q, s = O8.quantise(np.array([[127.0, 0.5, 1.5, 2.5, -0.5, -1.5, 63.5, 62.5]], np.float32))
     assert q.tolist() == [[127, 0, 2, 2, 0, -2, 64, 62]] and s[0] == 1.0
+
+
+def test_descriptors_are_the_headers(tmp_path):
+    """The packed descriptors against the C compiler's layout of include/shlo_cuda.h."""
+    import os
+    import subprocess
+    src = tmp_path / "sizes.c"
+    src.write_text('#include <stdio.h>\n#include "shlo_cuda.h"\nint main(void) {\n'
+                   '  printf("%zu %zu %zu %zu\\n", offsetof(shlo_norm_rope_args, weight_dtype) + 1, offsetof(shlo_mul_mat8_args, x_dtype) + 1,'
+                   ' offsetof(shlo_beam_args, dtype) + 1, offsetof(shlo_kv_fork_args, table_pages) + 4);\n'
+                   '  printf("%zu %zu %zu\\n", offsetof(shlo_norm_rope_args, tokens), offsetof(shlo_mul_mat8_args, rows),'
+                   ' offsetof(shlo_beam_args, seqs));\n  return 0;\n}\n')
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    subprocess.run(["gcc", "-I", include, str(src), "-o", str(tmp_path / "sizes")], check=True)
+    ends, middles = subprocess.run([str(tmp_path / "sizes")], check=True, capture_output=True, text=True).stdout.splitlines()
+    packed = (_lib.NORM_ROPE_ARGS, _lib.MUL_MAT8_ARGS, _lib.BEAM_ARGS, _lib.KV_FORK_ARGS)
+    assert [int(v) for v in ends.split()] == [a.size for a in packed]
+    assert [int(v) for v in middles.split()] == [_lib.struct.calcsize(f) for f in ("PqqPPPPPqqPqqPPPN", "PqPPqPPPqPN", "PqPPPPPPN")]
+
+
+def test_null_arguments_are_errors():
+    L = _lib.load()
+    for name in ("norm_rope", "norm_rope_grad", "mul_mat8", "linear8", "beam_select"):
+        assert getattr(L, "shlo_%s_noalloc" % name)(None, None) != 0
+        assert "null" in L.shlo_last_error().decode()
+    assert L.shlo_kv_fork_noalloc(None, None, None) != 0 and "null" in L.shlo_last_error().decode()

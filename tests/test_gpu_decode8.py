@@ -192,6 +192,45 @@ def test_norm_rope_far_values_and_absent_weights():
     assert bad.tobytes() == out.tobytes()
 
 
+def test_norm_rope_refusals():
+    x, pos = torch.zeros(3, 4, 16, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    phases, w = torch.zeros(8, dtype=torch.int64, device="cuda"), torch.ones(16, device="cuda")
+    kw = dict(q_heads=2, q_weight=w, k_weight=w, eps=1e-6)
+    wide = torch.zeros(3, 4, 600, device="cuda")
+    for args, change, text in (((x, pos, phases, x[:, :1].expand(3, 4, 16)), {}, "overlap"), ((x, pos, phases, torch.empty_like(x)[:1].expand(3, 4, 16)), {}, "overlap"),
+                               ((x, pos, phases, torch.empty_like(x)), dict(eps=0.0), "eps"), ((x, pos, phases, torch.empty_like(x)), dict(eps=float("nan")), "eps"),
+                               ((wide, pos, phases, torch.empty_like(wide)), dict(q_weight=None, k_weight=None), "600"),
+                               ((x[..., :8], pos, phases, torch.empty_like(x[..., :8])), dict(q_weight=w[:8], k_weight=w[:8]), "turned"),
+                               ((x[:2], pos[:2], phases, x[1:]), {}, "overlap")):
+        with pytest.raises(ShloError, match=text):
+            Dc.norm_rope_noalloc(*args, **dict(kw, **change))
+    dx, dw = torch.empty_like(x), torch.empty(2, 16, device="cuda")
+    for bad in (None, work(8), work(Dc.norm_rope_workspace() + 8)[4:]):
+        with pytest.raises(ShloError, match="workspace"):
+            Dc.norm_rope_grad_noalloc(x, x, pos, phases, dx, dw[0], dw[1], workspace=bad, **kw)
+
+
+def test_norm_rope_broadcast_operands():
+    """One head's values for all of them, one token's gradient for all: strides of 0 are read as they are."""
+    rng = np.random.default_rng(2)
+    T, H, D, R = 6, 4, 32, 32
+    phases, freqs = plan(R)
+    x, dy = cuda(rng.standard_normal((T, 1, D)).astype(np.float32)).expand(T, H, D), cuda(rng.standard_normal((1, H, D)).astype(np.float32)).expand(T, H, D)
+    pos = np.arange(T, dtype=np.int32)
+    wq, wk = (1 + 0.3 * rng.standard_normal((2, D))).astype(np.float32)
+    kw = dict(q_heads=3, q_weight=cuda(wq), k_weight=cuda(wk), eps=1e-6, stream=stream())
+    y, dx, dw = torch.empty(T, H, D, device="cuda"), torch.empty(T, H, D, device="cuda"), torch.empty(2, D, device="cuda")
+    Dc.norm_rope_noalloc(x, cuda(pos), cuda(phases), y, **kw)
+    Dc.norm_rope_grad_noalloc(x, dy, cuda(pos), cuda(phases), dx, dw[0], dw[1], workspace=work(Dc.norm_rope_workspace()), **kw)
+    xn, gn, eps = x.cpu().numpy(), dy.cpu().numpy(), np.float64(np.float32(1e-6))
+    want, mag = O8.norm_rope(xn, pos, freqs, wq, wk, 3, eps)
+    assert np.all(np.abs(y.cpu().numpy() - want) <= 2.0 ** -19 * mag)
+    want, mag, dq, dk, mq, mk = O8.norm_rope_grad(xn, gn, pos, freqs, wq, wk, 3, eps)
+    assert np.all(np.abs(dx.cpu().numpy() - want) <= 2.0 ** -18 * mag)
+    got = dw.cpu().numpy()
+    assert np.all(np.abs(got[0] - dq) <= 2.0 ** -16 * mq) and np.all(np.abs(got[1] - dk) <= 2.0 ** -16 * mk)
+
+
 def test_norm_rope_no_tokens():
     dw = torch.full((2, 8), 3.0, device="cuda")
     e = torch.empty(0, 2, 8, device="cuda")
@@ -496,3 +535,172 @@ def test_fork_refusals_and_no_rows():
         Dc.fork_noalloc(pool, t, l, i32(3), i32(2), i32(3, 2), i32(3))
     with pytest.raises(ShloError, match="kv_fork"):
         Dc.fork_noalloc(pool, t, l, i32(3), i32(3), i32(3, 3), i32(3))
+
+
+# --------------------------------------------------------------- together ----
+
+class Step:
+    """A decoder layer's step with beams, as a serving program runs it: projections in 8 bits, norm and rotation, the
+    cache, attention, the output over the vocabulary, selection, forks."""
+
+    def __init__(self, seed, seqs=2, beams=3, d=96, hq=4, hk=2, dim=32, vocab=777, page=16, length=21):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        rn = lambda *s: torch.randn(*s, device="cuda", generator=g)  # noqa: E731
+        self.seqs, self.beams, self.hq, self.hk, self.dim, rows = seqs, beams, hq, hk, dim, seqs * beams
+        i32 = lambda a: torch.tensor(a, dtype=torch.int32, device="cuda")  # noqa: E731
+        self.w = {}
+        for name, m, n in (("qkv", (hq + 2 * hk) * dim, d), ("o", d, hq * dim), ("head", vocab, d)):
+            pad = -(-n // 16) * 16
+            q, s = torch.zeros(m, pad, dtype=torch.int8, device="cuda")[:, :n], torch.empty(m, device="cuda")
+            Dc.quantise_rows_noalloc(rn(m, n) * n ** -0.5, q, s, stream=stream())
+            self.w[name] = q, s
+        self.wq, self.wk = 1 + 0.1 * rn(dim), 1 + 0.1 * rn(dim)
+        self.phases = cuda(Dc.rope_phases(dim)[0])
+        pages = rows * 4 + rows
+        shape = (pages, hk, page, dim)
+        self.pool = Dc.Pool(*[torch.randint(-127, 128, shape, dtype=torch.int8, device="cuda", generator=g) for _ in range(2)],
+                            *[torch.rand(pages, hk, device="cuda", generator=g) * 0.02 + 0.01 for _ in range(2)])
+        self.tables = torch.arange(rows * 4, dtype=torch.int32, device="cuda").view(rows, 4)
+        self.fresh = torch.arange(rows * 4, pages, dtype=torch.int32, device="cuda")
+        self.lens, self.starts = i32([length] * rows), torch.arange(rows + 1, dtype=torch.int32, device="cuda")
+        self.pos = i32([length - 1] * rows)
+        self.x, self.scores = rn(rows, d), -torch.rand(seqs, beams, device="cuda", generator=g)
+        self.space = [work(Dc.linear8_workspace(rows, max(d, hq * dim))), torch.zeros(Dc.attend_workspace(), dtype=torch.uint8, device="cuda"),
+                      work(Dc.beam_workspace(seqs, beams, beams, vocab))]
+        self.qkv, self.qk = torch.empty(rows, (hq + 2 * hk) * dim, device="cuda"), torch.empty(rows, hq + hk, dim, device="cuda")
+        self.att, self.h, self.z = torch.empty(rows, hq, dim, device="cuda"), torch.empty(rows, d, device="cuda"), torch.empty(rows, vocab, device="cuda")
+        self.next, self.parents, self.tokens = torch.empty(seqs, beams, device="cuda"), i32([[0] * beams] * seqs), i32([[0] * beams] * seqs)
+        self.tables2, self.lens2 = torch.empty_like(self.tables), torch.empty_like(self.lens)
+
+    def run(self):
+        st, rows = stream(), self.x.shape[0]
+        Dc.linear8_noalloc(self.x, *self.w["qkv"], self.qkv, workspace=self.space[0], stream=st)
+        heads = self.qkv.view(rows, self.hq + 2 * self.hk, self.dim)
+        both = self.hq + self.hk
+        Dc.norm_rope_noalloc(heads[:, :both], self.pos, self.phases, self.qk, q_heads=self.hq, q_weight=self.wq, k_weight=self.wk, eps=1e-6, stream=st)
+        Dc.append_noalloc(self.pool, self.qk[:, self.hq:], heads[:, both:], self.starts, self.lens, self.tables, stream=st)
+        Dc.attend_noalloc(self.pool, self.qk[:, :self.hq], self.starts, self.lens, self.tables, self.att, workspace=self.space[1], scale=self.dim ** -0.5, stream=st)
+        Dc.linear8_noalloc(self.att.view(rows, -1), *self.w["o"], self.h, workspace=self.space[0], stream=st)
+        Dc.linear8_noalloc(self.h, *self.w["head"], self.z, workspace=self.space[0], stream=st)
+        Dc.beam_select_noalloc(self.z, self.scores, self.next, self.parents, self.tokens, workspace=self.space[2], stream=st)
+        Dc.fork_noalloc(self.pool, self.tables, self.lens, self.parents, self.fresh, self.tables2, self.lens2, stream=st)
+
+    def result(self):
+        return [a.cpu().numpy().copy() for a in (self.qk, self.att, self.z, self.next, self.parents, self.tokens, self.tables2, self.lens2, *self.pool.keep)]
+
+
+def plain_step(s):
+    """The same by the oracles, from the device's inputs; each product from the device's own operands, so that a
+    rounding to 8 bits that falls the other way does not spread."""
+    rows, both = s.x.shape[0], s.hq + s.hk
+    cache = O.Cache(s.pool.c.pages, s.hk, s.pool.c.page_tokens, s.dim)
+    cache.k, cache.v, cache.ks, cache.vs = (a.cpu().numpy().copy() for a in s.pool.keep)
+
+    def product(x, name):
+        q, sc = O8.quantise(x)
+        return O8.mul_mat8(q, sc, s.w[name][0].cpu().numpy(), s.w[name][1].cpu().numpy())
+    qkv = product(s.x.cpu().numpy(), "qkv")
+    lens, tables = s.lens.cpu().numpy(), s.tables.cpu().numpy()
+    yield qkv
+    heads = qkv.reshape(rows, both + s.hk, s.dim)
+    qk, mag = O8.norm_rope(heads[:, :both], s.pos.cpu().numpy(), 10000.0 ** (-2.0 * np.arange(s.dim // 2) / s.dim), s.wq.cpu().numpy(), s.wk.cpu().numpy(),
+                           s.hq, np.float64(np.float32(1e-6)))
+    yield qk, 2.0 ** -19 * mag
+    dev = s.qk.cpu().numpy()
+    O.append(cache, dev[:, s.hq:], heads[:, both:], s.starts.cpu().numpy(), lens, tables)
+    att, _, _, vmax = O.attend(cache, dev[:, :s.hq], s.starts.cpu().numpy(), lens, tables, s.dim ** -0.5)
+    yield att, 2.0 ** -15 * vmax[..., None]
+    h = product(s.att.cpu().numpy().reshape(rows, -1), "o")
+    yield product(h, "head")
+    yield O8.beam(s.z.cpu().numpy(), s.scores.cpu().numpy(), s.beams)
+    parents = s.parents.cpu().numpy().reshape(-1)
+    yield (*O8.fork(cache, tables, lens, parents, s.fresh.cpu().numpy()), cache)
+
+
+def test_a_step_of_all_together():
+    s = Step(1)
+    want = plain_step(s)
+    qkv = next(want)
+    s.run()
+    assert s.qkv.cpu().numpy().tobytes() == qkv.tobytes()
+    for got in (s.qk, s.att):
+        w, tol = next(want)
+        assert np.all(np.abs(got.cpu().numpy() - w) <= tol)
+    assert s.z.cpu().numpy().tobytes() == next(want).tobytes()
+    same([a.cpu().numpy() for a in (s.next, s.parents, s.tokens)], next(want))
+    tables, lens, cache = next(want)
+    assert np.array_equal(s.tables2.cpu().numpy(), tables) and np.array_equal(s.lens2.cpu().numpy(), lens)
+    for got, w in zip(s.pool.keep, (cache.k, cache.v, cache.ks, cache.vs)):
+        assert np.array_equal(got.cpu().numpy(), w)
+
+
+def test_a_step_captured_and_two_at_once():
+    """Captured and replayed with other inputs, and two of them on streams of their own at the same time, each with its
+    own workspaces: the bits of one after the other."""
+    steps, fresh = [Step(2, vocab=5001), Step(3, seqs=5, length=37)], []
+    for s in steps:
+        kept = [a.clone() for a in s.pool.keep]
+        s.run()
+        fresh.append(s.result())
+        for a, b in zip(s.pool.keep, kept):
+            a.copy_(b)
+        s.kept = kept
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in steps]
+    graphs = []
+    for s, st in zip(steps, streams):
+        with torch.cuda.stream(st):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=st):
+                s.run()
+            graphs.append(g)
+    for turn in range(3):
+        for s, st, g in zip(steps, streams, graphs):
+            with torch.cuda.stream(st):
+                for a, b in zip(s.pool.keep, s.kept):
+                    a.copy_(b)
+                g.replay()
+        torch.cuda.synchronize()
+        for s, want in zip(steps, fresh):
+            assert all(a.tobytes() == b.tobytes() for a, b in zip(s.result(), want))
+    other = Step(4)  # a captured call reads what lies in its operands when it is replayed
+    steps[0].x.copy_(other.x)
+    for a, b in zip(steps[0].pool.keep, steps[0].kept):
+        a.copy_(b)
+    with torch.cuda.stream(streams[0]):
+        graphs[0].replay()
+    torch.cuda.synchronize()
+    got = steps[0].result()
+    for a, b in zip(steps[0].pool.keep, steps[0].kept):
+        a.copy_(b)
+    steps[0].run()
+    assert all(a.tobytes() == b.tobytes() for a, b in zip(got, steps[0].result()))
+    del graphs
+
+
+def test_host_threads_at_once():
+    import threading
+    steps, want, errors = [Step(5), Step(6, seqs=4)], [], []
+    for s in steps:
+        s.run()
+        want.append(s.result()[:6])
+    torch.cuda.synchronize()
+
+    def go(s, w):
+        try:
+            st = torch.cuda.Stream()
+            with torch.cuda.stream(st):
+                for _ in range(20):
+                    s.run()
+                st.synchronize()
+            # (the cache's tail pages take the same tokens again, which changes nothing)
+            if not all(a.tobytes() == b.tobytes() for a, b in zip(s.result()[:6], w)):
+                errors.append("bits")
+        except Exception as e:  # noqa: BLE001
+            errors.append(repr(e))
+    threads = [threading.Thread(target=go, args=a) for a in zip(steps, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert errors == []

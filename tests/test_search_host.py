@@ -125,6 +125,9 @@ def test_search_that_fails_frees_its_pages(decoder):
     with pytest.raises(ShloError, match="layer"):
         decoder.search([1, 2, 3], 3, 9)
     assert sorted(decoder.free) == list(range(40)) and not any(decoder.shared.values())
+    for prompt in ([], [11], [3, -1]):
+        with pytest.raises(ShloError, match="prompt"):
+            decoder.search(prompt, 3, 9)
     decoder.cfg = Dd.Config()
     with pytest.raises(ShloError, match="vocabulary"):
         decoder.search([1], 2, 3)
