@@ -11,6 +11,7 @@
 // float16 (101 MB) 24 us, 4.2 TB/s; 24 rows 3.1 us, a launch and four waits. The product
 // of linear8 begins while they are rounded, with its weights.
 #include <algorithm>
+#include <type_traits>
 
 #include "decode.cuh"
 
@@ -177,6 +178,195 @@ void launch_rows(const T *x, int64_t x_row, int64_t rows, int n, int8_t *q, int6
   else pick(std::integral_constant<int, 4>());
 }
 
+// Few rows: a warp a channel, whose bytes go through its lanes 16 at a time, against
+// the rows' in shared memory; each block rounds the rows for itself (T float16 or
+// float32; int8: they are rounded), so that a step of one sequence is one launch. The
+// first bytes of the weights are asked for before that. 1 row of 512 to 768 2.6 us, of
+// 4096 to 4096 (16.8 MB from HBM) 6.4, to 12288 11.7 (4.3 TB/s with launch and ramp).
+constexpr int kFewThreads = 256, kFewBytes = 64 * 1024;
+
+template <typename T, int R, typename Y>
+__global__ void __launch_bounds__(kFewThreads, 4) k_linear8_few(const Mm8Call c, int row_bytes, bool after_rows) {
+  constexpr int U = 4, WARPS = kFewThreads / 32;
+  constexpr bool ROUNDS = !std::is_same<T, int8_t>::value;
+  extern __shared__ uint4 xs[];  // [R][row_bytes]: zeros behind n
+  __shared__ uint32_t tops[WARPS];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, units = row_bytes / 16, row_units = row_bytes / 16;
+  const int full = c.n / 16;
+  auto weights = [&](int ch, int u) -> uint4 {
+    const int8_t *const w = c.w + (int64_t)ch * c.w_row + (int64_t)u * 16;
+    if (u < full) return __ldg(reinterpret_cast<const uint4 *>(w));
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (u == full)
+      for (int i = 0; i < c.n % 16; i++) reinterpret_cast<int8_t *>(&v)[i] = w[i];
+    return v;
+  };
+  const int step = gridDim.x * WARPS;
+  int ch = blockIdx.x * WARPS + warp;
+  uint4 w[U];
+#pragma unroll
+  for (int i = 0; i < U; i++)
+    if (ch < c.m && i * 32 + lane < units) w[i] = weights(ch, i * 32 + lane);
+
+  // The rows: a part of the threads each, up to KEEP vectors a thread on their way at once.
+  float scale = 0.0f;  // lane r: row r's
+  if constexpr (ROUNDS) {
+    constexpr int V = 16 / sizeof(T), TPR = kFewThreads / R, KEEP = 4;
+    const bool wide = (uintptr_t)c.x % 16 == 0 && (c.rows == 1 || c.x_row * (int64_t)sizeof(T) % 16 == 0);
+    const int r = threadIdx.x / TPR, t = threadIdx.x % TPR, vecs = r < c.rows ? (c.n + V - 1) / V : 0;
+    const T *const x = static_cast<const T *>(c.x) + (r < c.rows ? r : 0) * c.x_row;
+    auto load = [&](int i, T (&v)[V]) {
+      if (wide && i * V + V <= c.n) {
+        *reinterpret_cast<uint4 *>(v) = *reinterpret_cast<const uint4 *>(x + (int64_t)i * V);
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; j++) v[j] = i * V + j < c.n ? x[(int64_t)i * V + j] : T(0.0f);
+      }
+    };
+    T v[KEEP][V];
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < KEEP; k++)
+      if (t + k * TPR < vecs) load(t + k * TPR, v[k]);
+#pragma unroll
+    for (int k = 0; k < KEEP; k++)
+      if (t + k * TPR < vecs) top = max(top, top_bits(v[k]));
+    for (int i = t + KEEP * TPR; i < vecs; i += TPR) {
+      T u[V];
+      load(i, u);
+      top = max(top, top_bits(u));
+    }
+    top = __reduce_max_sync(~0u, top);
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
+    auto top_of = [&](int row) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < WARPS / R; i++) m = max(m, tops[row * (WARPS / R) + i]);
+      return m;
+    };
+    if (lane < R) {
+      const uint32_t m = top_of(lane);
+      scale = m < 0x7f800000u ? __uint_as_float(m) / 127.0f : __uint_as_float(0x7fc00000u);
+    }
+    top = top_of(r);
+    const float by = 127.0f / __uint_as_float(top);
+    const bool any = top > 0 && top < 0x7f800000u;
+    auto store = [&](int i, const T (&u)[V]) {
+      alignas(8) uint8_t b[V];
+#pragma unroll
+      for (int j = 0; j < V; j++) b[j] = 0;
+      if (any && i < vecs) quantise(u, __uint_as_float(top), by, b);
+      *reinterpret_cast<typename Raw<V>::T *>(reinterpret_cast<uint8_t *>(xs) + r * row_bytes + i * V) = *reinterpret_cast<const typename Raw<V>::T *>(b);
+    };
+#pragma unroll
+    for (int k = 0; k < KEEP; k++)
+      if (t + k * TPR < row_bytes / V) store(t + k * TPR, v[k]);
+    for (int i = t + KEEP * TPR; i < row_bytes / V; i += TPR) {
+      T u[V];
+      if (i < vecs) load(i, u);
+      store(i, u);
+    }
+  } else {
+    if (after_rows) cudaGridDependencySynchronize();
+    if (lane < c.rows) scale = c.x_scale[lane];
+    for (int i = threadIdx.x; i < R * units; i += kFewThreads) {
+      const int r = i / units, u = i - r * units;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      const int8_t *const x = static_cast<const int8_t *>(c.x) + r * c.x_row + (int64_t)u * 16;
+      if (r < c.rows && u < full) v = *reinterpret_cast<const uint4 *>(x);
+      else if (r < c.rows && u == full)
+        for (int j = 0; j < c.n % 16; j++) reinterpret_cast<int8_t *>(&v)[j] = x[j];
+      xs[i] = v;
+    }
+  }
+  __syncthreads();
+
+  for (; ch < c.m; ch += step) {
+    int sum[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) sum[r] = 0;
+    for (int u0 = 0; u0 < units; u0 += 32 * U) {
+      uint4 v[U];
+#pragma unroll
+      for (int i = 0; i < U; i++) v[i] = w[i];
+      // the bytes that follow: of this channel, or of the next
+      const bool more = u0 + 32 * U < units;
+      const int ch2 = more ? ch : ch + step, u2 = more ? u0 + 32 * U : 0;
+#pragma unroll
+      for (int i = 0; i < U; i++)
+        if (ch2 < c.m && u2 + i * 32 + lane < units) w[i] = weights(ch2, u2 + i * 32 + lane);
+#pragma unroll
+      for (int i = 0; i < U; i++) {
+        const int u = u0 + i * 32 + lane;
+        if (u < units) {
+#pragma unroll
+          for (int r = 0; r < R; r++) {
+            const uint4 x = xs[r * row_units + u];
+            sum[r] = __dp4a((int)x.x, (int)v[i].x, sum[r]);
+            sum[r] = __dp4a((int)x.y, (int)v[i].y, sum[r]);
+            sum[r] = __dp4a((int)x.z, (int)v[i].z, sum[r]);
+            sum[r] = __dp4a((int)x.w, (int)v[i].w, sum[r]);
+          }
+        }
+      }
+    }
+    int mine = 0;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const int all = __reduce_add_sync(~0u, sum[r]);
+      if (lane == r) mine = all;
+    }
+    if (lane < c.rows) {
+      float f = (float)mine * scale * c.w_scale[ch];
+      if (c.bias) f += c.bias[ch];
+      Y *const y = static_cast<Y *>(c.y) + lane * c.y_row + ch;
+      if constexpr (sizeof(Y) == 2) *y = __float2half_rn(f);
+      else *y = f;
+    }
+  }
+}
+
+template <typename T, typename Y>
+int launch_few(const Mm8Call &c, bool after_rows, int sms, cudaStream_t st) {
+  const int row_bytes = (c.n + 15) / 16 * 16, r = c.rows <= 1 ? 1 : c.rows <= 2 ? 2 : 4, bytes = r * row_bytes;
+  const auto kernel = r == 1 ? k_linear8_few<T, 1, Y> : r == 2 ? k_linear8_few<T, 2, Y> : k_linear8_few<T, 4, Y>;
+  if (bytes > 48 * 1024) {
+    static std::atomic<uint64_t> set[5]{};
+    int device;
+    SHLO_CUDA(cudaGetDevice(&device));
+    if (device >= 64 || !(set[r].load(std::memory_order_relaxed) >> device & 1)) {
+      SHLO_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewBytes));
+      if (device < 64) set[r].fetch_or(1ull << device);
+    }
+  }
+  // As many blocks as run at once, or as have a channel a warp.
+  const int64_t want = ((int64_t)c.m + kFewThreads / 32 - 1) / (kFewThreads / 32), most = (int64_t)sms * std::min(4, 200 * 1024 / std::max(bytes, 1));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)std::min(want, most));
+  cfg.blockDim = dim3(kFewThreads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = after_rows ? 1 : 0;
+  SHLO_CUDA(cudaLaunchKernelEx(&cfg, kernel, c, row_bytes, after_rows));
+  return launch_check(std::is_same<T, int8_t>::value ? "mul_mat8" : "linear8");
+}
+// Up to four rows, as long as a block's copy of them is small beside the weights that
+// it reads. (Products alone, us, this and the tiles: 1 row of 4096 to 4096 channels 5.4
+// and 9.0, 4 rows 6.8 and 9.1; 4 of 14336 to 4096 18.8 and 15.2.)
+bool few(const Mm8Call &c) {
+  const int64_t bytes = ((int64_t)c.n + 15) / 16 * 16;
+  return c.rows == 1 ? bytes <= kFewBytes : c.rows <= 4 && (c.rows == 2 ? 2 : 4) * bytes <= 24 * 1024;
+}
+// Whether each of those blocks also rounds the rows, instead of a launch of its own (us:
+// 1 row of 4096 to 4096 6.4 and 7.4, of 40000 46 and 43; 4 rows of 512 to 2048 3.4 and
+// 4.2, 2 of 2048 5.5 and 4.7, 4 of 4096 to 4096 12.5 and 9.5).
+bool few_round(const Mm8Call &c) { return c.rows == 1 ? c.n <= 16384 : c.rows * c.n <= 2048; }
+
 }  // namespace
 
 int launch_quantise_rows(const void *x, int64_t x_row, uint8_t dtype, int64_t rows, int32_t n, int8_t *q, int64_t q_row, float *scale,
@@ -221,6 +411,7 @@ int launch_mul_mat8(const Mm8Call &c, bool after_rows, int *err, int sms, cudaSt
   if ((uintptr_t)c.x % 16 || (c.rows > 1 && (c.x_row % 16 || c.x_row < c.n)))
     return fail("mul_mat8: rows of x begin on multiples of 16 bytes and do not overlap (a distance of %lld for %d values)", (long long)c.x_row, c.n);
   if ((uintptr_t)c.x_scale % 4) return fail("mul_mat8: an operand is not aligned to its type");
+  if (few(c)) return c.dtype == kF16 ? launch_few<int8_t, __half>(c, after_rows, sms, st) : launch_few<int8_t, float>(c, after_rows, sms, st);
   return launch_mul_mat8_tiles(c, after_rows, err, sms, st);
 }
 
@@ -237,6 +428,12 @@ int launch_linear8(const Mm8Call &call, int *err, int sms, cudaStream_t st) {
   if (!q || c.workspace_bytes < linear8_work_bytes(c.rows, c.n))
     return fail("linear8: a workspace of %zu bytes, %zu needed", q ? c.workspace_bytes : 0, linear8_work_bytes(c.rows, c.n));
   if ((uintptr_t)q % 16) return fail("linear8: the workspace does not begin on a multiple of 16 bytes");
+  if (!c.x) return fail("linear8: null pointer");
+  if ((uintptr_t)c.x % dtype_size(c.x_dtype)) return fail("linear8: an operand is not aligned to its type");
+  if (few(c) && few_round(c)) {
+    if (c.x_dtype == kF16) return c.dtype == kF16 ? launch_few<__half, __half>(c, false, sms, st) : launch_few<__half, float>(c, false, sms, st);
+    return c.dtype == kF16 ? launch_few<float, __half>(c, false, sms, st) : launch_few<float, float>(c, false, sms, st);
+  }
   c.x = q;
   c.x_row = quantised_row(c.n);
   c.x_scale = (const float *)(q + c.rows * c.x_row);

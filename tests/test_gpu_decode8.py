@@ -294,7 +294,8 @@ def weights(rng, m, n):
 @pytest.mark.parametrize("r,n,m", [(1, 1, 1), (1, 512, 768), (1, 4097, 130), (2, 16, 64), (3, 100, 1000), (5, 2000, 129), (8, 640, 257),
                                    (16, 1024, 4096), (17, 515, 300), (24, 4096, 515), (33, 31, 33), (64, 8192, 384), (65, 777, 1001),
                                    (130, 1300, 200), (257, 129, 640), (300, 512, 2050), (1000, 260, 1111), (2, 131071, 3),
-                                   (700, 1999, 2049), (2300, 1000, 2700), (100, 200, 40000)])
+                                   (700, 1999, 2049), (2300, 1000, 2700), (100, 200, 40000), (1, 16385, 40),
+                                   (1, 70001, 24), (2, 1500, 300), (4, 509, 1300), (4, 6145, 70), (3, 16, 5000), (1, 15, 20000)])
 def test_linear8(kind, r, n, m):
     rng = np.random.default_rng(r * 31 + n)
     x, (w, ws) = activations(rng, r, n, kind), weights(rng, m, n)
@@ -322,7 +323,7 @@ def test_linear8(kind, r, n, m):
 def test_linear8_extremes():
     """Sums at the ends of 32 bits; a row that is not finite is NaN and leaves the others alone."""
     n, m = 131071, 130
-    for r in (1, 20, 140):
+    for r in (1, 3, 20, 140):
         x, w = np.full((r, 131072), -128, np.int8), np.full((m, 131072), -128, np.int8)
         w[1] = 127
         xs, ws = np.ones(r, np.float32), np.ones(m, np.float32)
