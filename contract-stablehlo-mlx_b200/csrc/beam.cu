@@ -38,6 +38,7 @@ constexpr int kRoom = 512;  // candidates of a part at a time
 constexpr int kGroup = 4;   // stretches whose candidates are looked at together: 1, 1, 2, 4, 4, ...
 constexpr int kJoin = 256;  // the second kernel's threads
 constexpr int kPicked = 512;  // candidates that it ranks
+constexpr int kScan = 2048;   // entries of a sequence's lists that are all looked at
 constexpr int kSteps = 7;     // entries 2^j - 1 < kMaxKeep of a list
 static_assert(1 << (kSteps - 1) <= kMaxKeep, "entries of a list");
 
@@ -205,14 +206,17 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_parts(const BeamArgs a) {
     int2 above = make_int2(0, 0);
     k[0] = at < n ? found[at] : 0;
     k[1] = at + kThreads < n ? found[at + kThreads] : 0;
-    if (n <= kThreads)
+    if (n <= kThreads) {
+#pragma unroll 8
       for (int j = off; j < n; j += per) above.x += found[j] > k[0];
-    else
+    } else {
+#pragma unroll 8
       for (int j = 0; j < n; j++) {
         const uint64_t o = found[j];
         above.x += o > k[0];
         above.y += o > k[1];
       }
+    }
     for (int i = 1; i < per; i *= 2) above.x += __shfl_xor_sync(~0u, above.x, i);
     if (at >= n || off) above.x = kRoom;
     if (at + kThreads >= n || per > 1) above.y = kRoom;
@@ -282,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_parts(const BeamArgs a) {
         least = low > -INFINITY ? ordered(low) : kNegInf + 1;
         int have = __syncthreads_count(key >= least);
         if (have >= a.keep)
-          while (have > a.keep + 8 && over - least > 1 && over > least) {
+          for (int i = 0; i < 16 && have > a.keep + 8 && over - least > 1 && over > least; i++) {
             const uint32_t mid = least + (over - least) / 2;
             const int m = __syncthreads_count(key >= mid);
             if (m >= a.keep) least = mid, have = m;
@@ -614,39 +618,73 @@ __global__ void __launch_bounds__(kJoin) k_beam_join(const BeamArgs a) {
     }
   }
   const double least = far;  // (-infinity: all there are)
-  for (int l = threadIdx.x; l < lists; l += kJoin) {
-    const int name = named(l);
-    for (int at = 0;; at += 4) {
-      double t[4];
-      uint64_t k[4];
+  auto pick = [&](double t, uint64_t k, int name) {
+    const int i = atomicAdd(&picked, 1);
+    if (i < kPicked) total_of[i] = t, key_of[i] = k, list_of[i] = name;
+  };
+  if (lists * a.keep <= kScan) {  // (all entries at once: their loads wait for nothing)
+    for (int i0 = threadIdx.x; i0 < lists * a.keep; i0 += 8 * kJoin) {
+      uint64_t k[8];
 #pragma unroll
-      for (int j = 0; j < 4; j++) k[j] = entry(name, at + j, t[j]);
-      bool on = true;
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        on = on && k[j] && t[j] >= least;
-        if (on) {
-          const int i = atomicAdd(&picked, 1);
-          if (i < kPicked) total_of[i] = t[j], key_of[i] = k[j], list_of[i] = name;
-          else on = false;
-        }
+      for (int j = 0; j < 8; j++) {
+        const int i = i0 + j * kJoin;
+        k[j] = i < lists * a.keep ? a.best[(int64_t)seq * lists * a.keep + i] : 0;
       }
-      if (!on) break;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const int i = i0 + j * kJoin, l = i / a.keep;
+        if (i >= lists * a.keep) break;
+        const int b = l / a.parts;
+        double t = base[b];
+        if (ended[b]) k[j] = l == b * a.parts && i == l * a.keep ? ~0ull : 0;
+        else t += (double)of_ordered((uint32_t)(k[j] >> 32)) - (double)top_of[b];
+        if (k[j] && t >= least && t > none) pick(t, k[j], b << 16 | l);
+      }
+    }
+  } else {
+    for (int l = threadIdx.x; l < lists; l += kJoin) {
+      const int name = named(l);
+      for (int at = 0;; at += 4) {
+        double t[4];
+        uint64_t k[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) k[j] = entry(name, at + j, t[j]);
+        bool on = true;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          on = on && k[j] && t[j] >= least;
+          if (on) pick(t[j], k[j], name);
+        }
+        if (!on || picked > kPicked) break;
+      }
     }
   }
   __syncthreads();
   const int n = picked;
   if (n <= kPicked) {
-    for (int i = threadIdx.x; i < n; i += kJoin) {
-      const double t = total_of[i];
-      const uint64_t k = key_of[i];
-      const int l = list_of[i];
-      int before = 0;
-      for (int j = 0; j < n; j++) {
+    // (`per` lanes count for one; equal totals, which are rare, are told apart after)
+    const int per = n <= kJoin / 4 ? 4 : n <= kJoin / 2 ? 2 : 1, off = (int)threadIdx.x % per;
+    for (int i0 = 0; i0 < n; i0 += kJoin / per) {
+      const int i = i0 + (int)threadIdx.x / per;
+      const double t = i < n ? total_of[i] : none;
+      int before = 0, same = 0;
+#pragma unroll 8
+      for (int j = off; j < n; j += per) {
         const double t2 = total_of[j];
-        if (t2 >= t) before += j != i && better(t, k, l, t2, key_of[j], list_of[j]);
+        before += t2 > t;
+        same += t2 == t;
       }
-      if (before < a.keep) write(before, t, k, l);
+      for (int j = 1; j < per; j *= 2) {
+        before += __shfl_xor_sync(~0u, before, j);
+        same += __shfl_xor_sync(~0u, same, j);
+      }
+      if (i < n && off == 0) {
+        const uint64_t k = key_of[i];
+        const int l = list_of[i];
+        if (same > 1)
+          for (int j = 0; j < n; j++) before += j != i && total_of[j] == t && better(t, k, l, t, key_of[j], list_of[j]);
+        if (before < a.keep) write(before, t, k, l);
+      }
     }
     for (int i = n + threadIdx.x; i < a.keep; i += kJoin) write(i, none, 0, -1);
     return;
@@ -686,9 +724,9 @@ Cut cut(int64_t rows, int vocab, size_t size, int sms) {
     c.stretch = nv * kThreads * (16 / (int)size);
     return (vocab + c.stretch - 1) / c.stretch;
   };
-  // Shorter stretches where they would leave SMs without work.
+  // Shorter stretches where they would leave SMs without work, or be half empty.
   c.nv = size == 2 ? 4 : 8;
-  while (c.nv > 1 && rows * stretches(c.nv) < 2 * sms) c.nv /= 2;
+  while (c.nv > 1 && (rows * stretches(c.nv) < 2 * sms || stretches(c.nv / 2) == 1)) c.nv /= 2;
   const int n = stretches(c.nv);
   // Turns of blocks, four an SM, by the stretches of each, the first of which costs
   // two: its border has to be found. (512 rows of 128256: 47 us at 8 and 16 stretches a

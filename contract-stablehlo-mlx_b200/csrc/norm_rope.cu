@@ -19,6 +19,7 @@
 // blocks an SM (125 us, registers to memory) and two (91 us), no head ahead (88 us).
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "decode.cuh"
 
@@ -155,7 +156,7 @@ __device__ __forceinline__ void unpairs(const float2 (&a)[NS * VEC / 2], const f
 // BACK: the gradient. A block goes over tiles of 2^nt_log tokens, one in the
 // forward pass, for the heads of its part.
 template <typename T, int VEC, int NS, bool INTER, bool BACK>
-__global__ void __launch_bounds__(kThreads, BACK && sizeof(T) == 4 ? kBackBlocksPerSm : 2) k_norm_rope(const NormArgs a) {
+__global__ void __launch_bounds__(kThreads, BACK && (sizeof(T) == 4 || NS * VEC <= 4) ? kBackBlocksPerSm : 2) k_norm_rope(const NormArgs a) {
   // Backward: 8 P sums a thread; then the cosines and sines, [token][half] each, and at
   // the end the block's sums, [warp][dim], in their place.
   extern __shared__ double sh[];
@@ -251,6 +252,9 @@ __global__ void __launch_bounds__(kThreads, BACK && sizeof(T) == 4 ? kBackBlocks
       }
     }
   };
+  // (pair and token of this thread's angles, kThreads apart)
+  const int tt_first = half ? (int)threadIdx.x / half : 0, p_first = (int)threadIdx.x - tt_first * half;
+  const int dt = half ? kThreads / half : 0, dp = kThreads - dt * half;
   const float inv_dim = 1.0f / a.dim;
   const int64_t tiles = (a.tokens + nt - 1) >> a.nt_log;
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
@@ -272,8 +276,7 @@ __global__ void __launch_bounds__(kThreads, BACK && sizeof(T) == 4 ? kBackBlocks
       }
     }
     if (BACK && tile != (int64_t)blockIdx.x) __syncthreads();
-    for (int i = threadIdx.x; i < nt * half; i += kThreads) {
-      const int tt = i / half, p = i - tt * half;
+    for (int i = threadIdx.x, p = p_first, tt = tt_first; i < nt * half; i += kThreads) {
       if (t0 + tt < a.tokens) {
         const int64_t turns = (int64_t)((uint64_t)(int64_t)a.pos[t0 + tt] * (uint64_t)a.phases[p]) >> 32;
         float s, c;
@@ -281,6 +284,9 @@ __global__ void __launch_bounds__(kThreads, BACK && sizeof(T) == 4 ? kBackBlocks
         cs[i] = c * a.factor;
         sn[i] = s * a.factor;
       }
+      p += dp;
+      tt += dt;
+      if (p >= half) p -= half, tt++;
     }
     __syncthreads();
     // Forward: what a pair's two results take of its two values, weight and turn in
@@ -429,6 +435,7 @@ __global__ void __launch_bounds__(1024) k_norm_rope_dw(const double *partials, i
   const int c = threadIdx.x % 32, r = threadIdx.x / 32, i = blockIdx.x * 32 + c;
   float *const to = blockIdx.y ? dk : dq;
   if (!to) return;
+  cudaGridDependencySynchronize();  // (it may begin before the sums are there)
   double sum = 0.0;
   if (i < dim)
     for (int k = r; k < blocks; k += 32) sum += partials[((int64_t)k * 2 + blockIdx.y) * dim + i];
@@ -506,8 +513,9 @@ int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st)
     return half % v == 0 && rest % v == 0 && row(c.x, c.x_token, c.x_head) && row(c.y, c.y_token, c.y_head) && (!back || row(c.dy, c.dy_token, c.dy_head));
   };
   while (vec > 1 && !fits(vec)) vec /= 2;
+  // A lane's slots: as few as hold the head in 32 lanes (two pairs at least).
   const int units = half / vec + (rest / vec + 1) / 2;
-  const int slots = c.dtype == kF32 && vec == 4 && units <= 32 ? 1 : 8 / vec;
+  const int slots = units <= 32 ? (vec == 1 ? 2 : 1) : 8 / vec;
   NormArgs a;
   a.x = c.x; a.dy = c.dy; a.y = c.y; a.pos = c.positions; a.phases = c.phases; a.wq = c.q_weight; a.wk = c.k_weight;
   a.xt = c.x_token; a.xh = c.x_head; a.gt = c.dy_token; a.gh = c.dy_head; a.yt = c.y_token; a.yh = c.y_head;
@@ -529,32 +537,38 @@ int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st)
   dim3 grid((unsigned)tiles, (unsigned)((c.heads + a.hb - 1) / a.hb));
   // The backward pass has as many blocks as run at once (of float16, two an SM), each
   // with a row of sums.
-  if (back) grid.x = (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, (c.dtype == kF16 ? 2 * sms : back_blocks(sms)) / grid.y));
+  if (back) grid.x = (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, (c.dtype == kF16 && slots * vec > 4 ? 2 * sms : back_blocks(sms)) / grid.y));
   size_t smem = (size_t)(1 << a.nt_log) * half * 2 * sizeof(float);
   if (back) smem = std::max(smem, (size_t)(kThreads / 32) * c.dim * sizeof(double)) + (size_t)slots * vec * 4 * kThreads * sizeof(double);
   a.w_wide = true;
   for (const void *w : {c.q_weight, c.k_weight})
     if ((uintptr_t)w % (vec * wsize > 16 ? 16 : vec * wsize)) a.w_wide = false;
   const bool inter = (c.flags & 1) != 0;
-  if (c.dtype == kF16) {
-    switch (vec) {
-      case 8: SHLO_TRY((launch<__half, 8, 1>(a, inter, back, grid, smem, st))); break;
-      case 4: SHLO_TRY((launch<__half, 4, 2>(a, inter, back, grid, smem, st))); break;
-      case 2: SHLO_TRY((launch<__half, 2, 4>(a, inter, back, grid, smem, st))); break;
-      default: SHLO_TRY((launch<__half, 1, 8>(a, inter, back, grid, smem, st))); break;
-    }
-  } else {
-    switch (vec) {
-      case 4:
-        if (slots == 1) SHLO_TRY((launch<float, 4, 1>(a, inter, back, grid, smem, st)));
-        else SHLO_TRY((launch<float, 4, 2>(a, inter, back, grid, smem, st)));
-        break;
-      case 2: SHLO_TRY((launch<float, 2, 4>(a, inter, back, grid, smem, st))); break;
-      default: SHLO_TRY((launch<float, 1, 8>(a, inter, back, grid, smem, st))); break;
-    }
+  auto go = [&](auto v, auto n) {
+    constexpr int V = decltype(v)::value, N = decltype(n)::value;
+    if constexpr (V <= 4)
+      if (c.dtype == kF32) return launch<float, V, N>(a, inter, back, grid, smem, st);
+    return launch<__half, V, N>(a, inter, back, grid, smem, st);
+  };
+#define SHLO_INT(n) std::integral_constant<int, n>()
+  switch (vec) {
+    case 8: SHLO_TRY(go(SHLO_INT(8), SHLO_INT(1))); break;
+    case 4: SHLO_TRY(slots == 1 ? go(SHLO_INT(4), SHLO_INT(1)) : go(SHLO_INT(4), SHLO_INT(2))); break;
+    case 2: SHLO_TRY(slots == 1 ? go(SHLO_INT(2), SHLO_INT(1)) : go(SHLO_INT(2), SHLO_INT(4))); break;
+    default: SHLO_TRY(slots == 2 ? go(SHLO_INT(1), SHLO_INT(2)) : go(SHLO_INT(1), SHLO_INT(8))); break;
   }
+#undef SHLO_INT
   if (!sums) return 0;
-  k_norm_rope_dw<<<dim3((c.dim + 31) / 32, 2), 1024, 0, st>>>(a.partials, (int)(grid.x * grid.y), c.dim, c.dq_weight, c.dk_weight);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((c.dim + 31) / 32, 2);
+  cfg.blockDim = dim3(1024);
+  cfg.stream = st;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  SHLO_CUDA(cudaLaunchKernelEx(&cfg, k_norm_rope_dw, (const double *)a.partials, (int)(grid.x * grid.y), c.dim, c.dq_weight, c.dk_weight));
   return launch_check("norm_rope_grad");
 }
 
