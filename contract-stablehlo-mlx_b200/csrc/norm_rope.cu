@@ -28,7 +28,7 @@ namespace shlo {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBackBlocksPerSm = 3;  // float32's backward pass (float16's needs the registers of two)
+constexpr int kBackBlocksPerSm = 3;  // the backward pass's, with four pairs a lane or fewer (eight need the registers of two)
 
 struct NormArgs {
   const void *x, *dy;
@@ -156,7 +156,7 @@ __device__ __forceinline__ void unpairs(const float2 (&a)[NS * VEC / 2], const f
 // BACK: the gradient. A block goes over tiles of 2^nt_log tokens, one in the
 // forward pass, for the heads of its part.
 template <typename T, int VEC, int NS, bool INTER, bool BACK>
-__global__ void __launch_bounds__(kThreads, BACK && (sizeof(T) == 4 || NS * VEC <= 4) ? kBackBlocksPerSm : 2) k_norm_rope(const NormArgs a) {
+__global__ void __launch_bounds__(kThreads, BACK && NS * VEC <= 4 ? kBackBlocksPerSm : 2) k_norm_rope(const NormArgs a) {
   // Backward: 8 P sums a thread; then the cosines and sines, [token][half] each, and at
   // the end the block's sums, [warp][dim], in their place.
   extern __shared__ double sh[];
@@ -513,9 +513,14 @@ int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st)
     return half % v == 0 && rest % v == 0 && row(c.x, c.x_token, c.x_head) && row(c.y, c.y_token, c.y_head) && (!back || row(c.dy, c.dy_token, c.dy_head));
   };
   while (vec > 1 && !fits(vec)) vec /= 2;
-  // A lane's slots: as few as hold the head in 32 lanes (two pairs at least).
+  // A lane's slots: 8 / vec of them (as many as its registers are made for) where
+  // narrow vectors would leave it few values of a head, and there are heads enough for
+  // all lanes; else as few as hold the head in 32 lanes. (750000 tokens' heads of 72, 36
+  // turned, float16: 45 us with four slots and 84 with one; 55000 tokens of one such
+  // head: 57 and 42.)
   const int units = half / vec + (rest / vec + 1) / 2;
-  const int slots = units <= 32 ? (vec == 1 ? 2 : 1) : 8 / vec;
+  const bool narrow = c.dtype == kF16 ? vec <= 4 : vec <= 2;
+  const int slots = vec == 8 ? 1 : units > 32 || (narrow && c.heads >= 4) ? 8 / vec : vec == 1 ? 2 : 1;
   NormArgs a;
   a.x = c.x; a.dy = c.dy; a.y = c.y; a.pos = c.positions; a.phases = c.phases; a.wq = c.q_weight; a.wk = c.k_weight;
   a.xt = c.x_token; a.xh = c.x_head; a.gt = c.dy_token; a.gh = c.dy_head; a.yt = c.y_token; a.yh = c.y_head;
@@ -523,21 +528,21 @@ int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st)
   a.eps = c.eps; a.factor = c.factor; a.w_half = c.weight_dtype == kF16;
   a.partials = sums ? (double *)c.workspace : nullptr;
   a.lanes_log = 0;
-  while (a.lanes_log < 5 && (1 << a.lanes_log) < units) a.lanes_log++;
-  // A block's tokens, as long as every SM gets blocks; then its heads are shared among
-  // blocks while there are fewer than two a SM.
+  while (a.lanes_log < 5 && (slots << a.lanes_log) < units) a.lanes_log++;
+  // A block's tokens, as long as every SM gets blocks: eight, or more where their heads
+  // are fewer than its groups; then its heads are shared among blocks while there are
+  // fewer than two a SM.
   const int groups = kThreads >> a.lanes_log;
   a.nt_log = 0;
-  while ((2 << a.nt_log) <= groups && a.nt_log < 3 && (c.tokens >> (a.nt_log + 1)) >= 4 * sms) a.nt_log++;
+  while ((2 << a.nt_log) <= groups && (a.nt_log < 3 || (groups >> a.nt_log) > c.heads) && (c.tokens >> (a.nt_log + 1)) >= 4 * sms) a.nt_log++;
   const int64_t tiles = (c.tokens + (1 << a.nt_log) - 1) >> a.nt_log;
   const int step = std::max(1, groups >> a.nt_log);
   int parts = 1;
   while (tiles * parts < 2 * sms && parts < (c.heads + step - 1) / step) parts++;
   a.hb = (c.heads + parts - 1) / parts;
   dim3 grid((unsigned)tiles, (unsigned)((c.heads + a.hb - 1) / a.hb));
-  // The backward pass has as many blocks as run at once (of float16, two an SM), each
-  // with a row of sums.
-  if (back) grid.x = (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, (c.dtype == kF16 && slots * vec > 4 ? 2 * sms : back_blocks(sms)) / grid.y));
+  // The backward pass has as many blocks as run at once, each with a row of sums.
+  if (back) grid.x = (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, (slots * vec > 4 ? 2 * sms : back_blocks(sms)) / grid.y));
   size_t smem = (size_t)(1 << a.nt_log) * half * 2 * sizeof(float);
   if (back) smem = std::max(smem, (size_t)(kThreads / 32) * c.dim * sizeof(double)) + (size_t)slots * vec * 4 * kThreads * sizeof(double);
   a.w_wide = true;
