@@ -61,42 +61,33 @@ template <typename T, int V>
 __device__ __forceinline__ void quantise(const T (&v)[V], float top, float by, uint8_t (&q)[V]) {  // (q on a boundary of four)
   uint32_t m[V];
   float off = 0.0f;  // the farthest from its integer
-  if constexpr (V == 1) {
-    const float r = to_f32(v[0]) * by, s = r + 12582912.0f;
-    off = fabsf(r - (s - 12582912.0f));
-    m[0] = __float_as_uint(s);
-  } else {
 #pragma unroll
-    for (int j = 0; j < V; j += 2) {
-      const float2 r = __fmul2_rn(make_float2(to_f32(v[j]), to_f32(v[j + 1])), make_float2(by, by));
-      const float2 s = __fadd2_rn(r, make_float2(12582912.0f, 12582912.0f));
-      const float2 k = __fadd2_rn(s, make_float2(-12582912.0f, -12582912.0f));
-      const float2 d = __ffma2_rn(k, make_float2(-1.0f, -1.0f), r);
-      off = fmaxf(off, fmaxf(fabsf(d.x), fabsf(d.y)));
-      m[j] = __float_as_uint(s.x);
-      m[j + 1] = __float_as_uint(s.y);
-    }
+  for (int j = 0; j < V; j += 2) {
+    const float2 r = __fmul2_rn(make_float2(to_f32(v[j]), to_f32(v[j + 1])), make_float2(by, by));
+    const float2 s = __fadd2_rn(r, make_float2(12582912.0f, 12582912.0f));
+    const float2 k = __fadd2_rn(s, make_float2(-12582912.0f, -12582912.0f));
+    const float2 d = __ffma2_rn(k, make_float2(-1.0f, -1.0f), r);
+    off = fmaxf(off, fmaxf(fabsf(d.x), fabsf(d.y)));
+    m[j] = __float_as_uint(s.x);
+    m[j + 1] = __float_as_uint(s.y);
   }
   if (!(off < 0.5f - 0x1p-15f) || !(by < 0x1p120f)) {
 #pragma unroll
     for (int j = 0; j < V; j++) m[j] = (uint32_t)decide(to_f32(v[j]), top);
   }
-  if constexpr (V % 4 == 0) {
 #pragma unroll
-    for (int j = 0; j < V; j += 4)
-      *reinterpret_cast<uint32_t *>(q + j) = __byte_perm(__byte_perm(m[j], m[j + 1], 0x0040), __byte_perm(m[j + 2], m[j + 3], 0x0040), 0x5410);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; j++) q[j] = (uint8_t)m[j];
-  }
+  for (int j = 0; j < V; j += 4)
+    *reinterpret_cast<uint32_t *>(q + j) = __byte_perm(__byte_perm(m[j], m[j + 1], 0x0040), __byte_perm(m[j + 2], m[j + 3], 0x0040), 0x5410);
 }
 
-// TPR threads a row, vectors of V values; a row of up to KEEP TPR of them stays in
-// registers between the two passes, a longer one is read again from L2. V = 1 where
-// x does not allow vectors; WIDE where q allows stores of V bytes.
-template <typename T, int V, int TPR, int KEEP, bool WIDE>
-__global__ void __launch_bounds__(kQuantThreads, KEEP <= 2 && V > 1 ? 6 : 4) k_quantise_rows(const T *x, int64_t x_row, int64_t rows, int n, int8_t *q, int64_t q_row, float *scale, int fill) {
-  constexpr int ROWS = kQuantThreads / TPR;
+// TPR threads a row, V values of it at a time in loads of PIECE bytes (what x's
+// alignment allows); a row of up to KEEP TPR of them stays in registers between the two
+// passes, a longer one is read again from L2. `wide`: q allows stores of V bytes.
+template <typename T, int V, int PIECE, int TPR, int KEEP>
+__global__ void __launch_bounds__(kQuantThreads, KEEP <= 2 ? 6 : KEEP == 4 ? 5 : 4)
+k_quantise_rows(const T *x, int64_t x_row, int64_t rows, int n, int8_t *q, int64_t q_row, float *scale, int fill, bool wide) {
+  constexpr int ROWS = kQuantThreads / TPR, EACH = PIECE / (int)sizeof(T);
+  using R = typename Raw<PIECE>::T;
   __shared__ uint32_t tops[kQuantThreads / 32];
   // (a product that waits for these rows may begin to read its weights)
   cudaTriggerProgrammaticLaunchCompletion();
@@ -107,14 +98,16 @@ __global__ void __launch_bounds__(kQuantThreads, KEEP <= 2 && V > 1 ? 6 : 4) k_q
   q += (there ? row : 0) * q_row;
   const int vecs = there ? (n + V - 1) / V : 0;
   auto load = [&](int i, T (&v)[V]) {
+    const T *const from = x + (int64_t)i * V;
     if (i * V + V <= n) {
-      *reinterpret_cast<typename Raw<V * sizeof(T)>::T *>(v) = *reinterpret_cast<const typename Raw<V * sizeof(T)>::T *>(x + (int64_t)i * V);
+#pragma unroll
+      for (int j = 0; j < V; j += EACH) *reinterpret_cast<R *>(v + j) = *reinterpret_cast<const R *>(from + j);
     } else {
 #pragma unroll
-      for (int j = 0; j < V; j++) v[j] = i * V + j < n ? x[(int64_t)i * V + j] : T(0.0f);
+      for (int j = 0; j < V; j++) v[j] = i * V + j < n ? from[j] : T(0.0f);
     }
   };
-  T v[KEEP][V];
+  alignas(16) T v[KEEP][V];
   uint32_t bits = 0;
 #pragma unroll
   for (int k = 0; k < KEEP; k++)
@@ -122,8 +115,9 @@ __global__ void __launch_bounds__(kQuantThreads, KEEP <= 2 && V > 1 ? 6 : 4) k_q
 #pragma unroll
   for (int k = 0; k < KEEP; k++)
     if (t + k * TPR < vecs) bits = max(bits, top_bits(v[k]));
+#pragma unroll 2
   for (int i = t + KEEP * TPR; i < vecs; i += TPR) {
-    T w[V];
+    alignas(16) T w[V];
     load(i, w);
     bits = max(bits, top_bits(w));
   }
@@ -143,7 +137,7 @@ __global__ void __launch_bounds__(kQuantThreads, KEEP <= 2 && V > 1 ? 6 : 4) k_q
 #pragma unroll
     for (int j = 0; j < V; j++) b[j] = 0;
     if (any) quantise(w, top, by, b);
-    if (WIDE && i * V + V <= n) {
+    if (wide && i * V + V <= n) {
       *reinterpret_cast<typename Raw<V>::T *>(q + (int64_t)i * V) = *reinterpret_cast<const typename Raw<V>::T *>(b);
     } else {
 #pragma unroll
@@ -154,28 +148,26 @@ __global__ void __launch_bounds__(kQuantThreads, KEEP <= 2 && V > 1 ? 6 : 4) k_q
 #pragma unroll
   for (int k = 0; k < KEEP; k++)
     if (t + k * TPR < vecs) store(t + k * TPR, v[k]);
+#pragma unroll 2
   for (int i = t + KEEP * TPR; i < vecs; i += TPR) {
-    T w[V];
+    alignas(16) T w[V];
     load(i, w);
     store(i, w);
   }
   for (int i = n + t; i < fill; i += TPR) q[i] = 0;
 }
 
-template <typename T, int V>
+template <typename T, int V, int PIECE>
 void launch_rows(const T *x, int64_t x_row, int64_t rows, int n, int8_t *q, int64_t q_row, float *scale, int fill, cudaStream_t st) {
   const bool wide = (uintptr_t)q % V == 0 && (rows == 1 || q_row % V == 0);
-  auto go = [&](auto kernel, int per) { kernel<<<(unsigned)((rows + per - 1) / per), kQuantThreads, 0, st>>>(x, x_row, rows, n, q, q_row, scale, fill); };
-  // Threads a row: so many that few wait for one value, and all 256 for few rows.
+  auto go = [&](auto kernel, int per) { kernel<<<(unsigned)((rows + per - 1) / per), kQuantThreads, 0, st>>>(x, x_row, rows, n, q, q_row, scale, fill, wide); };
+  // Threads a row: a warp, or all 256 where that leaves a lane more than it keeps.
   const int vecs = (n + V - 1) / V;
-  auto pick = [&](auto keep) {
-    constexpr int K = decltype(keep)::value;
-    if (vecs <= 32 * K) go(wide ? k_quantise_rows<T, V, 32, K, true> : k_quantise_rows<T, V, 32, K, false>, 8);
-    else go(wide ? k_quantise_rows<T, V, 256, K, true> : k_quantise_rows<T, V, 256, K, false>, 1);
-  };
-  if (vecs <= 32 || (vecs > 64 && vecs <= 256)) pick(std::integral_constant<int, 1>());
-  else if (vecs <= 64 || (vecs > 128 && vecs <= 512)) pick(std::integral_constant<int, 2>());
-  else pick(std::integral_constant<int, 4>());
+  if (vecs <= 64) go(k_quantise_rows<T, V, PIECE, 32, 2>, 8);
+  else if (vecs <= 256 && rows > 1024) go(k_quantise_rows<T, V, PIECE, 32, 8>, 8);
+  else if (vecs <= 512) go(k_quantise_rows<T, V, PIECE, 256, 2>, 1);
+  else if (vecs <= 1024) go(k_quantise_rows<T, V, PIECE, 256, 4>, 1);
+  else go(k_quantise_rows<T, V, PIECE, 256, 8>, 1);
 }
 
 // Few rows: a warp a channel, whose bytes go through its lanes 16 at a time, against
@@ -378,14 +370,19 @@ int launch_quantise_rows(const void *x, int64_t x_row, uint8_t dtype, int64_t ro
   if (!x || !q || !scale) return fail("%s: null pointer", what);
   const size_t size = dtype_size(dtype);
   if ((uintptr_t)x % size || (uintptr_t)scale % 4) return fail("%s: an operand is not aligned to its type", what);
-  const bool wide = (uintptr_t)x % 16 == 0 && (rows == 1 || x_row * (int64_t)size % 16 == 0);
+  const uintptr_t at = (uintptr_t)x | (rows > 1 ? (uintptr_t)(x_row * (int64_t)size) : 0);
   const int end = fill ? (n + 15) / 16 * 16 : n;
   if (dtype == kF16) {
-    if (wide) launch_rows<__half, 8>((const __half *)x, x_row, rows, n, q, q_row, scale, end, st);
-    else launch_rows<__half, 1>((const __half *)x, x_row, rows, n, q, q_row, scale, end, st);
+    const __half *p = (const __half *)x;
+    if (at % 16 == 0) launch_rows<__half, 8, 16>(p, x_row, rows, n, q, q_row, scale, end, st);
+    else if (at % 8 == 0) launch_rows<__half, 4, 8>(p, x_row, rows, n, q, q_row, scale, end, st);
+    else if (at % 4 == 0) launch_rows<__half, 4, 4>(p, x_row, rows, n, q, q_row, scale, end, st);
+    else launch_rows<__half, 4, 2>(p, x_row, rows, n, q, q_row, scale, end, st);
   } else {
-    if (wide) launch_rows<float, 4>((const float *)x, x_row, rows, n, q, q_row, scale, end, st);
-    else launch_rows<float, 1>((const float *)x, x_row, rows, n, q, q_row, scale, end, st);
+    const float *p = (const float *)x;
+    if (at % 16 == 0) launch_rows<float, 4, 16>(p, x_row, rows, n, q, q_row, scale, end, st);
+    else if (at % 8 == 0) launch_rows<float, 4, 8>(p, x_row, rows, n, q, q_row, scale, end, st);
+    else launch_rows<float, 4, 4>(p, x_row, rows, n, q, q_row, scale, end, st);
   }
   return launch_check(what);
 }
