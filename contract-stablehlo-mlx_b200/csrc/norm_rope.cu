@@ -12,11 +12,11 @@
 // and goes over heads, so that its pairs' cosines and sines, and the weight, stay in
 // registers too (forward: their products); heads to come are asked for ahead, four of
 // them forward and one backward. Two pairs go through each packed instruction.
-// Measured on one B200: 16384 tokens x 40 heads x 128, float16 (336 MB) 62 us, 5.4 TB/s
+// Measured on one B200: 16384 tokens x 40 heads x 128, float16 (336 MB) 63 us, 5.3 TB/s
 // (rope.cu alone 55); the gradient of 24001 x 12 x 80 float32, 32 dimensions turned in
-// interleaved pairs (277 MB) 80 us, 3.5 TB/s: 330 instructions a group's head, and
-// lanes without values (10 units of 4 on 16 lanes). Measured and left there: four
-// blocks an SM (125 us, registers to memory) and two (91 us), no head ahead (88 us).
+// interleaved pairs (277 MB) 70 us, 3.9 TB/s: ten units of eight values a head, on ten
+// lanes, three heads a warp (84 us on 16 lanes). Measured and left there, on 16 lanes:
+// four blocks an SM (125 us, registers to memory) and two (91 us), no head ahead (88 us).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -39,9 +39,9 @@ struct NormArgs {
   int64_t xt, xh, gt, gh, yt, yh;  // token and head strides, in values (g: dy's)
   int64_t tokens;
   int heads, q_heads, dim, rot;
-  int lanes_log;  // lanes a group
-  int nt_log;     // tokens a block (at a time)
-  int hb;         // heads a block
+  int odd, lanes_log;  // lanes a group: odd << lanes_log
+  int nt_log;  // tokens a block (at a time)
+  int hb;      // heads a block
   float eps, factor;
   bool w_half, w_wide;  // the weights' type, and whether they allow wide loads
   double *partials;     // backward: [blocks][2][dim], nullptr without the weights' gradients
@@ -71,14 +71,14 @@ template <int NS> struct Places {
 };
 
 template <int VEC, int NS, bool INTER>
-__device__ __forceinline__ void places(const NormArgs &a, int lane, Places<NS> &p) {
+__device__ __forceinline__ void places(const NormArgs &a, int L, bool there, int lane, Places<NS> &p) {
   const int half = a.rot / 2, ru = half / VEC, cv = (a.dim - a.rot) / VEC;
 #pragma unroll
   for (int s = 0; s < NS; s++) {
-    const int u = lane + (s << a.lanes_log), c = 2 * (u - ru);
-    p.pair[s] = u < ru;
-    p.o[s] = u < ru ? (INTER ? 2 * VEC : VEC) * u : c < cv ? a.rot + c * VEC : -1;
-    p.o2[s] = u < ru ? p.o[s] + (INTER ? VEC : half) : c + 1 < cv ? a.rot + (c + 1) * VEC : -1;
+    const int u = lane + s * L, c = 2 * (u - ru);
+    p.pair[s] = there && u < ru;
+    p.o[s] = !there ? -1 : u < ru ? (INTER ? 2 * VEC : VEC) * u : c < cv ? a.rot + c * VEC : -1;
+    p.o2[s] = !there ? -1 : u < ru ? p.o[s] + (INTER ? VEC : half) : c + 1 < cv ? a.rot + (c + 1) * VEC : -1;
   }
 }
 template <typename T, int VEC, int NS>
@@ -112,8 +112,14 @@ __device__ __forceinline__ void clear_part(Part<T, VEC, NS> &r) {
 template <int VEC, bool INTER, typename V> __device__ __forceinline__ V &first(V (&v)[2][VEC], int j) { return INTER ? v[(2 * j) / VEC][(2 * j) % VEC] : v[0][j]; }
 template <int VEC, bool INTER, typename V> __device__ __forceinline__ V &second(V (&v)[2][VEC], int j) { return INTER ? v[(2 * j + 1) / VEC][(2 * j + 1) % VEC] : v[1][j]; }
 
-__device__ __forceinline__ float group_sum(float v, int lanes_log) {
-  for (int i = 0; i < lanes_log; i++) v += __shfl_xor_sync(~0u, v, 1 << i);
+// Over a group's lanes, the first of which is `base`: the same sum in each.
+template <bool ODD> __device__ __forceinline__ float group_sum(float v, const NormArgs &a, int base) {
+  for (int i = 0; i < a.lanes_log; i++) v += __shfl_xor_sync(~0u, v, 1 << i);
+  if (ODD) {
+    float sum = 0.0f;
+    for (int i = 0; i < a.odd; i++) sum += __shfl_sync(~0u, v, base + (i << a.lanes_log));
+    v = sum;
+  }
   return v;
 }
 
@@ -154,8 +160,9 @@ __device__ __forceinline__ void unpairs(const float2 (&a)[NS * VEC / 2], const f
 }
 
 // BACK: the gradient. A block goes over tiles of 2^nt_log tokens, one in the
-// forward pass, for the heads of its part.
-template <typename T, int VEC, int NS, bool INTER, bool BACK>
+// forward pass, for the heads of its part. ODD: a group's lanes are not a power of two;
+// a warp's last lanes may have no group.
+template <typename T, int VEC, int NS, bool INTER, bool BACK, bool ODD>
 __global__ void __launch_bounds__(kThreads, BACK && NS * VEC <= 4 ? kBackBlocksPerSm : 2) k_norm_rope(const NormArgs a) {
   // Backward: 8 P sums a thread; then the cosines and sines, [token][half] each, and at
   // the end the block's sums, [warp][dim], in their place.
@@ -163,11 +170,14 @@ __global__ void __launch_bounds__(kThreads, BACK && NS * VEC <= 4 ? kBackBlocksP
   constexpr int P = NS * VEC / 2, AHEAD = BACK ? 1 : 4;  // heads asked for beside the one in hand
   const int half = a.rot / 2, nt = 1 << a.nt_log;
   float *const cs = reinterpret_cast<float *>(sh + (BACK ? 8 * P * kThreads : 0)), *const sn = cs + nt * half;
-  const int lane = threadIdx.x & ((1 << a.lanes_log) - 1), group = threadIdx.x >> a.lanes_log;
-  const int groups = kThreads >> a.lanes_log;
+  const int warp = threadIdx.x / 32, wl = threadIdx.x % 32;
+  const int L = ODD ? a.odd << a.lanes_log : 1 << a.lanes_log, in_warp = ODD ? 32 / L : 32 >> a.lanes_log;  // groups
+  const int lane = ODD ? wl % L : wl & (L - 1), base = wl - lane, group = ODD ? warp * in_warp + wl / L : (int)threadIdx.x >> a.lanes_log;
+  const int groups = kThreads / 32 * in_warp;
+  const bool works = !ODD || wl < in_warp * L;
   const int h0 = blockIdx.y * a.hb, h1 = min(h0 + a.hb, a.heads);
   Places<NS> at;
-  places<VEC, NS, INTER>(a, lane, at);
+  places<VEC, NS, INTER>(a, L, works, lane, at);
   auto weight = [&](bool keys, float2 (&wa)[P], float2 (&wb)[P]) {
     const void *const wp = keys ? a.wk : a.wq;
     Part<float, VEC, NS> w;
@@ -214,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, BACK && NS * VEC <= 4 ? kBackBlocksP
     float cc[2 * P], ss[2 * P];
 #pragma unroll
     for (int i = 0; i < 2 * P; i += V) {
-      const int slot = i / VEC, p = t * half + (lane + (slot << a.lanes_log)) * VEC + i % VEC;
+      const int slot = i / VEC, p = t * half + (lane + slot * L) * VEC + i % VEC;
 #pragma unroll
       for (int j = 0; j < V; j++) cc[i + j] = 1.0f, ss[i + j] = 0.0f;
       if (at.pair[slot]) {
@@ -259,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, BACK && NS * VEC <= 4 ? kBackBlocksP
   const int64_t tiles = (a.tokens + nt - 1) >> a.nt_log;
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     const int64_t t0 = tile << a.nt_log;
-    const bool mine = t0 + t < a.tokens;
+    const bool mine = works && t0 + t < a.tokens;
     const T *x = static_cast<const T *>(a.x) + (t0 + t) * a.xt + h_first * a.xh;
     const T *g = BACK ? static_cast<const T *>(a.dy) + (t0 + t) * a.gt + h_first * a.gh : nullptr;
     T *y = static_cast<T *>(a.y) + (t0 + t) * a.yt + h_first * a.yh;
@@ -334,7 +344,7 @@ __global__ void __launch_bounds__(kThreads, BACK && NS * VEC <= 4 ? kBackBlocksP
         }
 #pragma unroll
         for (int i = 0; i < P; i++) sum = __ffma2_rn(xb[i], xb[i], __ffma2_rn(xa[i], xa[i], sum));
-        float ss = group_sum(sum.x + sum.y, a.lanes_log), scale = 1.0f, eps = a.eps;
+        float ss = group_sum<ODD>(sum.x + sum.y, a, base), scale = 1.0f, eps = a.eps;
         if (sizeof(T) == 4) {
           scale = safe_scale(ss, eps);
           if (__any_sync(~0u, scale != 1.0f)) {
@@ -346,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, BACK && NS * VEC <= 4 ? kBackBlocksP
               xb[i] = __fmul2_rn(xb[i], both(scale));
               sum = __ffma2_rn(xb[i], xb[i], __ffma2_rn(xa[i], xa[i], sum));
             }
-            ss = group_sum(sum.x + sum.y, a.lanes_log);
+            ss = group_sum<ODD>(sum.x + sum.y, a, base);
           }
         }
         // (2^-22 is enough where the result has 11 bits)
@@ -377,7 +387,7 @@ __global__ void __launch_bounds__(kThreads, BACK && NS * VEC <= 4 ? kBackBlocksP
             gb[i] = __fmul2_rn(q, wb[i]);
             dot = __ffma2_rn(gb[i], xb[i], __ffma2_rn(ga[i], xa[i], dot));
           }
-          const float gn = -(group_sum(dot.x + dot.y, a.lanes_log) * inv_dim);
+          const float gn = -(group_sum<ODD>(dot.x + dot.y, a, base) * inv_dim);
 #pragma unroll
           for (int i = 0; i < P; i++) {
             ya[i] = __fmul2_rn(__ffma2_rn(xa[i], both(gn), ga[i]), both(inv));
@@ -401,7 +411,6 @@ __global__ void __launch_bounds__(kThreads, BACK && NS * VEC <= 4 ? kBackBlocksP
     if (!a.partials) return;
     // The block's sums, of one weight and then of the other: a warp's groups, then the
     // warps one after the other.
-    const int L = 1 << a.lanes_log, warp = threadIdx.x / 32, wl = threadIdx.x % 32;
     if (has >= 0) flush();
     double *const rows = reinterpret_cast<double *>(cs);
     for (int k0 = 0; k0 < 2; k0++) {
@@ -414,7 +423,12 @@ __global__ void __launch_bounds__(kThreads, BACK && NS * VEC <= 4 ? kBackBlocksP
           const int s = p / V, j = p % V, k = INTER ? (2 * j + q) / V : q, at_j = INTER ? (2 * j + q) % V : j;
           const int o = k ? at.o2[s] : at.o[s];
           double v = sums[(k0 * 4 * P + p / 2 * 4 + 2 * q + p % 2) * kThreads];
-          for (int i = L; i < 32; i *= 2) v += __shfl_xor_sync(~0u, v, i);
+          if (!ODD) {
+            for (int i = L; i < 32; i *= 2) v += __shfl_xor_sync(~0u, v, i);
+          } else {
+            const double mine = v;
+            for (int i = 1; i < in_warp; i++) v += __shfl_sync(~0u, mine, (wl + i * L) % 32);
+          }
           if (wl < L && o >= 0) rows[warp * a.dim + o + at_j] = v;
         }
       __syncthreads();
@@ -448,10 +462,10 @@ __global__ void __launch_bounds__(1024) k_norm_rope_dw(const double *partials, i
   }
 }
 
-template <typename T, int VEC, int NS>
+template <typename T, int VEC, int NS, bool ODD>
 int launch(const NormArgs &a, bool inter, bool back, dim3 grid, size_t smem, cudaStream_t st) {
-  const auto kernel = back ? inter ? k_norm_rope<T, VEC, NS, true, true> : k_norm_rope<T, VEC, NS, false, true>
-                           : inter ? k_norm_rope<T, VEC, NS, true, false> : k_norm_rope<T, VEC, NS, false, false>;
+  const auto kernel = back ? inter ? k_norm_rope<T, VEC, NS, true, true, ODD> : k_norm_rope<T, VEC, NS, false, true, ODD>
+                           : inter ? k_norm_rope<T, VEC, NS, true, false, ODD> : k_norm_rope<T, VEC, NS, false, false, ODD>;
   if (smem > 48 * 1024) {
     static std::atomic<uint64_t> set[2]{};
     int device;
@@ -527,16 +541,35 @@ int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st)
   a.tokens = c.tokens; a.heads = c.heads; a.q_heads = c.q_heads; a.dim = c.dim; a.rot = c.rot;
   a.eps = c.eps; a.factor = c.factor; a.w_half = c.weight_dtype == kF16;
   a.partials = sums ? (double *)c.workspace : nullptr;
-  a.lanes_log = 0;
+  a.lanes_log = 0, a.odd = 1;
   while (a.lanes_log < 5 && (slots << a.lanes_log) < units) a.lanes_log++;
   // A block's tokens, as long as every SM gets blocks: eight, or more where their heads
   // are fewer than its groups; then its heads are shared among blocks while there are
   // fewer than two a SM.
-  const int groups = kThreads >> a.lanes_log;
-  a.nt_log = 0;
-  while ((2 << a.nt_log) <= groups && (a.nt_log < 3 || (groups >> a.nt_log) > c.heads) && (c.tokens >> (a.nt_log + 1)) >= 4 * sms) a.nt_log++;
+  int step = 1, groups = 0;
+  auto tokens_log = [&](int lanes) {
+    int n = 0;
+    groups = kThreads / 32 * (32 / lanes);
+    while (groups % (2 << n) == 0 && (n < 3 || (groups >> n) > c.heads) && (c.tokens >> (n + 1)) >= 4 * sms) n++;
+    step = groups >> n;
+    return n;
+  };
+  a.nt_log = tokens_log(1 << a.lanes_log);
+  // Five, six or ten lanes a group, where a block then takes fewer turns over its heads
+  // for as many tokens. (80 dimensions, 32 turned, float32, the gradient of 24001 x 12: ten
+  // lanes 70 us, sixteen 84; 40 heads of 72, float16: 58 and 67. Of vectors of two
+  // values, 40 heads of 80, float32: 91 and 79, their loads are apart.)
+  if (vec >= 4)
+    for (const int lanes : {5, 6, 10})
+      if (lanes < 1 << a.lanes_log && slots * lanes >= units) {
+        const int turns = (c.heads + step - 1) / step, n = tokens_log(lanes);
+        if (n == a.nt_log && (c.heads + step - 1) / step < turns) {
+          a.odd = lanes % 2 ? lanes : lanes / 2, a.lanes_log = lanes % 2 ? 0 : 1;
+          break;
+        }
+        tokens_log(1 << a.lanes_log);
+      }
   const int64_t tiles = (c.tokens + (1 << a.nt_log) - 1) >> a.nt_log;
-  const int step = std::max(1, groups >> a.nt_log);
   int parts = 1;
   while (tiles * parts < 2 * sms && parts < (c.heads + step - 1) / step) parts++;
   a.hb = (c.heads + parts - 1) / parts;
@@ -551,9 +584,13 @@ int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st)
   const bool inter = (c.flags & 1) != 0;
   auto go = [&](auto v, auto n) {
     constexpr int V = decltype(v)::value, N = decltype(n)::value;
+    if constexpr (V >= 4)
+      if (a.odd > 1 && c.dtype == kF16) return launch<__half, V, N, true>(a, inter, back, grid, smem, st);
+    if constexpr (V == 4)
+      if (a.odd > 1) return launch<float, V, N, true>(a, inter, back, grid, smem, st);
     if constexpr (V <= 4)
-      if (c.dtype == kF32) return launch<float, V, N>(a, inter, back, grid, smem, st);
-    return launch<__half, V, N>(a, inter, back, grid, smem, st);
+      if (c.dtype == kF32) return launch<float, V, N, false>(a, inter, back, grid, smem, st);
+    return launch<__half, V, N, false>(a, inter, back, grid, smem, st);
   };
 #define SHLO_INT(n) std::integral_constant<int, n>()
   switch (vec) {

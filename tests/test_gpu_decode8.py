@@ -98,6 +98,39 @@ def test_norm_rope_and_its_gradient(kind, inter, T, HQ, HK, D, R):
     assert torch.equal(again, out)
 
 
+# Heads of nine or ten units (ten lanes), five and six, in float32 or float16, with heads enough for a block's groups.
+UNEVEN = [(2500, 3, 2, 80, 32), (9, 20, 4, 72, 24), (9, 30, 10, 40, 40), (7, 30, 6, 48, 48), (9, 8, 40, 80, 80), (700, 30, 7, 96, 96),
+          (5, 23, 1, 160, 160), (9, 1, 39, 20, 0), (4000, 0, 3, 72, 72)]
+
+
+@pytest.mark.parametrize("kind", ["f16", "f32"])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("T,HQ,HK,D,R", UNEVEN)
+def test_norm_rope_of_heads_that_leave_lanes(kind, inter, T, HQ, HK, D, R):
+    test_norm_rope_and_its_gradient(kind, inter, T, HQ, HK, D, R)
+
+
+def test_norm_rope_of_heads_that_leave_lanes_far_values():
+    """float32 heads whose squares leave binary32's range, beside ones whose do not, ten lanes each."""
+    rng = np.random.default_rng(8)
+    T, H, D, R = 5, 24, 72, 24
+    x, dy = rng.standard_normal((2, T, H, D))
+    x = (x * np.where(rng.random((T, H, 1)) < 0.3, 1e25, 1.0)).astype(np.float32)
+    dy = dy.astype(np.float32)
+    w = (1 + 0.3 * rng.standard_normal(D)).astype(np.float32)
+    pos = rng.integers(0, 5000, T).astype(np.int32)
+    phases, freqs = plan(R)
+    args = dict(q_heads=H, q_weight=cuda(w), k_weight=None, eps=1e-5, stream=stream())
+    out = torch.empty(T, H, D, device="cuda")
+    Dc.norm_rope_noalloc(cuda(x), cuda(pos), cuda(phases), out, **args)
+    eps = np.float64(np.float32(1e-5))
+    want, mag = O8.norm_rope(x, pos, freqs, w, w, H, eps)
+    assert np.all(np.abs(out.cpu().numpy() - want) <= 2.0 ** -19 * mag)
+    Dc.norm_rope_grad_noalloc(cuda(x), cuda(dy), cuda(pos), cuda(phases), out, **args)
+    dx, mag = O8.norm_rope_grad(x, dy, pos, freqs, w, w, H, eps)[:2]
+    assert np.all(np.abs(out.cpu().numpy() - dx) <= 2.0 ** -18 * mag)
+
+
 def test_norm_rope_gradient_is_the_differences():
     """<dy, y(x, w)> by central differences of the 64-bit form: a step of 1e-4 leaves 1e-8 of the third derivative
     and 1e-12 of rounding, against 32-bit gradients to 2^-16."""
