@@ -18,11 +18,11 @@
 //
 // Bound: bytes (each logit read once), then the first kernel's ten instructions a
 // logit. Measured on one B200: 64 sequences of 8 beams over 128256 float16 logits (125
-// MB) 47 us; 5 of 32 over 50257 float32 logits, 64 kept 38 us; one of 4 over 32001 10
-// us. Measured and left: the polynomial for every term (64 us on the first case: the
-// heavy half of the FMA pipe), a part of one stretch each (73 us: every one searches
-// for its border), borders by halving over lists in memory (67 us for the second case's
-// join alone).
+// MB) 46 us, 36 of them the first kernel, at 512 blocks on 592 places; 5 of 32 over 50257
+// float32 logits, 64 kept 27 us; one of 4 over 32001 10 us. Measured and left: the
+// polynomial for every term (64 us on the first case: the heavy half of the FMA pipe), a
+// part of one stretch each (73 us: every one searches for its border), borders by
+// halving over lists in memory (67 us for the second case's join alone).
 #include <algorithm>
 #include <cmath>
 
@@ -730,7 +730,8 @@ Cut cut(int64_t rows, int vocab, size_t size, int sms) {
   const int n = stretches(c.nv);
   // Turns of blocks, four an SM, by the stretches of each, the first of which costs
   // two: its border has to be found. (512 rows of 128256: 47 us at 8 and 16 stretches a
-  // part, 53 at 4, 73 at 1; 160 rows of 50257: 38 us at 1, 47 at 2, 60 at 7.)
+  // part, 53 at 4, 73 at 1; 160 rows of 50257: with a join of 19 us, 38 at 1, 47 at 2,
+  // 60 at 7.)
   const int64_t slots = 4 * (int64_t)sms;
   int64_t least = INT64_MAX;
   c.turns = 1;
@@ -762,6 +763,15 @@ int launch_beam_select(const BeamCall &c, int sms, cudaStream_t st) {
   const size_t size = dtype_size(c.dtype);
   if ((uintptr_t)c.logits % size || ((uintptr_t)c.scores | (uintptr_t)c.ended | (uintptr_t)c.next | (uintptr_t)c.parents | (uintptr_t)c.tokens) % 4)
     return fail("beam_select: an operand is not aligned to its type");
+  // (a sequence's scores are read before its results are written, by the same block)
+  const int64_t out = 4 * (int64_t)c.seqs * c.keep;
+  const bool in_place = (const void *)c.next == c.scores && c.keep == c.beams;
+  for (const void *p : {(const void *)c.next, (const void *)c.parents, (const void *)c.tokens})
+    if ((!(in_place && p == c.next) && meet(p, out, c.scores, 4 * rows)) || meet(p, out, c.ended, 4 * rows) ||
+        meet(p, 1, 0, out, c.logits, rows, c.row * (int64_t)size, c.vocab * (int64_t)size))
+      return fail("beam_select: a result shares memory with an operand (the next scores may be the scores, where as many are kept as there are beams)");
+  if (meet(c.next, out, c.parents, out) || meet(c.next, out, c.tokens, out) || meet(c.parents, out, c.tokens, out))
+    return fail("beam_select: two results share memory");
   const size_t need = beam_work_bytes(rows, c.keep, c.vocab);
   if (!c.workspace || c.workspace_bytes < need) return fail("beam_select: a workspace of %zu bytes, %zu needed", c.workspace ? c.workspace_bytes : 0, need);
   if ((uintptr_t)c.workspace % 8) return fail("beam_select: misaligned workspace");

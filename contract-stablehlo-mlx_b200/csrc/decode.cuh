@@ -24,6 +24,21 @@ int launch_rope(const RopeCall &c, int sms, cudaStream_t st);
 // y [tokens][heads][dim] is x itself with its strides, or shares no value with it.
 int check_in_place(const void *x, int64_t x_token, int64_t x_head, const void *y, int64_t y_token, int64_t y_head, int64_t tokens,
                    int64_t heads, int64_t dim, size_t size, const char *what, const char *x_name, const char *y_name);
+// Whether rows of `bytes` bytes, `step` apart, at p share memory with those at q. (Rows
+// side by side in one buffer do not.)
+inline bool meet(const void *p, int64_t rows, int64_t step, int64_t bytes, const void *q, int64_t q_rows, int64_t q_step, int64_t q_bytes) {
+  if (!p || !q || rows < 1 || q_rows < 1) return false;
+  if (rows == 1) step = q_rows > 1 ? q_step : 0;
+  if (q_rows == 1) q_step = step;
+  const int64_t off = (intptr_t)q - (intptr_t)p;
+  auto low = [](int64_t n, int64_t s) { return s < 0 ? (double)(n - 1) * s : 0.0; };
+  auto high = [](int64_t n, int64_t s) { return s > 0 ? (double)(n - 1) * s : 0.0; };
+  if ((double)off + low(q_rows, q_step) >= high(rows, step) + bytes || (double)off + high(q_rows, q_step) + q_bytes <= low(rows, step)) return false;
+  if (step != q_step || step < 1) return true;
+  const int64_t at = (off % step + step) % step;
+  return at < bytes || at + q_bytes > step;
+}
+inline bool meet(const void *p, int64_t bytes, const void *q, int64_t q_bytes) { return meet(p, 1, 0, bytes, q, 1, 0, q_bytes); }
 
 // (dy: the gradient)
 using NormRopeCall = shlo_norm_rope_args;

@@ -8,8 +8,9 @@
 //            roundings (to binary32, two products, the bias) and the result's own.
 //
 // Rows, bound: bytes, and close behind them 4.7 instructions a value. 8192 rows of 4096
-// float16 (101 MB) 24 us, 4.2 TB/s; 24 rows 3.1 us, a launch and four waits. The product
-// of linear8 begins while they are rounded, with its weights.
+// float16 (101 MB) 26 us, 3.9 TB/s; 5893 rows of 5727 float32, which start at any
+// multiple of 4 bytes (169 MB) 41 us; 24 rows 3.1 us, a launch and four waits. The
+// product of linear8 begins while they are rounded, with its weights.
 #include <algorithm>
 #include <type_traits>
 
@@ -370,6 +371,9 @@ int launch_quantise_rows(const void *x, int64_t x_row, uint8_t dtype, int64_t ro
   if (!x || !q || !scale) return fail("%s: null pointer", what);
   const size_t size = dtype_size(dtype);
   if ((uintptr_t)x % size || (uintptr_t)scale % 4) return fail("%s: an operand is not aligned to its type", what);
+  if (meet(q, rows, q_row, n, x, rows, x_row * (int64_t)size, n * (int64_t)size) || meet(scale, 1, 0, 4 * rows, x, rows, x_row * (int64_t)size, n * (int64_t)size) ||
+      meet(scale, 1, 0, 4 * rows, q, rows, q_row, n))
+    return fail("%s: q, scale and x share memory", what);
   const uintptr_t at = (uintptr_t)x | (rows > 1 ? (uintptr_t)(x_row * (int64_t)size) : 0);
   const int end = fill ? (n + 15) / 16 * 16 : n;
   if (dtype == kF16) {
@@ -387,8 +391,8 @@ int launch_quantise_rows(const void *x, int64_t x_row, uint8_t dtype, int64_t ro
   return launch_check(what);
 }
 
-// What x does not enter into: the weights, the result and the sizes.
-static int check_mul_mat8(const Mm8Call &c, const char *what) {
+// The weights, the result and the sizes; x (of `x_size` bytes a value) where the result may not lie.
+static int check_mul_mat8(const Mm8Call &c, int64_t x_size, const char *what) {
   if (c.dtype != kF16 && c.dtype != kF32) return fail("%s: a result of %s not carried (float16 or float32)", what, dtype_name(c.dtype));
   if (c.rows < 0 || c.rows > (1 << 28) || c.m < 1 || c.n < 1 || c.n > 131071)
     return fail("%s: %lld rows, %d channels of %d values (32-bit sums hold 131071)", what, (long long)c.rows, c.m, c.n);
@@ -398,13 +402,20 @@ static int check_mul_mat8(const Mm8Call &c, const char *what) {
     return fail("%s: rows of w begin on multiples of 16 bytes and do not overlap (a distance of %lld for %d values)", what, (long long)c.w_row, c.n);
   if (c.rows > 1 && c.y_row < c.m) return fail("%s: rows of the result overlap", what);
   if ((uintptr_t)c.w_scale % 4 || (uintptr_t)c.bias % 4 || (uintptr_t)c.y % dtype_size(c.dtype)) return fail("%s: an operand is not aligned to its type", what);
+  const int64_t size = dtype_size(c.dtype);
+  auto hits = [&](const void *p, int64_t rows, int64_t step, int64_t bytes) { return meet(c.y, c.rows, c.y_row * size, c.m * size, p, rows, step, bytes); };
+  if (hits(c.x, c.rows, c.x_row * x_size, c.n * x_size) || hits(c.w, c.m, c.w_row, c.n) || hits(c.w_scale, 1, 0, 4 * (int64_t)c.m) ||
+      hits(c.bias, 1, 0, 4 * (int64_t)c.m))
+    return fail("%s: the result shares memory with an operand", what);
   return 0;
 }
 
 int launch_mul_mat8(const Mm8Call &c, bool after_rows, int *err, int sms, cudaStream_t st) {
-  SHLO_TRY(check_mul_mat8(c, "mul_mat8"));
+  SHLO_TRY(check_mul_mat8(c, 1, "mul_mat8"));
   if (c.rows == 0) return 0;
   if (!c.x || !c.x_scale) return fail("mul_mat8: null pointer");
+  if (meet(c.y, c.rows, c.y_row * (int64_t)dtype_size(c.dtype), c.m * (int64_t)dtype_size(c.dtype), c.x_scale, 1, 0, 4 * c.rows))
+    return fail("mul_mat8: the result shares memory with an operand");
   if ((uintptr_t)c.x % 16 || (c.rows > 1 && (c.x_row % 16 || c.x_row < c.n)))
     return fail("mul_mat8: rows of x begin on multiples of 16 bytes and do not overlap (a distance of %lld for %d values)", (long long)c.x_row, c.n);
   if ((uintptr_t)c.x_scale % 4) return fail("mul_mat8: an operand is not aligned to its type");
@@ -418,8 +429,8 @@ size_t linear8_work_bytes(int64_t rows, int32_t n) { return (size_t)rows * (quan
 
 int launch_linear8(const Mm8Call &call, int *err, int sms, cudaStream_t st) {
   Mm8Call c = call;
-  SHLO_TRY(check_mul_mat8(c, "linear8"));
   if (c.x_dtype != kF16 && c.x_dtype != kF32) return fail("linear8: %s not carried (float16 or float32)", dtype_name(c.x_dtype));
+  SHLO_TRY(check_mul_mat8(c, dtype_size(c.x_dtype), "linear8"));
   if (c.rows == 0) return 0;
   int8_t *const q = (int8_t *)c.workspace;
   if (!q || c.workspace_bytes < linear8_work_bytes(c.rows, c.n))

@@ -502,6 +502,7 @@ int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st)
   if ((uintptr_t)c.dq_weight % 4 || (uintptr_t)c.dk_weight % 4 || (sums && (uintptr_t)c.workspace % 8)) return fail("%s: misaligned gradient or workspace", what);
   if (sums && (!c.workspace || c.workspace_bytes < norm_rope_work_bytes(sms)))
     return fail("%s: a workspace of %zu bytes, %zu needed", what, c.workspace ? c.workspace_bytes : 0, norm_rope_work_bytes(sms));
+  if (sums && meet(c.dq_weight, c.dim * 4, c.dk_weight, c.dim * 4)) return fail("%s: the two weights' gradients share memory", what);
   if (c.tokens == 0) {
     if (c.dq_weight) SHLO_CUDA(cudaMemsetAsync(c.dq_weight, 0, c.dim * sizeof(float), st));
     if (c.dk_weight) SHLO_CUDA(cudaMemsetAsync(c.dk_weight, 0, c.dim * sizeof(float), st));

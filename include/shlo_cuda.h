@@ -263,7 +263,7 @@ int shlo_norm_rope_grad_noalloc(const shlo_norm_rope_args *args, void *stream);
    and scale [rows]: q = 127 x / top to the nearest whole number (of two the even
    one), scale = top / 127, top the row's largest magnitude. A row of zeros has
    scale 0; one with a value that is not finite zeros and scale NaN. Weights
-   [channels][n] are laid out by the same call. */
+   [channels][n] are laid out by the same call. x, q and scale share no memory. */
 int shlo_quantise_rows_noalloc(const void *x, int64_t x_row, int64_t rows, int32_t n, uint8_t dtype, int8_t *q, int64_t q_row,
                                float *scale, void *stream);
 /* y[r][c] = (sum over i < n of x[r][i] w[c][i]) x_scale[r] w_scale[c] + bias[c], for
@@ -304,7 +304,8 @@ int shlo_linear8_noalloc(const shlo_mul_mat8_args *args, void *stream);
    row whose logits hold a NaN or +inf, gives nothing to choose from; where less than
    `keep` is there, the rest has score -inf, parent -1 and token -1. Up to 64 beams
    and 64 kept, a vocabulary of up to 2^20. The workspace (8-byte boundary) holds
-   nothing between calls; calls that may run at once have one each. */
+   nothing between calls; calls that may run at once have one each. next may be
+   scores where keep is beams; else the results share no memory with the operands. */
 typedef struct {
 	const void *logits;
 	int64_t row;
@@ -366,7 +367,7 @@ int shlo_kv_gather_noalloc(const shlo_kv_pool *pool, const int32_t *tables, int6
    the first new row that continues its owner; for each later one its tokens and
    scales are copied into page fresh[r], which no row holds, and that is its last
    page. fresh[r] is not read otherwise. Entries behind a row's last page become -1.
-   out_tables and out_lens share no memory with tables and lens. A host that keeps
+   out_tables and out_lens share no memory with what is read. A host that keeps
    one table for several caches makes the call for each of them. */
 typedef struct {
 	const int32_t *tables, *lens; /* [rows][table_pages], table_stride apart; [rows] */

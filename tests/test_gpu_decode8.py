@@ -241,6 +241,9 @@ def test_norm_rope_refusals():
     for bad in (None, work(8), work(Dc.norm_rope_workspace() + 8)[4:]):
         with pytest.raises(ShloError, match="workspace"):
             Dc.norm_rope_grad_noalloc(x, x, pos, phases, dx, dw[0], dw[1], workspace=bad, **kw)
+    for dq, dk in ((dw[0], dw[0]), (dw.view(-1)[:16], dw.view(-1)[15:31])):
+        with pytest.raises(ShloError, match="share memory"):
+            Dc.norm_rope_grad_noalloc(x, x, pos, phases, dx, dq, dk, workspace=work(Dc.norm_rope_workspace()), **kw)
 
 
 def test_norm_rope_broadcast_operands():
@@ -391,6 +394,37 @@ def test_linear8_no_rows_and_refusals():
                             torch.zeros(1, 131072, dtype=torch.int8, device="cuda"), s[:1], y[:1, :1])
 
 
+def test_8_bits_results_in_operands_memory():
+    """Refused; rows side by side in one buffer are not the same memory."""
+    buf = torch.zeros(40, 256, dtype=torch.float16, device="cuda")
+    buf[:, :64] = torch.randn(40, 64, device="cuda")
+    w, s = torch.ones(64, 64, dtype=torch.int8, device="cuda"), torch.ones(64, device="cuda")
+    ws = work(Dc.linear8_workspace(40, 64))
+    x, y = buf[:, :64], torch.empty(40, 64, dtype=torch.float16, device="cuda")
+    Dc.linear8_noalloc(x, w, s, buf[:, 64:128], workspace=ws, stream=stream())
+    Dc.linear8_noalloc(x, w, s, y, workspace=ws, stream=stream())
+    assert torch.equal(buf[:, 64:128], y)
+    bits = buf.view(torch.int8)
+    for out in (x, buf[:, 32:96], buf[1:, :64], bits[:, :128].view(torch.float16)):
+        with pytest.raises(ShloError, match="shares memory"):
+            Dc.linear8_noalloc(x[:out.shape[0]], w, s, out, workspace=work(Dc.linear8_workspace(40, 64)))
+    for rows in (1, 4):
+        with pytest.raises(ShloError, match="shares memory"):
+            Dc.linear8_noalloc(x[:rows], w, s, x[:rows], workspace=ws)
+    with pytest.raises(ShloError, match="shares memory"):
+        Dc.linear8_noalloc(x, w[:16], s[:16], ws[:2560].view(torch.float16).view(40, 32)[:, :16], workspace=ws)
+    with pytest.raises(ShloError, match="shares memory"):
+        Dc.mul_mat8_noalloc(w[32:], s[:32], w[:16], s[:16], w.view(torch.float16)[:32, :16])
+    q, scale = torch.empty(40, 64, dtype=torch.int8, device="cuda"), torch.empty(40, device="cuda")
+    Dc.quantise_rows_noalloc(x, bits[:, 256:320], scale, stream=stream())
+    Dc.quantise_rows_noalloc(x, q, scale, stream=stream())
+    assert torch.equal(bits[:, 256:320], q)
+    with pytest.raises(ShloError, match="share memory"):
+        Dc.quantise_rows_noalloc(x, bits[:, 64:128], scale)
+    with pytest.raises(ShloError, match="share memory"):
+        Dc.quantise_rows_noalloc(x, q, q.view(-1).view(torch.float32)[:40])
+
+
 # ------------------------------------------------------------ beam_select ----
 
 def select(z, scores, keep, kind, ended=None, end=-1, view=None):
@@ -528,6 +562,27 @@ def test_beam_select_refusals():
                                torch.zeros(2, 65, dtype=torch.int32, device="cuda"), workspace=w)
 
 
+def test_beam_select_in_place_and_shared_results():
+    rng = np.random.default_rng(12)
+    z, scores = rng.standard_normal((6, 300)).astype(np.float32), rng.standard_normal((2, 3)).astype(np.float32)
+    w = work(Dc.beam_workspace(2, 3, 4, 300))
+    i32 = lambda n: torch.zeros(2, n, dtype=torch.int32, device="cuda")  # noqa: E731
+    zz, s, p, t = cuda(z), cuda(scores), i32(3), i32(3)
+    Dc.beam_select_noalloc(zz, s, s, p, t, workspace=w, stream=stream())
+    same((s.cpu().numpy(), p.cpu().numpy(), t.cpu().numpy()), O8.beam(z, scores, 3))
+    buf = torch.zeros(64, device="cuda")
+    ints = buf.view(torch.int32)
+    a, b = buf[:6].view(2, 3), ints[:8].view(2, 4)
+    four = torch.zeros(2, 4, device="cuda")
+    for args in ((zz, a, buf[2:10].view(2, 4), i32(4), i32(4)), (zz, a, four, b, i32(4)), (zz, a, four, i32(4), b),
+                 (zz, a, torch.zeros(2, 3, device="cuda"), ints[:6].view(2, 3), i32(3)), (zz, a, buf[16:24].view(2, 4), ints[20:28].view(2, 4), i32(4)),
+                 (zz, a, four, ints[20:28].view(2, 4), ints[27:35].view(2, 4)), (zz, a, zz.view(-1)[-8:].view(2, 4), i32(4), i32(4))):
+        with pytest.raises(ShloError, match="share"):
+            Dc.beam_select_noalloc(*args, workspace=w)
+    with pytest.raises(ShloError, match="share"):
+        Dc.beam_select_noalloc(zz, cuda(scores), torch.zeros(2, 3, device="cuda"), p, t, ended=p, workspace=w)
+
+
 # ------------------------------------------------------------------- fork ----
 
 @pytest.mark.parametrize("layout", ["heads", "tokens"])
@@ -569,6 +624,24 @@ def test_fork_refusals_and_no_rows():
         Dc.fork_noalloc(pool, t, l, i32(3), i32(2), i32(3, 2), i32(3))
     with pytest.raises(ShloError, match="kv_fork"):
         Dc.fork_noalloc(pool, t, l, i32(3), i32(3), i32(3, 3), i32(3))
+
+
+def test_fork_into_what_it_reads():
+    pool = Dc.Pool(*[torch.zeros(4, 2, 16, 16, dtype=torch.int8, device="cuda") for _ in range(2)],
+                   *[torch.zeros(4, 2, device="cuda") for _ in range(2)])
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    two = i32(3, 2, 2)  # tables and those to come, row by row side by side
+    two[:, 0] = torch.arange(6, device="cuda").view(3, 2) % 4
+    lens, parents = i32(3) + 32, torch.tensor([2, -1, 0], dtype=torch.int32, device="cuda")
+    out = i32(3)
+    Dc.fork_noalloc(pool, two[:, 0], lens, parents, i32(3), two[:, 1], out, stream=stream())
+    assert two[:, 1].tolist() == [[0, 1], [-1, -1], [0, 1]] and out.tolist() == [32, 0, 32]
+    t = i32(5, 2)
+    for args in ((t[:3], lens, parents, i32(3), t[2:], out), (t[:3], lens, parents, i32(3), i32(3, 2), lens),
+                 (t[:3], lens, parents, i32(3), i32(3, 2), parents), (t[:3], lens, parents, out, i32(3, 2), out),
+                 (t[:3], lens, parents, i32(3), t.view(-1)[3:9].view(3, 2), out), (i32(3, 2), lens, parents, i32(3), t[:3], t.view(-1)[4:7])):
+        with pytest.raises(ShloError, match="memory"):
+            Dc.fork_noalloc(pool, *args)
 
 
 # --------------------------------------------------------------- together ----
