@@ -7,10 +7,12 @@
 //            the sum in 32-bit integers, exact for up to 131071 terms; then four
 //            roundings (to binary32, two products, the bias) and the result's own.
 //
-// Rows, bound: bytes, and close behind them 4.7 instructions a value. 8192 rows of 4096
-// float16 (101 MB) 26 us, 3.9 TB/s; 5893 rows of 5727 float32, which start at any
-// multiple of 4 bytes (169 MB) 41 us; 24 rows 3.1 us, a launch and four waits. The
-// product of linear8 begins while they are rounded, with its weights.
+// Rows, bound: bytes, and close behind them ten instructions a value. 8192 rows of 4096
+// float16 (101 MB) 21 us, 4.8 TB/s; 5893 rows of 5727 float32,
+// which start at any multiple of 4 bytes (169 MB) 32 us; 24 rows of 4096 2.4 us, a launch
+// and four waits. Measured: the first of these with 256 threads a row and a check of its
+// end at every vector 27 us, with 64 threads 25, and no checks 21. The product of linear8
+// begins while they are rounded, with its weights.
 #include <algorithm>
 #include <type_traits>
 
@@ -32,32 +34,47 @@ template <> struct Raw<4> { using T = uint32_t; };
 template <> struct Raw<2> { using T = uint16_t; };
 template <> struct Raw<1> { using T = uint8_t; };
 
-// The largest magnitude's bits: those of values that are not finite are above all others'.
-template <int V> __device__ __forceinline__ uint32_t top_bits(const __half (&v)[V]) {
-  if constexpr (V == 8) {
-    const uint4 w = *reinterpret_cast<const uint4 *>(v);
-    const uint32_t m = 0x7fff7fffu, a = __vmaxu2(__vmaxu2(w.x & m, w.y & m), __vmaxu2(w.z & m, w.w & m)), h = max(a & 0xffffu, a >> 16);
-    return h >= 0x7c00u ? 0x7f800000u : __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
-  } else {
-    uint32_t t = 0;
+// The larger of three magnitudes; NaN if one is. (The first is one already.)
+__device__ __forceinline__ float top_of(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// The largest magnitude of what a thread has seen (float16: two of them), and its bits as
+// a float's: those of values that are not finite are above all others'.
+template <typename T> struct Top;
+template <> struct Top<float> {
+  float top = 0.0f;
+  template <int V> __device__ __forceinline__ void see(const float (&v)[V]) {
 #pragma unroll
-    for (int i = 0; i < V; i++) t = max(t, __float_as_uint(fabsf(__half2float(v[i]))));
-    return t;
+    for (int i = 0; i < V; i += 2) top = top_of(top, v[i], v[i + 1]);
   }
-}
-template <int V> __device__ __forceinline__ uint32_t top_bits(const float (&v)[V]) {
-  uint32_t t = 0;
+  __device__ __forceinline__ uint32_t bits() const { return __float_as_uint(fabsf(top)); }
+};
+template <> struct Top<__half> {
+  __half2 top = __half2half2(__ushort_as_half(0));
+  template <int V> __device__ __forceinline__ void see(const __half (&v)[V]) {
 #pragma unroll
-  for (int i = 0; i < V; i++) t = max(t, __float_as_uint(v[i]) & 0x7fffffffu);
-  return t;
-}
+    for (int i = 0; i < V; i += 2) top = __hmax2_nan(top, __habs2(__halves2half2(v[i], v[i + 1])));
+  }
+  __device__ __forceinline__ uint32_t bits() const { return __float_as_uint(fabsf(top_of(0.0f, __low2float(top), __high2float(top)))); }
+};
 
 // V values as the whole numbers nearest to 127 x / top. x times 127 / top is within
 // 2^-23 of that (2^-16 at 127) and mostly decides; it is rounded by an add of 1.5 2^23,
-// whose low byte then is the integer's. Where one of the values is near the middle
-// between two whole numbers (or 127 / top is not a number of 32 bits), 64 bits decide
-// for all: x and top have 24, so the quotient is the middle itself or 2^-33 of it away.
+// whose low byte then is the integer's. A value near the middle between two whole
+// numbers h and h + 1 is decided by 254 |x| against (2 h + 1) top, both exact: of 18 and
+// 19 bits where x has 11, else in 64. Where 127 / top is not a number of 32 bits, a
+// quotient of 64 bits decides: x and top have 24, so it is the middle itself or 2^-33 of
+// it away.
 __device__ __noinline__ int decide(float x, float top) { return (int)rint((double)x * 127.0 / (double)top); }
+template <typename T> __device__ __forceinline__ int middle(float x, float top, float r) {
+  using W = typename std::conditional<sizeof(T) == 2, float, double>::type;
+  const float h = floorf(fabsf(r));
+  const W a = (W)254.0f * (W)fabsf(x), b = (W)(2.0f * h + 1.0f) * (W)top;
+  const int k = (int)h, up = a > b || (a == b && (k & 1));
+  return r < 0.0f ? -(k + up) : k + up;
+}
 template <typename T, int V>
 __device__ __forceinline__ void quantise(const T (&v)[V], float top, float by, uint8_t (&q)[V]) {  // (q on a boundary of four)
   uint32_t m[V];
@@ -68,13 +85,19 @@ __device__ __forceinline__ void quantise(const T (&v)[V], float top, float by, u
     const float2 s = __fadd2_rn(r, make_float2(12582912.0f, 12582912.0f));
     const float2 k = __fadd2_rn(s, make_float2(-12582912.0f, -12582912.0f));
     const float2 d = __ffma2_rn(k, make_float2(-1.0f, -1.0f), r);
-    off = fmaxf(off, fmaxf(fabsf(d.x), fabsf(d.y)));
+    off = top_of(off, d.x, d.y);
     m[j] = __float_as_uint(s.x);
     m[j + 1] = __float_as_uint(s.y);
   }
-  if (!(off < 0.5f - 0x1p-15f) || !(by < 0x1p120f)) {
+  if (sizeof(T) == 4 && !(by < 0x1p120f)) {
 #pragma unroll
     for (int j = 0; j < V; j++) m[j] = (uint32_t)decide(to_f32(v[j]), top);
+  } else if (!(off < 0.5f - 0x1p-15f)) {
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+      const float r = to_f32(v[j]) * by, far = fabsf(r) - floorf(fabsf(r));
+      if (fabsf(far - 0.5f) <= 0x1p-15f) m[j] = (uint32_t)middle<T>(to_f32(v[j]), top, r);
+    }
   }
 #pragma unroll
   for (int j = 0; j < V; j += 4)
@@ -97,32 +120,33 @@ k_quantise_rows(const T *x, int64_t x_row, int64_t rows, int n, int8_t *q, int64
   const bool there = row < rows;
   x += (there ? row : 0) * x_row;
   q += (there ? row : 0) * q_row;
-  const int vecs = there ? (n + V - 1) / V : 0;
+  const int full = there ? n / V : 0;  // vectors; what is left of a row, less than one, has a thread
+  const bool rest = there && n % V && t == full % TPR;
   auto load = [&](int i, T (&v)[V]) {
-    const T *const from = x + (int64_t)i * V;
-    if (i * V + V <= n) {
 #pragma unroll
-      for (int j = 0; j < V; j += EACH) *reinterpret_cast<R *>(v + j) = *reinterpret_cast<const R *>(from + j);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; j++) v[j] = i * V + j < n ? from[j] : T(0.0f);
-    }
+    for (int j = 0; j < V; j += EACH) *reinterpret_cast<R *>(v + j) = *reinterpret_cast<const R *>(x + (int64_t)i * V + j);
   };
   alignas(16) T v[KEEP][V];
-  uint32_t bits = 0;
+  Top<T> most;
 #pragma unroll
-  for (int k = 0; k < KEEP; k++)
-    if (t + k * TPR < vecs) load(t + k * TPR, v[k]);
+  for (int k = 0; k < KEEP; k++) {
 #pragma unroll
-  for (int k = 0; k < KEEP; k++)
-    if (t + k * TPR < vecs) bits = max(bits, top_bits(v[k]));
+    for (int j = 0; j < V; j++) v[k][j] = T(0.0f);
+    if (t + k * TPR < full) load(t + k * TPR, v[k]);
+  }
+  alignas(16) T last[V];
+#pragma unroll
+  for (int j = 0; j < V; j++) last[j] = rest && full * V + j < n ? x[(int64_t)full * V + j] : T(0.0f);
+#pragma unroll
+  for (int k = 0; k < KEEP; k++) most.see(v[k]);
+  most.see(last);
 #pragma unroll 2
-  for (int i = t + KEEP * TPR; i < vecs; i += TPR) {
+  for (int i = t + KEEP * TPR; i < full; i += TPR) {
     alignas(16) T w[V];
     load(i, w);
-    bits = max(bits, top_bits(w));
+    most.see(w);
   }
-  bits = __reduce_max_sync(~0u, bits);
+  uint32_t bits = __reduce_max_sync(~0u, most.bits());
   if (TPR > 32) {
     if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = bits;
     __syncthreads();
@@ -131,29 +155,42 @@ k_quantise_rows(const T *x, int64_t x_row, int64_t rows, int n, int8_t *q, int64
   }
   if (!there) return;
   const float top = __uint_as_float(bits), by = 127.0f / top;
-  const bool finite = bits < 0x7f800000u, any = finite && bits > 0;
+  const bool finite = bits < 0x7f800000u;
   if (t == 0) scale[row] = finite ? top / 127.0f : __uint_as_float(0x7fc00000u);
+  if (!finite || bits == 0) {
+    for (int i = t; i < max(n, fill); i += TPR) q[i] = 0;
+    return;
+  }
+  auto some = [&](int i, const T (&w)[V], int count) {  // of a vector's results the first few, one by one
+    alignas(8) uint8_t b[V];
+    quantise(w, top, by, b);
+#pragma unroll
+    for (int j = 0; j < V; j++)
+      if (j < count) q[(int64_t)i * V + j] = (int8_t)b[j];
+  };
   auto store = [&](int i, const T (&w)[V]) {
     alignas(8) uint8_t b[V];
-#pragma unroll
-    for (int j = 0; j < V; j++) b[j] = 0;
-    if (any) quantise(w, top, by, b);
-    if (wide && i * V + V <= n) {
-      *reinterpret_cast<typename Raw<V>::T *>(q + (int64_t)i * V) = *reinterpret_cast<const typename Raw<V>::T *>(b);
-    } else {
-#pragma unroll
-      for (int j = 0; j < V; j++)
-        if (i * V + j < n) q[(int64_t)i * V + j] = (int8_t)b[j];
-    }
+    quantise(w, top, by, b);
+    *reinterpret_cast<typename Raw<V>::T *>(q + (int64_t)i * V) = *reinterpret_cast<const typename Raw<V>::T *>(b);
   };
+  if (rest) some(full, last, n - full * V);
+  if (wide) {
 #pragma unroll
-  for (int k = 0; k < KEEP; k++)
-    if (t + k * TPR < vecs) store(t + k * TPR, v[k]);
+    for (int k = 0; k < KEEP; k++)
+      if (t + k * TPR < full) store(t + k * TPR, v[k]);
 #pragma unroll 2
-  for (int i = t + KEEP * TPR; i < vecs; i += TPR) {
-    alignas(16) T w[V];
-    load(i, w);
-    store(i, w);
+    for (int i = t + KEEP * TPR; i < full; i += TPR) {
+      alignas(16) T w[V];
+      load(i, w);
+      store(i, w);
+    }
+  } else {
+#pragma unroll 1
+    for (int i = t; i < full; i += TPR) {
+      alignas(16) T w[V];
+      load(i, w);
+      some(i, w, V);
+    }
   }
   for (int i = n + t; i < fill; i += TPR) q[i] = 0;
 }
@@ -162,10 +199,14 @@ template <typename T, int V, int PIECE>
 void launch_rows(const T *x, int64_t x_row, int64_t rows, int n, int8_t *q, int64_t q_row, float *scale, int fill, cudaStream_t st) {
   const bool wide = (uintptr_t)q % V == 0 && (rows == 1 || q_row % V == 0);
   auto go = [&](auto kernel, int per) { kernel<<<(unsigned)((rows + per - 1) / per), kQuantThreads, 0, st>>>(x, x_row, rows, n, q, q_row, scale, fill, wide); };
-  // Threads a row: a warp, or all 256 where that leaves a lane more than it keeps.
+  // Threads a row: a warp, or as many as keep the row; where there are rows for all SMs
+  // few threads with much of it each, whose shares of the work for a row as a whole
+  // are then small.
   const int vecs = (n + V - 1) / V;
   if (vecs <= 64) go(k_quantise_rows<T, V, PIECE, 32, 2>, 8);
   else if (vecs <= 256 && rows > 1024) go(k_quantise_rows<T, V, PIECE, 32, 8>, 8);
+  else if (vecs <= 512 && rows > 2048) go(k_quantise_rows<T, V, PIECE, 64, 8>, 4);
+  else if (vecs <= 1024 && rows > 4096) go(k_quantise_rows<T, V, PIECE, 128, 8>, 2);
   else if (vecs <= 512) go(k_quantise_rows<T, V, PIECE, 256, 2>, 1);
   else if (vecs <= 1024) go(k_quantise_rows<T, V, PIECE, 256, 4>, 1);
   else go(k_quantise_rows<T, V, PIECE, 256, 8>, 1);
@@ -217,32 +258,32 @@ __global__ void __launch_bounds__(kFewThreads, 4) k_linear8_few(const Mm8Call c,
       }
     };
     T v[KEEP][V];
-    uint32_t top = 0;
+    Top<T> most;
 #pragma unroll
     for (int k = 0; k < KEEP; k++)
       if (t + k * TPR < vecs) load(t + k * TPR, v[k]);
 #pragma unroll
     for (int k = 0; k < KEEP; k++)
-      if (t + k * TPR < vecs) top = max(top, top_bits(v[k]));
+      if (t + k * TPR < vecs) most.see(v[k]);
     for (int i = t + KEEP * TPR; i < vecs; i += TPR) {
       T u[V];
       load(i, u);
-      top = max(top, top_bits(u));
+      most.see(u);
     }
-    top = __reduce_max_sync(~0u, top);
+    uint32_t top = __reduce_max_sync(~0u, most.bits());
     if (lane == 0) tops[warp] = top;
     __syncthreads();
-    auto top_of = [&](int row) {
+    auto row_top = [&](int row) {
       uint32_t m = 0;
 #pragma unroll
       for (int i = 0; i < WARPS / R; i++) m = max(m, tops[row * (WARPS / R) + i]);
       return m;
     };
     if (lane < R) {
-      const uint32_t m = top_of(lane);
+      const uint32_t m = row_top(lane);
       scale = m < 0x7f800000u ? __uint_as_float(m) / 127.0f : __uint_as_float(0x7fc00000u);
     }
-    top = top_of(r);
+    top = row_top(r);
     const float by = 127.0f / __uint_as_float(top);
     const bool any = top > 0 && top < 0x7f800000u;
     auto store = [&](int i, const T (&u)[V]) {
