@@ -61,7 +61,8 @@ __device__ __forceinline__ void of_f32(float &d, float f) { d = f; }
 // A lane's part of a head: NS slots of two vectors of VEC values. The first
 // rot / 2 / VEC slots of a head hold pairs (the vectors half the part apart, or
 // side by side); the others two vectors of the part that is not turned, the last
-// of which may have one only.
+// of which may have one only. Side by side, a slot may be turned in part: the pairs
+// of the rest of it are turned by nothing, and rot need be no multiple of anything.
 template <typename T, int VEC, int NS> struct Part {
   T v[NS][2][VEC];
 };
@@ -72,13 +73,18 @@ template <int NS> struct Places {
 
 template <int VEC, int NS, bool INTER>
 __device__ __forceinline__ void places(const NormArgs &a, int L, bool there, int lane, Places<NS> &p) {
-  const int half = a.rot / 2, ru = half / VEC, cv = (a.dim - a.rot) / VEC;
+  const int half = a.rot / 2, ru = (half + VEC - 1) / VEC, cv = INTER ? 0 : (a.dim - a.rot) / VEC;
 #pragma unroll
   for (int s = 0; s < NS; s++) {
     const int u = lane + s * L, c = 2 * (u - ru);
     p.pair[s] = there && u < ru;
-    p.o[s] = !there ? -1 : u < ru ? (INTER ? 2 * VEC : VEC) * u : c < cv ? a.rot + c * VEC : -1;
-    p.o2[s] = !there ? -1 : u < ru ? p.o[s] + (INTER ? VEC : half) : c + 1 < cv ? a.rot + (c + 1) * VEC : -1;
+    if (INTER) {
+      p.o[s] = there && 2 * VEC * u < a.dim ? 2 * VEC * u : -1;
+      p.o2[s] = there && 2 * VEC * u + VEC < a.dim ? 2 * VEC * u + VEC : -1;
+    } else {
+      p.o[s] = !there ? -1 : u < ru ? VEC * u : c < cv ? a.rot + c * VEC : -1;
+      p.o2[s] = !there ? -1 : u < ru ? p.o[s] + half : c + 1 < cv ? a.rot + (c + 1) * VEC : -1;
+    }
   }
 }
 template <typename T, int VEC, int NS>
@@ -168,8 +174,8 @@ __global__ void __launch_bounds__(kThreads, BACK && NS * VEC <= 4 ? kBackBlocksP
   // the end the block's sums, [warp][dim], in their place.
   extern __shared__ double sh[];
   constexpr int P = NS * VEC / 2, AHEAD = BACK ? 1 : 4;  // heads asked for beside the one in hand
-  const int half = a.rot / 2, nt = 1 << a.nt_log;
-  float *const cs = reinterpret_cast<float *>(sh + (BACK ? 8 * P * kThreads : 0)), *const sn = cs + nt * half;
+  const int half = a.rot / 2, row = (half + VEC - 1) / VEC * VEC, nt = 1 << a.nt_log;  // (row: a token's cosines)
+  float *const cs = reinterpret_cast<float *>(sh + (BACK ? 8 * P * kThreads : 0)), *const sn = cs + nt * row;
   const int warp = threadIdx.x / 32, wl = threadIdx.x % 32;
   const int L = ODD ? a.odd << a.lanes_log : 1 << a.lanes_log, in_warp = ODD ? 32 / L : 32 >> a.lanes_log;  // groups
   const int lane = ODD ? wl % L : wl & (L - 1), base = wl - lane, group = ODD ? warp * in_warp + wl / L : (int)threadIdx.x >> a.lanes_log;
@@ -224,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, BACK && NS * VEC <= 4 ? kBackBlocksP
     float cc[2 * P], ss[2 * P];
 #pragma unroll
     for (int i = 0; i < 2 * P; i += V) {
-      const int slot = i / VEC, p = t * half + (lane + slot * L) * VEC + i % VEC;
+      const int slot = i / VEC, p = t * row + (lane + slot * L) * VEC + i % VEC;
 #pragma unroll
       for (int j = 0; j < V; j++) cc[i + j] = 1.0f, ss[i + j] = 0.0f;
       if (at.pair[slot]) {
@@ -263,8 +269,8 @@ __global__ void __launch_bounds__(kThreads, BACK && NS * VEC <= 4 ? kBackBlocksP
     }
   };
   // (pair and token of this thread's angles, kThreads apart)
-  const int tt_first = half ? (int)threadIdx.x / half : 0, p_first = (int)threadIdx.x - tt_first * half;
-  const int dt = half ? kThreads / half : 0, dp = kThreads - dt * half;
+  const int tt_first = row ? (int)threadIdx.x / row : 0, p_first = (int)threadIdx.x - tt_first * row;
+  const int dt = row ? kThreads / row : 0, dp = kThreads - dt * row;
   const float inv_dim = 1.0f / a.dim;
   const int64_t tiles = (a.tokens + nt - 1) >> a.nt_log;
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
@@ -286,17 +292,21 @@ __global__ void __launch_bounds__(kThreads, BACK && NS * VEC <= 4 ? kBackBlocksP
       }
     }
     if (BACK && tile != (int64_t)blockIdx.x) __syncthreads();
-    for (int i = threadIdx.x, p = p_first, tt = tt_first; i < nt * half; i += kThreads) {
+    for (int i = threadIdx.x, p = p_first, tt = tt_first; i < nt * row; i += kThreads) {
       if (t0 + tt < a.tokens) {
-        const int64_t turns = (int64_t)((uint64_t)(int64_t)a.pos[t0 + tt] * (uint64_t)a.phases[p]) >> 32;
-        float s, c;
-        sincospif((float)turns * 0x1p-31f, &s, &c);
-        cs[i] = c * a.factor;
-        sn[i] = s * a.factor;
+        float s = 0.0f, c = 1.0f;
+        if (!INTER || p < half) {
+          const int64_t turns = (int64_t)((uint64_t)(int64_t)a.pos[t0 + tt] * (uint64_t)a.phases[p]) >> 32;
+          sincospif((float)turns * 0x1p-31f, &s, &c);
+          c *= a.factor;
+          s *= a.factor;
+        }
+        cs[i] = c;
+        sn[i] = s;
       }
       p += dp;
       tt += dt;
-      if (p >= half) p -= half, tt++;
+      if (p >= row) p -= row, tt++;
     }
     __syncthreads();
     // Forward: what a pair's two results take of its two values, weight and turn in
@@ -517,15 +527,18 @@ int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st)
   SHLO_TRY(check_in_place(c.x, c.x_token, c.x_head, c.y, c.y_token, c.y_head, c.tokens, c.heads, c.dim, size, what, "x", back ? "dx" : "y"));
   if (back)
     SHLO_TRY(check_in_place(c.dy, c.dy_token, c.dy_head, c.y, c.y_token, c.y_head, c.tokens, c.heads, c.dim, size, what, "dy", "dx"));
-  // The widest vector (16 bytes at most) that every offset is a multiple of.
+  // The widest vector (16 bytes at most) that every offset is a multiple of. (40 heads of
+  // 72, 18 turned, float16, pairs side by side: 36 us with eight values, which needs no
+  // half of them to be whole vectors, 105 with one; the gradient 73 and 280.)
   const int half = c.rot / 2, rest = c.dim - c.rot;
+  const bool inter = (c.flags & 1) != 0;
   int vec = (int)(16 / size);
   const bool strided_h = c.heads > 1, strided_t = c.tokens > 1;
   auto fits = [&](int v) {
     auto row = [&](const void *p, int64_t token, int64_t head) {
       return (uintptr_t)p % (v * size) == 0 && (!strided_t || token % v == 0) && (!strided_h || head % v == 0);
     };
-    return half % v == 0 && rest % v == 0 && row(c.x, c.x_token, c.x_head) && row(c.y, c.y_token, c.y_head) && (!back || row(c.dy, c.dy_token, c.dy_head));
+    return (inter ? c.dim % v == 0 : half % v == 0 && rest % v == 0) && row(c.x, c.x_token, c.x_head) && row(c.y, c.y_token, c.y_head) && (!back || row(c.dy, c.dy_token, c.dy_head));
   };
   while (vec > 1 && !fits(vec)) vec /= 2;
   // A lane's slots: 8 / vec of them (as many as its registers are made for) where
@@ -533,7 +546,7 @@ int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st)
   // all lanes; else as few as hold the head in 32 lanes. (750000 tokens' heads of 72, 36
   // turned, float16: 45 us with four slots and 84 with one; 55000 tokens of one such
   // head: 57 and 42.)
-  const int units = half / vec + (rest / vec + 1) / 2;
+  const int units = inter ? (c.dim / vec + 1) / 2 : half / vec + (rest / vec + 1) / 2;
   const bool narrow = c.dtype == kF16 ? vec <= 4 : vec <= 2;
   const int slots = vec == 8 ? 1 : units > 32 || (narrow && c.heads >= 4) ? 8 / vec : vec == 1 ? 2 : 1;
   NormArgs a;
@@ -577,12 +590,11 @@ int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st)
   dim3 grid((unsigned)tiles, (unsigned)((c.heads + a.hb - 1) / a.hb));
   // The backward pass has as many blocks as run at once, each with a row of sums.
   if (back) grid.x = (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, (slots * vec > 4 ? 2 * sms : back_blocks(sms)) / grid.y));
-  size_t smem = (size_t)(1 << a.nt_log) * half * 2 * sizeof(float);
+  size_t smem = (size_t)(1 << a.nt_log) * ((half + vec - 1) / vec * vec) * 2 * sizeof(float);
   if (back) smem = std::max(smem, (size_t)(kThreads / 32) * c.dim * sizeof(double)) + (size_t)slots * vec * 4 * kThreads * sizeof(double);
   a.w_wide = true;
   for (const void *w : {c.q_weight, c.k_weight})
     if ((uintptr_t)w % (vec * wsize > 16 ? 16 : vec * wsize)) a.w_wide = false;
-  const bool inter = (c.flags & 1) != 0;
   auto go = [&](auto v, auto n) {
     constexpr int V = decltype(v)::value, N = decltype(n)::value;
     if constexpr (V >= 4)

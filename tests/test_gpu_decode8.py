@@ -98,9 +98,10 @@ def test_norm_rope_and_its_gradient(kind, inter, T, HQ, HK, D, R):
     assert torch.equal(again, out)
 
 
-# Heads of nine or ten units (ten lanes), five and six, in float32 or float16, with heads enough for a block's groups.
+# Heads of nine or ten units (ten lanes), five and six, in float32 or float16, with heads enough for a block's groups; a
+# turned part that ends inside a vector.
 UNEVEN = [(2500, 3, 2, 80, 32), (9, 20, 4, 72, 24), (9, 30, 10, 40, 40), (7, 30, 6, 48, 48), (9, 8, 40, 80, 80), (700, 30, 7, 96, 96),
-          (5, 23, 1, 160, 160), (9, 1, 39, 20, 0), (4000, 0, 3, 72, 72)]
+          (5, 23, 1, 160, 160), (9, 1, 39, 20, 0), (4000, 0, 3, 72, 72), (2500, 3, 2, 72, 18), (3000, 2, 0, 20, 6), (1300, 5, 1, 66, 34)]
 
 
 @pytest.mark.parametrize("kind", ["f16", "f32"])
