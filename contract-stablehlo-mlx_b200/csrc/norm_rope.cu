@@ -10,8 +10,8 @@
 // Bound: bytes (each value read once and written once), and close behind them the
 // instructions. A group of 1 to 32 lanes holds a head in registers; it keeps one token
 // and goes over heads, so that its pairs' cosines and sines, and the weight, stay in
-// registers too (forward: their products); heads to come are asked for ahead, four of
-// them forward and one backward. Two pairs go through each packed instruction.
+// registers too (forward: their products); heads to come are asked for ahead, up to four
+// of them forward and one backward. Two pairs go through each packed instruction.
 // Measured on one B200: 16384 tokens x 40 heads x 128, float16 (336 MB) 63 us, 5.3 TB/s
 // (rope.cu alone 55); the gradient of 24001 x 12 x 80 float32, 32 dimensions turned in
 // interleaved pairs (277 MB) 70 us, 3.9 TB/s: ten units of eight values a head, on ten
@@ -167,13 +167,17 @@ __device__ __forceinline__ void unpairs(const float2 (&a)[NS * VEC / 2], const f
 
 // BACK: the gradient. A block goes over tiles of 2^nt_log tokens, one in the
 // forward pass, for the heads of its part. ODD: a group's lanes are not a power of two;
-// a warp's last lanes may have no group.
-template <typename T, int VEC, int NS, bool INTER, bool BACK, bool ODD>
-__global__ void __launch_bounds__(kThreads, BACK && NS * VEC <= 4 ? kBackBlocksPerSm : 2) k_norm_rope(const NormArgs a) {
+// a warp's last lanes may have no group. FEW: a group has few heads of a token, and more
+// blocks take the place of heads asked for ahead.
+constexpr int blocks_per_sm(int values, bool back, bool few) {
+  return back ? (values <= 4 ? kBackBlocksPerSm : 2) : values <= 4 ? (few ? 4 : 3) : (few ? 3 : 2);
+}
+template <typename T, int VEC, int NS, bool INTER, bool BACK, bool ODD, bool FEW>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(NS * VEC, BACK, FEW)) k_norm_rope(const NormArgs a) {
   // Backward: 8 P sums a thread; then the cosines and sines, [token][half] each, and at
   // the end the block's sums, [warp][dim], in their place.
   extern __shared__ double sh[];
-  constexpr int P = NS * VEC / 2, AHEAD = BACK ? 1 : 4;  // heads asked for beside the one in hand
+  constexpr int P = NS * VEC / 2, AHEAD = BACK ? 1 : P <= 2 ? 2 : FEW ? 1 : 4;  // heads asked for beside the one in hand
   const int half = a.rot / 2, row = (half + VEC - 1) / VEC * VEC, nt = 1 << a.nt_log;  // (row: a token's cosines)
   float *const cs = reinterpret_cast<float *>(sh + (BACK ? 8 * P * kThreads : 0)), *const sn = cs + nt * row;
   const int warp = threadIdx.x / 32, wl = threadIdx.x % 32;
@@ -473,9 +477,10 @@ __global__ void __launch_bounds__(1024) k_norm_rope_dw(const double *partials, i
 }
 
 template <typename T, int VEC, int NS, bool ODD>
-int launch(const NormArgs &a, bool inter, bool back, dim3 grid, size_t smem, cudaStream_t st) {
-  const auto kernel = back ? inter ? k_norm_rope<T, VEC, NS, true, true, ODD> : k_norm_rope<T, VEC, NS, false, true, ODD>
-                           : inter ? k_norm_rope<T, VEC, NS, true, false, ODD> : k_norm_rope<T, VEC, NS, false, false, ODD>;
+int launch(const NormArgs &a, bool inter, bool back, bool few, dim3 grid, size_t smem, cudaStream_t st) {
+  const auto kernel = back ? inter ? k_norm_rope<T, VEC, NS, true, true, ODD, false> : k_norm_rope<T, VEC, NS, false, true, ODD, false>
+                      : few ? inter ? k_norm_rope<T, VEC, NS, true, false, ODD, true> : k_norm_rope<T, VEC, NS, false, false, ODD, true>
+                            : inter ? k_norm_rope<T, VEC, NS, true, false, ODD, false> : k_norm_rope<T, VEC, NS, false, false, ODD, false>;
   if (smem > 48 * 1024) {
     static std::atomic<uint64_t> set[2]{};
     int device;
@@ -587,6 +592,11 @@ int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st)
   int parts = 1;
   while (tiles * parts < 2 * sms && parts < (c.heads + step - 1) / step) parts++;
   a.hb = (c.heads + parts - 1) / parts;
+  // (us: 16384 x 40 x 128 float16, 20 turns, 64 with four heads ahead and two blocks on an
+  // SM, 70 with one and three; of 3 heads of 64, one turn, 68 and 56; 40 heads of 64, five,
+  // 30 and 32; 7 of 256, four, 25 and 23. Four values a lane, 40 heads of 128 float32, 20
+  // turns, 47 with three blocks and 51 with four; of 80, 14 turns, 51 and 48.)
+  const bool few = (a.hb + step - 1) / step <= (slots * vec > 4 ? 4 : 14);
   dim3 grid((unsigned)tiles, (unsigned)((c.heads + a.hb - 1) / a.hb));
   // The backward pass has as many blocks as run at once, each with a row of sums.
   if (back) grid.x = (unsigned)std::max<int64_t>(1, std::min<int64_t>(tiles, (slots * vec > 4 ? 2 * sms : back_blocks(sms)) / grid.y));
@@ -598,12 +608,12 @@ int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st)
   auto go = [&](auto v, auto n) {
     constexpr int V = decltype(v)::value, N = decltype(n)::value;
     if constexpr (V >= 4)
-      if (a.odd > 1 && c.dtype == kF16) return launch<__half, V, N, true>(a, inter, back, grid, smem, st);
+      if (a.odd > 1 && c.dtype == kF16) return launch<__half, V, N, true>(a, inter, back, few, grid, smem, st);
     if constexpr (V == 4)
-      if (a.odd > 1) return launch<float, V, N, true>(a, inter, back, grid, smem, st);
+      if (a.odd > 1) return launch<float, V, N, true>(a, inter, back, few, grid, smem, st);
     if constexpr (V <= 4)
-      if (c.dtype == kF32) return launch<float, V, N, false>(a, inter, back, grid, smem, st);
-    return launch<__half, V, N, false>(a, inter, back, grid, smem, st);
+      if (c.dtype == kF32) return launch<float, V, N, false>(a, inter, back, few, grid, smem, st);
+    return launch<__half, V, N, false>(a, inter, back, few, grid, smem, st);
   };
 #define SHLO_INT(n) std::integral_constant<int, n>()
   switch (vec) {
