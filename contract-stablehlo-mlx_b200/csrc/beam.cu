@@ -65,6 +65,7 @@ __device__ __forceinline__ float of_ordered(uint32_t u) {
   return __uint_as_float(u ^ ((int32_t)u < 0 ? 0x80000000u : 0xffffffffu));
 }
 constexpr uint32_t kNegInf = 0x007fffffu;  // ordered(-infinity)
+constexpr uint32_t kInf = 0xff800000u;     // ordered(infinity): above it is NaN alone
 
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -324,7 +325,8 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_parts(const BeamArgs a) {
     __syncthreads();
     if (n > kRoom) {
       // More of them than there is room for (many equal ones, or rows that rise): the
-      // exact border of these stretches, and which of the logits that equal it.
+      // exact border of these stretches, and which of the logits that equal it. (What is
+      // not a number was no candidate and is none here: all of them would have no room.)
       auto counted = [&](uint32_t t, uint32_t last) {  // logits above t, and those at t whose ~token is at least last
         int c = 0;
         for (int at = group; at < group_end; at += STRETCH)
@@ -334,7 +336,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_parts(const BeamArgs a) {
 #pragma unroll
             for (int j = 0; j < W; j++) {
               const uint32_t u = ordered(V::value(w, j));
-              if (u > t || (u == t && (uint32_t)~token(at, i, j) >= last)) c++;
+              if ((u > t && u <= kInf) || (u == t && (uint32_t)~token(at, i, j) >= last)) c++;
             }
           }
         c = __reduce_add_sync(~0u, c);
@@ -346,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_parts(const BeamArgs a) {
         for (int i = 0; i < kWarps; i++) c += __float_as_int(tops[i]);
         return c;
       };
-      uint32_t t0 = least, t1 = 0xff800001u;  // enough reach t0; t1 is above all numbers
+      uint32_t t0 = least, t1 = kInf + 1;  // enough reach t0; t1 is above all numbers
       while (t1 - t0 > 1) {
         const uint32_t mid = t0 + (t1 - t0) / 2;
         if (counted(mid, 0) >= a.keep) t0 = mid;
@@ -368,11 +370,14 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_parts(const BeamArgs a) {
 #pragma unroll
           for (int j = 0; j < W; j++) {
             const uint32_t u = ordered(V::value(w, j)), last = ~token(at, i, j);
-            if (u > t0 || (u == t0 && last >= l0)) found[atomicAdd(&count, 1)] = (uint64_t)u << 32 | last;
+            if ((u > t0 && u <= kInf) || (u == t0 && last >= l0)) {
+              const int k = atomicAdd(&count, 1);
+              if (k < kRoom) found[k] = (uint64_t)u << 32 | last;
+            }
           }
         }
       __syncthreads();
-      n = count;
+      n = min(count, kRoom);
       __syncthreads();
     }
     // The best of them, in order; later stretches' candidates are above the last (of

@@ -1,0 +1,53 @@
+"""The norm with rotation, the products in 8 bits, beam search's selection and the cache's reordering on the GPU where
+values, masks or memory are unusual; the tolerances of tests/test_gpu_decode8.py, whose helpers these use, unless a test
+says otherwise."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+import decode8_oracle as O8  # noqa: E402
+from shlo import mlx as M  # noqa: E402
+from test_gpu_decode8 import NP, same, select  # noqa: E402
+
+
+@pytest.fixture(scope="module", autouse=True)
+def device():
+    torch.cuda.set_device(0)
+    M.set_device(0)
+    yield
+    torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------ beam_select ----
+
+def not_numbers(z, rows, lo, hi, rng):
+    """NaNs of both signs in columns lo to hi, of the rows' type."""
+    nan = np.copysign(np.nan, rng.choice([-1.0, 1.0, 1.0], (len(rows), hi - lo)))
+    z[rows, lo:hi] = nan.astype(z.dtype)
+
+
+@pytest.mark.parametrize("kind", ["f16", "f32"])
+@pytest.mark.parametrize("seqs,beams,v", [(1, 4, 8192), (64, 8, 41003), (1, 2, 3000), (2, 3, 131072)])
+def test_beam_select_of_many_nans_beside_equal_logits(kind, seqs, beams, v):
+    """More equal logits than a block has room for, and more NaNs: at the beginning, in later stretches, everywhere,
+    in every other place. Their rows give nothing, the others what they gave."""
+    rng = np.random.default_rng(v)
+    z = rng.standard_normal((seqs * beams, v)).astype(NP[kind])
+    odd = np.arange(0, seqs * beams, 2)
+    for i, r in enumerate(odd):
+        r = np.array([r])
+        z[r] = [0, -3, 5][i % 3]
+        where = [(0, v // 2), (v // 2, v), (v // 4, v // 4 + 600), (0, v), (v - 700, v)][i % 5]
+        if i % 7 == 6:
+            z[r, ::2] = np.nan
+        else:
+            not_numbers(z, r, *where, rng)
+        if i % 11 == 10:
+            z[r, :v // 3] = np.inf
+    z[1] = 2.0
+    scores = -rng.random((seqs, beams)).astype(np.float32)
+    for keep in (1, 8, 64):
+        same(select(z, scores, keep, kind), O8.beam(z, scores, keep))
