@@ -460,7 +460,7 @@ int shlo_linear8(shlo_arr x, shlo_arr x_scale, shlo_arr w, shlo_arr w_scale, shl
   SHLO_TRY(whole(dev, w_scale, what, "w_scale", held, &s));
   if (x->ndim != 2 || w->ndim != 2 || w->dtype != kI8) return fail("%s: x is not [rows, values], or w not int8 [channels, values]", what);
   const int64_t rows = x->shape[0], n = x->shape[1], m = w->shape[0], row = (n + 15) / 16 * 16;
-  if (n < 1 || n > 131071 || m < 1 || m > 0x7fffffff || rows > (1 << 28)) return fail("%s: %lld rows, %lld channels of %lld values", what, (long long)rows, (long long)m, (long long)n);
+  if (n < 1 || n > 131071 || m < 1 || m > (1 << 30) || rows > (1 << 28)) return fail("%s: %lld rows, %lld channels of %lld values", what, (long long)rows, (long long)m, (long long)n);
   if (w->shape[1] != row) return fail("%s: rows of w of %lld values, x's %lld and zeros up to a multiple of 16 expected", what, (long long)w->shape[1], (long long)n);
   SHLO_TRY(shaped(w_scale, kF32, {m}, what, "w_scale"));
   if (bias) {

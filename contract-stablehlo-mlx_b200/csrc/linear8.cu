@@ -435,8 +435,9 @@ int launch_quantise_rows(const void *x, int64_t x_row, uint8_t dtype, int64_t ro
 // The weights, the result and the sizes; x (of `x_size` bytes a value) where the result may not lie.
 static int check_mul_mat8(const Mm8Call &c, int64_t x_size, const char *what) {
   if (c.dtype != kF16 && c.dtype != kF32) return fail("%s: a result of %s not carried (float16 or float32)", what, dtype_name(c.dtype));
-  if (c.rows < 0 || c.rows > (1 << 28) || c.m < 1 || c.n < 1 || c.n > 131071)
-    return fail("%s: %lld rows, %d channels of %d values (32-bit sums hold 131071)", what, (long long)c.rows, c.m, c.n);
+  // (the kernels count channels in 32 bits, up to a grid's or a tile's beyond the last)
+  if (c.rows < 0 || c.rows > (1 << 28) || c.m < 1 || c.m > (1 << 30) || c.n < 1 || c.n > 131071)
+    return fail("%s: %lld rows, %d channels (at most 2^30) of %d values (32-bit sums hold 131071)", what, (long long)c.rows, c.m, c.n);
   if (c.rows == 0) return 0;
   if (!c.w || !c.w_scale || !c.y) return fail("%s: null pointer", what);
   if ((uintptr_t)c.w % 16 || (c.m > 1 && (c.w_row % 16 || c.w_row < c.n)))

@@ -267,10 +267,10 @@ int shlo_norm_rope_grad_noalloc(const shlo_norm_rope_args *args, void *stream);
 int shlo_quantise_rows_noalloc(const void *x, int64_t x_row, int64_t rows, int32_t n, uint8_t dtype, int8_t *q, int64_t q_row,
                                float *scale, void *stream);
 /* y[r][c] = (sum over i < n of x[r][i] w[c][i]) x_scale[r] w_scale[c] + bias[c], for
-   `rows` rows and m channels; y of `dtype`, y_row values apart, bias float32 [m] or
-   NULL. The sum is exact (32-bit integers; n up to 131071). w begins on a 16-byte
-   boundary and has rows a multiple of 16 bytes apart; what lies between rows is not
-   read. y shares no memory with the operands. */
+   `rows` rows (up to 2^28) and m channels (up to 2^30); y of `dtype`, y_row values
+   apart, bias float32 [m] or NULL. The sum is exact (32-bit integers; n up to
+   131071). w begins on a 16-byte boundary and has rows a multiple of 16 bytes apart;
+   what lies between rows is not read. y shares no memory with the operands. */
 typedef struct {
 	const void *x;
 	int64_t x_row; /* in values */
