@@ -105,6 +105,8 @@ def _workspace(x, at):
             _elsewhere(x, at)
     except AttributeError:
         _elsewhere(x, at)
+    if not x.is_contiguous():  # (its values are fewer bytes, or others, than it names)
+        raise ShloError("a workspace that is not contiguous")
     return x.data_ptr(), x.numel() * x.element_size()
 
 
@@ -213,18 +215,14 @@ def attend_noalloc(pool: Pool, q, starts, lens, tables, out, *, workspace, scale
     if m != n or do != dt:
         raise ShloError("kv_attend: out is not q's shape and type")
     lp = None
-    try:
-        if workspace.get_device() != at:
-            _elsewhere(workspace, at)
-    except AttributeError:
-        _elsewhere(workspace, at)
+    wp, wn = _workspace(workspace, at)
     if lse is not None:
         if _code(lse, at) != _F32 or lse.shape != (t, h) or (t and h and not lse.is_contiguous()):
             raise ShloError("kv_attend: lse is not a contiguous float32 [%d, %d]" % (t, h))
         lp = lse.data_ptr()
     check(lib.shlo_kv_attend_noalloc(c, _batch(starts, lens, tables, t, at), q.data_ptr(), qs[0], qs[1], h, dt, scale,
                                      1 if causal else 0, window, out.data_ptr(), os_[0], os_[1], lp,
-                                     workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream))
+                                     wp, wn, stream))
 
 
 def _weights(q_weight, k_weight, q_heads, h, d, what, at):
