@@ -780,6 +780,10 @@ int launch_beam_select(const BeamCall &c, int sms, cudaStream_t st) {
   const size_t need = beam_work_bytes(rows, c.keep, c.vocab);
   if (!c.workspace || c.workspace_bytes < need) return fail("beam_select: a workspace of %zu bytes, %zu needed", c.workspace ? c.workspace_bytes : 0, need);
   if ((uintptr_t)c.workspace % 8) return fail("beam_select: misaligned workspace");
+  bool used = meet(c.workspace, 1, 0, (int64_t)need, c.logits, rows, c.row * (int64_t)size, c.vocab * (int64_t)size) ||
+              meet(c.workspace, (int64_t)need, c.scores, 4 * rows) || meet(c.workspace, (int64_t)need, c.ended, 4 * rows);
+  for (const void *p : {(const void *)c.next, (const void *)c.parents, (const void *)c.tokens}) used = used || meet(c.workspace, (int64_t)need, p, out);
+  if (used) return fail("beam_select: the workspace shares memory with an operand or a result");
   const Cut how = cut(rows, c.vocab, size, sms);
   BeamArgs a;
   a.z = c.logits; a.row = c.row; a.scores = c.scores; a.ended = c.ended; a.next = c.next; a.parents = c.parents; a.tokens = c.tokens;

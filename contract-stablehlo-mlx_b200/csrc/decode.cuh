@@ -1,5 +1,8 @@
 // The decoder operators' calls inside the library: rotary positions (rope.cu),
-// the 8-bit paged cache (kv_cache.cu) and the attention over it (kv_attend.cu).
+// the 8-bit paged cache (kv_cache.cu) and the attention over it (kv_attend.cu),
+// the norm of queries and keys with the rotation (norm_rope.cu), products in 8-bit
+// integers (linear8.cu, linear8_tiles.cu), beam search's selection (beam.cu) and the
+// reordering of the cache after it (kv_fork.cu).
 // The C entry points on caller-owned memory and those on arrays both end here.
 #pragma once
 
@@ -39,6 +42,19 @@ inline bool meet(const void *p, int64_t rows, int64_t step, int64_t bytes, const
   return at < bytes || at + q_bytes > step;
 }
 inline bool meet(const void *p, int64_t bytes, const void *q, int64_t q_bytes) { return meet(p, 1, 0, bytes, q, 1, 0, q_bytes); }
+// The same of [tokens][heads] rows at p, and `q_bytes` bytes at q.
+inline bool meet(const void *p, int64_t tokens, int64_t token, int64_t heads, int64_t head, int64_t bytes, const void *q, int64_t q_bytes) {
+  if (!p || !q || tokens < 1 || heads < 1) return false;
+  const char *x = static_cast<const char *>(p);
+  if (token < 0) x += (tokens - 1) * token, token = -token;
+  if (head < 0) x += (heads - 1) * head, head = -head;
+  const double off = (double)((intptr_t)q - (intptr_t)x);
+  if (off >= (double)(tokens - 1) * token + (double)(heads - 1) * head + bytes || off + q_bytes <= 0.0) return false;
+  const bool by_heads = heads <= tokens;  // the shorter axis is gone through
+  for (int64_t i = 0; i < (by_heads ? heads : tokens); i++)
+    if (by_heads ? meet(x + i * head, tokens, token, bytes, q, 1, 0, q_bytes) : meet(x + i * token, heads, head, bytes, q, 1, 0, q_bytes)) return true;
+  return false;
+}
 
 // (dy: the gradient)
 using NormRopeCall = shlo_norm_rope_args;

@@ -479,6 +479,11 @@ int launch_linear8(const Mm8Call &call, int *err, int sms, cudaStream_t st) {
     return fail("linear8: a workspace of %zu bytes, %zu needed", q ? c.workspace_bytes : 0, linear8_work_bytes(c.rows, c.n));
   if ((uintptr_t)q % 16) return fail("linear8: the workspace does not begin on a multiple of 16 bytes");
   if (!c.x) return fail("linear8: null pointer");
+  const int64_t need = (int64_t)linear8_work_bytes(c.rows, c.n), x_size = dtype_size(c.x_dtype), y_size = dtype_size(c.dtype);
+  auto hits = [&](const void *p, int64_t rows, int64_t step, int64_t bytes) { return meet(q, 1, 0, need, p, rows, step, bytes); };
+  if (hits(c.x, c.rows, c.x_row * x_size, c.n * x_size) || hits(c.w, c.m, c.w_row, c.n) || hits(c.w_scale, 1, 0, 4 * (int64_t)c.m) ||
+      hits(c.bias, 1, 0, 4 * (int64_t)c.m) || hits(c.y, c.rows, c.y_row * y_size, c.m * y_size))
+    return fail("linear8: the workspace shares memory with an operand or the result");
   if ((uintptr_t)c.x % dtype_size(c.x_dtype)) return fail("linear8: an operand is not aligned to its type");
   if (few(c) && few_round(c)) {
     if (c.x_dtype == kF16) return c.dtype == kF16 ? launch_few<__half, __half>(c, false, sms, st) : launch_few<__half, float>(c, false, sms, st);

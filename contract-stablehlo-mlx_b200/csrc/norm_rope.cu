@@ -518,6 +518,27 @@ int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st)
   if (sums && (!c.workspace || c.workspace_bytes < norm_rope_work_bytes(sms)))
     return fail("%s: a workspace of %zu bytes, %zu needed", what, c.workspace ? c.workspace_bytes : 0, norm_rope_work_bytes(sms));
   if (sums && meet(c.dq_weight, c.dim * 4, c.dk_weight, c.dim * 4)) return fail("%s: the two weights' gradients share memory", what);
+  // What is written beside the rows, against what is read, and the rows against that.
+  const int64_t w_bytes = c.dim * (int64_t)wsize, work = sums ? (int64_t)norm_rope_work_bytes(sms) : 0;
+  const struct { const void *p; int64_t bytes; } small[4] = {
+      {c.q_weight, w_bytes}, {c.k_weight, w_bytes}, {c.rot ? c.positions : nullptr, 4 * c.tokens}, {c.rot ? c.phases : nullptr, 4 * (int64_t)c.rot}};
+  auto in_rows = [&](const void *p, int64_t bytes) {
+    auto rows = [&](const void *x, int64_t token, int64_t head) {
+      return meet(x, c.tokens, token * (int64_t)size, c.heads, head * (int64_t)size, c.dim * (int64_t)size, p, bytes);
+    };
+    return rows(c.x, c.x_token, c.x_head) || rows(c.y, c.y_token, c.y_head) || (back && rows(c.dy, c.dy_token, c.dy_head));
+  };
+  const struct { const void *p; int64_t bytes; } made[3] = {{back ? c.dq_weight : nullptr, 4 * (int64_t)c.dim}, {back ? c.dk_weight : nullptr, 4 * (int64_t)c.dim}, {sums ? c.workspace : nullptr, work}};
+  for (const auto &m : made) {
+    bool used = in_rows(m.p, m.bytes);
+    for (const auto &i : small) used = used || meet(m.p, m.bytes, i.p, i.bytes);
+    if (used) return fail("%s: a weight's gradient or the workspace shares memory with an operand or dx", what);
+  }
+  if (sums && (meet(c.workspace, work, c.dq_weight, 4 * (int64_t)c.dim) || meet(c.workspace, work, c.dk_weight, 4 * (int64_t)c.dim)))
+    return fail("%s: a weight's gradient shares memory with the workspace", what);
+  for (const auto &i : small)
+    if (meet(c.y, c.tokens, c.y_token * (int64_t)size, c.heads, c.y_head * (int64_t)size, c.dim * (int64_t)size, i.p, i.bytes))
+      return fail("%s: %s shares memory with a weight, positions or phases", what, back ? "dx" : "y");
   if (c.tokens == 0) {
     if (c.dq_weight) SHLO_CUDA(cudaMemsetAsync(c.dq_weight, 0, c.dim * sizeof(float), st));
     if (c.dk_weight) SHLO_CUDA(cudaMemsetAsync(c.dk_weight, 0, c.dim * sizeof(float), st));

@@ -254,8 +254,9 @@ int shlo_norm_rope_workspace(size_t *bytes);
 /* Its gradient: dx of x's type from dy of the same type (dx may be x or dy itself;
    else it shares no value with them), and the weights', sums over all tokens and
    their heads. The workspace (8-byte boundary) holds nothing between calls (NULL
-   without the weights' gradients); calls that may run at once have one each. The
-   same call gives the same bits. */
+   without the weights' gradients); calls that may run at once have one each. What is
+   written shares no memory with what else is read or written. The same call gives
+   the same bits. */
 int shlo_norm_rope_grad_noalloc(const shlo_norm_rope_args *args, void *stream);
 
 /* Products in 8-bit integers with a scale for each row of both sides. Rows of n
@@ -289,8 +290,8 @@ typedef struct {
 /* Of x in int8 with its scales, laid out as w is (no workspace; x_dtype is not read). */
 int shlo_mul_mat8_noalloc(const shlo_mul_mat8_args *args, void *stream);
 /* Of activations of `x_dtype`, rounded row by row into the workspace (begins on a
-   16-byte boundary; it holds nothing between calls; calls that may run at once have
-   one each; x_scale is not read). */
+   16-byte boundary; it holds nothing between calls, and shares no memory with the
+   operands or y; calls that may run at once have one each; x_scale is not read). */
 int shlo_linear8_workspace(int64_t rows, int32_t n, size_t *bytes);
 int shlo_linear8_noalloc(const shlo_mul_mat8_args *args, void *stream);
 
@@ -305,7 +306,8 @@ int shlo_linear8_noalloc(const shlo_mul_mat8_args *args, void *stream);
    `keep` is there, the rest has score -inf, parent -1 and token -1. Up to 64 beams
    and 64 kept, a vocabulary of up to 2^20. The workspace (8-byte boundary) holds
    nothing between calls; calls that may run at once have one each. next may be
-   scores where keep is beams; else the results share no memory with the operands. */
+   scores where keep is beams; else the results and the workspace share no memory
+   with the operands or each other. */
 typedef struct {
 	const void *logits;
 	int64_t row;

@@ -9,7 +9,7 @@ torch = pytest.importorskip("torch")
 import test_decode8_host as H  # noqa: E402
 import test_decode_devices as Hd  # noqa: E402
 from shlo import mlx as M  # noqa: E402
-from shlo._lib import MUL_MAT8_ARGS, ShloError, load  # noqa: E402
+from shlo._lib import BEAM_ARGS, MUL_MAT8_ARGS, NORM_ROPE_ARGS, ShloError, load  # noqa: E402
 from test_decode8_host import calls  # noqa: E402, F401
 
 # (with a device what is not refused would run, on addresses where nothing lies)
@@ -50,6 +50,83 @@ def test_more_channels_than_are_counted(entry, rows):
     assert product(entry, rows=rows) == ""
     for m in ((1 << 30) + 1, (1 << 31) - 4736, (1 << 31) - 1):
         assert "at most 2^30" in product(entry, rows=rows, m=m, y_row=m)
+
+
+# Operands of 5 rows of 64 float32 values (or 8-bit ones), 100 channels.
+@pytest.mark.parametrize("rows", [1, 5])
+@pytest.mark.parametrize("name,at,length", [("x", FAR, 64 * 4), ("w", 3 * FAR, 99 * 64 + 64), ("w_scale", 4 * FAR, 400), ("bias", 5 * FAR, 400),
+                                            ("y", 6 * FAR, 400)])
+def test_linear8_workspace_in_other_memory(rows, name, at, length):
+    need = rows * (64 + 4) + 16
+    length += (rows - 1) * {"x": 256, "y": 400}.get(name, 0)
+    inside = [at - need // 16 * 16, at, at + (length - 1) // 16 * 16]
+    for work in inside:
+        assert "workspace shares memory" in product("linear8", rows=rows, work=work, work_bytes=need)
+    for work in (at - (need + 15) // 16 * 16, at + (length + 15) // 16 * 16):
+        assert product("linear8", rows=rows, work=work, work_bytes=need) == ""
+    # (what lies behind the bytes that are needed is the caller's)
+    assert product("linear8", rows=rows, work=at - (need + 15) // 16 * 16, work_bytes=1 << 30) == ""
+
+
+def beam(**change):
+    a = dict(logits=FAR, row=1000, scores=2 * FAR, ended=3 * FAR, next=4 * FAR, parents=5 * FAR, tokens=6 * FAR, work=7 * FAR,
+             work_bytes=1 << 30, seqs=2, beams=3, keep=4, vocab=1000, end=-1, dtype=M.dtF32)
+    a.update(change)
+    return launch("_ZN4shlo18launch_beam_selectERK14shlo_beam_argsiP11CUstream_st", BEAM_ARGS.pack(*a.values()), SMS, None)
+
+
+@pytest.mark.parametrize("at,length", [(FAR, 6 * 4000), (2 * FAR, 24), (3 * FAR, 24), (4 * FAR, 32), (5 * FAR, 32), (6 * FAR, 32)])
+def test_beam_workspace_in_other_memory(at, length):
+    n = ctypes.c_size_t()
+    assert load().shlo_beam_workspace(2, 3, 4, 1000, ctypes.byref(n)) == 0
+    need = n.value
+    for work in (at, at - need // 8 * 8 + 8, at + length - 8):
+        assert "workspace shares memory" in beam(work=work, work_bytes=need)
+    for work in (at - (need + 7) // 8 * 8, at + length):
+        assert beam(work=work, work_bytes=need) == ""
+    assert beam(work=FAR + 4000, work_bytes=need, row=1000 + (need + 3) // 4 * 2) == ""  # between rows
+
+
+def norm_rope(back, **change):
+    a = dict(x=FAR, x_token=4 * 16, x_head=16, positions=2 * FAR, phases=3 * FAR, wq=4 * FAR, wk=5 * FAR, y=6 * FAR, y_token=4 * 16, y_head=16,
+             dy=7 * FAR, dy_token=4 * 16, dy_head=16, dq=8 * FAR, dk=9 * FAR, work=10 * FAR, work_bytes=1 << 30, tokens=3, heads=4, dim=16,
+             rot=8, q_heads=2, eps=1e-6, factor=1.0, flags=0, dtype=M.dtF32, wtype=M.dtF16)
+    a.update(change)
+    return launch("_ZN4shlo16launch_norm_ropeERK19shlo_norm_rope_argsbiP11CUstream_st", NORM_ROPE_ARGS.pack(*a.values()), back, SMS, None)
+
+
+ROWS = 3 * 4 * 16 * 4
+
+
+@pytest.mark.parametrize("at,length", [(FAR, ROWS), (2 * FAR, 12), (3 * FAR, 32), (4 * FAR, 32), (5 * FAR, 32), (6 * FAR, ROWS), (7 * FAR, ROWS)])
+def test_norm_rope_grad_sums_in_other_memory(at, length):
+    """The weights' gradients and the workspace in x, positions, phases, the weights, dx, dy, or each other."""
+    need = 3 * SMS * 2 * 512 * 8  # (shlo_norm_rope_workspace's)
+    assert norm_rope(True, work_bytes=need - 1) != "" and norm_rope(True, work_bytes=need) == ""
+    last = at + (length - 1) // 8 * 8
+    for name, size in (("dq", 64), ("dk", 64), ("work", need)):
+        for p in (at, last, at - size + 8):
+            assert "shares memory" in norm_rope(True, **{name: p})
+        for p in (at + (length + 7) // 8 * 8, at - size):
+            assert norm_rope(True, **{name: p}) == ""
+        assert norm_rope(False, **{name: at}) == ""  # (the forward pass has none)
+    for name in ("dq", "dk"):
+        assert "shares memory" in norm_rope(True, work=9 * FAR if name == "dk" else 8 * FAR)
+        assert norm_rope(True, **{name: FAR + 32}, x_head=24, x_token=96) != ""  # in the first head's second half
+        assert norm_rope(True, **{name: FAR + 64}, x_head=32, x_token=128) == ""  # between two heads
+        assert norm_rope(True, **{name: FAR + 64 - 4 * 32}, x_head=-32, x_token=128) == ""
+        assert norm_rope(True, **{name: FAR - 4 * 32}, x_head=-32, x_token=128) != ""
+
+
+@pytest.mark.parametrize("back", [False, True])
+@pytest.mark.parametrize("name,length", [("positions", 12), ("phases", 32), ("wq", 32), ("wk", 32)])
+def test_norm_rope_rows_in_what_is_read(back, name, length):
+    for off in (0, 8, ROWS - 8, 8 - length):
+        assert "shares memory" in norm_rope(back, **{name: 6 * FAR + off})
+    for off in (ROWS, -length - length % 8):
+        assert norm_rope(back, **{name: 6 * FAR + off}) == ""
+    assert norm_rope(back, **{name: 6 * FAR + 64}, y_head=32, y_token=128) == ""
+    assert (norm_rope(back, **{name: 6 * FAR}, rot=0) == "") == (name in ("positions", "phases"))  # (then they are not read)
 
 
 # ---- of the Python forms ----
