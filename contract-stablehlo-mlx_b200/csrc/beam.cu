@@ -420,13 +420,14 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_parts(const BeamArgs a) {
   }
   const int64_t place = (int64_t)row * a.parts + blockIdx.x;
   uint64_t *const best = a.best + place * a.keep;
-  if (n == a.keep) {  // (in order already)
-    if ((int)threadIdx.x < n) best[threadIdx.x] = found[threadIdx.x];
-  } else {
+  if (n < a.keep) {  // (else in order already; the order is the sum's below too, and not that of the atomics)
     uint64_t k[2];
     const int above = rank(n, k).x;  // (fewer than keep: one a thread)
-    if (above < a.keep) best[above] = k[0];
+    __syncthreads();
+    if (above < n) found[above] = k[0];
+    __syncthreads();
   }
+  if ((int)threadIdx.x < n) best[threadIdx.x] = found[threadIdx.x];
   for (int i = n + threadIdx.x; i < a.keep; i += kThreads) best[i] = 0;
   // The part's sum, the candidates' terms by the polynomial.
   if ((int)threadIdx.x < n) {

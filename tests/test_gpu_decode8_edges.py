@@ -51,3 +51,22 @@ def test_beam_select_of_many_nans_beside_equal_logits(kind, seqs, beams, v):
     scores = -rng.random((seqs, beams)).astype(np.float32)
     for keep in (1, 8, 64):
         same(select(z, scores, keep, kind), O8.beam(z, scores, keep))
+
+
+@pytest.mark.parametrize("kind", ["f16", "f32"])
+@pytest.mark.parametrize("seqs,beams,v,left", [(8, 8, 5000, 3), (40, 16, 5000, 20), (20, 40, 8000, 60), (64, 8, 41003, 33)])
+def test_beam_select_equal_rows_with_few_logits_left(kind, seqs, beams, v, left):
+    """Rows of which a mask leaves fewer than are kept, the same for all beams of a sequence: their sums are the same bits,
+    so that the lowest beam comes first, and two calls give the same. (Terms far below the largest: sums of a few near ones
+    are exact in 64 bits, in any order.)"""
+    rng = np.random.default_rng(left)
+    z = np.full((seqs, 1, v), -np.inf, NP[kind])
+    for s in range(seqs):
+        z[s, 0, rng.choice(v, left, replace=False)] = -45 * rng.random(left)
+    z = np.repeat(z, beams, 1).reshape(seqs * beams, v)
+    scores = np.repeat(-rng.random((seqs, 1)).astype(np.float32), beams, 1)
+    want = O8.beam(z, scores, 64)
+    first = select(z, scores, 64, kind)
+    assert np.array_equal(first[1], want[1]) and np.array_equal(first[2], want[2])
+    for _ in range(50):
+        assert all(np.array_equal(a, b) for a, b in zip(select(z, scores, 64, kind), first))
