@@ -4,17 +4,22 @@
 // in descending order, of equal ones the lowest beam first, then the lowest token.
 //
 // Two kernels. The first gives a block a part of a row, which it reads once, a stretch
-// of registers at a time: each thread's largest logit so far and the sum of
-// e^(logit - largest), and the part's `keep` largest logits, of which the first
-// stretch gives a border that few of the later ones pass. The second joins a
-// sequence's parts: a row's sum, then its parts' lists.
+// of registers at a time: each thread's sum of e^(logit - largest), the largest of the
+// first stretch or of what the thread has seen since, and the part's `keep` largest
+// logits, of which the first stretch gives a border that few of the later ones pass. The
+// second joins a sequence's parts: a row's sum, then its parts' lists.
 //
 // Two beams' continuations may lie closer together than binary32 tells apart, and
-// the order between them is part of the result. A term of the sum is ex2.approx's,
-// within 2^-22, eight of them are added in binary32 and the rest in 64 bits; the
-// terms of the candidates, which are most of a peaked row's sum, are replaced by a
-// polynomial's, right to 2^-24. What is left is 2^-22 of the light terms' share, and
-// averages out where they are many.
+// the order between them is part of the result. A term of the sum is ex2.approx's, off
+// by 2.1 10^-7 of it at most where it lies up to 2 above or below what is counted from
+// (farther down by more, but of less), eight of them are added in binary32 and the rest
+// in 64 bits; the terms of the candidates, which are most of a peaked row's sum, are
+// replaced by a polynomial's, off by 7 10^-8. What is left is that share of the light
+// terms, which averages out where they are many and not equal. (A thread counts from a
+// logit of its own where that is more than 2 above the first stretch's largest: a plateau
+// 57 above that would move the logarithm by 3 10^-6. Of 512 rows of 128256 normal logits,
+// us: from the first stretch's alone 47.3, from beyond 2 above it 47.9, from any above it
+// 49.4.)
 //
 // Bound: bytes (each logit read once), then the first kernel's ten instructions a
 // logit. Measured on one B200: 64 sequences of 8 beams over 128256 float16 logits (125
@@ -24,6 +29,7 @@
 // part of one stretch each (73 us: every one searches for its border), borders by
 // halving over lists in memory (67 us for the second case's join alone).
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "decode.cuh"
@@ -49,7 +55,7 @@ struct BeamArgs {
   const int32_t *ended;
   float *next;
   int32_t *parents, *tokens;
-  uint64_t *best;  // [rows][parts][keep]: ordered logit above, ~token below; 0: none
+  uint64_t *best;  // [rows][parts][keep]: entries; 0: none
   double *sum;     // [rows][parts]
   float *top;      // [rows][parts]: what the sum counts from; NaN: a value that is not a number, or infinity
   int vocab, beams, keep, parts, part, end_token;  // part: logits a part
@@ -78,7 +84,8 @@ __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
 // e^d for -87 <= d <= 87: d = i ln 2 + r (ln 2 rounded: 2.7 10^-9 of d), e^r = 1 + r +
 // r^2 g(r), g of degree 4 fitted to the smallest largest relative error (2^-28,
-// 3 10^-10 on average).
+// 3 10^-10 on average). With its roundings, over all d: 3 10^-8 up to |d| = 0.06, 6.8
+// 10^-8 up to 2, 1.1 10^-7 up to 16, 2.8 10^-7 up to 80.
 __device__ __forceinline__ float2 exp_near(float2 d) {
   const float2 m = __ffma2_rn(d, both(0x1.715476p+0f), both(12582912.0f));
   const float2 i = __fadd2_rn(m, both(-12582912.0f));
@@ -95,7 +102,10 @@ __device__ __forceinline__ float2 exp_near(float2 d) {
   return g;
 }
 
-// The same within 2^-22, and 0 for -infinity: 2^(d log2(e)), the product in two parts.
+// The same for d <= kRise, 1 for 0 and 0 for -infinity: 2^(d log2(e)), the product in two
+// parts. What its roundings lose grows with d: over all d 1.8 10^-7 up to |d| = 1, 2.1
+// 10^-7 up to 2, 2.7 10^-7 up to 4, 4.9 10^-7 up to 8, 9.3 10^-7 up to 16. (A factor for what
+// is lost would hold it at 2 10^-7, and costs 2 us of 47 for 512 rows of 128256.)
 __device__ __forceinline__ float2 exp_fast(float2 d) {
   const float2 t = __ffma2_rn(d, both(0x1.4ae0c0p-26f), __fmul2_rn(d, both(0x1.715476p+0f)));
   float2 e;
@@ -103,6 +113,40 @@ __device__ __forceinline__ float2 exp_fast(float2 d) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
   return e;
 }
+constexpr float kRise = 2.0f;
+
+// What a candidate's term is more by the polynomial than by the other.
+__device__ __forceinline__ double replaced(float d) {
+  const float2 near = make_float2(fmaxf(d, -80.0f), 0.0f);
+  return (double)exp_near(near).x - (double)exp_fast(near).x;
+}
+
+// A sum counted from `from`, counted from `to` above it: times e^d, by the power series
+// of degree 9 (8 10^-12; a call of exp takes four times as long, which all wait for).
+// (Both are rare: their code is not the loop's.)
+__device__ __noinline__ double recounted(double sum, float from, float to) {
+  const double d = fmax((double)from - (double)to, -600.0), i = rint(d * 1.4426950408889634), r = fma(i, -0.69314718055994531, d);
+  double p = 1.0 / 362880.0;
+  p = fma(p, r, 1.0 / 40320.0);
+  p = fma(p, r, 1.0 / 5040.0);
+  p = fma(p, r, 1.0 / 720.0);
+  p = fma(p, r, 1.0 / 120.0);
+  p = fma(p, r, 1.0 / 24.0);
+  p = fma(p, r, 1.0 / 6.0);
+  p = fma(p, r, 0.5);
+  p = fma(p, r, 1.0);
+  p = fma(p, r, 1.0);
+  return sum * __hiloint2double(__double2hiint(p) + ((int)i << 20), __double2loint(p));
+}
+__device__ __noinline__ double replaced_apart(float d) { return d < 0.0f ? replaced(d) : 0.0; }
+
+// A candidate: in the order of the logits, of equal ones the lowest token first; the
+// lowest bit is no part of the order (tokens are below 2^20), and says that its term is
+// the polynomial's already. 0 is below all.
+__device__ __forceinline__ uint64_t entry_of(float logit, int token, bool done) {
+  return (uint64_t)ordered(logit) << 32 | (uint32_t)~token << 1 | (uint32_t)done;
+}
+__device__ __forceinline__ int token_of(uint64_t e) { return (int)(~(uint32_t)e >> 1); }
 
 // What a type's vectors of 16 bytes need: the largest of their values (NaN where
 // one is), their values less the largest of all, the values themselves.
@@ -149,6 +193,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_parts(const BeamArgs a) {
   __shared__ uint64_t found[kRoom];
   __shared__ int count;
   __shared__ uint32_t least_shared;
+  __shared__ float first_top;
   const int row = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   if (a.ended && a.ended[row]) return;  // it goes on with one token, whatever its logits
   const T *const z = static_cast<const T *>(a.z) + row * a.row;
@@ -228,9 +273,9 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_parts(const BeamArgs a) {
   __shared__ uint4 ahead[NV * kThreads];
   int asked = -1;
   double sum = 0.0;        // the sum of e^(logit - from) over this thread's logits,
-  float from = -INFINITY;  // the first stretch's largest
-  bool odd = false;        // whether one is not a number, or infinity,
-  bool far = false;        // or too far above `from`
+  float from = -INFINITY;  // the first stretch's largest, or one of the thread's own more than kRise above it
+  bool odd = false;        // whether one is not a number, or infinity
+  int risen = INT_MAX;     // the stretch that has the first such of its own
   uint32_t least = 0;     // candidates are the logits that reach this, in order
   int n = 0;              // candidates so far
   if (threadIdx.x == 0) count = 0;
@@ -283,6 +328,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_parts(const BeamArgs a) {
           low = fminf(low, lows[i]);
         }
         from = top;
+        if (threadIdx.x == 0) first_top = top;
         uint32_t over = ordered(top) + 1;
         least = low > -INFINITY ? ordered(low) : kNegInf + 1;
         int have = __syncthreads_count(key >= least);
@@ -295,7 +341,11 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_parts(const BeamArgs a) {
           }
       }
 
-      far = far || mine > from + 60.0f;
+      if (mine > from + kRise) {
+        sum = recounted(sum, from, mine);
+        from = mine;
+        risen = min(risen, lo);
+      }
       sum += exps(v, from);
 
       if (key >= least) {
@@ -314,7 +364,8 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_parts(const BeamArgs a) {
           for (int j = 0; j < W; j++)
             if (V::value(w, j) >= border) {
               const int k = atomicAdd(&count, 1);
-              if (k < kRoom) found[k] = (uint64_t)ordered(V::value(w, j)) << 32 | (uint32_t)~token(lo, i, j);
+              if (k < kRoom) found[k] = entry_of(V::value(w, j), token(lo, i, j), risen <= lo);
+              if (risen <= lo) sum += replaced_apart(V::value(w, j) - from);
             }
         }
       }
@@ -372,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_parts(const BeamArgs a) {
             const uint32_t u = ordered(V::value(w, j)), last = ~token(at, i, j);
             if ((u > t0 && u <= kInf) || (u == t0 && last >= l0)) {
               const int k = atomicAdd(&count, 1);
-              if (k < kRoom) found[k] = (uint64_t)u << 32 | last;
+              if (k < kRoom) found[k] = entry_of(V::value(w, j), token(at, i, j), risen <= at);
             }
           }
         }
@@ -396,30 +447,6 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_parts(const BeamArgs a) {
     }
   }
 
-  // A row whose first stretch is far below what follows (or masked) is added up once
-  // more, from its largest.
-  if (__syncthreads_or(far)) {
-    float most = -INFINITY;
-    for (int lo = begin; lo < end; lo += STRETCH)
-#pragma unroll 1
-      for (int i = 0; i < NV; i++) most = fmaxf(most, V::top(load(lo, i)));
-#pragma unroll
-    for (int i = 16; i; i /= 2) most = fmaxf(most, __shfl_xor_sync(~0u, most, i));
-    if (lane == 0) tops[warp] = most;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kWarps; i++) most = fmaxf(most, tops[i]);
-    from = most;
-    sum = 0.0;
-    for (int lo = begin; lo < end; lo += STRETCH) {
-      uint4 v[NV];
-#pragma unroll
-      for (int i = 0; i < NV; i++) v[i] = load(lo, i);
-      sum += exps(v, from);
-    }
-  }
-  const int64_t place = (int64_t)row * a.parts + blockIdx.x;
-  uint64_t *const best = a.best + place * a.keep;
   if (n < a.keep) {  // (else in order already; the order is the sum's below too, and not that of the atomics)
     uint64_t k[2];
     const int above = rank(n, k).x;  // (fewer than keep: one a thread)
@@ -427,13 +454,19 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_parts(const BeamArgs a) {
     if (above < n) found[above] = k[0];
     __syncthreads();
   }
+  // The candidates' terms by the polynomial. A thread's own sum is the first stretch's
+  // with it, a risen thread's candidates are done.
+  double more = 0.0;
+  if ((int)threadIdx.x < n && !(found[threadIdx.x] & 1)) more = replaced(of_ordered((uint32_t)(found[threadIdx.x] >> 32)) - first_top);
+  // All from the part's largest logit, if a thread has risen to it: it is a candidate.
+  const float largest = n ? of_ordered((uint32_t)(found[0] >> 32)) : first_top, most = largest > first_top + kRise ? largest : first_top;
+  if (from < most) sum = recounted(sum, from, most);
+  if (first_top < most && more != 0.0) more = recounted(more, first_top, most);
+  sum += more;
+  const int64_t place = (int64_t)row * a.parts + blockIdx.x;
+  uint64_t *const best = a.best + place * a.keep;
   if ((int)threadIdx.x < n) best[threadIdx.x] = found[threadIdx.x];
   for (int i = n + threadIdx.x; i < a.keep; i += kThreads) best[i] = 0;
-  // The part's sum, the candidates' terms by the polynomial.
-  if ((int)threadIdx.x < n) {
-    const float d = of_ordered((uint32_t)(found[threadIdx.x] >> 32)) - from;
-    sum += (double)exp_near(make_float2(fmaxf(d, -80.0f), 0.0f)).x - (double)exp_fast(make_float2(d, 0.0f)).x;
-  }
 #pragma unroll
   for (int i = 16; i; i /= 2) sum += __shfl_xor_sync(~0u, sum, i);
   if (lane == 0) sums[warp] = sum;
@@ -443,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_beam_parts(const BeamArgs a) {
 #pragma unroll
     for (int i = 0; i < kWarps; i++) all += sums[i];
     a.sum[place] = all;
-    a.top[place] = odd ? __uint_as_float(0x7fc00000u) : from;
+    a.top[place] = odd ? __uint_as_float(0x7fc00000u) : most;
   }
 }
 
@@ -527,7 +560,7 @@ __global__ void __launch_bounds__(kJoin) k_beam_join(const BeamArgs a) {
     const int64_t to = (int64_t)seq * a.keep + i;
     a.next[to] = l < 0 ? -INFINITY : (float)t;
     a.parents[to] = l < 0 ? -1 : seq * a.beams + (l >> 16);
-    a.tokens[to] = l < 0 ? -1 : k == ~0ull ? a.end_token : (int32_t)~(uint32_t)k;
+    a.tokens[to] = l < 0 ? -1 : k == ~0ull ? a.end_token : token_of(k);
   };
   // The best of this thread's heads.
   double total;

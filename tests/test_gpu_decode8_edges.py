@@ -67,6 +67,39 @@ def test_beam_select_equal_rows_with_few_logits_left(kind, seqs, beams, v, left)
     scores = np.repeat(-rng.random((seqs, 1)).astype(np.float32), beams, 1)
     want = O8.beam(z, scores, 64)
     first = select(z, scores, 64, kind)
-    assert np.array_equal(first[1], want[1]) and np.array_equal(first[2], want[2])
+    same(first, want)
     for _ in range(50):
         assert all(np.array_equal(a, b) for a, b in zip(select(z, scores, 64, kind), first))
+
+
+@pytest.mark.parametrize("kind", ["f16", "f32"])
+@pytest.mark.parametrize("rise", [3, 10, 30, 57.22, 59.9])
+def test_beam_select_rows_that_rise(kind, rise):
+    """Rows that a block goes over in several turns, which rise above the first: plateaus of equal logits, more than are
+    kept, that begin in a later turn; the same in steps; single logits and noise up there. The scores cancel the
+    logarithm, so that its error is what is left: 2^-23."""
+    rng = np.random.default_rng(int(rise))
+    seqs, v = 512, 41003
+    z = (rng.standard_normal((seqs, v)) * 0.3).astype(NP[kind])
+    z[0::4, 20000:] = rise
+    z[1::4, 9000:] = rise / 3
+    z[1::4, 18000:] = rise
+    z[2::4, 20000:] += NP[kind](rise)
+    z[3::4, 30001] = rise
+    z[4::8, 2000:2003] = rise  # (in the first turn too: what follows is no higher)
+    z[5::8, :17000] = -np.inf
+    l = z.astype(np.float64)
+    top = l.max(1, keepdims=True)
+    lse = top[:, 0] + np.log(np.exp(l - top).sum(1))
+    scores = (lse - top[:, 0]).astype(np.float32)[:, None]
+    want = O8.beam(z, scores, 64)
+    # A plateau no more than 2 above the first turn's largest is counted from that: a term is then off by 2.06 10^-7 at
+    # most (ex2.approx and the roundings of its argument, over all arguments up to 2; 2^-22 is 2.38 10^-7), and equal
+    # terms add up without rounding, so the logarithm is off by 2^-22 at most.
+    first = l[:, :8192].max(1)
+    near = (top[:, 0] > first) & (top[:, 0] <= first + 2.1)
+    for keep in (1, 8, 64):
+        got, w = select(z, scores, keep, kind), [a[:, :keep] for a in want]
+        same([a[~near] for a in got], [a[~near] for a in w])
+        assert all(np.array_equal(a[near], b[near]) for a, b in zip(got[1:], w[1:]))
+        assert np.all(np.abs(got[0][near] - w[0][near]) <= 2.0 ** -22 + 2.0 ** -24 * np.abs(w[0][near]))
