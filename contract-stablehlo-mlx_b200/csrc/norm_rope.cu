@@ -28,6 +28,7 @@ namespace shlo {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kRun = 16;  // heads of a token that the weights' gradients are summed over in binary32
 constexpr int kBackBlocksPerSm = 3;  // the backward pass's, with four pairs a lane or fewer (eight need the registers of two)
 
 struct NormArgs {
@@ -248,8 +249,12 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NS * VEC, BACK, FEW)) 
       s[i] = make_float2(ss[2 * i], ss[2 * i + 1]);
     }
   };
-  // Backward: a weight, and the sums of its gradient over a few heads; then they go to
-  // the thread's sums in 64 bits, [weight][4 P], in shared memory.
+  // Backward: a weight, and the sums of its gradient over kRun heads of a token at most;
+  // then they go to the thread's sums in 64 bits, [weight][4 P], in shared memory, also
+  // where the next heads are of the same kind (us, sums of the same kind kept over all
+  // tokens and not: 16384 x 32 x 128 float16 98 and 100, 55000 x 1 x 64 21.1 and 22.4;
+  // kept over up to 16 heads of several tokens 24001 x 12 x 80 float32 would take 77
+  // instead of 69.5).
   float2 dwa[BACK ? P : 1], dwb[BACK ? P : 1], wa[BACK ? P : 1], wb[BACK ? P : 1];
   double *const sums = reinterpret_cast<double *>(sh) + threadIdx.x;
   int has = -1;  // whose weight is in registers: 0 the queries', 1 the keys'
@@ -324,108 +329,111 @@ __global__ void __launch_bounds__(kThreads, blocks_per_sm(NS * VEC, BACK, FEW)) 
       has = -1;
     }
     // (a warp's groups take the same number of turns: its shuffles name all lanes)
-    for (int h = h0; h < h1; h += AHEAD * h_step) {
+    for (int h = h0, stop = BACK ? h0 : h1; h < h1;) {
+      if (BACK) stop = min(stop + kRun * h_step, h1);
+      for (; h < stop; h += AHEAD * h_step) {
 #pragma unroll
-      for (int ahead = 0; ahead < AHEAD; ahead++) {
-        if (AHEAD > 1 && h + ahead * h_step >= h1) break;
-        const int hh = h + ahead * h_step + (group >> a.nt_log);
-        const bool there = mine && hh < h1;
-        if (has != (int)(hh >= a.q_heads)) {
-          if (BACK && has >= 0) flush();
-          has = hh >= a.q_heads;
-          if constexpr (BACK) {
-            weight(has, wa, wb);
+        for (int ahead = 0; ahead < AHEAD; ahead++) {
+          if (AHEAD > 1 && h + ahead * h_step >= h1) break;
+          const int hh = h + ahead * h_step + (group >> a.nt_log);
+          const bool there = mine && hh < h1;
+          if (has != (int)(hh >= a.q_heads)) {
+            if (BACK && has >= 0) flush();
+            has = hh >= a.q_heads;
+            if constexpr (BACK) {
+              weight(has, wa, wb);
+            } else {
+              float2 c[P], s[P], u[P], v[P];
+              turn(c, s);
+              weight(has, u, v);
+#pragma unroll
+              for (int i = 0; i < P; i++) {
+                ca[i] = __fmul2_rn(u[i], c[i]);
+                sa[i] = __fmul2_rn(u[i], s[i]);
+                cb[i] = __fmul2_rn(v[i], c[i]);
+                sb[i] = __fmul2_rn(v[i], neg(s[i]));
+              }
+            }
+          }
+          float2 xa[P], xb[P], sum = both(0.0f);
+          pairs<T, VEC, NS, INTER>(next[ahead], xa, xb);
+          Part<T, VEC, NS> in_g;
+          if (BACK) in_g = next_g[ahead];
+          if (mine && hh + AHEAD * h_step < h1) {
+            load_part(x + AHEAD * x_step, at, next[ahead]);
+            if (BACK) load_part(g + AHEAD * g_step, at, next_g[ahead]);
+          }
+#pragma unroll
+          for (int i = 0; i < P; i++) sum = __ffma2_rn(xb[i], xb[i], __ffma2_rn(xa[i], xa[i], sum));
+          float ss = group_sum<ODD>(sum.x + sum.y, a, base), scale = 1.0f, eps = a.eps;
+          if (sizeof(T) == 4) {
+            scale = safe_scale(ss, eps);
+            if (__any_sync(~0u, scale != 1.0f)) {
+              eps = eps * scale * scale;  // (scale^2 itself has no place in 32 bits)
+              sum = both(0.0f);
+#pragma unroll
+              for (int i = 0; i < P; i++) {
+                xa[i] = __fmul2_rn(xa[i], both(scale));
+                xb[i] = __fmul2_rn(xb[i], both(scale));
+                sum = __ffma2_rn(xb[i], xb[i], __ffma2_rn(xa[i], xa[i], sum));
+              }
+              ss = group_sum<ODD>(sum.x + sum.y, a, base);
+            }
+          }
+          // (2^-22 is enough where the result has 11 bits)
+          const float inv = sizeof(T) == 2 ? rsqrtf(__fmaf_rn(ss, inv_dim, eps)) : __frsqrt_rn(__fmaf_rn(ss, inv_dim, eps));
+          float2 ya[P], yb[P];
+          if constexpr (!BACK) {
+#pragma unroll
+            for (int i = 0; i < P; i++) {
+              const float2 p = __fmul2_rn(xa[i], both(inv)), q = __fmul2_rn(xb[i], both(inv));
+              ya[i] = __ffma2_rn(q, sb[i], __fmul2_rn(p, ca[i]));
+              yb[i] = __ffma2_rn(q, cb[i], __fmul2_rn(p, sa[i]));
+            }
           } else {
-            float2 c[P], s[P], u[P], v[P];
-            turn(c, s);
-            weight(has, u, v);
+            float2 ga[P], gb[P], dot = both(0.0f);
+            pairs<T, VEC, NS, INTER>(in_g, ga, gb);
 #pragma unroll
             for (int i = 0; i < P; i++) {
-              ca[i] = __fmul2_rn(u[i], c[i]);
-              sa[i] = __fmul2_rn(u[i], s[i]);
-              cb[i] = __fmul2_rn(v[i], c[i]);
-              sb[i] = __fmul2_rn(v[i], neg(s[i]));
+              xa[i] = __fmul2_rn(xa[i], both(inv));
+              xb[i] = __fmul2_rn(xb[i], both(inv));
+              // turned back
+              const float2 p = __ffma2_rn(ga[i], ca[i], __fmul2_rn(gb[i], sa[i]));
+              const float2 q = __ffma2_rn(ga[i], sb[i], __fmul2_rn(gb[i], ca[i]));
+              if (there) {
+                dwa[i] = __ffma2_rn(p, xa[i], dwa[i]);
+                dwb[i] = __ffma2_rn(q, xb[i], dwb[i]);
+              }
+              ga[i] = __fmul2_rn(p, wa[i]);
+              gb[i] = __fmul2_rn(q, wb[i]);
+              dot = __ffma2_rn(gb[i], xb[i], __ffma2_rn(ga[i], xa[i], dot));
             }
-          }
-        }
-        float2 xa[P], xb[P], sum = both(0.0f);
-        pairs<T, VEC, NS, INTER>(next[ahead], xa, xb);
-        Part<T, VEC, NS> in_g;
-        if (BACK) in_g = next_g[ahead];
-        if (mine && hh + AHEAD * h_step < h1) {
-          load_part(x + AHEAD * x_step, at, next[ahead]);
-          if (BACK) load_part(g + AHEAD * g_step, at, next_g[ahead]);
-        }
-#pragma unroll
-        for (int i = 0; i < P; i++) sum = __ffma2_rn(xb[i], xb[i], __ffma2_rn(xa[i], xa[i], sum));
-        float ss = group_sum<ODD>(sum.x + sum.y, a, base), scale = 1.0f, eps = a.eps;
-        if (sizeof(T) == 4) {
-          scale = safe_scale(ss, eps);
-          if (__any_sync(~0u, scale != 1.0f)) {
-            eps = eps * scale * scale;  // (scale^2 itself has no place in 32 bits)
-            sum = both(0.0f);
+            const float gn = -(group_sum<ODD>(dot.x + dot.y, a, base) * inv_dim);
 #pragma unroll
             for (int i = 0; i < P; i++) {
-              xa[i] = __fmul2_rn(xa[i], both(scale));
-              xb[i] = __fmul2_rn(xb[i], both(scale));
-              sum = __ffma2_rn(xb[i], xb[i], __ffma2_rn(xa[i], xa[i], sum));
+              ya[i] = __fmul2_rn(__ffma2_rn(xa[i], both(gn), ga[i]), both(inv));
+              yb[i] = __fmul2_rn(__ffma2_rn(xb[i], both(gn), gb[i]), both(inv));
+              if (sizeof(T) == 4) {
+                ya[i] = __fmul2_rn(ya[i], both(scale));
+                yb[i] = __fmul2_rn(yb[i], both(scale));
+              }
             }
-            ss = group_sum<ODD>(sum.x + sum.y, a, base);
           }
+          Part<T, VEC, NS> out;
+          unpairs<T, VEC, NS, INTER>(ya, yb, out);
+          if (there) store_part(y, at, out);
+          x += x_step;
+          y += y_step;
+          if (BACK) g += g_step;
         }
-        // (2^-22 is enough where the result has 11 bits)
-        const float inv = sizeof(T) == 2 ? rsqrtf(__fmaf_rn(ss, inv_dim, eps)) : __frsqrt_rn(__fmaf_rn(ss, inv_dim, eps));
-        float2 ya[P], yb[P];
-        if constexpr (!BACK) {
-#pragma unroll
-          for (int i = 0; i < P; i++) {
-            const float2 p = __fmul2_rn(xa[i], both(inv)), q = __fmul2_rn(xb[i], both(inv));
-            ya[i] = __ffma2_rn(q, sb[i], __fmul2_rn(p, ca[i]));
-            yb[i] = __ffma2_rn(q, cb[i], __fmul2_rn(p, sa[i]));
-          }
-        } else {
-          float2 ga[P], gb[P], dot = both(0.0f);
-          pairs<T, VEC, NS, INTER>(in_g, ga, gb);
-#pragma unroll
-          for (int i = 0; i < P; i++) {
-            xa[i] = __fmul2_rn(xa[i], both(inv));
-            xb[i] = __fmul2_rn(xb[i], both(inv));
-            // turned back
-            const float2 p = __ffma2_rn(ga[i], ca[i], __fmul2_rn(gb[i], sa[i]));
-            const float2 q = __ffma2_rn(ga[i], sb[i], __fmul2_rn(gb[i], ca[i]));
-            if (there) {
-              dwa[i] = __ffma2_rn(p, xa[i], dwa[i]);
-              dwb[i] = __ffma2_rn(q, xb[i], dwb[i]);
-            }
-            ga[i] = __fmul2_rn(p, wa[i]);
-            gb[i] = __fmul2_rn(q, wb[i]);
-            dot = __ffma2_rn(gb[i], xb[i], __ffma2_rn(ga[i], xa[i], dot));
-          }
-          const float gn = -(group_sum<ODD>(dot.x + dot.y, a, base) * inv_dim);
-#pragma unroll
-          for (int i = 0; i < P; i++) {
-            ya[i] = __fmul2_rn(__ffma2_rn(xa[i], both(gn), ga[i]), both(inv));
-            yb[i] = __fmul2_rn(__ffma2_rn(xb[i], both(gn), gb[i]), both(inv));
-            if (sizeof(T) == 4) {
-              ya[i] = __fmul2_rn(ya[i], both(scale));
-              yb[i] = __fmul2_rn(yb[i], both(scale));
-            }
-          }
-        }
-        Part<T, VEC, NS> out;
-        unpairs<T, VEC, NS, INTER>(ya, yb, out);
-        if (there) store_part(y, at, out);
-        x += x_step;
-        y += y_step;
-        if (BACK) g += g_step;
       }
+      if (BACK) flush(), has = -1;
     }
   }
   if constexpr (BACK) {
     if (!a.partials) return;
     // The block's sums, of one weight and then of the other: a warp's groups, then the
     // warps one after the other.
-    if (has >= 0) flush();
     double *const rows = reinterpret_cast<double *>(cs);
     for (int k0 = 0; k0 < 2; k0++) {
       __syncthreads();

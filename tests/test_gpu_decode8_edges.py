@@ -9,8 +9,9 @@ pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
 import decode8_oracle as O8  # noqa: E402
+from shlo import decode as Dc  # noqa: E402
 from shlo import mlx as M  # noqa: E402
-from test_gpu_decode8 import NP, same, select  # noqa: E402
+from test_gpu_decode8 import NP, TT, cuda, same, select, stream, work  # noqa: E402
 
 
 @pytest.fixture(scope="module", autouse=True)
@@ -19,6 +20,30 @@ def device():
     M.set_device(0)
     yield
     torch.cuda.empty_cache()
+
+
+# -------------------------------------------------------------- norm_rope ----
+
+@pytest.mark.parametrize("kind", ["f16", "f32"])
+@pytest.mark.parametrize("q_heads", [0, 8])
+def test_norm_rope_grad_of_many_tokens_of_one_kind(kind, q_heads):
+    """Queries alone, keys alone: a thread's terms of one weight's gradient are as many as 900 in a row, of one sign and
+    here all the same, so that what an addition loses, it loses each time. What is summed in binary32 are 16 heads: 2^-20 of
+    the sum of magnitudes, as much again the norm (16 + 5 roundings, 2^-24 each, and the root's), and the result's own
+    rounding: 2^-18, however many tokens."""
+    T, H, D = 400000, 8, 512
+    rng = np.random.default_rng(q_heads + 5)
+    x, dy = rng.uniform(0.5, 2, (2, 1, 1, D)).astype(NP[kind])
+    w = (1 + 0.3 * rng.standard_normal(D)).astype(np.float32)
+    pos, phases = torch.zeros(T, dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda")
+    dx, dw = torch.empty(T, H, D, dtype=TT[kind], device="cuda"), torch.full((2, D), np.nan, device="cuda")
+    Dc.norm_rope_grad_noalloc(cuda(x).expand(T, H, D), cuda(dy).expand(T, H, D), pos, phases, dx, dw[0], dw[1], q_heads=q_heads,
+                              q_weight=cuda(w), k_weight=cuda(w), eps=1e-5, workspace=work(Dc.norm_rope_workspace()), stream=stream())
+    n = x.astype(np.float64) / np.sqrt((x.astype(np.float64) ** 2).mean() + np.float64(np.float32(1e-5)))
+    want = T * H * (n * dy.astype(np.float64))[0, 0]
+    got = dw.cpu().numpy().astype(np.float64)
+    assert np.all(np.abs(got[0 if q_heads else 1] - want) <= 2.0 ** -18 * want)
+    assert np.all(got[1 if q_heads else 0] == 0)
 
 
 # ------------------------------------------------------------ beam_select ----
