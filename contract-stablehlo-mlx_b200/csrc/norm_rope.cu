@@ -513,8 +513,9 @@ int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st)
   const char *const what = back ? "norm_rope_grad" : "norm_rope";
   if (c.dtype != kF16 && c.dtype != kF32) return fail("%s: %s not carried (float16 or float32)", what, dtype_name(c.dtype));
   if (c.weight_dtype != kF16 && c.weight_dtype != kF32) return fail("%s: weights of %s not carried (float16 or float32)", what, dtype_name(c.weight_dtype));
-  if (c.tokens < 0 || c.heads < 1 || c.dim < 1 || c.dim > 512)
-    return fail("%s: %lld tokens, %d heads of %d (1 to 512)", what, (long long)c.tokens, c.heads, c.dim);
+  // (the kernel counts heads in 32 bits, up to a block's turns beyond the last)
+  if (c.tokens < 0 || c.heads < 1 || c.heads > (1 << 30) || c.dim < 1 || c.dim > 512)
+    return fail("%s: %lld tokens, %d heads (1 to 2^30) of %d (1 to 512)", what, (long long)c.tokens, c.heads, c.dim);
   if (c.q_heads < 0 || c.q_heads > c.heads) return fail("%s: %d query heads of %d", what, c.q_heads, c.heads);
   if (c.rot < 0 || c.rot > c.dim || c.rot % 2) return fail("%s: %d of %d dimensions turned (an even number)", what, c.rot, c.dim);
   if (c.flags & ~1u) return fail("%s: flags 0x%x", what, c.flags);

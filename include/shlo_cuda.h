@@ -226,8 +226,8 @@ int shlo_rope_noalloc(const void *x, int64_t x_token, int64_t x_head, const int3
    y = turn(n w), n = x / sqrt(mean of x^2 over the head's dim values + eps), the
    turn shlo_rope_noalloc's (flags: 1 alone). The first q_heads heads have the
    weight q_weight [dim], the others k_weight [dim] (float16 or float32,
-   `weight_dtype`; NULL: ones). dim up to 512; y as shlo_rope_noalloc's. Strides
-   are in values. */
+   `weight_dtype`; NULL: ones). dim up to 512, heads up to 2^30; y as
+   shlo_rope_noalloc's, and not in what else is read. Strides are in values. */
 typedef struct {
 	const void *x;
 	int64_t x_token, x_head;

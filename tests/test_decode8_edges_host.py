@@ -129,6 +129,13 @@ def test_norm_rope_rows_in_what_is_read(back, name, length):
     assert (norm_rope(back, **{name: 6 * FAR}, rot=0) == "") == (name in ("positions", "phases"))  # (then they are not read)
 
 
+@pytest.mark.parametrize("back", [False, True])
+def test_more_heads_than_are_counted(back):
+    for heads in ((1 << 30) + 1, (1 << 31) - 1):
+        assert "2^30" in norm_rope(back, tokens=1, heads=heads, dim=1, rot=0, x_head=1, y_head=1, dy_head=1)
+    assert norm_rope(back, tokens=1, heads=1 << 30, dim=1, rot=0, x_head=1, y_head=1, dy_head=1) == ""
+
+
 # ---- of the Python forms ----
 
 @pytest.mark.parametrize("work", [torch.zeros(1, dtype=torch.uint8).expand(1 << 20), torch.zeros(1 << 21, dtype=torch.uint8)[::2],
