@@ -23,6 +23,14 @@ from ._lib import BEAM_ARGS, KV_FORK_ARGS, MUL_MAT8_ARGS, NORM_ROPE_ARGS, KvBatc
 _UNPACKED = (struct.error, OverflowError)  # a number that a descriptor's field does not hold
 _norm_rope, _mul_mat8, _beam, _fork = NORM_ROPE_ARGS.pack, MUL_MAT8_ARGS.pack, BEAM_ARGS.pack, KV_FORK_ARGS.pack
 
+
+def _words(what, *numbers):
+    """Numbers that go as 32-bit arguments, which would be cut to what fits."""
+    for v in numbers:
+        if not -1 << 31 <= v < 1 << 31:
+            raise ShloError("%s: %d is no 32-bit number" % (what, v))
+
+
 SCALINGS = {"none": 0, "linear": 1, "base": 2, "ramp": 3, "blend": 4}
 
 _NAMES = {"torch.float16": M.dtF16, "torch.float32": M.dtF32, "torch.int32": M.dtI32, "torch.int64": M.dtI64,
@@ -339,6 +347,7 @@ def quantise_rows_noalloc(x, q, scale, *, stream=0):
         raise ShloError("quantise_rows: q is not x's shape")
     if r > 1 and qs < n:
         raise ShloError("quantise_rows: rows of q overlap")
+    _words("quantise_rows", n)
     check(lib.shlo_quantise_rows_noalloc(x.data_ptr(), xs, r, n, dt, q.data_ptr(), qs, _scales(scale, r, "quantise_rows: scale", at),
                                          stream))
 
@@ -371,6 +380,7 @@ def mul_mat8_noalloc(x, x_scale, w, w_scale, out, *, bias=None, stream=0):
 
 def linear8_workspace(rows: int, n: int) -> int:
     """Bytes of the workspace that linear8_noalloc needs for so many rows of n values."""
+    _words("linear8_workspace", n)
     b = ctypes.c_size_t()
     check(load().shlo_linear8_workspace(rows, n, ctypes.byref(b)))
     return b.value
@@ -395,6 +405,7 @@ def _grid(x, code, shape, what, at):
 
 def beam_workspace(seqs: int, beams: int, keep: int, vocab: int) -> int:
     """Bytes of the workspace that beam_select_noalloc needs."""
+    _words("beam_workspace", seqs, beams, keep, vocab)
     n = ctypes.c_size_t()
     check(load().shlo_beam_workspace(seqs, beams, keep, vocab, ctypes.byref(n)))
     return n.value
@@ -444,10 +455,13 @@ def fork_noalloc(pool: Pool, tables, lens, parents, fresh, out_tables, out_lens,
                         % (rows, news, width))
     if news > 1 and ostride < width:
         raise ShloError("kv_fork: rows of out_tables overlap")
-    if lib.shlo_kv_fork_noalloc(
-            pool.c, _fork(tables.data_ptr(), lens.data_ptr(), stride, parents.data_ptr(), fresh.data_ptr(), out_tables.data_ptr(),
-                          out_lens.data_ptr(), ostride, rows, news, width), stream):
-        check(1)
+    try:
+        if lib.shlo_kv_fork_noalloc(
+                pool.c, _fork(tables.data_ptr(), lens.data_ptr(), stride, parents.data_ptr(), fresh.data_ptr(), out_tables.data_ptr(),
+                              out_lens.data_ptr(), ostride, rows, news, width), stream):
+            check(1)
+    except _UNPACKED as e:
+        raise ShloError("kv_fork: %s" % e) from None
 
 
 # ---- on arrays (mlx.Arr), in the library's own memory ----
@@ -471,6 +485,8 @@ def norm_rope(x: M.Arr, positions: M.Arr, phases: M.Arr, q_weight: M.Arr, k_weig
     """x [tokens, heads, dim], each head normed, weighted (the first q_heads by q_weight, the others by k_weight, [dim])
     and turned by positions. May be called inside a compiled function, as may what follows up to Cache."""
     t, h, d = M.shape(x)
+    if not 0 <= q_heads <= h:
+        raise ShloError("norm_rope: %d query heads of %d" % (q_heads, h))
     words = [t, h, d, 2 * M.shape(phases)[0], 1 if interleaved else 0, _bits(factor), q_heads, _bits(eps)]
     return M.kernel_apply(Run.kernel("norm_rope"), [x, positions, phases, q_weight, k_weight, Run.params(words)], [[t, h, d]],
                           bytes([M.dtype(x)]), [max(t, 1), 1, 1], [64, 1, 1])[0]
@@ -483,6 +499,7 @@ def _outs(n):
 def norm_rope_grad(x: M.Arr, dy: M.Arr, positions: M.Arr, phases: M.Arr, q_weight: M.Arr, k_weight: M.Arr, *, q_heads: int,
                    eps: float, interleaved=False, factor=1.0):
     """(dx, dq_weight, dk_weight) of norm_rope."""
+    _words("norm_rope_grad", q_heads)
     o = _outs(3)
     check(load().shlo_norm_rope_grad(x.h, dy.h, positions.h, phases.h, q_weight.h, k_weight.h, q_heads, eps,
                                      1 if interleaved else 0, factor, *[ctypes.byref(a) for a in o]))
@@ -507,6 +524,7 @@ def linear8(x: M.Arr, w: M.Arr, w_scale: M.Arr, *, x_scale: M.Arr | None = None,
 
 def beam_select(logits: M.Arr, scores: M.Arr, keep: int, *, ended: M.Arr | None = None, end_token=-1):
     """(scores, parents, tokens) [sequences, keep] of logits [sequences * beams, vocabulary], scores [sequences, beams]."""
+    _words("beam_select", keep, end_token)
     o = _outs(3)
     check(load().shlo_beam_select(logits.h, scores.h, ended.h if ended else None, end_token, keep,
                                   *[ctypes.byref(a) for a in o]))

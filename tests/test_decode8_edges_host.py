@@ -1,6 +1,7 @@
 """What the launch functions of the norm with rotation, the products in 8 bits, beam search and the cache's reordering
 refuse, and what their Python forms do, where no GPU is needed: the checks come before anything is launched or read."""
 import ctypes
+import types
 
 import pytest
 
@@ -167,3 +168,41 @@ def test_attention_over_a_workspace_that_is_not_contiguous(monkeypatch):
     with pytest.raises(ShloError, match="contiguous"):
         attend(Hd.On(torch.zeros(1, dtype=torch.uint8).expand(1 << 20)))
     assert len(made) == 1
+
+
+class Wide(H.On):
+    """A tensor that says it has other sizes than it has."""
+
+    def __init__(self, t, shape, stride=None):
+        super().__init__(t)
+        self.shape, self.strides = shape, stride
+
+    def stride(self):
+        return self.strides or self.t.stride()
+
+
+def test_numbers_that_would_be_cut_to_32_bits(calls, monkeypatch):  # noqa: F811
+    t = H.operands()
+    n = (1 << 32) + 32
+    with pytest.raises(ShloError, match="quantise_rows.*32-bit"):
+        H.Dc.quantise_rows_noalloc(Wide(t["a"].t, (5, n), (n, 1)), Wide(t["q"].t, (5, n), (n, 1)), t["s"])
+    wide = torch.zeros(1, 2, dtype=torch.int32).expand(1 << 31, 2)
+    with pytest.raises(ShloError, match="kv_fork"):
+        H.Dc.fork_noalloc(H.Dc.Pool(t["k"], t["v"], t["ks"], t["vs"]), H.On(wide), Wide(t["lens"].t, (1 << 31,), (1,)), t["parents"], t["fresh"],
+                          t["tables2"], t["lens2"])
+    assert calls == []
+    monkeypatch.undo()  # (the library itself)
+    for args in ((n, 1, 1, 9), (1, n, 1, 9), (1, 1, n, 9), (1, 1, 1, n)):
+        with pytest.raises(ShloError):
+            H.Dc.beam_workspace(*args)
+    with pytest.raises(ShloError):
+        H.Dc.linear8_workspace(1, n)
+    arr = types.SimpleNamespace(h=None)
+    for f in (lambda: H.Dc.beam_select(arr, arr, n), lambda: H.Dc.beam_select(arr, arr, 4, end_token=-n),
+              lambda: H.Dc.norm_rope_grad(arr, arr, arr, arr, arr, arr, q_heads=n, eps=1e-6)):
+        with pytest.raises(ShloError, match="32-bit"):
+            f()
+    monkeypatch.setattr(H.Dc.M, "shape", lambda a: (3, 4, 16))
+    for q_heads in (-1, 5, n):
+        with pytest.raises(ShloError, match="query heads"):
+            H.Dc.norm_rope(arr, arr, arr, arr, arr, q_heads=q_heads, eps=1e-6)
