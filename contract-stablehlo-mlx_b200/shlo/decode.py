@@ -447,7 +447,7 @@ def fork_noalloc(pool: Pool, tables, lens, parents, fresh, out_tables, out_lens,
         _pool(pool, at)
     # (a selection's parents come as [sequences, beams])
     n = parents.shape
-    flat = n[0] if len(n) == 1 else n[0] * n[1] if len(n) == 2 and parents.is_contiguous() else -1
+    flat = n[0] if len(n) == 1 else parents.numel() if len(n) and parents.is_contiguous() else -1
     if _code(parents, at) != _I32 or flat != news or (len(n) == 1 and news > 1 and parents.stride()[0] != 1):
         raise ShloError("kv_fork: parents are not int32 of %d rows" % news)
     if w != width or _list(lens, _I32, "kv_fork: lens", at) != rows or _list(fresh, _I32, "kv_fork: fresh", at) != news or \

@@ -208,13 +208,13 @@ def test_numbers_that_would_be_cut_to_32_bits(calls, monkeypatch):  # noqa: F811
             H.Dc.norm_rope(arr, arr, arr, arr, arr, q_heads=q_heads, eps=1e-6)
 
 
-@pytest.mark.parametrize("shape", [(), (2, 4, 1), (2, 4, 5), (8, 1, 2), (0,)])
-def test_fork_of_parents_of_other_ranks(calls, shape):  # noqa: F811
-    """Of the rows' parents a vector or [sequences, beams]: not the first of more."""
+@pytest.mark.parametrize("shape", [(), (2, 4, 5), (8, 1, 2), (0,)])
+def test_fork_of_more_parents_than_rows(calls, shape):  # noqa: F811
+    """The rows' parents are all that there are: not the first of more."""
     t = H.operands()
     args = (H.Dc.Pool(t["k"], t["v"], t["ks"], t["vs"]), t["tables"], t["lens"])
-    for parents in (t["parents"], H.On(torch.zeros(8, dtype=torch.int32))):
+    for parents in (t["parents"], H.On(torch.zeros(8, dtype=torch.int32)), H.On(torch.zeros(2, 4, 1, dtype=torch.int32))):
         H.Dc.fork_noalloc(*args, parents, t["fresh"], t["tables2"], t["lens2"])
     with pytest.raises(ShloError, match="parents"):
         H.Dc.fork_noalloc(*args, H.On(torch.zeros(shape, dtype=torch.int32)), t["fresh"], t["tables2"], t["lens2"])
-    assert calls == 2 * ["kv_fork"]
+    assert calls == 3 * ["kv_fork"]
