@@ -113,6 +113,11 @@ class Decoder:
     def fork(self, rows, parents):
         """New sequences, number i going on from rows[parents[i]] as it is now; the rows themselves stop. Full pages are
         shared; a last page that is not full is copied for all but the first that go on from its owner."""
+        if len({id(s) for s in rows}) != len(rows):
+            raise ShloError("decoder: a sequence named twice in one fork")
+        for p in parents:
+            if not 0 <= p < len(rows):
+                raise ShloError("decoder: a parent %d of %d rows" % (p, len(rows)))
         page = self.cfg.page_tokens
         seen, copied = set(), []
         for i, p in enumerate(parents):
