@@ -156,19 +156,19 @@ class Decoder:
         rows, texts, scores, y = [s], [[]], np.zeros((1, 1), np.float32), y[-1:]
         ended = np.zeros((1, 1), np.int32)
         try:
-            for _ in range(steps):
+            for left in range(steps, 0, -1):
                 z = self._dense(M.of_numpy(np.ascontiguousarray(y)), "head", "chead", cfg.vocab, cfg.d, len(rows))
                 got = D.beam_select(M.reshape(z, [len(rows), cfg.vocab]), M.of_numpy(scores), beams, ended=M.of_numpy(ended),
                                     end_token=end)
                 scores, parents, tokens = (M.to_numpy(a) for a in got)
                 live = [(int(p), int(t)) for p, t in zip(parents[0], tokens[0]) if p >= 0]  # (a vocabulary may be smaller)
-                rows = self.fork(rows, [p for p, _ in live])
                 over = [bool(ended[0, p]) for p, _ in live]
                 texts = [texts[p] if o else texts[p] + [t] for (p, t), o in zip(live, over)]
                 scores = np.ascontiguousarray(scores[:, :len(live)])
                 ended = np.array([[o or t == end for (_, t), o in zip(live, over)]], np.int32)
-                if ended.all():
+                if ended.all() or left == 1:  # (no page is taken for what nobody reads)
                     break
+                rows = self.fork(rows, [p for p, _ in live])
                 # (a beam that has ended takes its token again: nothing reads what follows)
                 y = self.step([(r, self.embed[[max(t, 0)]]) for r, (_, t) in zip(rows, live)])
         finally:
