@@ -227,7 +227,12 @@ int shlo_rope_noalloc(const void *x, int64_t x_token, int64_t x_head, const int3
    turn shlo_rope_noalloc's (flags: 1 alone). The first q_heads heads have the
    weight q_weight [dim], the others k_weight [dim] (float16 or float32,
    `weight_dtype`; NULL: ones). dim up to 512, heads up to 2^30; y as
-   shlo_rope_noalloc's, and not in what else is read. Strides are in values. */
+   shlo_rope_noalloc's, and not in what else is read. Strides are in values. A head
+   with a NaN is all NaN. Of one with an infinity the values are 0, and NaN at the
+   infinity and at what is turned with it, or at one other where neither is turned. A
+   weight that is not finite makes NaN of the same places in every head that it meets,
+   a dy of a head's whole dx and of those places of the weight's gradient. Other heads
+   are as without it. */
 typedef struct {
 	const void *x;
 	int64_t x_token, x_head;
@@ -365,8 +370,9 @@ int shlo_kv_gather_noalloc(const shlo_kv_pool *pool, const int32_t *tables, int6
                            void *stream);
 /* Rows that go on as other rows, as a beam search's: new row r (of `news`, up to
    65536) gets the length and the pages of row parents[r] of `rows` (outside them: no
-   tokens, no pages). Full pages are shared. A last page that is not full stays with
-   the first new row that continues its owner; for each later one its tokens and
+   tokens, no pages). Full pages are shared. A last page that is not full belongs to one
+   old row (of two rows that name the same one both would go on in it); it stays with
+   the first new row that continues that row; for each later one its tokens and
    scales are copied into page fresh[r], which no row holds, and that is its last
    page. fresh[r] is not read otherwise. Entries behind a row's last page become -1.
    out_tables and out_lens share no memory with what is read. A host that keeps
