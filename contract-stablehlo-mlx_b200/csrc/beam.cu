@@ -21,10 +21,11 @@
 // us: from the first stretch's alone 47.3, from beyond 2 above it 47.9, from any above it
 // 49.4.)
 //
-// Bound: bytes (each logit read once), then the first kernel's ten instructions a
-// logit. Measured on one B200: 64 sequences of 8 beams over 128256 float16 logits (125
-// MB) 46 us, 36 of them the first kernel, at 512 blocks on 592 places; 5 of 32 over 50257
-// float32 logits, 64 kept 27 us; one of 4 over 32001 10 us. Measured and left: the
+// Bound: bytes (each logit read once); what keeps the first kernel from their rate are its
+// ten instructions a logit and their waits: issue slots 57 % used, DRAM 38 %, 14 warps on
+// an SM on average. Measured on one B200: 64 sequences of 8 beams over 128256 float16
+// logits (125 MB) 47 us, 37 of them the first kernel, at 512 blocks on 592 places; 5 of 32
+// over 50257 float32 logits, 64 kept 28 us; one of 4 over 32001 10 us. Measured and left: the
 // polynomial for every term (64 us on the first case: the heavy half of the FMA pipe), a
 // part of one stretch each (73 us: every one searches for its border), borders by
 // halving over lists in memory (67 us for the second case's join alone).

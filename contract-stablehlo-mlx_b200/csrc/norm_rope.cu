@@ -7,15 +7,18 @@
 //   dz = turn(dy, -position),  dw = sum of dz n over tokens and heads,
 //   g = dz w,   dx = (g - n mean(g n)) / sqrt(mean(x^2) + eps).
 //
-// Bound: bytes (each value read once and written once), and close behind them the
-// instructions. A group of 1 to 32 lanes holds a head in registers; it keeps one token
-// and goes over heads, so that its pairs' cosines and sines, and the weight, stay in
-// registers too (forward: their products); heads to come are asked for ahead, up to four
-// of them forward and one backward. Two pairs go through each packed instruction.
+// Bound: bytes (each value read once and written once); what keeps it from a copy's rate
+// are waits, with the 16 warps an SM that the registers leave (the gradient: 24), whose
+// issue slots are 51 % used (63 %): for the loads, of which few are ahead, and for the
+// sums over a group, two of them one after the other in the gradient. A group of 1 to 32
+// lanes holds a head in registers; it keeps one token and goes over heads, so that its
+// pairs' cosines and sines, and the weight, stay in registers too (forward: their
+// products); heads to come are asked for ahead, up to four of them forward and one
+// backward. Two pairs go through each packed instruction.
 // Measured on one B200: 16384 tokens x 40 heads x 128, float16 (336 MB) 63 us, 5.3 TB/s
 // (rope.cu alone 55); the gradient of 24001 x 12 x 80 float32, 32 dimensions turned in
 // interleaved pairs (277 MB) 70 us, 3.9 TB/s: ten units of eight values a head, on ten
-// lanes, three heads a warp (84 us on 16 lanes). Measured and left there, on 16 lanes:
+// lanes, three heads a warp (82 us on 16 lanes). Measured and left there, on 16 lanes:
 // four blocks an SM (125 us, registers to memory) and two (91 us), no head ahead (88 us).
 #include <algorithm>
 #include <cmath>
@@ -562,9 +565,10 @@ int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st)
   SHLO_TRY(check_in_place(c.x, c.x_token, c.x_head, c.y, c.y_token, c.y_head, c.tokens, c.heads, c.dim, size, what, "x", back ? "dx" : "y"));
   if (back)
     SHLO_TRY(check_in_place(c.dy, c.dy_token, c.dy_head, c.y, c.y_token, c.y_head, c.tokens, c.heads, c.dim, size, what, "dy", "dx"));
-  // The widest vector (16 bytes at most) that every offset is a multiple of. (40 heads of
-  // 72, 18 turned, float16, pairs side by side: 36 us with eight values, which needs no
-  // half of them to be whole vectors, 105 with one; the gradient 73 and 280.)
+  // The widest vector (16 bytes at most) that every offset is a multiple of. (16384 tokens
+  // of 40 heads of 72, 18 turned, float16, pairs side by side: 48 us with eight values,
+  // which needs no half of them to be whole vectors, 144 with one; the gradient 92 and 260.
+  // Half the turned part apart they are 144 and 293: one value at a time.)
   const int half = c.rot / 2, rest = c.dim - c.rot;
   const bool inter = (c.flags & 1) != 0;
   int vec = (int)(16 / size);
@@ -606,8 +610,10 @@ int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st)
   a.nt_log = tokens_log(1 << a.lanes_log);
   // Five, six or ten lanes a group, where a block then takes fewer turns over its heads
   // for as many tokens. (80 dimensions, 32 turned, float32, the gradient of 24001 x 12: ten
-  // lanes 70 us, sixteen 84; 40 heads of 72, float16: 58 and 67. Of vectors of two
-  // values, 40 heads of 80, float32: 91 and 79, their loads are apart.)
+  // lanes 69 us, sixteen 82.5; 16384 tokens of 40 heads of 72, 18 turned, side by side,
+  // float16: 48 and 53.6, all turned, the gradient: 93.6 and 110. Of vectors of two values,
+  // which are apart in memory, 8192 x 40 x 80 float32, 36 turned, would take 81 instead of
+  // 72, and the gradient 98 instead of 118.)
   if (vec >= 4)
     for (const int lanes : {5, 6, 10})
       if (lanes < 1 << a.lanes_log && slots * lanes >= units) {
@@ -622,10 +628,12 @@ int launch_norm_rope(const NormRopeCall &c, bool back, int sms, cudaStream_t st)
   int parts = 1;
   while (tiles * parts < 2 * sms && parts < (c.heads + step - 1) / step) parts++;
   a.hb = (c.heads + parts - 1) / parts;
-  // (us: 16384 x 40 x 128 float16, 20 turns, 64 with four heads ahead and two blocks on an
-  // SM, 70 with one and three; of 3 heads of 64, one turn, 68 and 56; 40 heads of 64, five,
-  // 30 and 32; 7 of 256, four, 25 and 23. Four values a lane, 40 heads of 128 float32, 20
-  // turns, 47 with three blocks and 51 with four; of 80, 14 turns, 51 and 48.)
+  // (us, with four heads ahead and two blocks on an SM, and with one and three; tokens x
+  // heads x dimensions, float16: 16384 x 40 x 128, ten turns, 62.7 and 68.5; 32768 x 40 x 64,
+  // five, 68.4 and 72.9; 16384 x 7 x 256, four, 32.8 and 31.1; 436000 x 3 x 64, two, 182 and
+  // 146. Four values a lane, two heads ahead, three blocks and four, float32: 8192 x 40 x
+  // 80, 14 turns, 45.9 and 43.3; of 128 dimensions, 20 turns, it goes by the
+  // tokens of 40 heads: 6100 45.3 and 50.7, 8192 62.6 and 60.4, 16384 112 and 114.)
   const bool few = (a.hb + step - 1) / step <= (slots * vec > 4 ? 4 : 14);
   dim3 grid((unsigned)tiles, (unsigned)((c.heads + a.hb - 1) / a.hb));
   // The backward pass has as many blocks as run at once, each with a row of sums.
