@@ -122,22 +122,10 @@ __device__ __forceinline__ double replaced(float d) {
   return (double)exp_near(near).x - (double)exp_fast(near).x;
 }
 
-// A sum counted from `from`, counted from `to` above it: times e^d, by the power series
-// of degree 9 (8 10^-12; a call of exp takes four times as long, which all wait for).
-// (Both are rare: their code is not the loop's.)
+// A sum counted from `from`, counted from `to` above it. (This and the next are rare:
+// their code is not the loop's, whose registers it would take.)
 __device__ __noinline__ double recounted(double sum, float from, float to) {
-  const double d = fmax((double)from - (double)to, -600.0), i = rint(d * 1.4426950408889634), r = fma(i, -0.69314718055994531, d);
-  double p = 1.0 / 362880.0;
-  p = fma(p, r, 1.0 / 40320.0);
-  p = fma(p, r, 1.0 / 5040.0);
-  p = fma(p, r, 1.0 / 720.0);
-  p = fma(p, r, 1.0 / 120.0);
-  p = fma(p, r, 1.0 / 24.0);
-  p = fma(p, r, 1.0 / 6.0);
-  p = fma(p, r, 0.5);
-  p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  return sum * __hiloint2double(__double2hiint(p) + ((int)i << 20), __double2loint(p));
+  return from > -INFINITY ? sum * exp((double)from - (double)to) : 0.0;
 }
 __device__ __noinline__ double replaced_apart(float d) { return d < 0.0f ? replaced(d) : 0.0; }
 
